@@ -75,7 +75,7 @@ int pkv_device_available(void);
 enum pkv_codec_kind { PKV_CODEC_TURBO = 1, PKV_CODEC_FIB = 2 };
 enum pkv_turbo_mode { PKV_TURBO_POLAR_ONLY = 0, PKV_TURBO_POLAR_WITH_QJL = 1 };
 enum pkv_radii_codec { PKV_RADII_F32 = 0, PKV_RADII_LOG_U8 = 1 };
-enum pkv_dtype { PKV_F32 = 0, PKV_BF16 = 1, PKV_F16 = 2 };
+enum pkv_dtype { PKV_F32 = 0, PKV_BF16 = 1, PKV_F16 = 2, PKV_FP4 = 3 /* cache views (pkv_kv_view) only */ };
 
 /* Replaces TurboQuantizer::new_with_mode (turbo-quant/src/turbo.rs:124-188)
  * as built by TurboQuantAdapter (proveKV/src/codec.rs:249-250): FastHadamard
@@ -495,6 +495,146 @@ int pkv_score_status(const uint32_t* host_status, uint32_t nseg, pkv_error* err)
 int pkv_turbo_score_batch(pkv_ctx* ctx, const pkv_profile* prof, const uint8_t* payload, uint64_t len,
                           const float* queries, uint32_t nq, float post_scale, float* scores, uint64_t scores_cap,
                           uint64_t* n_out, pkv_error* err);
+
+/* ---------------------------------------------------------------- live caches
+ * Attention over a KV cache on the device, the 4-bit cache, and eviction: what
+ * a serving loop does with the caches pkv_decode_segments_ex rehydrates.  No
+ * counterpart in the reference, whose harness hands the decoded cache to a
+ * framework's own attention (proveKV/scripts/ppl_validate_multi_agent.py:226-272).
+ *
+ * A cache view: keys and values of `copies` caches x `layers` x `heads`, each
+ * `slots` rows of `dim` (64 or 128) elements.  Row j of (copy c, layer l, head
+ * h) starts at element c * copy_stride + l * layer_stride + h * head_stride +
+ * j * slot_stride of d_keys and of d_values; elems bounds every such row's end
+ * (checked), so it is the element count behind each of the two pointers.
+ *   PKV_F32, PKV_BF16, PKV_F16: pointers 16-byte aligned, strides a multiple
+ *     of 16 bytes; scale pointers NULL.
+ *   PKV_FP4: OCP MX FP4.  Two 4-bit codes a byte (even element low) of the
+ *     e2m1 values 0, .5, 1, 1.5, 2, 3, 4, 6 (bit 3: sign), blocks of 32 along
+ *     dim with one scale byte b, standing for code value * 2^(b - 127); b = 255
+ *     makes the block NaN.  d_keys / d_values are the codes (byte = element /
+ *     2), d_key_scales / d_value_scales the scale bytes (byte = element / 32),
+ *     16- and 4-byte aligned, strides a multiple of dim. */
+typedef struct pkv_kv_view {
+    void* d_keys;
+    void* d_values;
+    uint8_t* d_key_scales;
+    uint8_t* d_value_scales;
+    uint64_t copy_stride, layer_stride, head_stride, slot_stride;
+    uint64_t elems;
+    uint32_t copies, layers, heads, slots, dim;
+    int32_t dtype;
+} pkv_kv_view;
+
+/* Attention of nq query rows per copy and query head over one layer's view
+ * (layers == 1).  Query row i of copy c, i < q_len(c), stands at slot
+ *     p = len(c) - q_len(c) + i      (the last q_len slots are the rows' own)
+ * and sees slot j when 0 <= j <= p and (window == 0 or p - j < window or
+ * j < sinks): causal, the last `window` slots, and the first `sinks` always.
+ *     s_j = scale <q, k_j>,   w_j = exp(s_j - max s) / sum,   out = sum w_j v_j
+ * Query head g belongs to KV head g / (q_heads / heads).  A row that sees no
+ * slot, or only slots whose logit is -inf, gives out = 0 and lse = -inf.
+ * Slots that a row does not see never reach it, whatever they hold (NaN too).
+ *   q, out   element (c, i, g, 0) at c * copy_stride + i * row_stride + g *
+ *            head_stride, of dtype: the cache's, or for PKV_FP4 any of
+ *            PKV_F32 / PKV_BF16 / PKV_F16; 16-byte aligned, strides a multiple
+ *            of 16 bytes.  Rows i >= q_len(c) of out are left as they were.
+ *   d_lens   [copies] int32 device words: len(c), taken into 0 .. max_len
+ *   d_q_lens [copies] int32 device words, taken into 0 .. nq, or NULL (nq)
+ *   d_lse    NULL, or f32 [copies][q_heads][nq]: natural log of the sum of
+ *            exp(s_j) (rows i >= q_len(c) left as they were)
+ *   d_weights NULL, or f32 (c, h, j) at c * weight_copy_stride + h *
+ *            weight_head_stride + j: each slot's w_j summed over the rows and
+ *            the query heads of its KV head is added to it
+ *   max_len  <= slots: no len(c) is above it (0: slots); the launch is sized
+ *            by it, so a tight one is faster, and a captured graph wants the
+ *            largest its replays use
+ *   d_workspace  pkv_attend_workspace(op) bytes, 256-byte aligned, used until
+ *            the call's work on `stream` is done; calls that may run at the
+ *            same time need one each (a captured graph holds on to its own)
+ * Logits, softmax and sums are held in 32 bits.  Asynchronous on `stream`; the
+ * call can be captured. */
+typedef struct pkv_attend_op {
+    pkv_kv_view cache;
+    const void* d_q;
+    void* d_out;
+    uint64_t q_copy_stride, q_row_stride, q_head_stride;
+    uint64_t out_copy_stride, out_row_stride, out_head_stride;
+    const int32_t* d_lens;
+    const int32_t* d_q_lens;
+    float* d_lse;
+    float* d_weights;
+    uint64_t weight_copy_stride, weight_head_stride;
+    void* d_workspace;
+    uint64_t workspace_bytes;
+    float scale;              /* > 0, finite */
+    int32_t dtype;            /* of q and out */
+    uint32_t q_heads, nq, max_len, window, sinks;
+    uint32_t reserved;        /* 0 */
+} pkv_attend_op;
+/* Workspace bytes of a call with these shapes (pointers and strides are not
+ * looked at); 0 for shapes pkv_attend refuses. */
+uint64_t pkv_attend_workspace(const pkv_attend_op* op);
+int pkv_attend(pkv_ctx* ctx, const pkv_attend_op* op, void* stream);
+
+/* Rows into and out of a PKV_FP4 cache.  Element (c, l, h, i, 0) of keys and
+ * values at c * copy_stride + l * layer_stride + h * head_stride + i *
+ * row_stride of a dtype tensor (16-byte aligned, strides a multiple of 16
+ * bytes); row i of copy c belongs to slot d_first[c] + i, for i < count(c)
+ * (d_counts: int32 device words taken into 0 .. rows, or NULL: all rows).
+ * A row whose slot lies outside 0 .. slots - 1, or behind count(c), is not
+ * stored, and loaded as 0.  d_keys or d_values may be NULL (that side is left
+ * alone).
+ *   store: each block of 32 takes the smallest scale 2^e with max |x| <= 7 *
+ *     2^e, e in -125 .. 125 (so that no value is off by more than half the
+ *     format's widest step, 4 to 6), each value the nearest code, half way to
+ *     the even one; a block that holds an infinity or NaN becomes NaN.  Two
+ *     rows must not name the same slot of a (copy, layer, head).
+ *   load: the values the codes stand for (exact in f32 and bf16; f16 rounds
+ *     to nearest even). */
+typedef struct pkv_rows_op {
+    pkv_kv_view cache;
+    void* d_keys;             /* read by a store, written by a load */
+    void* d_values;
+    uint64_t copy_stride, layer_stride, head_stride, row_stride;
+    const int32_t* d_first;
+    const int32_t* d_counts;
+    int32_t dtype;
+    uint32_t rows;
+} pkv_rows_op;
+int pkv_fp4_store(pkv_ctx* ctx, const pkv_rows_op* op, void* stream);
+int pkv_fp4_load(pkv_ctx* ctx, const pkv_rows_op* op, void* stream);
+
+/* Shorten every (copy, layer, head) of a cache to at most `budget` slots.
+ * With n = len(c) (taken into 0 .. slots): n <= budget keeps every slot; else
+ * the first `sinks`, the last `recent` and, of the others, the budget - sinks
+ * - recent with the largest weight are kept (equal weights: the lower slot; a
+ * NaN counts as -inf).  Kept rows go to slots 0, 1, .. of `into` in their
+ * order: of the same memory and strides as `cache` (in place), or of memory
+ * that does not overlap it.  Slots of `into` behind them keep what they held.
+ *   d_kept        int32 [copies][layers][heads][budget]: kept slots ascending,
+ *                 then -1
+ *   d_new_lens    int32 [copies]: min(n, budget); not d_lens
+ *   d_weights     f32 (c, l, h, j) at c * weight_strides[0] + l *
+ *                 weight_strides[1] + h * weight_strides[2] + j
+ *   d_weights_out the same with out_strides, into.slots per head: the kept
+ *                 slots' weights, then 0 up to into.slots; may be d_weights
+ *                 with its strides (in place)
+ * sinks + recent <= budget, budget >= 1, into.slots >= min(budget, slots).
+ * Asynchronous on `stream`; the call can be captured. */
+typedef struct pkv_evict_op {
+    pkv_kv_view cache;
+    pkv_kv_view into;
+    const int32_t* d_lens;
+    int32_t* d_new_lens;
+    int32_t* d_kept;
+    const float* d_weights;
+    float* d_weights_out;
+    uint64_t weight_strides[3], out_strides[3];
+    uint32_t budget, sinks, recent;
+    uint32_t reserved;        /* 0 */
+} pkv_evict_op;
+int pkv_evict(pkv_ctx* ctx, const pkv_evict_op* op, void* stream);
 
 /* ---------------------------------------------------------------- diagnostics
  * Validation hook, no counterpart in the reference: the encode kernels take

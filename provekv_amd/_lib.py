@@ -38,6 +38,7 @@ RADII_LOG_U8 = 1
 DT_F32 = 0
 DT_BF16 = 1
 DT_F16 = 2
+DT_FP4 = 3
 
 # every symbol include/pkv_codec.h declares
 EXPORTS = (
@@ -56,6 +57,7 @@ EXPORTS = (
     "pkv_blake3_tier_digests", "pkv_blake3_build_digests", "pkv_blake3",
     "pkv_host_angle_bins", "pkv_host_octant_bins", "pkv_host_logf", "pkv_host_expf", "pkv_host_expf_fused",
     "pkv_host_div255", "pkv_host_f32_stable_rel50", "pkv_code_from_json", "pkv_fib_digests", "pkv_host_blake3",
+    "pkv_attend_workspace", "pkv_attend", "pkv_fp4_store", "pkv_fp4_load", "pkv_evict",
 )
 
 
@@ -76,6 +78,42 @@ class DigestTier(C.Structure):
     _fields_ = [("d_buf", C.c_void_p), ("buf_bytes", C.c_uint64), ("ranges", C.c_void_p),
                 ("d_blob_digests", C.c_void_p), ("d_layer_digests", C.c_void_p), ("n", C.c_uint32),
                 ("reserved", C.c_uint32)]
+
+
+class KvView(C.Structure):
+    """pkv_kv_view"""
+    _fields_ = [("d_keys", C.c_void_p), ("d_values", C.c_void_p), ("d_key_scales", C.c_void_p),
+                ("d_value_scales", C.c_void_p), ("copy_stride", C.c_uint64), ("layer_stride", C.c_uint64),
+                ("head_stride", C.c_uint64), ("slot_stride", C.c_uint64), ("elems", C.c_uint64),
+                ("copies", C.c_uint32), ("layers", C.c_uint32), ("heads", C.c_uint32), ("slots", C.c_uint32),
+                ("dim", C.c_uint32), ("dtype", C.c_int32)]
+
+
+class AttendOp(C.Structure):
+    """pkv_attend_op"""
+    _fields_ = [("cache", KvView), ("d_q", C.c_void_p), ("d_out", C.c_void_p), ("q_copy_stride", C.c_uint64),
+                ("q_row_stride", C.c_uint64), ("q_head_stride", C.c_uint64), ("out_copy_stride", C.c_uint64),
+                ("out_row_stride", C.c_uint64), ("out_head_stride", C.c_uint64), ("d_lens", C.c_void_p),
+                ("d_q_lens", C.c_void_p), ("d_lse", C.c_void_p), ("d_weights", C.c_void_p),
+                ("weight_copy_stride", C.c_uint64), ("weight_head_stride", C.c_uint64), ("d_workspace", C.c_void_p),
+                ("workspace_bytes", C.c_uint64), ("scale", C.c_float), ("dtype", C.c_int32),
+                ("q_heads", C.c_uint32), ("nq", C.c_uint32), ("max_len", C.c_uint32), ("window", C.c_uint32),
+                ("sinks", C.c_uint32), ("reserved", C.c_uint32)]
+
+
+class RowsOp(C.Structure):
+    """pkv_rows_op"""
+    _fields_ = [("cache", KvView), ("d_keys", C.c_void_p), ("d_values", C.c_void_p), ("copy_stride", C.c_uint64),
+                ("layer_stride", C.c_uint64), ("head_stride", C.c_uint64), ("row_stride", C.c_uint64),
+                ("d_first", C.c_void_p), ("d_counts", C.c_void_p), ("dtype", C.c_int32), ("rows", C.c_uint32)]
+
+
+class EvictOp(C.Structure):
+    """pkv_evict_op"""
+    _fields_ = [("cache", KvView), ("into", KvView), ("d_lens", C.c_void_p), ("d_new_lens", C.c_void_p),
+                ("d_kept", C.c_void_p), ("d_weights", C.c_void_p), ("d_weights_out", C.c_void_p),
+                ("weight_strides", C.c_uint64 * 3), ("out_strides", C.c_uint64 * 3), ("budget", C.c_uint32),
+                ("sinks", C.c_uint32), ("recent", C.c_uint32), ("reserved", C.c_uint32)]
 
 
 class Seg(C.Structure):
@@ -209,6 +247,11 @@ def _declare(L):
         "pkv_code_from_json": ([P, P, U64, P, U64, P, P], I32),
         "pkv_fib_digests": ([P, P, P, P], I32),
         "pkv_host_blake3": ([P, U64, P], None),
+        "pkv_attend_workspace": ([P], U64),
+        "pkv_attend": ([P, P, P], I32),
+        "pkv_fp4_store": ([P, P, P], I32),
+        "pkv_fp4_load": ([P, P, P], I32),
+        "pkv_evict": ([P, P, P], I32),
     }
     for name, (args, res) in sig.items():
         fn = getattr(L, name)

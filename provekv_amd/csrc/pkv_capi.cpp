@@ -116,6 +116,8 @@ struct pkv_ctx {
     NoallocScratch* noalloc = nullptr;  // this device's `scratch` (pkv_decode_segments_noalloc)
 };
 
+int pkv::ctx_device(const pkv_ctx* ctx) { return ctx->device; }
+
 struct pkv_profile {
     pkv_ctx* ctx = nullptr;
     int kind = 0;

@@ -8,6 +8,8 @@
 
 namespace pkv {
 
+int ctx_device(const pkv_ctx* ctx);   // pkv_capi.cpp
+
 // Status-word kinds (low 4 bits of a per-segment status word; the vector
 // index sits above them).
 enum Kind : uint32_t {

@@ -215,6 +215,19 @@ def default_context() -> Context:
         return _default_ctx
 
 
+_device_ctx: dict = {}
+
+
+def device_context(device: int) -> Context:
+    """The process's context of one device (the default context for device 0)."""
+    if device == 0:
+        return default_context()
+    with _default_lock:
+        if device not in _device_ctx:
+            _device_ctx[device] = Context(device)
+        return _device_ctx[device]
+
+
 class Profile:
     """pkv_profile: constants resident on the device."""
 

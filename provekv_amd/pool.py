@@ -22,6 +22,7 @@ import numpy as np
 
 from . import _lib as L
 from .device import SEG_DTYPE
+from .live import FourBitKVCache, LiveCache  # noqa: F401
 
 
 def read_fb2_n_blocks(payload: bytes):
@@ -69,12 +70,13 @@ def _tier(owners, layers: int, heads: int, dim: int, corpus_tokens: int, hdr: in
     return TierLayout(np.array(enc, dtype=SEG_DTYPE), np.array(dec, dtype=SEG_DTYPE), wire, out, blobs)
 
 
-class DeviceKVCache:
+class DeviceKVCache(LiveCache):
     """A KV cache in HuggingFace ``DynamicCache`` layout on the GPU: per layer
     one K and one V tensor [1, H, T, D] (float32, bfloat16 or float16), all in
     one allocation [copies][layers][K|V][H][T][D].  ``copies`` independent
     caches (one per agent served on this GPU) share the allocation so that one
-    decode can fan out to all of them.
+    decode can fan out to all of them.  ``attend`` and ``evict`` (LiveCache)
+    read and shorten it.
 
     Implements proveKV's ``CacheTarget`` (proveKV/src/pool.rs:646-658):
     ``num_layers``, ``append_key``, ``append_value``, ``seq_len``; a key or
@@ -88,6 +90,30 @@ class DeviceKVCache:
         self.layers, self.heads, self.tokens, self.dim, self.copies = layers, heads, tokens, dim, copies
         self.buf = torch.zeros((copies, layers, 2, heads, tokens, dim), dtype=dtype or torch.float32, device=device)
         self._seq_len = 0
+
+    @classmethod
+    def over(cls, buf) -> "DeviceKVCache":
+        """A cache over a caller's tensor [copies, layers, 2, heads, tokens, dim]
+        (contiguous; kept, not copied)."""
+        if buf.dim() != 6 or buf.shape[2] != 2 or not buf.is_contiguous():
+            raise ValueError("buf must be a contiguous [copies, layers, 2, heads, tokens, dim] tensor")
+        self = cls.__new__(cls)
+        self.copies, self.layers, _, self.heads, self.tokens, self.dim = buf.shape
+        self.buf = buf
+        self._seq_len = 0
+        return self
+
+    def _pointers(self):
+        import torch
+        dts = {torch.float32: L.DT_F32, torch.bfloat16: L.DT_BF16, torch.float16: L.DT_F16}
+        if self.buf.dtype not in dts:
+            raise TypeError("a cache is float32, bfloat16 or float16")
+        p, side = self.buf.data_ptr(), self.heads * self.tokens * self.dim
+        return dts[self.buf.dtype], self.buf.element_size(), p, p + side * self.buf.element_size(), 0, 0
+
+    @property
+    def device(self):
+        return self.buf.device
 
     # ---- layout
     @property
