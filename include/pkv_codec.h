@@ -507,6 +507,7 @@ int pkv_turbo_score_batch(pkv_ctx* ctx, const pkv_profile* prof, const uint8_t* 
  * h) starts at element c * copy_stride + l * layer_stride + h * head_stride +
  * j * slot_stride of d_keys and of d_values; elems bounds every such row's end
  * (checked), so it is the element count behind each of the two pointers.
+ * slot_stride is at most 2^22.
  *   PKV_F32, PKV_BF16, PKV_F16: pointers 16-byte aligned, strides a multiple
  *     of 16 bytes; scale pointers NULL.
  *   PKV_FP4: OCP MX FP4.  Two 4-bit codes a byte (even element low) of the
@@ -572,8 +573,8 @@ typedef struct pkv_attend_op {
     uint32_t q_heads, nq, max_len, window, sinks;
     uint32_t reserved;        /* 0 */
 } pkv_attend_op;
-/* Workspace bytes of a call with these shapes (pointers and strides are not
- * looked at); 0 for shapes pkv_attend refuses. */
+/* Workspace bytes of a call with these shapes (of the pointers only whether
+ * d_weights is NULL counts); 0 for shapes pkv_attend refuses. */
 uint64_t pkv_attend_workspace(const pkv_attend_op* op);
 int pkv_attend(pkv_ctx* ctx, const pkv_attend_op* op, void* stream);
 

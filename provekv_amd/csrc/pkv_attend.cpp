@@ -67,6 +67,9 @@ bool overlap(const void* a, uint64_t an, const void* b, uint64_t bn) {
 }
 
 constexpr uint32_t kMaxCount = 0x7fffffffu;
+// Elements from a slot to the next: a kernel's tile of 64 slots stays within
+// 32-bit offsets of its first.
+constexpr uint64_t kMaxSlotStride = 1u << 22;
 
 int check_view(const pkv_kv_view& v, bool written) {
     if (v.dim != 64 && v.dim != 128) return PKV_ERR_UNSUPPORTED;
@@ -83,6 +86,7 @@ int check_view(const pkv_kv_view& v, bool written) {
     } else if (v.d_key_scales || v.d_value_scales) {
         return PKV_ERR_INVALID_ARG;
     }
+    if (v.slot_stride > kMaxSlotStride) return PKV_ERR_INVALID_ARG;
     if (v.copy_stride % unit || v.layer_stride % unit || v.head_stride % unit || v.slot_stride % unit)
         return PKV_ERR_INVALID_ARG;
     const Axis a[4] = {{v.copy_stride, v.copies}, {v.layer_stride, v.layers}, {v.head_stride, v.heads},

@@ -152,6 +152,438 @@ __global__ __launch_bounds__(256) void weights_kernel(AttendDev a) {
     a.weights[c * a.w_copy + h * a.w_head + j] += sum;
 }
 
+// ------------------------------------------------------------ few rows: split over the slots
+typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
+typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
+typedef float f32x4 __attribute__((ext_vector_type(4)));
+typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
+typedef _Float16 f16x2 __attribute__((ext_vector_type(2)));
+typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
+
+// Type of the matrix products over a cache: its own, bf16 for 4-bit codes
+// (every code times its scale is exact in bf16).
+constexpr int mat_type(int ct) { return ct == PKV_FP4 ? PKV_BF16 : ct; }
+// A query of QT over 4-bit codes is the sum of this many bf16 terms (exact: 8
+// bits each), any other query is its own single term.
+constexpr int query_terms(int ct, int qt) { return ct != PKV_FP4 ? 1 : qt == PKV_F32 ? 3 : qt == PKV_F16 ? 2 : 1; }
+
+template <int MT>
+__device__ inline f32x4 mma16(u32x4 a, u32x4 b, f32x4 c) {
+    if constexpr (MT == PKV_BF16)
+        return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), c,
+                                                       0, 0, 0);
+    else
+        return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(f16x8, a), __builtin_bit_cast(f16x8, b), c, 0,
+                                                      0, 0);
+}
+
+// (a, b) rounded to the matrix type, and what the rounding left of each.
+template <int MT>
+__device__ inline uint32_t pack_term(float& a, float& b) {
+    if constexpr (MT == PKV_BF16) {
+        const bf16x2 h = {static_cast<__bf16>(a), static_cast<__bf16>(b)};
+        a -= static_cast<float>(h[0]);
+        b -= static_cast<float>(h[1]);
+        return __builtin_bit_cast(uint32_t, h);
+    } else {
+        const f16x2 h = {static_cast<_Float16>(a), static_cast<_Float16>(b)};
+        a -= static_cast<float>(h[0]);
+        b -= static_cast<float>(h[1]);
+        return __builtin_bit_cast(uint32_t, h);
+    }
+}
+
+// Two 16-bit values that hold an infinity or NaN.
+template <int MT>
+__device__ inline bool nonfinite2(uint32_t x) {
+    constexpr uint32_t e = MT == PKV_BF16 ? 0x7f80u : 0x7c00u;
+    return (x & e) == e || (x >> 16 & e) == e;
+}
+
+// The slots that the rows of a tile see, as tiles of `step` slots: [0, first)
+// with the always-visible slots, then [second, second + count - first).
+struct Tiles {
+    int first, second, count;
+    int low, high;          // rows see slots < a.sinks (with a window) and low .. high - 1
+    __device__ int slot(int t, int step) const { return (t < first ? t : second + t - first) * step; }
+};
+__device__ inline Tiles tiles_of(const AttendDev& a, int pos0, int pos1, int step) {
+    Tiles t;
+    t.high = max(pos1 + 1, 0);
+    t.low = a.window ? static_cast<int>(max(static_cast<int64_t>(pos0) - a.window + 1, static_cast<int64_t>(0))) : 0;
+    const int sink = static_cast<int>(min(static_cast<uint32_t>(min(t.low, t.high)), a.sinks));
+    t.first = (sink + step - 1) / step;
+    t.second = max(t.first, t.low / step);
+    t.count = t.first + max((t.high + step - 1) / step - t.second, 0);
+    return t;
+}
+// Every row between pos0 and pos1 sees all of lo .. hi.
+__device__ inline bool all_visible(const AttendDev& a, int pos0, int pos1, int lo, int hi) {
+    return hi <= pos0 && (!a.window || static_cast<uint32_t>(pos1 - lo) < a.window || static_cast<uint32_t>(hi) < a.sinks);
+}
+// Some row of the tile list's rows sees slot j.
+__device__ inline bool any_visible(const AttendDev& a, const Tiles& t, int j) {
+    return j < t.high && (j >= t.low || static_cast<uint32_t>(j) < a.sinks);
+}
+
+// Up to 16 query rows (rows x group of one KV head) against a share of the
+// slots, the whole product on the matrix cores with nothing staged in LDS:
+//   S^T = K Q^T   A = 16 slots (lane % 16) x 8 channels a lane group (lane /
+//                 16); B = 16 rows (lane % 16).  Any order of the channels will
+//                 do as long as q has the same, so a lane reads 16 bytes of a
+//                 row.  Result: row lane % 16, slots 4 (lane / 16) + r.
+//   O^T = V^T P^T A wants, for one channel a lane, the slots its lane group
+//                 has in S^T: the softmax's registers are B as they are.  Lane
+//                 i of a group reads channels 8i .. of its 4 (x 2) slots and
+//                 v_perm gathers each channel across them; channel order
+//                 along M is free again, so O^T tile e holds channels 8m + e.
+// Bound by the cache's bytes: 32 slots cost a wave 16 + 32 matrix
+// instructions at head_dim 128 against 16 KB of bf16, a sixth of the time HBM
+// needs for them.
+template <int CT, int D>
+struct SlotTile {
+    static constexpr int kSub = CT == PKV_F32 ? 1 : 2;        // 16-slot pieces
+    static constexpr int kStep = 16 * kSub;
+    static constexpr int kKRegs = CT == PKV_FP4 ? 1 : CT == PKV_F32 ? D / 16 : D / 32;   // 16-byte reads of a key
+    static constexpr int kVRegs = CT == PKV_F32 ? D / 64 : 1;
+    static constexpr int kPer = CT == PKV_F32 ? 4 : D / 16;   // channels of a value that a lane reads at once
+    u32x4 k[kSub][kKRegs];
+    u32x4 v[kSub][4][kVRegs];
+    uint32_t ks[kSub], vs[kSub][4];
+
+    __device__ static uint32_t bytes(uint32_t e) { return CT == PKV_FP4 ? e / 2 : CT == PKV_F32 ? e * 4 : e * 2; }
+
+    // kp, vp, ksp, vsp: slot 0 of the head.  Slots past `last` read the last one.
+    __device__ void load(const uint8_t* kp, const uint8_t* vp, const uint8_t* ksp, const uint8_t* vsp, uint64_t stride,
+                         int slot, int last, uint32_t lane) {
+        const uint32_t i = lane % 16, g = lane / 16;
+        const uint64_t base = static_cast<uint64_t>(slot) * stride;
+        const uint8_t* kt = kp + (CT == PKV_FP4 ? base / 2 : CT == PKV_F32 ? base * 4 : base * 2);
+        const uint8_t* vt = vp + (CT == PKV_FP4 ? base / 2 : CT == PKV_F32 ? base * 4 : base * 2);
+        const uint32_t st = static_cast<uint32_t>(stride);
+        const int room = last - slot;      // >= 0
+        for (int t = 0; t < kSub; ++t) {
+            const uint32_t e = static_cast<uint32_t>(min(16 * t + static_cast<int>(i), room)) * st;
+            const uint8_t* p = kt + bytes(e);
+            if constexpr (CT == PKV_FP4) {
+                if constexpr (D == 128) k[t][0] = *reinterpret_cast<const u32x4*>(p + 16 * g);
+                else {
+                    const u32x2 x = *reinterpret_cast<const u32x2*>(p + 8 * g);
+                    k[t][0] = u32x4{x[0], x[1], 0, 0};
+                }
+                ks[t] = (ksp + base / 32)[e / 32 + (D == 128 ? g : g / 2)];
+            } else {
+                for (int s = 0; s < kKRegs; ++s) k[t][s] = *reinterpret_cast<const u32x4*>(p + 64 * s + 16 * g);
+            }
+        }
+        for (int t = 0; t < kSub; ++t)
+            for (int j = 0; j < 4; ++j) {
+                const uint32_t e = static_cast<uint32_t>(min(16 * t + 4 * static_cast<int>(g) + j, room)) * st;
+                const uint8_t* p = vt + bytes(e);
+                if constexpr (CT == PKV_FP4) {
+                    if constexpr (D == 128) v[t][j][0][0] = *reinterpret_cast<const uint32_t*>(p + 4 * i);
+                    else v[t][j][0][0] = *reinterpret_cast<const uint16_t*>(p + 2 * i);
+                    vs[t][j] = (vsp + base / 32)[e / 32 + (D == 128 ? i / 4 : i / 8)];
+                } else if constexpr (CT == PKV_F32) {
+                    for (int q = 0; q < kVRegs; ++q)
+                        v[t][j][q] = *reinterpret_cast<const u32x4*>(p + 256 * q + 16 * i);
+                } else if constexpr (D == 128) {
+                    v[t][j][0] = *reinterpret_cast<const u32x4*>(p + 16 * i);
+                } else {
+                    const u32x2 x = *reinterpret_cast<const u32x2*>(p + 8 * i);
+                    v[t][j][0] = u32x4{x[0], x[1], 0, 0};
+                }
+            }
+    }
+    // 4-bit codes to bf16: eight channels of dword `w` under scale byte b.
+    __device__ static u32x4 expand(uint32_t w, uint32_t b) {
+        const float s = block_scale(b);
+        return u32x4{__builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(w, s, 0)),
+                     __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(w, s, 1)),
+                     __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(w, s, 2)),
+                     __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(w, s, 3))};
+    }
+    __device__ void expand_values() {
+        if constexpr (CT == PKV_FP4)
+            for (int t = 0; t < kSub; ++t)
+                for (int j = 0; j < 4; ++j) v[t][j][0] = expand(v[t][j][0][0], vs[t][j]);
+    }
+    // The channel that word `word` of step `s` of a lane's keys starts at (two channels a word, 16-bit types).
+    __device__ static uint32_t channel(int s, uint32_t g) {
+        return CT == PKV_FP4 ? (D / 4) * g + 8 * s : CT == PKV_F32 ? 16 * s + 4 * g : 32 * s + 8 * g;
+    }
+};
+
+struct Partial {
+    float* o;        // [copy][kv head][split][16 rows][D]
+    float* ml;       // [copy][kv head][split][16 rows][2]: largest logit (unscaled), sum
+    float* logits;   // [copy][kv head][rows x group][ld], unscaled
+    uint32_t splits, ld;
+};
+
+template <int CT, int QT, int D, bool LOGITS>
+__global__ __launch_bounds__(256, 2) void decode_kernel(AttendDev a, Partial part) {
+    using T = typename Elem<QT>::T;
+    using Tile = SlotTile<CT, D>;
+    constexpr int MT = mat_type(CT), NQ = query_terms(CT, QT), NP = QT == PKV_F32 ? 3 : 2, kSub = Tile::kSub;
+    constexpr int kQ = CT == PKV_F32 ? D / 16 : D / 32;          // query registers (16 bytes) per term
+    constexpr int kO = D / 16;                                   // 16-channel tiles of the output
+    const uint32_t lane = threadIdx.x % 64, wave = __builtin_amdgcn_readfirstlane(threadIdx.x / 64);
+    const uint32_t split = blockIdx.x % part.splits, ch = blockIdx.x / part.splits, c = ch / a.heads, h = ch % a.heads;
+    const uint32_t row = lane % 16, g = lane / 16;
+    const Span sp = span(a, c);
+    const int R = sp.rows * static_cast<int>(a.group);
+    const int pos1 = sp.first + sp.rows - 1;
+    const bool real = static_cast<int>(row) < R;
+    const int qi = row / a.group, pos = real ? sp.first + qi : -1;
+    const Tiles tl = tiles_of(a, sp.first, sp.rows ? pos1 : -1, Tile::kStep);
+    const int per = (tl.count + part.splits - 1) / part.splits;
+    const int t0 = split * per, t1 = min(t0 + per, tl.count);
+
+    const T* qp = reinterpret_cast<const T*>(a.q) + c * a.q_copy + (real ? qi : 0) * a.q_row +
+                  (h * a.group + (real ? row % a.group : 0)) * a.q_head;
+    u32x4 q[NQ][kQ];
+    for (int s = 0; s < kQ; ++s) {
+        const uint32_t d = Tile::channel(s, g);
+        if constexpr (CT == PKV_F32) {
+            q[0][s] = real ? *reinterpret_cast<const u32x4*>(qp + d) : u32x4{};
+        } else if constexpr (NQ == 1) {
+            q[0][s] = real ? *reinterpret_cast<const u32x4*>(qp + d) : u32x4{};
+        } else {
+            for (int w = 0; w < 4; ++w) {
+                float x = real ? static_cast<float>(qp[d + 2 * w]) : 0.0f;
+                float y = real ? static_cast<float>(qp[d + 2 * w + 1]) : 0.0f;
+                for (int n = 0; n < NQ; ++n) q[n][s][w] = pack_term<PKV_BF16>(x, y);
+            }
+        }
+    }
+
+    const uint64_t base = c * a.kv.copy + h * a.kv.head;
+    const uint64_t byte = CT == PKV_FP4 ? base / 2 : CT == PKV_F32 ? base * 4 : base * 2;
+    const uint8_t *kp = a.kv.k + byte, *vp = a.kv.v + byte;
+    const uint8_t *ksp = CT == PKV_FP4 ? a.kv.ks + base / 32 : nullptr;
+    const uint8_t *vsp = CT == PKV_FP4 ? a.kv.vs + base / 32 : nullptr;
+
+    float m = -kInf, l = 0.0f;
+    f32x4 o[kO] = {};
+    for (int t = t0 + static_cast<int>(wave); t < t1; t += 4) {
+        const int slot = tl.slot(t, Tile::kStep);
+        Tile x;
+        x.load(kp, vp, ksp, vsp, a.kv.slot, slot, tl.high - 1, lane);
+        // logits
+        f32x4 sc[kSub] = {};
+        for (int u = 0; u < kSub; ++u)
+            for (int s = 0; s < kQ; ++s) {
+                if constexpr (CT == PKV_F32) {
+                    for (int e = 0; e < 4; ++e)
+                        sc[u] = __builtin_amdgcn_mfma_f32_16x16x4f32(__uint_as_float(x.k[u][s][e]),
+                                                                     __uint_as_float(q[0][s][e]), sc[u], 0, 0, 0);
+                } else {
+                    const u32x4 ka = CT == PKV_FP4 ? Tile::expand(x.k[u][0][s], x.ks[u]) : x.k[u][s];
+                    for (int n = NQ - 1; n >= 0; --n) sc[u] = mma16<MT>(ka, q[n][s], sc[u]);
+                }
+            }
+        const bool full = all_visible(a, sp.first, pos1, slot, slot + Tile::kStep - 1);
+        if (LOGITS && real)
+            for (int u = 0; u < kSub; ++u)
+                *reinterpret_cast<f32x4*>(part.logits + (static_cast<uint64_t>(ch) * a.nq * a.group + row) * part.ld +
+                                          slot + 16 * u + 4 * g) = sc[u];
+        x.expand_values();
+        bool odd = false;   // a value that must not meet the weight 0 of a row that does not see it
+        if (!full) {
+            for (int u = 0; u < kSub; ++u)
+                for (int j = 0; j < 4; ++j) {
+                    const int key = slot + 16 * u + 4 * static_cast<int>(g) + j;
+                    if (!visible(a, pos, key)) sc[u][j] = -kInf;
+                    const bool any = any_visible(a, tl, key);
+                    for (int n = 0; n < Tile::kVRegs; ++n)
+                        for (int w = 0; w < 4; ++w) {
+                            if (!any) x.v[u][j][n][w] = 0;
+                            if constexpr (CT == PKV_F32) odd |= (x.v[u][j][n][w] & 0x7f800000u) == 0x7f800000u;
+                            else if (w < kO / 2) odd |= nonfinite2<MT>(x.v[u][j][n][w]);
+                        }
+                }
+        }
+        // running maximum; rescaled only when it grows by more than 2^8 (weights
+        // stay below 2^8 times the largest, exact all the same)
+        float top = fmaxf(fmaxf(sc[0][0], sc[0][1]), fmaxf(sc[0][2], sc[0][3]));
+        for (int u = 1; u < kSub; ++u)
+            top = fmaxf(top, fmaxf(fmaxf(sc[u][0], sc[u][1]), fmaxf(sc[u][2], sc[u][3])));
+        top = fmaxf(top, __shfl_xor(top, 16));
+        top = fmaxf(top, __shfl_xor(top, 32));
+        const bool grow = m == -kInf ? top > -kInf : (top - m) * a.scale2 > 8.0f;
+        if (__any(grow)) {
+            const float mn = fmaxf(m, top);
+            const float f = m == -kInf ? 1.0f : exp2f((m - mn) * a.scale2);
+            if (mn > m) {
+                l *= f;
+                for (int e = 0; e < kO; ++e) o[e] *= f;
+                m = mn;
+            }
+        }
+        const float mc = m == -kInf ? 0.0f : m * a.scale2;
+        float p[kSub][4];
+        for (int u = 0; u < kSub; ++u)
+            for (int j = 0; j < 4; ++j) {
+                p[u][j] = __builtin_amdgcn_exp2f(__builtin_fmaf(sc[u][j], a.scale2, -mc));
+                l += p[u][j];
+            }
+        // weighted values
+        auto gather = [&](f32x4 (&acc)[kO], const Tile& y) {
+            if constexpr (CT == PKV_F32) {
+                for (int j = 0; j < 4; ++j)
+                    for (int n = 0; n < Tile::kVRegs; ++n)
+                        for (int e = 0; e < 4; ++e)
+                            acc[4 * n + e] = __builtin_amdgcn_mfma_f32_16x16x4f32(__uint_as_float(y.v[0][j][n][e]),
+                                                                                  p[0][j], acc[4 * n + e], 0, 0, 0);
+            } else {
+                float r[kSub][4];
+                for (int u = 0; u < kSub; ++u)
+                    for (int j = 0; j < 4; ++j) r[u][j] = p[u][j];
+                u32x4 pt[NP];
+                for (int n = 0; n < NP; ++n)
+                    pt[n] = u32x4{pack_term<MT>(r[0][0], r[0][1]), pack_term<MT>(r[0][2], r[0][3]),
+                                  pack_term<MT>(r[1][0], r[1][1]), pack_term<MT>(r[1][2], r[1][3])};
+                for (int e = 0; e < kO; ++e) {
+                    const uint32_t sel = e % 2 ? 0x07060302u : 0x05040100u;
+                    const u32x4 va = {__builtin_amdgcn_perm(y.v[0][1][0][e / 2], y.v[0][0][0][e / 2], sel),
+                                      __builtin_amdgcn_perm(y.v[0][3][0][e / 2], y.v[0][2][0][e / 2], sel),
+                                      __builtin_amdgcn_perm(y.v[1][1][0][e / 2], y.v[1][0][0][e / 2], sel),
+                                      __builtin_amdgcn_perm(y.v[1][3][0][e / 2], y.v[1][2][0][e / 2], sel)};
+                    for (int n = NP - 1; n >= 0; --n) acc[e] = mma16<MT>(va, pt[n], acc[e]);
+                }
+            }
+        };
+        if (__builtin_expect(__any(odd) && sp.rows > 1, 0)) {
+            // an infinity or NaN in a slot that only some rows see: each query
+            // row by itself, with the slots it does not see cleared
+            for (int i = 0; i < sp.rows; ++i) {
+                Tile y = x;
+                for (int u = 0; u < kSub; ++u)
+                    for (int j = 0; j < 4; ++j)
+                        if (!visible(a, sp.first + i, slot + 16 * u + 4 * static_cast<int>(g) + j))
+                            for (int n = 0; n < Tile::kVRegs; ++n) y.v[u][j][n] = u32x4{};
+                f32x4 acc[kO];
+                for (int e = 0; e < kO; ++e) acc[e] = o[e];
+                gather(acc, y);
+                if (qi == i)
+                    for (int e = 0; e < kO; ++e) o[e] = acc[e];
+            }
+        } else {
+            gather(o, x);
+        }
+    }
+    l += __shfl_xor(l, 16);
+    l += __shfl_xor(l, 32);
+
+    // the four waves' shares joined; channel of o[e][r]: see SlotTile
+    __shared__ float so[4][16][D + 4], sm[4][16], sl[4][16];
+    for (int r = 0; r < 4; ++r)
+        for (int e = 0; e < kO; ++e) {
+            const int w = 4 * g + r;
+            const int d = CT == PKV_F32 ? 64 * (e / 4) + 4 * w + e % 4 : kO * w + e;
+            so[wave][row][d] = o[e][r];
+        }
+    if (g == 0) { sm[wave][row] = m; sl[wave][row] = l; }
+    __syncthreads();
+    for (uint32_t x = threadIdx.x; x < static_cast<uint32_t>(R) * (D / 4); x += 256) {
+        const uint32_t r = x / (D / 4), d = x % (D / 4) * 4;
+        const float top = fmaxf(fmaxf(sm[0][r], sm[1][r]), fmaxf(sm[2][r], sm[3][r])), mu = top == -kInf ? 0.0f : top;
+        float sum = 0.0f;
+        f32x4 acc = {};
+        for (int w = 0; w < 4; ++w) {
+            const float f = sm[w][r] == -kInf ? 0.0f : sm[w][r] == mu ? 1.0f : exp2f((sm[w][r] - mu) * a.scale2);
+            sum += sl[w][r] * f;
+            if (f != 0.0f) acc += *reinterpret_cast<const f32x4*>(&so[w][r][d]) * f;
+        }
+        const uint64_t at = (static_cast<uint64_t>(ch) * part.splits + split) * 16 + r;
+        *reinterpret_cast<f32x4*>(part.o + at * D + d) = acc;
+        if (d == 0) {
+            part.ml[2 * at] = top;
+            part.ml[2 * at + 1] = sum;
+        }
+    }
+}
+
+// The splits of a row joined: largest logit and the sum under it.
+__device__ inline void join_splits(const float* ml, uint32_t splits, float scale2, uint32_t lane, float* mu, float* sum) {
+    float top = -kInf;
+    for (uint32_t s = lane; s < splits; s += 64) top = fmaxf(top, ml[32 * s]);
+    for (int x = 32; x; x >>= 1) top = fmaxf(top, __shfl_xor(top, x));
+    float l = 0.0f;
+    for (uint32_t s = lane; s < splits; s += 64) {
+        // a share without a largest logit holds the sum 0, or NaN from NaN logits
+        const float ms = ml[32 * s];
+        l += ml[32 * s + 1] * (ms == top || ms == -kInf ? 1.0f : exp2f((ms - top) * scale2));
+    }
+    *sum = wave_sum(l);
+    *mu = top == -kInf ? 0.0f : top;
+}
+
+// The splits' shares joined, a wave a row; then, with weights, a wave's rows
+// of softmax statistics against the stored logits, four slots a thread.
+// blockIdx.x < outs: 4 rows of all copies x heads x rows; else 1,024 slots.
+template <int QT, int D>
+__global__ __launch_bounds__(256) void join_kernel(AttendDev a, Partial part, uint32_t outs) {
+    using T = typename Elem<QT>::T;
+    const uint32_t lane = threadIdx.x % 64, wave = threadIdx.x / 64, all = a.nq * a.group;
+    if (blockIdx.x < outs) {
+        const uint32_t x = blockIdx.x * 4 + wave;
+        if (x >= a.copies * a.heads * all) return;
+        const uint32_t r = x % all, ch = x / all, c = ch / a.heads, h = ch % a.heads, i = r / a.group, g = r % a.group;
+        if (static_cast<int>(i) >= span(a, c).rows) return;
+        const uint64_t at = static_cast<uint64_t>(ch) * part.splits * 16 + r;
+        float mu, sum;
+        join_splits(part.ml + 2 * at, part.splits, a.scale2, lane, &mu, &sum);
+        float o[D / 64] = {};
+        for (uint32_t s = 0; s < part.splits; ++s) {
+            const float ms = part.ml[2 * (at + 16 * s)];
+            const float f = ms == -kInf ? 0.0f : ms == mu ? 1.0f : exp2f((ms - mu) * a.scale2);
+            if (f == 0.0f) continue;
+            const float* p = part.o + (at + 16ull * s) * D + lane * (D / 64);
+            for (int e = 0; e < D / 64; ++e) o[e] += p[e] * f;
+        }
+        T* out = reinterpret_cast<T*>(a.out) + c * a.o_copy + i * a.o_row + (h * a.group + g) * a.o_head;
+        for (int e = 0; e < D / 64; ++e)
+            out[lane * (D / 64) + e] = static_cast<T>(sum == 0.0f ? 0.0f : o[e] / sum);
+        if (a.lse && lane == 0)
+            a.lse[(static_cast<uint64_t>(c) * a.heads * a.group + h * a.group + g) * a.nq + i] =
+                sum == 0.0f ? -kInf : (mu * a.scale2 + log2f(sum)) * kLn2;
+        return;
+    }
+    const uint32_t chunks = (a.max_len + 1023) / 1024;
+    const uint32_t x = blockIdx.x - outs, chunk = x % chunks, ch = x / chunks, c = ch / a.heads, h = ch % a.heads;
+    const Span sp = span(a, c);
+    const int j0 = chunk * 1024, rows = sp.rows * static_cast<int>(a.group);
+    const Tiles tl = tiles_of(a, sp.first, sp.rows ? sp.first + sp.rows - 1 : -1, 1);
+    if (j0 >= tl.high || (j0 + 1023 < tl.low && static_cast<uint32_t>(j0) >= a.sinks)) return;
+    __shared__ float st[16][2];
+    for (int r = wave; r < rows; r += 4) {
+        float mu, sum;
+        join_splits(part.ml + 2 * (static_cast<uint64_t>(ch) * part.splits * 16 + r), part.splits, a.scale2, lane, &mu,
+                    &sum);
+        if (lane == 0) {
+            st[r][0] = -mu * a.scale2;
+            st[r][1] = sum == 0.0f ? 0.0f : 1.0f / sum;
+        }
+    }
+    __syncthreads();
+    const int j = j0 + 4 * static_cast<int>(threadIdx.x);
+    if (j >= tl.high) return;
+    float w[4] = {};
+    for (int r = 0; r < rows; ++r) {
+        const int pos = sp.first + r / static_cast<int>(a.group);
+        // reads up to three logits that no tile wrote: unused
+        const f32x4 s = *reinterpret_cast<const f32x4*>(part.logits + (static_cast<uint64_t>(ch) * all + r) * part.ld + j);
+        for (int e = 0; e < 4; ++e)
+            if (visible(a, pos, j + e) && st[r][1] != 0.0f)
+                w[e] += __builtin_amdgcn_exp2f(__builtin_fmaf(s[e], a.scale2, st[r][0])) * st[r][1];
+    }
+    float* out = a.weights + c * a.w_copy + h * a.w_head + j;
+    for (int e = 0; e < 4; ++e)
+        if (any_visible(a, tl, j + e)) out[e] += w[e];
+}
+
 // ------------------------------------------------------------ the 4-bit cache
 struct Row {
     uint64_t src, dst;   // element offsets in the rows' tensor and in the cache
@@ -383,8 +815,46 @@ __global__ __launch_bounds__(256) void move_kernel(EvictDev a) {
     }
 }
 
+uint64_t round256(uint64_t x) { return (x + 255) & ~255ull; }
+
+constexpr uint32_t kDecodeRows = 16;   // rows x group that decode_kernel takes
+
+// How a call of few rows is cut: `splits` shares of the slots for each (copy,
+// head), so that the chip is full (768 workgroups, three a CU) while every wave
+// of a share has a tile.
+struct DecodePlan {
+    uint32_t splits, ld;
+    uint64_t ml, logits, bytes;   // offsets in the workspace (partial outputs first), all of it
+};
+DecodePlan decode_plan(const AttendDev& a, uint32_t dim, int cache_dtype) {
+    DecodePlan p;
+    const uint32_t step = cache_dtype == PKV_F32 ? 16 : 32, heads = a.copies * a.heads;
+    // slots that a call can see: all, or the window, the rows before the last and the sinks, each up to a tile more
+    uint64_t most = a.max_len;
+    if (a.window) most = std::min<uint64_t>(most, static_cast<uint64_t>(a.window) + a.nq + a.sinks + 2 * step);
+    const uint64_t tiles = (most + step - 1) / step;
+    p.splits = static_cast<uint32_t>(std::max<uint64_t>(1, std::min<uint64_t>((768 + heads - 1) / heads, tiles / 4)));
+    p.ld = (a.max_len + 31) / 32 * 32 + 4;
+    const uint64_t parts = static_cast<uint64_t>(heads) * p.splits * kDecodeRows;
+    p.ml = round256(parts * dim * 4);
+    p.logits = p.ml + round256(parts * 8);
+    p.bytes = p.logits + (a.weights ? round256(4ull * heads * a.nq * a.group * p.ld) : 0);
+    return p;
+}
+
 template <int CT, int QT, int D>
 int attend_typed(AttendDev a, uint8_t* ws, hipStream_t st) {
+    if (a.nq * a.group <= kDecodeRows) {
+        const DecodePlan p = decode_plan(a, D, CT);
+        const Partial part{reinterpret_cast<float*>(ws), reinterpret_cast<float*>(ws + p.ml),
+                           reinterpret_cast<float*>(ws + p.logits), p.splits, p.ld};
+        const uint32_t heads = a.copies * a.heads, outs = (heads * a.nq * a.group + 3) / 4;
+        if (a.weights) decode_kernel<CT, QT, D, true><<<heads * p.splits, 256, 0, st>>>(a, part);
+        else decode_kernel<CT, QT, D, false><<<heads * p.splits, 256, 0, st>>>(a, part);
+        const uint32_t chunks = a.weights ? (a.max_len + 1023) / 1024 * heads : 0;
+        join_kernel<QT, D><<<outs + chunks, 256, 0, st>>>(a, part, outs);
+        return hipGetLastError();
+    }
     a.stats = a.weights ? reinterpret_cast<float*>(ws) : nullptr;
     attend_kernel<CT, QT, D><<<dim3(a.nq * a.group, a.heads, a.copies), 256, 0, st>>>(a);
     if (a.weights)
@@ -399,7 +869,8 @@ int attend_dim(const AttendDev& a, uint32_t dim, uint8_t* ws, hipStream_t st) {
 
 }  // namespace
 
-uint64_t attend_workspace(const AttendDev& a, uint32_t, int, int) {
+uint64_t attend_workspace(const AttendDev& a, uint32_t dim, int cache_dtype, int) {
+    if (a.nq * a.group <= kDecodeRows) return decode_plan(a, dim, cache_dtype).bytes;
     return 8ull * a.copies * a.heads * a.nq * a.group;
 }
 
