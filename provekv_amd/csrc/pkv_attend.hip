@@ -5,6 +5,7 @@
 
 #include <algorithm>
 #include <cmath>
+#include <type_traits>
 
 #include "pkv_attend.h"
 
@@ -56,102 +57,6 @@ __device__ inline float wave_sum(float x) {
     return x;
 }
 
-// One workgroup per (row, head, copy), four waves over every fourth visible
-// slot, each with its own running maximum and sum.
-template <int CT, int QT, int D>
-__global__ __launch_bounds__(256) void attend_kernel(AttendDev a) {
-    using T = typename Elem<QT>::T;
-    const uint32_t r = blockIdx.x, h = blockIdx.y, c = blockIdx.z;
-    const uint32_t i = r / a.group, g = r % a.group, lane = threadIdx.x % 64, wave = threadIdx.x / 64;
-    const Span s = span(a, c);
-    if (static_cast<int>(i) >= s.rows) return;
-    const int pos = s.first + static_cast<int>(i);
-    __shared__ float sq[D], so[4][D], sm[4], sl[4];
-    const T* q = reinterpret_cast<const T*>(a.q) + c * a.q_copy + i * a.q_row + (h * a.group + g) * a.q_head;
-    if (threadIdx.x < D) sq[threadIdx.x] = static_cast<float>(q[threadIdx.x]);
-    __syncthreads();
-    const uint64_t base = c * a.kv.copy + h * a.kv.head;
-    const uint32_t d0 = 2 * lane;
-    const float q0 = d0 < D ? sq[d0] : 0.0f, q1 = d0 < D ? sq[d0 + 1] : 0.0f;
-    float m = -kInf, l = 0.0f, o0 = 0.0f, o1 = 0.0f;
-    for (int j = wave; j <= pos; j += 4) {
-        if (!visible(a, pos, j)) continue;
-        const uint64_t row = base + static_cast<uint64_t>(j) * a.kv.slot;
-        float t = 0.0f;
-        if (d0 < D) {
-            const f32x2 k = load2<CT>(a.kv.k, a.kv.ks, row, d0);
-            t = q0 * k[0] + q1 * k[1];
-        }
-        t = wave_sum(t) * a.scale2;
-        const float mn = fmaxf(m, t), mu = mn == -kInf ? 0.0f : mn;
-        const float p = exp2f(t - mu), f = exp2f(m - mu);
-        l = l * f + p;
-        if (d0 < D) {
-            const f32x2 v = load2<CT>(a.kv.v, a.kv.vs, row, d0);
-            o0 = o0 * f + p * v[0];
-            o1 = o1 * f + p * v[1];
-        }
-        m = mn;
-    }
-    if (lane == 0) { sm[wave] = m; sl[wave] = l; }
-    if (d0 < D) { so[wave][d0] = o0; so[wave][d0 + 1] = o1; }
-    __syncthreads();
-    const float top = fmaxf(fmaxf(sm[0], sm[1]), fmaxf(sm[2], sm[3])), mu = top == -kInf ? 0.0f : top;
-    float sum = 0.0f, f[4];
-    for (int w = 0; w < 4; ++w) {
-        f[w] = exp2f(sm[w] - mu);
-        sum += sl[w] * f[w];
-    }
-    const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
-    if (threadIdx.x < D) {
-        float o = 0.0f;
-        for (int w = 0; w < 4; ++w) o += so[w][threadIdx.x] * f[w];
-        T* out = reinterpret_cast<T*>(a.out) + c * a.o_copy + i * a.o_row + (h * a.group + g) * a.o_head;
-        out[threadIdx.x] = static_cast<T>(sum == 0.0f ? 0.0f : o * inv);
-    }
-    if (threadIdx.x == 0) {
-        if (a.lse) {
-            const uint64_t hq = static_cast<uint64_t>(c) * a.heads * a.group + h * a.group + g;
-            a.lse[hq * a.nq + i] = sum == 0.0f ? -kInf : (mu + log2f(sum)) * kLn2;
-        }
-        if (a.stats) {
-            float* st = a.stats + 2 * ((static_cast<uint64_t>(c) * a.heads + h) * a.nq * a.group + r);
-            st[0] = mu;
-            st[1] = inv;
-        }
-    }
-}
-
-// One thread per slot: its weights over every row, in row order.
-template <int CT, int QT, int D>
-__global__ __launch_bounds__(256) void weights_kernel(AttendDev a) {
-    using T = typename Elem<QT>::T;
-    const uint32_t h = blockIdx.y, c = blockIdx.z;
-    const int j = blockIdx.x * 256 + threadIdx.x;
-    const Span s = span(a, c);
-    if (j >= s.len) return;
-    const uint64_t row = c * a.kv.copy + h * a.kv.head + static_cast<uint64_t>(j) * a.kv.slot;
-    float k[D];
-    for (int d = 0; d < D; d += 2) {
-        const f32x2 x = load2<CT>(a.kv.k, a.kv.ks, row, d);
-        k[d] = x[0];
-        k[d + 1] = x[1];
-    }
-    const float* st = a.stats + 2 * (static_cast<uint64_t>(c) * a.heads + h) * a.nq * a.group;
-    float sum = 0.0f;
-    for (uint32_t i = 0; i < static_cast<uint32_t>(s.rows); ++i) {
-        if (!visible(a, s.first + static_cast<int>(i), j)) continue;
-        for (uint32_t g = 0; g < a.group; ++g) {
-            const T* q = reinterpret_cast<const T*>(a.q) + c * a.q_copy + i * a.q_row + (h * a.group + g) * a.q_head;
-            float t = 0.0f;
-            for (int d = 0; d < D; ++d) t += static_cast<float>(q[d]) * k[d];
-            const float* x = st + 2 * (i * a.group + g);
-            sum += exp2f(t * a.scale2 - x[0]) * x[1];
-        }
-    }
-    a.weights[c * a.w_copy + h * a.w_head + j] += sum;
-}
-
 // ------------------------------------------------------------ few rows: split over the slots
 typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
 typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
@@ -198,6 +103,15 @@ template <int MT>
 __device__ inline bool nonfinite2(uint32_t x) {
     constexpr uint32_t e = MT == PKV_BF16 ? 0x7f80u : 0x7c00u;
     return (x & e) == e || (x >> 16 & e) == e;
+}
+
+// Infinities and NaN of the two cleared.
+template <int MT>
+__device__ inline uint32_t finite_or_0(uint32_t x) {
+    constexpr uint32_t e = MT == PKV_BF16 ? 0x7f80u : 0x7c00u;
+    if ((x & e) == e) x &= 0xffff0000u;
+    if ((x >> 16 & e) == e) x &= 0x0000ffffu;
+    return x;
 }
 
 // The slots that the rows of a tile see, as tiles of `step` slots: [0, first)
@@ -315,10 +229,10 @@ struct SlotTile {
 };
 
 struct Partial {
-    float* o;        // [copy][kv head][split][16 rows][D]
-    float* ml;       // [copy][kv head][split][16 rows][2]: largest logit (unscaled), sum
-    float* logits;   // [copy][kv head][rows x group][ld], unscaled
-    uint32_t splits, ld;
+    float* o;        // [copy][kv head][split][rows][D]
+    float* ml;       // [copy][kv head][split][rows][2]: largest logit (unscaled), sum
+    float* logits;   // [copy][kv head][rows x group][ld], unscaled (few rows)
+    uint32_t splits, ld, rows;
 };
 
 template <int CT, int QT, int D, bool LOGITS>
@@ -496,7 +410,7 @@ __global__ __launch_bounds__(256, 2) void decode_kernel(AttendDev a, Partial par
             sum += sl[w][r] * f;
             if (f != 0.0f) acc += *reinterpret_cast<const f32x4*>(&so[w][r][d]) * f;
         }
-        const uint64_t at = (static_cast<uint64_t>(ch) * part.splits + split) * 16 + r;
+        const uint64_t at = (static_cast<uint64_t>(ch) * part.splits + split) * part.rows + r;
         *reinterpret_cast<f32x4*>(part.o + at * D + d) = acc;
         if (d == 0) {
             part.ml[2 * at] = top;
@@ -506,15 +420,17 @@ __global__ __launch_bounds__(256, 2) void decode_kernel(AttendDev a, Partial par
 }
 
 // The splits of a row joined: largest logit and the sum under it.
-__device__ inline void join_splits(const float* ml, uint32_t splits, float scale2, uint32_t lane, float* mu, float* sum) {
+__device__ inline void join_splits(const float* ml, uint32_t splits, uint32_t rows, float scale2, uint32_t lane,
+                                   float* mu, float* sum) {
+    const uint32_t step = 2 * rows;
     float top = -kInf;
-    for (uint32_t s = lane; s < splits; s += 64) top = fmaxf(top, ml[32 * s]);
+    for (uint32_t s = lane; s < splits; s += 64) top = fmaxf(top, ml[step * s]);
     for (int x = 32; x; x >>= 1) top = fmaxf(top, __shfl_xor(top, x));
     float l = 0.0f;
     for (uint32_t s = lane; s < splits; s += 64) {
         // a share without a largest logit holds the sum 0, or NaN from NaN logits
-        const float ms = ml[32 * s];
-        l += ml[32 * s + 1] * (ms == top || ms == -kInf ? 1.0f : exp2f((ms - top) * scale2));
+        const float ms = ml[step * s];
+        l += ml[step * s + 1] * (ms == top || ms == -kInf ? 1.0f : exp2f((ms - top) * scale2));
     }
     *sum = wave_sum(l);
     *mu = top == -kInf ? 0.0f : top;
@@ -532,15 +448,15 @@ __global__ __launch_bounds__(256) void join_kernel(AttendDev a, Partial part, ui
         if (x >= a.copies * a.heads * all) return;
         const uint32_t r = x % all, ch = x / all, c = ch / a.heads, h = ch % a.heads, i = r / a.group, g = r % a.group;
         if (static_cast<int>(i) >= span(a, c).rows) return;
-        const uint64_t at = static_cast<uint64_t>(ch) * part.splits * 16 + r;
+        const uint64_t at = static_cast<uint64_t>(ch) * part.splits * part.rows + r;
         float mu, sum;
-        join_splits(part.ml + 2 * at, part.splits, a.scale2, lane, &mu, &sum);
+        join_splits(part.ml + 2 * at, part.splits, part.rows, a.scale2, lane, &mu, &sum);
         float o[D / 64] = {};
         for (uint32_t s = 0; s < part.splits; ++s) {
-            const float ms = part.ml[2 * (at + 16 * s)];
+            const float ms = part.ml[2 * (at + static_cast<uint64_t>(part.rows) * s)];
             const float f = ms == -kInf ? 0.0f : ms == mu ? 1.0f : exp2f((ms - mu) * a.scale2);
             if (f == 0.0f) continue;
-            const float* p = part.o + (at + 16ull * s) * D + lane * (D / 64);
+            const float* p = part.o + (at + static_cast<uint64_t>(part.rows) * s) * D + lane * (D / 64);
             for (int e = 0; e < D / 64; ++e) o[e] += p[e] * f;
         }
         T* out = reinterpret_cast<T*>(a.out) + c * a.o_copy + i * a.o_row + (h * a.group + g) * a.o_head;
@@ -549,6 +465,10 @@ __global__ __launch_bounds__(256) void join_kernel(AttendDev a, Partial part, ui
         if (a.lse && lane == 0)
             a.lse[(static_cast<uint64_t>(c) * a.heads * a.group + h * a.group + g) * a.nq + i] =
                 sum == 0.0f ? -kInf : (mu * a.scale2 + log2f(sum)) * kLn2;
+        if (a.stats && lane == 0) {
+            a.stats[2 * (static_cast<uint64_t>(ch) * all + r)] = -mu * a.scale2;
+            a.stats[2 * (static_cast<uint64_t>(ch) * all + r) + 1] = sum == 0.0f ? 0.0f : 1.0f / sum;
+        }
         return;
     }
     const uint32_t chunks = (a.max_len + 1023) / 1024;
@@ -560,8 +480,8 @@ __global__ __launch_bounds__(256) void join_kernel(AttendDev a, Partial part, ui
     __shared__ float st[16][2];
     for (int r = wave; r < rows; r += 4) {
         float mu, sum;
-        join_splits(part.ml + 2 * (static_cast<uint64_t>(ch) * part.splits * 16 + r), part.splits, a.scale2, lane, &mu,
-                    &sum);
+        join_splits(part.ml + 2 * (static_cast<uint64_t>(ch) * part.splits * part.rows + r), part.splits, part.rows,
+                    a.scale2, lane, &mu, &sum);
         if (lane == 0) {
             st[r][0] = -mu * a.scale2;
             st[r][1] = sum == 0.0f ? 0.0f : 1.0f / sum;
@@ -582,6 +502,512 @@ __global__ __launch_bounds__(256) void join_kernel(AttendDev a, Partial part, ui
     float* out = a.weights + c * a.w_copy + h * a.w_head + j;
     for (int e = 0; e < 4; ++e)
         if (any_visible(a, tl, j + e)) out[e] += w[e];
+}
+
+// ------------------------------------------------------------ many rows: tiles of rows through LDS
+typedef float f32x16 __attribute__((ext_vector_type(16)));
+
+template <int MT>
+__device__ inline f32x16 mma32(u32x4 a, u32x4 b, f32x16 c) {
+    if constexpr (MT == PKV_BF16)
+        return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), c,
+                                                       0, 0, 0);
+    else
+        return __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(f16x8, a), __builtin_bit_cast(f16x8, b), c, 0,
+                                                      0, 0);
+}
+// Row of a 32x32 result that register r of lane half `half` holds.
+__device__ constexpr int row32(int r, int half) { return 8 * (r / 4) + 4 * half + r % 4; }
+
+// The query of one row as matrix operands, a lane half its half of every 16
+// channels (f32: of every 8): channel_of(s, half) onwards, 16 bytes a register.
+template <int CT, int QT, int D>
+struct Query {
+    using T = typename Elem<QT>::T;
+    static constexpr int kTerms = query_terms(CT, QT);
+    static constexpr int kRegs = CT == PKV_F32 ? D / 8 : D / 16;
+    u32x4 q[kTerms][kRegs];
+    __device__ void load(const T* p, bool real, uint32_t half) {
+        for (int s = 0; s < kRegs; ++s) {
+            const uint32_t d = CT == PKV_F32 ? 8 * s + 4 * half : 16 * s + 8 * half;
+            if constexpr (kTerms == 1) {
+                q[0][s] = real ? *reinterpret_cast<const u32x4*>(p + d) : u32x4{};
+            } else {
+                for (int w = 0; w < 4; ++w) {
+                    float x = real ? static_cast<float>(p[d + 2 * w]) : 0.0f;
+                    float y = real ? static_cast<float>(p[d + 2 * w + 1]) : 0.0f;
+                    for (int n = 0; n < kTerms; ++n) q[n][s][w] = pack_term<PKV_BF16>(x, y);
+                }
+            }
+        }
+    }
+};
+
+// A tile of slots on its way from the cache to LDS.
+//   keys    [slot][D], 16-byte pieces at piece ^ (slot % pieces): the 32 lanes
+//           of an operand read 32 slots at one channel
+//   values  16-bit types: [channel][slot], transposed on the way (v_perm over
+//           8 slots a thread), the 8 slots of a piece in the order in which a
+//           lane half holds them in S^T (row32), piece ^ turn(channel);
+//           f32: [slot][D], channel ^ 32 in every other 4 slots
+// so that every operand is one 16-byte read (f32 values: 4 bytes) without bank
+// conflicts, S^T's registers are the second product's operand as they are, and
+// the transposition is paid once a workgroup instead of once a wave.
+template <int CT, int D>
+struct Stage {
+    static constexpr int kSlots = CT == PKV_F32 ? 32 : 64;
+    static constexpr int kPieces = CT == PKV_F32 ? D / 4 : D / 8;       // 16-byte pieces of a key
+    static constexpr int kKeyBytes = kSlots * kPieces * 16, kBytes = 2 * kKeyBytes;
+    static constexpr int kK = CT == PKV_FP4 ? 1 : kSlots * kPieces / 256;
+    static constexpr int kPer = D / 32;                                 // channels of a value a thread transposes
+    u32x4 k[kK];
+    u32x2 v[CT == PKV_F32 ? 1 : 8];
+    u32x4 vf[CT == PKV_F32 ? kK : 1];
+    uint32_t ks, vs[CT == PKV_FP4 ? 8 : 1];
+
+    __device__ static uint32_t turn(uint32_t d) { return (d >> 1 ^ d >> 4) & 7; }
+    __device__ static int slot_of(int piece, int j) { return 16 * (piece / 2) + 4 * (piece % 2) + j % 4 + 8 * (j / 4); }
+    __device__ static uint32_t key_at(uint32_t slot, uint32_t piece) {
+        return (slot * kPieces + (piece ^ (slot % (kPieces < 16 ? kPieces : 16)))) * 16;
+    }
+    __device__ static uint32_t value_at(uint32_t d, uint32_t piece) { return kKeyBytes + d * 128 + (piece ^ turn(d)) * 16; }
+    __device__ static uint32_t value32_at(uint32_t slot, uint32_t d) {
+        return kKeyBytes + (slot * D + (d ^ (slot / 4 % 2 * 32))) * 4;
+    }
+
+    __device__ void load(const uint8_t* kp, const uint8_t* vp, const uint8_t* ksp, const uint8_t* vsp, uint64_t stride,
+                         int slot, int last) {
+        const uint32_t t = threadIdx.x, st = static_cast<uint32_t>(stride);
+        const uint64_t base = static_cast<uint64_t>(slot) * stride;
+        const int room = last - slot;
+        const uint64_t bytes = CT == PKV_FP4 ? base / 2 : CT == PKV_F32 ? base * 4 : base * 2;
+        const uint8_t *kt = kp + bytes, *vt = vp + bytes;
+        if constexpr (CT == PKV_FP4) {
+            const uint32_t e = static_cast<uint32_t>(min(static_cast<int>(t / 4), room)) * st, b = t % 4;
+            if constexpr (D == 128) {
+                k[0] = *reinterpret_cast<const u32x4*>(kt + e / 2 + 16 * b);
+            } else {
+                const u32x2 x = *reinterpret_cast<const u32x2*>(kt + e / 2 + 8 * b);
+                k[0] = u32x4{x[0], x[1], 0, 0};
+            }
+            ks = (ksp + base / 32)[e / 32 + (D == 128 ? b : b / 2)];
+            const uint32_t dg = t % 32;
+            for (int j = 0; j < 8; ++j) {
+                const uint32_t ev = static_cast<uint32_t>(min(slot_of(t / 32, j), room)) * st;
+                v[j][0] = kPer == 4 ? *reinterpret_cast<const uint16_t*>(vt + ev / 2 + 2 * dg) : (vt + ev / 2)[dg];
+                vs[j] = (vsp + base / 32)[ev / 32 + dg * kPer / 32];
+            }
+        } else {
+            constexpr uint32_t kSize = CT == PKV_F32 ? 4 : 2;
+            for (int n = 0; n < kK; ++n) {
+                const uint32_t x = t + 256 * n;
+                const uint32_t e = static_cast<uint32_t>(min(static_cast<int>(x / kPieces), room)) * st;
+                k[n] = *reinterpret_cast<const u32x4*>(kt + e * kSize + x % kPieces * 16);
+                if constexpr (CT == PKV_F32) vf[n] = *reinterpret_cast<const u32x4*>(vt + e * kSize + x % kPieces * 16);
+            }
+            if constexpr (CT != PKV_F32) {
+                const uint32_t dg = t % 32;
+                for (int j = 0; j < 8; ++j) {
+                    const uint8_t* p = vt + static_cast<uint32_t>(min(slot_of(t / 32, j), room)) * st * kSize + dg * kPer * 2;
+                    if constexpr (kPer == 4) v[j] = *reinterpret_cast<const u32x2*>(p);
+                    else v[j][0] = *reinterpret_cast<const uint32_t*>(p);
+                }
+            }
+        }
+    }
+
+    // A staged value.
+    __device__ static float value(const uint8_t* lds, int slot, uint32_t d) {
+        if constexpr (CT == PKV_F32) return *reinterpret_cast<const float*>(lds + value32_at(slot, d));
+        const int piece = slot / 16 * 2 + slot / 4 % 2, j = slot % 4 + slot / 8 % 2 * 4;   // slot_of(piece, j) == slot
+        return static_cast<float>(
+            reinterpret_cast<const typename Elem<mat_type(CT)>::T*>(lds + value_at(d, piece))[j]);
+    }
+
+    // Into LDS.  any(j): some row of the workgroup sees slot + j (the values of
+    // the others are cleared), asked only if !full.  True when a value is an
+    // infinity or NaN and rows differ in what they see.
+    template <class Any>
+    __device__ bool store(uint8_t* lds, bool full, Any any) {
+        const uint32_t t = threadIdx.x;
+        constexpr int MT = mat_type(CT);
+        bool odd = false;
+        if constexpr (CT == PKV_FP4) {
+            const uint32_t row = t / 4, b = t % 4;
+            for (int w = 0; w < (D == 128 ? 4 : 2); ++w)
+                *reinterpret_cast<u32x4*>(lds + key_at(row, b * (D / 32) + w)) = SlotTile<CT, D>::expand(k[0][w], ks);
+            for (int j = 0; j < 8; ++j) {
+                const float s = block_scale(vs[j]);
+                const uint32_t w = v[j][0];
+                v[j][0] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(w, s, 0));
+                if (kPer == 4) v[j][1] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(w, s, 1));
+            }
+        } else {
+            for (int n = 0; n < kK; ++n) {
+                const uint32_t x = t + 256 * n;
+                *reinterpret_cast<u32x4*>(lds + key_at(x / kPieces, x % kPieces)) = k[n];
+            }
+        }
+        if constexpr (CT == PKV_F32) {
+            for (int n = 0; n < kK; ++n) {
+                const uint32_t x = t + 256 * n, slot = x / kPieces;
+                if (!full) {
+                    const bool keep = any(static_cast<int>(slot));
+                    for (int w = 0; w < 4; ++w) {
+                        if (!keep) vf[n][w] = 0;
+                        odd |= (vf[n][w] & 0x7f800000u) == 0x7f800000u;
+                    }
+                }
+                *reinterpret_cast<u32x4*>(lds + value32_at(slot, x % kPieces * 4)) = vf[n];
+            }
+        } else {
+            const uint32_t dg = t % 32, piece = t / 32;
+            if (!full)
+                for (int j = 0; j < 8; ++j) {
+                    const bool keep = any(slot_of(piece, j));
+                    for (int w = 0; w < kPer / 2; ++w) {
+                        if (!keep) v[j][w] = 0;
+                        odd |= nonfinite2<MT>(v[j][w]);
+                    }
+                }
+            for (int e = 0; e < kPer; ++e) {
+                const uint32_t sel = e % 2 ? 0x07060302u : 0x05040100u;
+                const u32x4 x = {__builtin_amdgcn_perm(v[1][e / 2], v[0][e / 2], sel),
+                                 __builtin_amdgcn_perm(v[3][e / 2], v[2][e / 2], sel),
+                                 __builtin_amdgcn_perm(v[5][e / 2], v[4][e / 2], sel),
+                                 __builtin_amdgcn_perm(v[7][e / 2], v[6][e / 2], sel)};
+                *reinterpret_cast<u32x4*>(lds + value_at(dg * kPer + e, piece)) = x;
+            }
+        }
+        return odd;
+    }
+};
+
+// S^T of 32 slots (piece u of a staged tile) and 32 query rows.
+template <int CT, int QT, int D>
+__device__ inline f32x16 logits32(const uint8_t* lds, int u, const Query<CT, QT, D>& q, uint32_t lane) {
+    constexpr int MT = mat_type(CT);
+    f32x16 s = {};
+    for (int x = 0; x < Query<CT, QT, D>::kRegs; ++x) {
+        const u32x4 k = *reinterpret_cast<const u32x4*>(lds + Stage<CT, D>::key_at(32 * u + lane % 32, 2 * x + lane / 32));
+        if constexpr (CT == PKV_F32) {
+            for (int e = 0; e < 4; ++e)
+                s = __builtin_amdgcn_mfma_f32_32x32x2f32(__uint_as_float(k[e]), __uint_as_float(q.q[0][x][e]), s, 0, 0, 0);
+        } else {
+            for (int n = Query<CT, QT, D>::kTerms - 1; n >= 0; --n) s = mma32<MT>(k, q.q[n][x], s);
+        }
+    }
+    return s;
+}
+
+constexpr uint32_t kRowTile = 128;   // query rows (rows x group of one KV head) of a workgroup
+
+// Query rows in tiles of 128, 32 a wave, against tiles of 64 slots (f32: 32)
+// staged through LDS in two buffers, one barrier a tile:
+//   S^T = K Q^T (32x32 tiles; a lane holds one query row and half of each
+//   piece's slots), softmax in registers, O^T += V^T P^T with the rounded
+//   weights straight from those registers.
+// Weights of a 16-bit call are rounded once to its type (half a step of the
+// output's own rounding for each, independent, so the output's error grows by
+// less than half); over 4-bit codes they are as many bf16 terms as the query.
+// Bound, at head_dim 128, by the softmax's vector instructions beside the
+// matrix instructions (16 exponentials' 16 cycles each per 8 + 8 matrix
+// instructions of 32) -- see the table of measurements.
+template <int CT, int QT, int D>
+__global__ __launch_bounds__(256, (query_terms(CT, QT) * D > 256 ? 1 : 2)) void rows_kernel(AttendDev a, Partial part, uint32_t row_tiles) {
+    using T = typename Elem<QT>::T;
+    using St = Stage<CT, D>;
+    constexpr int MT = mat_type(CT), kU = St::kSlots / 32, kO = D / 32;
+    constexpr int NP = CT == PKV_FP4 ? query_terms(CT, QT) : 1;
+    __shared__ __align__(16) uint8_t lds[2][St::kBytes];
+    __shared__ uint32_t s_odd[2][4];
+    const uint32_t lane = threadIdx.x % 64, wave = __builtin_amdgcn_readfirstlane(threadIdx.x / 64);
+    const uint32_t n = lane % 32, half = lane / 32;
+    // heads fastest, so that a head's workgroups share an XCD's L2 where the heads are a multiple of 8; row tiles
+    // from the last, whose rows see most
+    const uint32_t heads = a.copies * a.heads;
+    const uint32_t ch = blockIdx.x % heads, c = ch / a.heads, h = ch % a.heads;
+    const uint32_t split = blockIdx.x / heads % part.splits, tile = row_tiles - 1 - blockIdx.x / heads / part.splits;
+    const Span sp = span(a, c);
+    const int R = sp.rows * static_cast<int>(a.group), r0 = static_cast<int>(tile * kRowTile), G = static_cast<int>(a.group);
+    if (r0 >= R) return;
+    const int last = min(r0 + static_cast<int>(kRowTile), R) - 1;
+    const int pos0 = sp.first + r0 / G, pos1 = sp.first + last / G;
+    const Tiles tl = tiles_of(a, pos0, pos1, St::kSlots);
+    const int per = (tl.count + static_cast<int>(part.splits) - 1) / static_cast<int>(part.splits);
+    const int t0 = static_cast<int>(split) * per, t1 = min(t0 + per, tl.count);
+
+    const int w0 = r0 + 32 * static_cast<int>(wave), w1 = min(w0 + 31, last), r = w0 + static_cast<int>(n);
+    const bool real = r <= last;
+    const int qi = (real ? r : last) / G, pos = real ? sp.first + qi : -1;
+    const int wpos0 = sp.first + w0 / G, wpos1 = sp.first + w1 / G;   // of the wave's rows (w0 > last: none)
+    const Tiles wt = tiles_of(a, wpos0, w0 <= last ? wpos1 : -1, 1);
+    Query<CT, QT, D> q;
+    q.load(reinterpret_cast<const T*>(a.q) + c * a.q_copy + qi * a.q_row + (h * a.group + (real ? r : last) % G) * a.q_head,
+           real, half);
+
+    const uint64_t base = c * a.kv.copy + h * a.kv.head;
+    const uint64_t byte = CT == PKV_FP4 ? base / 2 : CT == PKV_F32 ? base * 4 : base * 2;
+    const uint8_t *kp = a.kv.k + byte, *vp = a.kv.v + byte;
+    const uint8_t *ksp = CT == PKV_FP4 ? a.kv.ks + base / 32 : nullptr;
+    const uint8_t *vsp = CT == PKV_FP4 ? a.kv.vs + base / 32 : nullptr;
+
+    float m = -kInf, l = 0.0f;
+    f32x16 o[kO] = {};
+    St st;
+    auto put = [&](int t) {
+        const int slot = tl.slot(t, St::kSlots);
+        const bool full = all_visible(a, pos0, pos1, slot, slot + St::kSlots - 1);
+        const bool odd = st.store(lds[(t - t0) & 1], full, [&](int j) { return any_visible(a, tl, slot + j); });
+        const bool some = __any(odd);
+        if (lane == 0) s_odd[(t - t0) & 1][wave] = some;
+    };
+    if (t0 < t1) {
+        st.load(kp, vp, ksp, vsp, a.kv.slot, tl.slot(t0, St::kSlots), tl.high - 1);
+        put(t0);
+        if (t0 + 1 < t1) st.load(kp, vp, ksp, vsp, a.kv.slot, tl.slot(t0 + 1, St::kSlots), tl.high - 1);
+    }
+    __syncthreads();
+    for (int t = t0; t < t1; ++t) {
+        const uint8_t* buf = lds[(t - t0) & 1];
+        const uint32_t* odds = s_odd[(t - t0) & 1];
+        const bool odd = (odds[0] | odds[1] | odds[2] | odds[3]) != 0;
+        if (t + 1 < t1) {
+            put(t + 1);
+            if (t + 2 < t1) st.load(kp, vp, ksp, vsp, a.kv.slot, tl.slot(t + 2, St::kSlots), tl.high - 1);
+        }
+        const int slot = tl.slot(t, St::kSlots), end = slot + St::kSlots - 1;
+        // no row of the wave sees any of it
+        if (slot >= wt.high || (end < wt.low && static_cast<uint32_t>(slot) >= a.sinks)) {
+            __syncthreads();
+            continue;
+        }
+        f32x16 sc[kU];
+        for (int u = 0; u < kU; ++u) sc[u] = logits32<CT, QT, D>(buf, u, q, lane);
+        const bool full = all_visible(a, wpos0, wpos1, slot, end);
+        if (!full)
+            for (int u = 0; u < kU; ++u)
+                for (int x = 0; x < 16; ++x)
+                    if (!visible(a, pos, slot + 32 * u + row32(x, half))) sc[u][x] = -kInf;
+        float top = sc[0][0];
+        for (int u = 0; u < kU; ++u)
+            for (int x = 0; x < 16; ++x) top = fmaxf(top, sc[u][x]);
+        top = fmaxf(top, __shfl_xor(top, 32));
+        const bool grow = m == -kInf ? top > -kInf : (top - m) * a.scale2 > 8.0f;
+        if (__any(grow)) {   // as in decode_kernel
+            const float mn = fmaxf(m, top);
+            const float f = m == -kInf ? 1.0f : exp2f((m - mn) * a.scale2);
+            if (mn > m) {
+                l *= f;
+                for (int e = 0; e < kO; ++e) o[e] *= f;
+                m = mn;
+            }
+        }
+        const float mc = m == -kInf ? 0.0f : m * a.scale2;
+        for (int u = 0; u < kU; ++u)
+            for (int x = 0; x < 16; ++x) {
+                sc[u][x] = __builtin_amdgcn_exp2f(__builtin_fmaf(sc[u][x], a.scale2, -mc));
+                l += sc[u][x];
+            }
+        // O^T += V^T P^T, infinities and NaN taken out first if `clean`
+        auto weigh = [&](auto clean) {
+            for (int u = 0; u < kU; ++u) {
+                if constexpr (CT == PKV_F32) {
+                    for (int x = 0; x < 16; ++x)
+                        for (int e = 0; e < kO; ++e) {
+                            float v = *reinterpret_cast<const float*>(
+                                buf + St::value32_at(32 * u + row32(x, half), 32 * e + n));
+                            if (clean && (__float_as_uint(v) & 0x7f800000u) == 0x7f800000u) v = 0.0f;
+                            o[e] = __builtin_amdgcn_mfma_f32_32x32x2f32(v, sc[u][x], o[e], 0, 0, 0);
+                        }
+                } else {
+                    for (int y = 0; y < 2; ++y) {
+                        float p[8];
+                        for (int x = 0; x < 8; ++x) p[x] = sc[u][8 * y + x];
+                        u32x4 pt[NP];
+                        for (int k = 0; k < NP; ++k)
+                            pt[k] = u32x4{pack_term<MT>(p[0], p[1]), pack_term<MT>(p[2], p[3]), pack_term<MT>(p[4], p[5]),
+                                          pack_term<MT>(p[6], p[7])};
+                        for (int e = 0; e < kO; ++e) {
+                            u32x4 v = *reinterpret_cast<const u32x4*>(
+                                buf + St::value_at(32 * e + n, 4 * u + 2 * y + half));
+                            if (clean)
+                                for (int k = 0; k < 4; ++k) v[k] = finite_or_0<MT>(v[k]);
+                            for (int k = NP - 1; k >= 0; --k) o[e] = mma32<MT>(v, pt[k], o[e]);
+                        }
+                    }
+                }
+            }
+        };
+        if (__builtin_expect(odd && !full, 0)) {
+            // infinities or NaN among the values, in slots that some of the
+            // wave's rows do not see: the products without them, then each of
+            // them to the rows that do
+            weigh(std::true_type{});
+#pragma unroll 1
+            for (int j = 0; j < St::kSlots; ++j) {
+                // register and half that hold slot j's weights
+                const int reg = j % 32 / 8 * 4 + j % 4 + 16 * (j / 32), side = j / 4 % 2;
+                float p = 0.0f;
+                for (int u = 0; u < kU; ++u)
+                    for (int x = 0; x < 16; ++x) p = reg == 16 * u + x ? sc[u][x] : p;
+                p = __shfl(p, static_cast<int>(n) + 32 * side);
+                const bool sees = visible(a, pos, slot + j);
+                for (int e = 0; e < kO; ++e)
+                    for (int x = 0; x < 16; ++x) {
+                        const float v = St::value(buf, j, 32 * e + row32(x, half));
+                        if (sees && (__float_as_uint(v) & 0x7f800000u) == 0x7f800000u) o[e][x] += p * v;
+                    }
+            }
+        } else {
+            weigh(std::false_type{});
+        }
+        __syncthreads();
+    }
+    l += __shfl_xor(l, 32);
+    if (!real) return;
+    const uint64_t all = static_cast<uint64_t>(a.nq) * a.group;
+    if (part.splits > 1) {
+        const uint64_t at = (static_cast<uint64_t>(ch) * part.splits + split) * part.rows + r;
+        for (int e = 0; e < kO; ++e)
+            for (int x = 0; x < 4; ++x)
+                *reinterpret_cast<f32x4*>(part.o + at * D + 32 * e + 8 * x + 4 * half) =
+                    f32x4{o[e][4 * x], o[e][4 * x + 1], o[e][4 * x + 2], o[e][4 * x + 3]};
+        if (half == 0) {
+            part.ml[2 * at] = m;
+            part.ml[2 * at + 1] = l;
+        }
+        return;
+    }
+    const float inv = l == 0.0f ? 0.0f : 1.0f / l, mu = m == -kInf ? 0.0f : m;
+    const uint32_t g = static_cast<uint32_t>(r % G);
+    T* out = reinterpret_cast<T*>(a.out) + c * a.o_copy + qi * a.o_row + (h * a.group + g) * a.o_head;
+    for (int e = 0; e < kO; ++e)
+        for (int x = 0; x < 4; ++x) {
+            typedef T T4 __attribute__((ext_vector_type(4)));
+            T4 y;
+            for (int k = 0; k < 4; ++k) y[k] = static_cast<T>(l == 0.0f ? 0.0f : o[e][4 * x + k] * inv);
+            *reinterpret_cast<T4*>(out + 32 * e + 8 * x + 4 * half) = y;
+        }
+    if (half == 0) {
+        if (a.lse)
+            a.lse[(static_cast<uint64_t>(c) * a.heads * a.group + h * a.group + g) * a.nq + qi] =
+                l == 0.0f ? -kInf : (mu * a.scale2 + log2f(l)) * kLn2;
+        if (a.stats) {
+            a.stats[2 * (ch * all + r)] = -mu * a.scale2;
+            a.stats[2 * (ch * all + r) + 1] = inv;
+        }
+    }
+}
+
+// Accumulated weights of many rows: 32 slots a wave, its keys held in registers
+// as the S^T operand, all rows that can see them streamed through LDS 32 at a
+// time (four waves share them); every slot belongs to one wave, so sums have
+// one order.  S^T, one multiply-add and one exponential a logit: half of
+// rows_kernel's matrix work, its softmax work without maximum and rounding.
+template <int CT, int QT, int D>
+__global__ __launch_bounds__(256, 2) void weights_kernel(AttendDev a) {
+    using T = typename Elem<QT>::T;
+    using Q = Query<CT, QT, D>;
+    constexpr int MT = mat_type(CT), kPieces = CT == PKV_F32 ? D / 4 : D / 8, kTerms = Q::kTerms;
+    constexpr uint32_t kTermBytes = 32 * kPieces * 16;
+    __shared__ __align__(16) uint8_t lds[2][kTerms * kTermBytes];
+    __shared__ float s_stat[2][32][2];
+    const uint32_t lane = threadIdx.x % 64, wave = __builtin_amdgcn_readfirstlane(threadIdx.x / 64);
+    const uint32_t n = lane % 32, half = lane / 32, heads = a.copies * a.heads;
+    const uint32_t ch = blockIdx.x % heads, c = ch / a.heads, h = ch % a.heads;
+    const Span sp = span(a, c);
+    const int G = static_cast<int>(a.group), b0 = static_cast<int>(blockIdx.x / heads) * 128, s0 = b0 + 32 * static_cast<int>(wave);
+    const int high = sp.first + sp.rows;                 // slots below it are seen by the last row or hidden by its window
+    if (b0 >= high || sp.rows == 0) return;
+    // rows i0 .. i1 see something of b0 .. b0 + 127
+    const int i0 = max(b0 - sp.first, 0);
+    const int64_t reach = !a.window || static_cast<uint32_t>(b0) < a.sinks
+                              ? sp.rows - 1
+                              : static_cast<int64_t>(b0) + 126 + a.window - sp.first;
+    const int i1 = static_cast<int>(min(reach, static_cast<int64_t>(sp.rows - 1)));
+    if (i0 > i1) return;
+    const int r0 = i0 * G, r1 = i1 * G + G;
+
+    // the wave's keys as operand A: slot n, channels as Query
+    u32x4 k[Q::kRegs];
+    {
+        const uint64_t e = c * a.kv.copy + h * a.kv.head + static_cast<uint64_t>(min(s0 + static_cast<int>(n), high - 1)) * a.kv.slot;
+        if constexpr (CT == PKV_FP4) {
+            for (int s = 0; s < Q::kRegs; ++s) {
+                const uint64_t x = e + 16 * s + 8 * half;
+                k[s] = SlotTile<CT, D>::expand(*reinterpret_cast<const uint32_t*>(a.kv.k + x / 2), a.kv.ks[x / 32]);
+            }
+        } else {
+            const uint8_t* p = a.kv.k + e * (CT == PKV_F32 ? 4 : 2);
+            for (int s = 0; s < Q::kRegs; ++s) k[s] = *reinterpret_cast<const u32x4*>(p + 32 * s + 16 * half);
+        }
+    }
+    const uint64_t all = static_cast<uint64_t>(a.nq) * a.group;
+    const T* qp = reinterpret_cast<const T*>(a.q) + c * a.q_copy + static_cast<uint64_t>(h) * a.group * a.q_head;
+    auto stage = [&](int r, uint32_t b) {
+        for (uint32_t x = threadIdx.x; x < 32 * kPieces; x += 256) {
+            const int row = min(r + static_cast<int>(x / kPieces), r1 - 1);
+            const uint32_t piece = x % kPieces;
+            const T* p = qp + static_cast<uint64_t>(row / G) * a.q_row + static_cast<uint64_t>(row % G) * a.q_head;
+            const uint32_t at = (x / kPieces * kPieces + (piece ^ (x / kPieces % (kPieces < 16 ? kPieces : 16)))) * 16;
+            if constexpr (kTerms == 1) {
+                *reinterpret_cast<u32x4*>(lds[b] + at) = reinterpret_cast<const u32x4*>(p)[piece];
+            } else {
+                u32x4 w[kTerms];
+                for (int y = 0; y < 4; ++y) {
+                    float f0 = static_cast<float>(p[8 * piece + 2 * y]), f1 = static_cast<float>(p[8 * piece + 2 * y + 1]);
+                    for (int z = 0; z < kTerms; ++z) w[z][y] = pack_term<PKV_BF16>(f0, f1);
+                }
+                for (int z = 0; z < kTerms; ++z) *reinterpret_cast<u32x4*>(lds[b] + z * kTermBytes + at) = w[z];
+            }
+        }
+        if (threadIdx.x < 32) {
+            const bool in = r + static_cast<int>(threadIdx.x) < r1;
+            const float* st = a.stats + 2 * (ch * all + min(r + static_cast<int>(threadIdx.x), r1 - 1));
+            s_stat[b][threadIdx.x][0] = st[0];
+            s_stat[b][threadIdx.x][1] = in ? st[1] : 0.0f;
+        }
+    };
+    float w[16] = {};
+    stage(r0, 0);
+    __syncthreads();
+    uint32_t b = 0;
+    for (int r = r0; r < r1; r += 32, b ^= 1) {
+        if (r + 32 < r1) stage(r + 32, b ^ 1);
+        f32x16 s = {};
+        for (int x = 0; x < Q::kRegs; ++x)
+            for (int z = kTerms - 1; z >= 0; --z) {
+                const uint32_t piece = 2 * x + half;
+                const u32x4 y = *reinterpret_cast<const u32x4*>(
+                    lds[b] + z * kTermBytes + (n * kPieces + (piece ^ (n % (kPieces < 16 ? kPieces : 16)))) * 16);
+                if constexpr (CT == PKV_F32) {
+                    for (int e = 0; e < 4; ++e)
+                        s = __builtin_amdgcn_mfma_f32_32x32x2f32(__uint_as_float(k[x][e]), __uint_as_float(y[e]), s, 0, 0, 0);
+                } else {
+                    s = mma32<MT>(k[x], y, s);
+                }
+            }
+        const float mc = s_stat[b][n][0], inv = s_stat[b][n][1];
+        const int pos = sp.first + (r + static_cast<int>(n)) / G;
+        if (all_visible(a, sp.first + r / G, sp.first + min(r + 31, r1 - 1) / G, s0, s0 + 31) && r + 32 <= r1) {
+            for (int x = 0; x < 16; ++x)
+                w[x] = __builtin_fmaf(__builtin_amdgcn_exp2f(__builtin_fmaf(s[x], a.scale2, mc)), inv, w[x]);
+        } else {
+            for (int x = 0; x < 16; ++x)
+                if (r + static_cast<int>(n) < r1 && inv != 0.0f && visible(a, pos, s0 + row32(x, half)))
+                    w[x] = __builtin_fmaf(__builtin_amdgcn_exp2f(__builtin_fmaf(s[x], a.scale2, mc)), inv, w[x]);
+        }
+        __syncthreads();
+    }
+    for (int x = 0; x < 16; ++x)
+        for (int y = 16; y; y >>= 1) w[x] += __shfl_xor(w[x], y);
+    float* out = a.weights + c * a.w_copy + h * a.w_head;
+    for (int x = 0; x < 16; ++x) {
+        const int j = s0 + row32(x, half);
+        if (n == 0 && j < high && (!a.window || j >= sp.first - static_cast<int64_t>(a.window) + 1 || static_cast<uint32_t>(j) < a.sinks))
+            out[j] += w[x];
+    }
 }
 
 // ------------------------------------------------------------ the 4-bit cache
@@ -819,46 +1245,54 @@ uint64_t round256(uint64_t x) { return (x + 255) & ~255ull; }
 
 constexpr uint32_t kDecodeRows = 16;   // rows x group that decode_kernel takes
 
-// How a call of few rows is cut: `splits` shares of the slots for each (copy,
-// head), so that the chip is full (768 workgroups, three a CU) while every wave
-// of a share has a tile.
-struct DecodePlan {
-    uint32_t splits, ld;
-    uint64_t ml, logits, bytes;   // offsets in the workspace (partial outputs first), all of it
+// How a call is cut: row tiles (one of at most 16 rows, or tiles of 128) times
+// `splits` shares of the slots, so that the chip is full (kFew / kMany
+// workgroups) while a share has work for its waves.
+struct Plan {
+    uint32_t row_tiles, splits, rows, ld;
+    uint64_t ml, logits, stats, bytes;   // offsets in the workspace (partial outputs first), all of it
 };
-DecodePlan decode_plan(const AttendDev& a, uint32_t dim, int cache_dtype) {
-    DecodePlan p;
-    const uint32_t step = cache_dtype == PKV_F32 ? 16 : 32, heads = a.copies * a.heads;
-    // slots that a call can see: all, or the window, the rows before the last and the sinks, each up to a tile more
+Plan plan_of(const AttendDev& a, uint32_t dim, int cache_dtype) {
+    Plan p{};
+    const uint64_t all = static_cast<uint64_t>(a.nq) * a.group, heads = static_cast<uint64_t>(a.copies) * a.heads;
+    const bool few = all <= kDecodeRows;
+    const uint32_t step = (few ? 32 : 64) / (cache_dtype == PKV_F32 ? 2 : 1);
+    p.row_tiles = few ? 1 : static_cast<uint32_t>((all + kRowTile - 1) / kRowTile);
+    p.rows = few ? kDecodeRows : p.row_tiles * kRowTile;
+    // slots that a row tile can see: all, or the window, the rows before its last and the sinks, each up to a tile more
     uint64_t most = a.max_len;
-    if (a.window) most = std::min<uint64_t>(most, static_cast<uint64_t>(a.window) + a.nq + a.sinks + 2 * step);
-    const uint64_t tiles = (most + step - 1) / step;
-    p.splits = static_cast<uint32_t>(std::max<uint64_t>(1, std::min<uint64_t>((768 + heads - 1) / heads, tiles / 4)));
-    p.ld = (a.max_len + 31) / 32 * 32 + 4;
-    const uint64_t parts = static_cast<uint64_t>(heads) * p.splits * kDecodeRows;
-    p.ml = round256(parts * dim * 4);
-    p.logits = p.ml + round256(parts * 8);
-    p.bytes = p.logits + (a.weights ? round256(4ull * heads * a.nq * a.group * p.ld) : 0);
+    if (a.window)
+        most = std::min<uint64_t>(most, static_cast<uint64_t>(a.window) + std::min<uint64_t>(a.nq, p.rows) + a.sinks + 2 * step);
+    const uint64_t tiles = (most + step - 1) / step, groups = heads * p.row_tiles;
+    // few rows: 768 workgroups are three a CU, every wave of a share has a tile; many rows: two a CU, four tiles a share
+    const uint64_t want = few ? (768 + groups - 1) / groups : 512 / groups;
+    p.splits = static_cast<uint32_t>(std::max<uint64_t>(1, std::min<uint64_t>(want, tiles / 4)));
+    const bool parts = few || p.splits > 1;
+    p.ld = few && a.weights ? (a.max_len + 31) / 32 * 32 + 4 : 0;
+    p.ml = parts ? round256(heads * p.splits * p.rows * dim * 4) : 0;
+    p.logits = p.ml + (parts ? round256(heads * p.splits * p.rows * 8) : 0);
+    p.stats = p.logits + round256(4 * heads * all * p.ld);
+    p.bytes = p.stats + (!few && a.weights ? round256(8 * heads * all) : 0);
     return p;
 }
 
 template <int CT, int QT, int D>
 int attend_typed(AttendDev a, uint8_t* ws, hipStream_t st) {
+    const Plan p = plan_of(a, D, CT);
+    const Partial part{reinterpret_cast<float*>(ws), reinterpret_cast<float*>(ws + p.ml),
+                       reinterpret_cast<float*>(ws + p.logits), p.splits, p.ld, p.rows};
+    const uint32_t heads = a.copies * a.heads, outs = (heads * a.nq * a.group + 3) / 4;
     if (a.nq * a.group <= kDecodeRows) {
-        const DecodePlan p = decode_plan(a, D, CT);
-        const Partial part{reinterpret_cast<float*>(ws), reinterpret_cast<float*>(ws + p.ml),
-                           reinterpret_cast<float*>(ws + p.logits), p.splits, p.ld};
-        const uint32_t heads = a.copies * a.heads, outs = (heads * a.nq * a.group + 3) / 4;
         if (a.weights) decode_kernel<CT, QT, D, true><<<heads * p.splits, 256, 0, st>>>(a, part);
         else decode_kernel<CT, QT, D, false><<<heads * p.splits, 256, 0, st>>>(a, part);
         const uint32_t chunks = a.weights ? (a.max_len + 1023) / 1024 * heads : 0;
         join_kernel<QT, D><<<outs + chunks, 256, 0, st>>>(a, part, outs);
         return hipGetLastError();
     }
-    a.stats = a.weights ? reinterpret_cast<float*>(ws) : nullptr;
-    attend_kernel<CT, QT, D><<<dim3(a.nq * a.group, a.heads, a.copies), 256, 0, st>>>(a);
-    if (a.weights)
-        weights_kernel<CT, QT, D><<<dim3((a.max_len + 255) / 256, a.heads, a.copies), 256, 0, st>>>(a);
+    a.stats = a.weights ? reinterpret_cast<float*>(ws + p.stats) : nullptr;
+    rows_kernel<CT, QT, D><<<heads * p.row_tiles * p.splits, 256, 0, st>>>(a, part, p.row_tiles);
+    if (p.splits > 1) join_kernel<QT, D><<<outs, 256, 0, st>>>(a, part, outs);
+    if (a.weights) weights_kernel<CT, QT, D><<<(a.max_len + 127) / 128 * heads, 256, 0, st>>>(a);
     return hipGetLastError();
 }
 
@@ -870,8 +1304,7 @@ int attend_dim(const AttendDev& a, uint32_t dim, uint8_t* ws, hipStream_t st) {
 }  // namespace
 
 uint64_t attend_workspace(const AttendDev& a, uint32_t dim, int cache_dtype, int) {
-    if (a.nq * a.group <= kDecodeRows) return decode_plan(a, dim, cache_dtype).bytes;
-    return 8ull * a.copies * a.heads * a.nq * a.group;
+    return plan_of(a, dim, cache_dtype).bytes;
 }
 
 int launch_attend(const AttendDev& a, uint32_t dim, int cache_dtype, int dtype, uint8_t* ws, void* stream) {
