@@ -105,6 +105,15 @@ __device__ inline bool nonfinite2(uint32_t x) {
     return (x & e) == e || (x >> 16 & e) == e;
 }
 
+// One word's part of a dot product.
+template <int MT>
+__device__ inline float dot_word(uint32_t a, uint32_t b) {
+    if constexpr (MT == PKV_F32) return __uint_as_float(a) * __uint_as_float(b);
+    using T2 = typename std::conditional<MT == PKV_BF16, bf16x2, f16x2>::type;
+    const T2 x = __builtin_bit_cast(T2, a), y = __builtin_bit_cast(T2, b);
+    return static_cast<float>(x[0]) * static_cast<float>(y[0]) + static_cast<float>(x[1]) * static_cast<float>(y[1]);
+}
+
 // Infinities and NaN of the two cleared.
 template <int MT>
 __device__ inline uint32_t finite_or_0(uint32_t x) {
@@ -543,141 +552,144 @@ struct Query {
     }
 };
 
-// A tile of slots on its way from the cache to LDS.
-//   keys    [slot][D], 16-byte pieces at piece ^ (slot % pieces): the 32 lanes
-//           of an operand read 32 slots at one channel
-//   values  16-bit types: [channel][slot], transposed on the way (v_perm over
-//           8 slots a thread), the 8 slots of a piece in the order in which a
-//           lane half holds them in S^T (row32), piece ^ turn(channel);
-//           f32: [slot][D], channel ^ 32 in every other 4 slots
-// so that every operand is one 16-byte read (f32 values: 4 bytes) without bank
-// conflicts, S^T's registers are the second product's operand as they are, and
-// the transposition is paid once a workgroup instead of once a wave.
+// 16 bytes a lane from global memory straight to LDS (lane i at `to` + 16 i; to
+// is uniform), nothing held in registers on the way.  Done when the wave waits
+// (copies_done): the compiler, which would wait at the next LDS read of any
+// kind, does not see them.  M0 is put back, since the compiler may hold a value there.
+__device__ inline void copy_to_lds(uint32_t to, const uint8_t* from, uint32_t offset) {
+    uint32_t m0;
+    asm volatile("s_mov_b32 %0, m0\n\ts_mov_b32 m0, %1\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %2, %3\n\ts_mov_b32 m0, %0"
+                 : "=&s"(m0)
+                 : "s"(to), "v"(offset), "s"(from)
+                 : "memory");
+}
+__device__ inline void copies_done() { asm volatile("s_waitcnt vmcnt(0)" ::: "memory"); }
+
+typedef __attribute__((address_space(3))) uint8_t LdsByte;
+
+// A tile of slots in LDS: keys [slot][D], then values [slot][D], 4-bit codes
+// as bf16, in 16-byte pieces at piece ^ turn(slot) so that no read meets a bank
+// conflict: an operand of the first product is one piece of 32 slots, one of
+// the second 4 slots x 16 channels, transposed by the read itself
+// (ds_read_tr16_b64; f32: 32 channels of a slot, no transposition).  f32 keys
+// meet two lanes a bank: their products take four times longer than the read.
+// 16- and 32-bit rows go from memory to LDS without registers; a lane reads
+// the piece that its place holds.
 template <int CT, int D>
 struct Stage {
     static constexpr int kSlots = CT == PKV_F32 ? 32 : 64;
-    static constexpr int kPieces = CT == PKV_F32 ? D / 4 : D / 8;       // 16-byte pieces of a key
-    static constexpr int kKeyBytes = kSlots * kPieces * 16, kBytes = 2 * kKeyBytes;
-    static constexpr int kK = CT == PKV_FP4 ? 1 : kSlots * kPieces / 256;
-    static constexpr int kPer = D / 32;                                 // channels of a value a thread transposes
-    u32x4 k[kK];
-    u32x2 v[CT == PKV_F32 ? 1 : 8];
-    u32x4 vf[CT == PKV_F32 ? kK : 1];
-    uint32_t ks, vs[CT == PKV_FP4 ? 8 : 1];
+    static constexpr int kRow = CT == PKV_F32 ? D * 4 : D * 2, kPieces = kRow / 16;
+    static constexpr int kKeyBytes = kSlots * kRow, kBytes = 2 * kKeyBytes;
+    static constexpr int kCopies = kKeyBytes / 4096;            // wave-wide copies of 1,024 bytes, a side
+    static constexpr int kCopyRows = 1024 / kRow, kCopyStep = 4 * kCopyRows;
+    u32x4 k, v;                                                 // 4-bit codes on their way
+    uint32_t ks, vs;
 
-    __device__ static uint32_t turn(uint32_t d) { return (d >> 1 ^ d >> 4) & 7; }
-    __device__ static int slot_of(int piece, int j) { return 16 * (piece / 2) + 4 * (piece % 2) + j % 4 + 8 * (j / 4); }
+    __device__ static uint32_t turn(uint32_t slot, bool values) {
+        if constexpr (CT == PKV_F32) return values ? slot / 4 % 2 * 8 : slot % 8;
+        else if constexpr (D == 128) return slot % 4 * 4 + slot / 4 % 4;
+        else return slot / 2 % 2 * 4 + slot / 4 % 4;
+    }
     __device__ static uint32_t key_at(uint32_t slot, uint32_t piece) {
-        return (slot * kPieces + (piece ^ (slot % (kPieces < 16 ? kPieces : 16)))) * 16;
+        return slot * kRow + (piece ^ turn(slot, false)) * 16;
     }
-    __device__ static uint32_t value_at(uint32_t d, uint32_t piece) { return kKeyBytes + d * 128 + (piece ^ turn(d)) * 16; }
-    __device__ static uint32_t value32_at(uint32_t slot, uint32_t d) {
-        return kKeyBytes + (slot * D + (d ^ (slot / 4 % 2 * 32))) * 4;
+    __device__ static uint32_t value_at(uint32_t slot, uint32_t piece) {
+        return kKeyBytes + slot * kRow + (piece ^ turn(slot, true)) * 16;
+    }
+    // The slot that thread t's 4-bit codes belong to, 16 a wave: 16 lanes write 16 different places of the banks.
+    __device__ static uint32_t code_slot(uint32_t t) {
+        const uint32_t i = t % 64;
+        return t / 64 * 16 + (D == 128 ? i / 16 + i / 4 % 4 * 4 : i / 4 % 2 + i / 8 % 2 * 4 + i / 16 % 2 * 2 + i / 32 * 8);
     }
 
-    __device__ void load(const uint8_t* kp, const uint8_t* vp, const uint8_t* ksp, const uint8_t* vsp, uint64_t stride,
-                         int slot, int last) {
-        const uint32_t t = threadIdx.x, st = static_cast<uint32_t>(stride);
+    // Start a tile on its way.  kp, vp, ksp, vsp: slot 0 of the head; slots past `last` read the last one.
+    __device__ void fetch(uint32_t lds, const uint8_t* kp, const uint8_t* vp, const uint8_t* ksp, const uint8_t* vsp,
+                          uint64_t stride, int slot, int last) {
         const uint64_t base = static_cast<uint64_t>(slot) * stride;
+        const uint32_t st = static_cast<uint32_t>(stride);
         const int room = last - slot;
-        const uint64_t bytes = CT == PKV_FP4 ? base / 2 : CT == PKV_F32 ? base * 4 : base * 2;
-        const uint8_t *kt = kp + bytes, *vt = vp + bytes;
         if constexpr (CT == PKV_FP4) {
-            const uint32_t e = static_cast<uint32_t>(min(static_cast<int>(t / 4), room)) * st, b = t % 4;
+            const uint32_t t = threadIdx.x, b = t % 4;
+            const uint32_t e = static_cast<uint32_t>(min(static_cast<int>(code_slot(t)), room)) * st;
+            const uint8_t *kt = kp + base / 2 + e / 2, *vt = vp + base / 2 + e / 2;
             if constexpr (D == 128) {
-                k[0] = *reinterpret_cast<const u32x4*>(kt + e / 2 + 16 * b);
+                k = *reinterpret_cast<const u32x4*>(kt + 16 * b);
+                v = *reinterpret_cast<const u32x4*>(vt + 16 * b);
             } else {
-                const u32x2 x = *reinterpret_cast<const u32x2*>(kt + e / 2 + 8 * b);
-                k[0] = u32x4{x[0], x[1], 0, 0};
+                const u32x2 x = *reinterpret_cast<const u32x2*>(kt + 8 * b), y = *reinterpret_cast<const u32x2*>(vt + 8 * b);
+                k = u32x4{x[0], x[1], 0, 0};
+                v = u32x4{y[0], y[1], 0, 0};
             }
-            ks = (ksp + base / 32)[e / 32 + (D == 128 ? b : b / 2)];
-            const uint32_t dg = t % 32;
-            for (int j = 0; j < 8; ++j) {
-                const uint32_t ev = static_cast<uint32_t>(min(slot_of(t / 32, j), room)) * st;
-                v[j][0] = kPer == 4 ? *reinterpret_cast<const uint16_t*>(vt + ev / 2 + 2 * dg) : (vt + ev / 2)[dg];
-                vs[j] = (vsp + base / 32)[ev / 32 + dg * kPer / 32];
-            }
+            const uint64_t sb = base / 32 + e / 32 + (D == 128 ? b : b / 2);
+            ks = ksp[sb];
+            vs = vsp[sb];
         } else {
             constexpr uint32_t kSize = CT == PKV_F32 ? 4 : 2;
-            for (int n = 0; n < kK; ++n) {
-                const uint32_t x = t + 256 * n;
-                const uint32_t e = static_cast<uint32_t>(min(static_cast<int>(x / kPieces), room)) * st;
-                k[n] = *reinterpret_cast<const u32x4*>(kt + e * kSize + x % kPieces * 16);
-                if constexpr (CT == PKV_F32) vf[n] = *reinterpret_cast<const u32x4*>(vt + e * kSize + x % kPieces * 16);
-            }
-            if constexpr (CT != PKV_F32) {
-                const uint32_t dg = t % 32;
-                for (int j = 0; j < 8; ++j) {
-                    const uint8_t* p = vt + static_cast<uint32_t>(min(slot_of(t / 32, j), room)) * st * kSize + dg * kPer * 2;
-                    if constexpr (kPer == 4) v[j] = *reinterpret_cast<const u32x2*>(p);
-                    else v[j][0] = *reinterpret_cast<const uint32_t*>(p);
-                }
+            const uint32_t lane = threadIdx.x % 64, wave = __builtin_amdgcn_readfirstlane(threadIdx.x / 64);
+            // turn() of the row is the same for all of a lane's copies
+            const uint32_t row = kCopyRows * wave + lane / kPieces, piece = lane % kPieces;
+            const uint32_t kc = (piece ^ turn(row, false)) * 16, vc = (piece ^ turn(row, true)) * 16;
+            const uint8_t *kt = kp + base * kSize, *vt = vp + base * kSize;
+            for (int x = 0; x < kCopies; ++x) {
+                const uint32_t e = min(kCopyStep * x + static_cast<int>(row), room) * st * kSize;
+                const uint32_t to = lds + (kCopyStep * x + kCopyRows * wave) * kRow;
+                copy_to_lds(to, kt, e + kc);
+                copy_to_lds(to + kKeyBytes, vt, e + vc);
             }
         }
     }
-
-    // A staged value.
-    __device__ static float value(const uint8_t* lds, int slot, uint32_t d) {
-        if constexpr (CT == PKV_F32) return *reinterpret_cast<const float*>(lds + value32_at(slot, d));
-        const int piece = slot / 16 * 2 + slot / 4 % 2, j = slot % 4 + slot / 8 % 2 * 4;   // slot_of(piece, j) == slot
-        return static_cast<float>(
-            reinterpret_cast<const typename Elem<mat_type(CT)>::T*>(lds + value_at(d, piece))[j]);
-    }
-
-    // Into LDS.  any(j): some row of the workgroup sees slot + j (the values of
-    // the others are cleared), asked only if !full.  True when a value is an
-    // infinity or NaN and rows differ in what they see.
-    template <class Any>
-    __device__ bool store(uint8_t* lds, bool full, Any any) {
-        const uint32_t t = threadIdx.x;
-        constexpr int MT = mat_type(CT);
-        bool odd = false;
+    // What fetch started, into LDS (a barrier follows).
+    __device__ void land(uint8_t* lds) {
         if constexpr (CT == PKV_FP4) {
-            const uint32_t row = t / 4, b = t % 4;
-            for (int w = 0; w < (D == 128 ? 4 : 2); ++w)
-                *reinterpret_cast<u32x4*>(lds + key_at(row, b * (D / 32) + w)) = SlotTile<CT, D>::expand(k[0][w], ks);
-            for (int j = 0; j < 8; ++j) {
-                const float s = block_scale(vs[j]);
-                const uint32_t w = v[j][0];
-                v[j][0] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(w, s, 0));
-                if (kPer == 4) v[j][1] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(w, s, 1));
+            const uint32_t t = threadIdx.x, row = code_slot(t), b = t % 4;
+            for (int w = 0; w < D / 32; ++w) {
+                *reinterpret_cast<u32x4*>(lds + key_at(row, b * (D / 32) + w)) = SlotTile<CT, D>::expand(k[w], ks);
+                *reinterpret_cast<u32x4*>(lds + value_at(row, b * (D / 32) + w)) = SlotTile<CT, D>::expand(v[w], vs);
             }
         } else {
-            for (int n = 0; n < kK; ++n) {
-                const uint32_t x = t + 256 * n;
-                *reinterpret_cast<u32x4*>(lds + key_at(x / kPieces, x % kPieces)) = k[n];
-            }
+            copies_done();
         }
-        if constexpr (CT == PKV_F32) {
-            for (int n = 0; n < kK; ++n) {
-                const uint32_t x = t + 256 * n, slot = x / kPieces;
-                if (!full) {
-                    const bool keep = any(static_cast<int>(slot));
-                    for (int w = 0; w < 4; ++w) {
-                        if (!keep) vf[n][w] = 0;
-                        odd |= (vf[n][w] & 0x7f800000u) == 0x7f800000u;
+    }
+    // Operand of O^T += V^T P^T for channels 32 e .. and 16 slots from `slot` on: a lane's channel 32 e + lane % 32,
+    // the slots of row32 in its half of them.
+    __device__ static u32x4 values16(const uint8_t* lds, uint32_t slot, uint32_t e, uint32_t lane) {
+        const uint32_t s = lane % 16, piece = 4 * e + lane / 16 % 2 * 2 + s % 4 / 2;
+        const uint32_t row = slot + lane / 32 * 4 + s / 4;
+        typedef short s16x4 __attribute__((ext_vector_type(4)));
+        typedef __attribute__((address_space(3))) s16x4* Ptr;
+        const LdsByte* p = (const LdsByte*)lds;
+        const s16x4 a = __builtin_amdgcn_ds_read_tr16_b64_v4i16((Ptr)(p + value_at(row, piece) + s % 2 * 8));
+        const s16x4 b = __builtin_amdgcn_ds_read_tr16_b64_v4i16((Ptr)(p + value_at(row + 8, piece) + s % 2 * 8));
+        const u32x2 x = __builtin_bit_cast(u32x2, a), y = __builtin_bit_cast(u32x2, b);
+        return u32x4{x[0], x[1], y[0], y[1]};
+    }
+    __device__ static uint32_t value32_at(uint32_t slot, uint32_t d) { return value_at(slot, d / 4) + d % 4 * 4; }
+    // A staged value.
+    __device__ static float value(const uint8_t* lds, uint32_t slot, uint32_t d) {
+        if constexpr (CT == PKV_F32) return *reinterpret_cast<const float*>(lds + value32_at(slot, d));
+        else return static_cast<float>(
+            reinterpret_cast<const typename Elem<mat_type(CT)>::T*>(lds + value_at(slot, d / 8))[d % 8]);
+    }
+    // Infinities and NaN among a staged tile's values to 0; true if this thread had any.
+    __device__ static bool clean(uint8_t* lds) {
+        bool odd = false;
+        for (uint32_t x = threadIdx.x; x < kKeyBytes / 16; x += 256) {
+            u32x4* p = reinterpret_cast<u32x4*>(lds + kKeyBytes) + x;
+            u32x4 w = *p;
+            bool any = false;
+            for (int y = 0; y < 4; ++y) {
+                if constexpr (CT == PKV_F32) {
+                    if ((w[y] & 0x7f800000u) == 0x7f800000u) {
+                        w[y] = 0;
+                        any = true;
                     }
+                } else {
+                    any |= nonfinite2<mat_type(CT)>(w[y]);
+                    w[y] = finite_or_0<mat_type(CT)>(w[y]);
                 }
-                *reinterpret_cast<u32x4*>(lds + value32_at(slot, x % kPieces * 4)) = vf[n];
             }
-        } else {
-            const uint32_t dg = t % 32, piece = t / 32;
-            if (!full)
-                for (int j = 0; j < 8; ++j) {
-                    const bool keep = any(slot_of(piece, j));
-                    for (int w = 0; w < kPer / 2; ++w) {
-                        if (!keep) v[j][w] = 0;
-                        odd |= nonfinite2<MT>(v[j][w]);
-                    }
-                }
-            for (int e = 0; e < kPer; ++e) {
-                const uint32_t sel = e % 2 ? 0x07060302u : 0x05040100u;
-                const u32x4 x = {__builtin_amdgcn_perm(v[1][e / 2], v[0][e / 2], sel),
-                                 __builtin_amdgcn_perm(v[3][e / 2], v[2][e / 2], sel),
-                                 __builtin_amdgcn_perm(v[5][e / 2], v[4][e / 2], sel),
-                                 __builtin_amdgcn_perm(v[7][e / 2], v[6][e / 2], sel)};
-                *reinterpret_cast<u32x4*>(lds + value_at(dg * kPer + e, piece)) = x;
-            }
+            if (any) *p = w;
+            odd |= any;
         }
         return odd;
     }
@@ -713,14 +725,19 @@ constexpr uint32_t kRowTile = 128;   // query rows (rows x group of one KV head)
 // Bound, at head_dim 128, by the softmax's vector instructions beside the
 // matrix instructions (16 exponentials' 16 cycles each per 8 + 8 matrix
 // instructions of 32) -- see the table of measurements.
+//
+// A weight 0 times an infinity or NaN would be NaN in rows that do not see the
+// slot.  The loop does not look for those: an output that is not finite sends
+// the workgroup through it again, with infinities and NaN taken out of the
+// staged values and each added afterwards to the rows that see it.
 template <int CT, int QT, int D>
-__global__ __launch_bounds__(256, (query_terms(CT, QT) * D > 256 ? 1 : 2)) void rows_kernel(AttendDev a, Partial part, uint32_t row_tiles) {
+__global__ __launch_bounds__(256, (query_terms(CT, QT) * D >= 256 ? 1 : 2)) void rows_kernel(AttendDev a, Partial part,
+                                                                                        uint32_t row_tiles) {
+    __shared__ __align__(16) uint8_t lds[2 * Stage<CT, D>::kBytes];
     using T = typename Elem<QT>::T;
     using St = Stage<CT, D>;
     constexpr int MT = mat_type(CT), kU = St::kSlots / 32, kO = D / 32;
     constexpr int NP = CT == PKV_FP4 ? query_terms(CT, QT) : 1;
-    __shared__ __align__(16) uint8_t lds[2][St::kBytes];
-    __shared__ uint32_t s_odd[2][4];
     const uint32_t lane = threadIdx.x % 64, wave = __builtin_amdgcn_readfirstlane(threadIdx.x / 64);
     const uint32_t n = lane % 32, half = lane / 32;
     // heads fastest, so that a head's workgroups share an XCD's L2 where the heads are a multiple of 8; row tiles
@@ -752,117 +769,130 @@ __global__ __launch_bounds__(256, (query_terms(CT, QT) * D > 256 ? 1 : 2)) void 
     const uint8_t *ksp = CT == PKV_FP4 ? a.kv.ks + base / 32 : nullptr;
     const uint8_t *vsp = CT == PKV_FP4 ? a.kv.vs + base / 32 : nullptr;
 
-    float m = -kInf, l = 0.0f;
-    f32x16 o[kO] = {};
+    const uint32_t at = static_cast<uint32_t>(reinterpret_cast<uintptr_t>((LdsByte*)lds));
+    float m, l;
+    f32x16 o[kO];
     St st;
-    auto put = [&](int t) {
-        const int slot = tl.slot(t, St::kSlots);
-        const bool full = all_visible(a, pos0, pos1, slot, slot + St::kSlots - 1);
-        const bool odd = st.store(lds[(t - t0) & 1], full, [&](int j) { return any_visible(a, tl, slot + j); });
-        const bool some = __any(odd);
-        if (lane == 0) s_odd[(t - t0) & 1][wave] = some;
+    auto fetch = [&](int t) {
+        st.fetch(at + ((t - t0) & 1) * St::kBytes, kp, vp, ksp, vsp, a.kv.slot, tl.slot(t, St::kSlots), tl.high - 1);
     };
-    if (t0 < t1) {
-        st.load(kp, vp, ksp, vsp, a.kv.slot, tl.slot(t0, St::kSlots), tl.high - 1);
-        put(t0);
-        if (t0 + 1 < t1) st.load(kp, vp, ksp, vsp, a.kv.slot, tl.slot(t0 + 1, St::kSlots), tl.high - 1);
-    }
-    __syncthreads();
-    for (int t = t0; t < t1; ++t) {
-        const uint8_t* buf = lds[(t - t0) & 1];
-        const uint32_t* odds = s_odd[(t - t0) & 1];
-        const bool odd = (odds[0] | odds[1] | odds[2] | odds[3]) != 0;
-        if (t + 1 < t1) {
-            put(t + 1);
-            if (t + 2 < t1) st.load(kp, vp, ksp, vsp, a.kv.slot, tl.slot(t + 2, St::kSlots), tl.high - 1);
+    // no row of the wave sees any of the tile
+    auto skip = [&](int slot) {
+        return slot >= wt.high || (slot + St::kSlots <= wt.low && static_cast<uint32_t>(slot) >= a.sinks);
+    };
+    for (bool clean = false;; clean = true) {
+        m = -kInf;
+        l = 0.0f;
+        for (int e = 0; e < kO; ++e) o[e] = f32x16{};
+        if (t0 < t1) {
+            fetch(t0);
+            st.land(lds);
         }
-        const int slot = tl.slot(t, St::kSlots), end = slot + St::kSlots - 1;
-        // no row of the wave sees any of it
-        if (slot >= wt.high || (end < wt.low && static_cast<uint32_t>(slot) >= a.sinks)) {
-            __syncthreads();
-            continue;
-        }
-        f32x16 sc[kU];
-        for (int u = 0; u < kU; ++u) sc[u] = logits32<CT, QT, D>(buf, u, q, lane);
-        const bool full = all_visible(a, wpos0, wpos1, slot, end);
-        if (!full)
-            for (int u = 0; u < kU; ++u)
-                for (int x = 0; x < 16; ++x)
-                    if (!visible(a, pos, slot + 32 * u + row32(x, half))) sc[u][x] = -kInf;
-        float top = sc[0][0];
-        for (int u = 0; u < kU; ++u)
-            for (int x = 0; x < 16; ++x) top = fmaxf(top, sc[u][x]);
-        top = fmaxf(top, __shfl_xor(top, 32));
-        const bool grow = m == -kInf ? top > -kInf : (top - m) * a.scale2 > 8.0f;
-        if (__any(grow)) {   // as in decode_kernel
-            const float mn = fmaxf(m, top);
-            const float f = m == -kInf ? 1.0f : exp2f((m - mn) * a.scale2);
-            if (mn > m) {
-                l *= f;
-                for (int e = 0; e < kO; ++e) o[e] *= f;
-                m = mn;
+        __syncthreads();
+        for (int t = t0; t < t1; ++t) {
+            uint8_t* buf = lds + ((t - t0) & 1) * St::kBytes;
+            if (t + 1 < t1) fetch(t + 1);
+            const int slot = tl.slot(t, St::kSlots);
+            if (__builtin_expect(clean, 0)) {
+                St::clean(buf);
+                __syncthreads();
             }
-        }
-        const float mc = m == -kInf ? 0.0f : m * a.scale2;
-        for (int u = 0; u < kU; ++u)
-            for (int x = 0; x < 16; ++x) {
-                sc[u][x] = __builtin_amdgcn_exp2f(__builtin_fmaf(sc[u][x], a.scale2, -mc));
-                l += sc[u][x];
-            }
-        // O^T += V^T P^T, infinities and NaN taken out first if `clean`
-        auto weigh = [&](auto clean) {
-            for (int u = 0; u < kU; ++u) {
-                if constexpr (CT == PKV_F32) {
-                    for (int x = 0; x < 16; ++x)
-                        for (int e = 0; e < kO; ++e) {
-                            float v = *reinterpret_cast<const float*>(
-                                buf + St::value32_at(32 * u + row32(x, half), 32 * e + n));
-                            if (clean && (__float_as_uint(v) & 0x7f800000u) == 0x7f800000u) v = 0.0f;
-                            o[e] = __builtin_amdgcn_mfma_f32_32x32x2f32(v, sc[u][x], o[e], 0, 0, 0);
-                        }
-                } else {
-                    for (int y = 0; y < 2; ++y) {
-                        float p[8];
-                        for (int x = 0; x < 8; ++x) p[x] = sc[u][8 * y + x];
-                        u32x4 pt[NP];
-                        for (int k = 0; k < NP; ++k)
-                            pt[k] = u32x4{pack_term<MT>(p[0], p[1]), pack_term<MT>(p[2], p[3]), pack_term<MT>(p[4], p[5]),
-                                          pack_term<MT>(p[6], p[7])};
-                        for (int e = 0; e < kO; ++e) {
-                            u32x4 v = *reinterpret_cast<const u32x4*>(
-                                buf + St::value_at(32 * e + n, 4 * u + 2 * y + half));
-                            if (clean)
-                                for (int k = 0; k < 4; ++k) v[k] = finite_or_0<MT>(v[k]);
-                            for (int k = NP - 1; k >= 0; --k) o[e] = mma32<MT>(v, pt[k], o[e]);
+            if (!skip(slot)) {
+                f32x16 sc[kU];
+                for (int u = 0; u < kU; ++u) sc[u] = logits32<CT, QT, D>(buf, u, q, lane);
+                if (!all_visible(a, wpos0, wpos1, slot, slot + St::kSlots - 1))
+                    for (int u = 0; u < kU; ++u)
+                        for (int x = 0; x < 16; ++x)
+                            if (!visible(a, pos, slot + 32 * u + row32(x, half))) sc[u][x] = -kInf;
+                float top = sc[0][0];
+                for (int u = 0; u < kU; ++u)
+                    for (int x = 0; x < 16; ++x) top = fmaxf(top, sc[u][x]);
+                top = fmaxf(top, __shfl_xor(top, 32));
+                const bool grow = m == -kInf ? top > -kInf : (top - m) * a.scale2 > 8.0f;
+                if (__any(grow)) {   // as in decode_kernel
+                    const float mn = fmaxf(m, top);
+                    const float f = m == -kInf ? 1.0f : exp2f((m - mn) * a.scale2);
+                    if (mn > m) {
+                        l *= f;
+                        for (int e = 0; e < kO; ++e) o[e] *= f;
+                        m = mn;
+                    }
+                }
+                const float mc = m == -kInf ? 0.0f : m * a.scale2;
+                for (int u = 0; u < kU; ++u)
+                    for (int x = 0; x < 16; ++x) {
+                        sc[u][x] = __builtin_amdgcn_exp2f(__builtin_fmaf(sc[u][x], a.scale2, -mc));
+                        l += sc[u][x];
+                    }
+                for (int u = 0; u < kU; ++u) {
+                    if constexpr (CT == PKV_F32) {
+                        for (int x = 0; x < 16; ++x)
+                            for (int e = 0; e < kO; ++e)
+                                o[e] = __builtin_amdgcn_mfma_f32_32x32x2f32(
+                                    *reinterpret_cast<const float*>(
+                                        buf + St::value32_at(32 * u + row32(x, half), 32 * e + n)),
+                                    sc[u][x], o[e], 0, 0, 0);
+                    } else {
+                        for (int y = 0; y < 2; ++y) {
+                            float p[8];
+                            for (int x = 0; x < 8; ++x) p[x] = sc[u][8 * y + x];
+                            u32x4 pt[NP];
+                            for (int k = 0; k < NP; ++k)
+                                pt[k] = u32x4{pack_term<MT>(p[0], p[1]), pack_term<MT>(p[2], p[3]),
+                                              pack_term<MT>(p[4], p[5]), pack_term<MT>(p[6], p[7])};
+                            for (int e = 0; e < kO; ++e) {
+                                const u32x4 v = St::values16(buf, 32 * u + 16 * y, e, lane);
+                                for (int k = NP - 1; k >= 0; --k) o[e] = mma32<MT>(v, pt[k], o[e]);
+                            }
                         }
                     }
                 }
             }
-        };
-        if (__builtin_expect(odd && !full, 0)) {
-            // infinities or NaN among the values, in slots that some of the
-            // wave's rows do not see: the products without them, then each of
-            // them to the rows that do
-            weigh(std::true_type{});
+            if (t + 1 < t1) st.land(lds + ((t + 1 - t0) & 1) * St::kBytes);
+            __syncthreads();
+        }
+        if (!clean) {
+            bool odd = false;
+            for (int e = 0; e < kO; ++e)
+                for (int x = 0; x < 16; ++x) odd |= (__float_as_uint(o[e][x]) & 0x7f800000u) == 0x7f800000u;
+            if (!__syncthreads_or(odd && real)) break;
+            continue;
+        }
+        const float mc = m == -kInf ? 0.0f : m * a.scale2;
+#pragma unroll 1
+        for (int t = t0; t < t1; ++t) {
+            const int slot = tl.slot(t, St::kSlots);
+            uint8_t* buf = lds + ((t - t0) & 1) * St::kBytes;
+            fetch(t);
+            st.land(buf);
+            __syncthreads();
+            if (!__syncthreads_or(St::clean(buf))) continue;
+            fetch(t);
+            st.land(buf);
+            __syncthreads();
 #pragma unroll 1
             for (int j = 0; j < St::kSlots; ++j) {
-                // register and half that hold slot j's weights
-                const int reg = j % 32 / 8 * 4 + j % 4 + 16 * (j / 32), side = j / 4 % 2;
-                float p = 0.0f;
-                for (int u = 0; u < kU; ++u)
-                    for (int x = 0; x < 16; ++x) p = reg == 16 * u + x ? sc[u][x] : p;
-                p = __shfl(p, static_cast<int>(n) + 32 * side);
                 const bool sees = visible(a, pos, slot + j);
+                if (!__any(sees)) continue;
+                uint32_t hf = half;
+                asm volatile("" : "+v"(hf));   // this rare loop's addresses are not kept over the main one
+                float dot = 0.0f;
+                for (int x = 0; x < Query<CT, QT, D>::kRegs; ++x) {
+                    const u32x4 k = *reinterpret_cast<const u32x4*>(buf + St::key_at(j, 2 * x + hf));
+                    for (int w = 0; w < 4; ++w)
+                        for (int y = 0; y < Query<CT, QT, D>::kTerms; ++y) dot += dot_word<MT>(k[w], q.q[y][x][w]);
+                }
+                dot += __shfl_xor(dot, 32);
+                const float p = __builtin_amdgcn_exp2f(__builtin_fmaf(dot, a.scale2, -mc));
                 for (int e = 0; e < kO; ++e)
                     for (int x = 0; x < 16; ++x) {
-                        const float v = St::value(buf, j, 32 * e + row32(x, half));
+                        const float v = St::value(buf, j, 32 * e + row32(x, hf));
                         if (sees && (__float_as_uint(v) & 0x7f800000u) == 0x7f800000u) o[e][x] += p * v;
                     }
             }
-        } else {
-            weigh(std::false_type{});
+            __syncthreads();
         }
-        __syncthreads();
+        break;
     }
     l += __shfl_xor(l, 32);
     if (!real) return;
@@ -898,6 +928,7 @@ __global__ __launch_bounds__(256, (query_terms(CT, QT) * D > 256 ? 1 : 2)) void 
             a.stats[2 * (ch * all + r) + 1] = inv;
         }
     }
+    return;
 }
 
 // Accumulated weights of many rows: 32 slots a wave, its keys held in registers
