@@ -431,7 +431,7 @@ __global__ __launch_bounds__(256, 2) void decode_kernel(AttendDev a, Partial par
 // The splits of a row joined: largest logit and the sum under it.
 __device__ inline void join_splits(const float* ml, uint32_t splits, uint32_t rows, float scale2, uint32_t lane,
                                    float* mu, float* sum) {
-    const uint32_t step = 2 * rows;
+    const uint64_t step = 2ull * rows;
     float top = -kInf;
     for (uint32_t s = lane; s < splits; s += 64) top = fmaxf(top, ml[step * s]);
     for (int x = 32; x; x >>= 1) top = fmaxf(top, __shfl_xor(top, x));
@@ -445,38 +445,51 @@ __device__ inline void join_splits(const float* ml, uint32_t splits, uint32_t ro
     *mu = top == -kInf ? 0.0f : top;
 }
 
-// The splits' shares joined, a wave a row; then, with weights, a wave's rows
-// of softmax statistics against the stored logits, four slots a thread.
-// blockIdx.x < outs: 4 rows of all copies x heads x rows; else 1,024 slots.
+// The splits' shares joined, a workgroup a row: every wave the row's largest
+// logit and sum, then 1024 / D shares at a time, 4 channels a thread.  With
+// weights of few rows, then, a workgroup's rows of softmax statistics against
+// the stored logits, four slots a thread.  blockIdx.x < outs: rows of all
+// copies x heads; else 1,024 slots.
 template <int QT, int D>
 __global__ __launch_bounds__(256) void join_kernel(AttendDev a, Partial part, uint32_t outs) {
     using T = typename Elem<QT>::T;
     const uint32_t lane = threadIdx.x % 64, wave = threadIdx.x / 64, all = a.nq * a.group;
     if (blockIdx.x < outs) {
-        const uint32_t x = blockIdx.x * 4 + wave;
-        if (x >= a.copies * a.heads * all) return;
-        const uint32_t r = x % all, ch = x / all, c = ch / a.heads, h = ch % a.heads, i = r / a.group, g = r % a.group;
+        const uint32_t r = blockIdx.x % all, ch = blockIdx.x / all, c = ch / a.heads, h = ch % a.heads;
+        const uint32_t i = r / a.group, g = r % a.group;
         if (static_cast<int>(i) >= span(a, c).rows) return;
         const uint64_t at = static_cast<uint64_t>(ch) * part.splits * part.rows + r;
+        constexpr uint32_t kLanes = D / 4, kShares = 256 / kLanes;
+        const uint32_t first = threadIdx.x / kLanes, d = threadIdx.x % kLanes * 4;
         float mu, sum;
         join_splits(part.ml + 2 * at, part.splits, part.rows, a.scale2, lane, &mu, &sum);
-        float o[D / 64] = {};
-        for (uint32_t s = 0; s < part.splits; ++s) {
-            const float ms = part.ml[2 * (at + static_cast<uint64_t>(part.rows) * s)];
-            const float f = ms == -kInf ? 0.0f : ms == mu ? 1.0f : exp2f((ms - mu) * a.scale2);
-            if (f == 0.0f) continue;
-            const float* p = part.o + (at + static_cast<uint64_t>(part.rows) * s) * D + lane * (D / 64);
-            for (int e = 0; e < D / 64; ++e) o[e] += p[e] * f;
+        f32x4 o = {};
+        for (uint32_t s = first; s < part.splits; s += kShares) {
+            const uint64_t x = at + static_cast<uint64_t>(part.rows) * s;
+            const float ms = part.ml[2 * x];
+            const f32x4 p = *reinterpret_cast<const f32x4*>(part.o + x * D + d);
+            const float f = ms == mu ? 1.0f : exp2f((ms - mu) * a.scale2);
+            if (ms != -kInf) o += p * f;
         }
-        T* out = reinterpret_cast<T*>(a.out) + c * a.o_copy + i * a.o_row + (h * a.group + g) * a.o_head;
-        for (int e = 0; e < D / 64; ++e)
-            out[lane * (D / 64) + e] = static_cast<T>(sum == 0.0f ? 0.0f : o[e] / sum);
-        if (a.lse && lane == 0)
-            a.lse[(static_cast<uint64_t>(c) * a.heads * a.group + h * a.group + g) * a.nq + i] =
-                sum == 0.0f ? -kInf : (mu * a.scale2 + log2f(sum)) * kLn2;
-        if (a.stats && lane == 0) {
-            a.stats[2 * (static_cast<uint64_t>(ch) * all + r)] = -mu * a.scale2;
-            a.stats[2 * (static_cast<uint64_t>(ch) * all + r) + 1] = sum == 0.0f ? 0.0f : 1.0f / sum;
+        __shared__ f32x4 so[256];
+        so[threadIdx.x] = o;
+        __syncthreads();
+        if (first == 0) {
+            for (uint32_t s = 1; s < kShares; ++s) o += so[threadIdx.x + s * kLanes];
+            T* out = reinterpret_cast<T*>(a.out) + c * a.o_copy + i * a.o_row + (h * a.group + g) * a.o_head;
+            typedef T T4 __attribute__((ext_vector_type(4)));
+            T4 y;
+            for (int e = 0; e < 4; ++e) y[e] = static_cast<T>(sum == 0.0f ? 0.0f : o[e] / sum);
+            *reinterpret_cast<T4*>(out + d) = y;
+        }
+        if (threadIdx.x == 0) {
+            if (a.lse)
+                a.lse[(static_cast<uint64_t>(c) * a.heads * a.group + h * a.group + g) * a.nq + i] =
+                    sum == 0.0f ? -kInf : (mu * a.scale2 + log2f(sum)) * kLn2;
+            if (a.stats) {
+                a.stats[2 * (static_cast<uint64_t>(ch) * all + r)] = -mu * a.scale2;
+                a.stats[2 * (static_cast<uint64_t>(ch) * all + r) + 1] = sum == 0.0f ? 0.0f : 1.0f / sum;
+            }
         }
         return;
     }
@@ -561,6 +574,14 @@ __device__ inline void copy_to_lds(uint32_t to, const uint8_t* from, uint32_t of
     asm volatile("s_mov_b32 %0, m0\n\ts_mov_b32 m0, %1\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %2, %3\n\ts_mov_b32 m0, %0"
                  : "=&s"(m0)
                  : "s"(to), "v"(offset), "s"(from)
+                 : "memory");
+}
+// The same from an address of each lane's own.
+__device__ inline void copy_row_to_lds(uint32_t to, const uint8_t* from) {
+    uint32_t m0;
+    asm volatile("s_mov_b32 %0, m0\n\ts_mov_b32 m0, %1\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %2, off\n\ts_mov_b32 m0, %0"
+                 : "=&s"(m0)
+                 : "s"(to), "v"(from)
                  : "memory");
 }
 __device__ inline void copies_done() { asm volatile("s_waitcnt vmcnt(0)" ::: "memory"); }
@@ -932,18 +953,21 @@ __global__ __launch_bounds__(256, (query_terms(CT, QT) * D >= 256 ? 1 : 2)) void
 }
 
 // Accumulated weights of many rows: 32 slots a wave, its keys held in registers
-// as the S^T operand, all rows that can see them streamed through LDS 32 at a
-// time (four waves share them); every slot belongs to one wave, so sums have
-// one order.  S^T, one multiply-add and one exponential a logit: half of
-// rows_kernel's matrix work, its softmax work without maximum and rounding.
+// as the S^T operand, all rows that can see them streamed through LDS (four
+// waves share them) 64 at a time (queries of more than one term: 32), straight
+// from memory while the rows before are worked on; every slot belongs to one
+// wave, so sums have one order.  S^T, one multiply-add, one exponential and one
+// more multiply-add a logit: half of rows_kernel's matrix work, its softmax
+// work without maximum and rounding.
 template <int CT, int QT, int D>
 __global__ __launch_bounds__(256, 2) void weights_kernel(AttendDev a) {
     using T = typename Elem<QT>::T;
     using Q = Query<CT, QT, D>;
-    constexpr int MT = mat_type(CT), kPieces = CT == PKV_F32 ? D / 4 : D / 8, kTerms = Q::kTerms;
-    constexpr uint32_t kTermBytes = 32 * kPieces * 16;
+    using St = Stage<CT, D>;
+    constexpr int MT = mat_type(CT), kPieces = St::kPieces, kTerms = Q::kTerms;
+    constexpr int kRows = kTerms == 1 ? 64 : 32, kU = kRows / 32;
+    constexpr uint32_t kTermBytes = kRows * St::kRow;
     __shared__ __align__(16) uint8_t lds[2][kTerms * kTermBytes];
-    __shared__ float s_stat[2][32][2];
     const uint32_t lane = threadIdx.x % 64, wave = __builtin_amdgcn_readfirstlane(threadIdx.x / 64);
     const uint32_t n = lane % 32, half = lane / 32, heads = a.copies * a.heads;
     const uint32_t ch = blockIdx.x % heads, c = ch / a.heads, h = ch % a.heads;
@@ -976,69 +1000,129 @@ __global__ __launch_bounds__(256, 2) void weights_kernel(AttendDev a) {
     }
     const uint64_t all = static_cast<uint64_t>(a.nq) * a.group;
     const T* qp = reinterpret_cast<const T*>(a.q) + c * a.q_copy + static_cast<uint64_t>(h) * a.group * a.q_head;
-    auto stage = [&](int r, uint32_t b) {
-        for (uint32_t x = threadIdx.x; x < 32 * kPieces; x += 256) {
-            const int row = min(r + static_cast<int>(x / kPieces), r1 - 1);
-            const uint32_t piece = x % kPieces;
-            const T* p = qp + static_cast<uint64_t>(row / G) * a.q_row + static_cast<uint64_t>(row % G) * a.q_head;
-            const uint32_t at = (x / kPieces * kPieces + (piece ^ (x / kPieces % (kPieces < 16 ? kPieces : 16)))) * 16;
-            if constexpr (kTerms == 1) {
-                *reinterpret_cast<u32x4*>(lds[b] + at) = reinterpret_cast<const u32x4*>(p)[piece];
-            } else {
-                u32x4 w[kTerms];
-                for (int y = 0; y < 4; ++y) {
-                    float f0 = static_cast<float>(p[8 * piece + 2 * y]), f1 = static_cast<float>(p[8 * piece + 2 * y + 1]);
-                    for (int z = 0; z < kTerms; ++z) w[z][y] = pack_term<PKV_BF16>(f0, f1);
-                }
-                for (int z = 0; z < kTerms; ++z) *reinterpret_cast<u32x4*>(lds[b] + z * kTermBytes + at) = w[z];
-            }
+    const uint32_t at = static_cast<uint32_t>(reinterpret_cast<uintptr_t>((LdsByte*)&lds[0][0]));
+    // Row that this thread fetches a piece of, as (row, head of the group); steps of rows without dividing again.
+    struct At {
+        int i, g;
+    };
+    auto step = [&](At x, int rows_i, int rows_g) {
+        x.i += rows_i;
+        x.g += rows_g;
+        if (x.g >= G) {
+            x.g -= G;
+            ++x.i;
         }
-        if (threadIdx.x < 32) {
-            const bool in = r + static_cast<int>(threadIdx.x) < r1;
-            const float* st = a.stats + 2 * (ch * all + min(r + static_cast<int>(threadIdx.x), r1 - 1));
-            s_stat[b][threadIdx.x][0] = st[0];
-            s_stat[b][threadIdx.x][1] = in ? st[1] : 0.0f;
+        return x;
+    };
+    constexpr int kCopies = kRows * St::kRow / 4096, kStep = St::kCopyStep;
+    const uint32_t mine = kTerms == 1 ? St::kCopyRows * wave + lane / kPieces : threadIdx.x / kPieces;
+    constexpr int kMoves = kTerms == 1 ? kCopies : kRows * kPieces / 256, kMoveStep = kTerms == 1 ? kStep : 256 / kPieces;
+    At here[kMoves];
+    for (int x = 0; x < kMoves; ++x) {
+        const int row = static_cast<int>(mine) + kMoveStep * x;
+        here[x] = At{i0 + row / G, row % G};
+    }
+    const int adv_i = kRows / G, adv_g = kRows % G;
+    u32x4 w[kTerms == 1 ? 1 : kMoves];      // a multi-term query on its way (f16: 8 values; f32: the first half)
+    u32x4 w2[QT == PKV_F32 && kTerms > 1 ? kMoves : 1];
+    auto fetch = [&](uint32_t b) {
+        const uint32_t piece = (kTerms == 1 ? lane : threadIdx.x) % kPieces;
+        for (int x = 0; x < kMoves; ++x) {
+            const At r = here[x].i <= i1 ? here[x] : At{i1, G - 1};
+            const T* p = qp + static_cast<uint64_t>(r.i) * a.q_row + static_cast<uint64_t>(r.g) * a.q_head;
+            if constexpr (kTerms == 1) {
+                const uint32_t row = mine + kStep * x;
+                copy_row_to_lds(at + b * kTermBytes + (kStep * x + St::kCopyRows * wave) * St::kRow,
+                                reinterpret_cast<const uint8_t*>(p) + (piece ^ St::turn(row, false)) * 16);
+            } else {
+                w[x] = reinterpret_cast<const u32x4*>(p + 8 * piece)[0];
+                if constexpr (QT == PKV_F32) w2[x] = reinterpret_cast<const u32x4*>(p + 8 * piece)[1];
+            }
+            here[x] = step(here[x], adv_i, adv_g);
         }
     };
-    float w[16] = {};
-    stage(r0, 0);
+    auto land = [&](uint32_t b) {
+        if constexpr (kTerms == 1) {
+            copies_done();
+        } else {
+            for (int x = 0; x < kMoves; ++x) {
+                const uint32_t row = mine + kMoveStep * x, to = St::key_at(row, threadIdx.x % kPieces);
+                u32x4 y[kTerms];
+                for (int e = 0; e < 4; ++e) {
+                    float f0, f1;
+                    if constexpr (QT == PKV_F32) {
+                        f0 = __uint_as_float(e < 2 ? w[x][2 * e] : w2[x][2 * e - 4]);
+                        f1 = __uint_as_float(e < 2 ? w[x][2 * e + 1] : w2[x][2 * e - 3]);
+                    } else {
+                        const uint32_t word = w[x][e];   // not bit_cast of the element itself: that reads element 0
+                        const f16x2 f = __builtin_bit_cast(f16x2, word);
+                        f0 = static_cast<float>(f[0]);
+                        f1 = static_cast<float>(f[1]);
+                    }
+                    for (int z = 0; z < kTerms; ++z) y[z][e] = pack_term<PKV_BF16>(f0, f1);
+                }
+                for (int z = 0; z < kTerms; ++z) *reinterpret_cast<u32x4*>(lds[b] + z * kTermBytes + to) = y[z];
+            }
+        }
+    };
+    float sum[16] = {};
+    typedef float f32x2u __attribute__((ext_vector_type(2)));
+    const f32x2u* stats = reinterpret_cast<const f32x2u*>(a.stats) + ch * all;
+    f32x2u next[kU], now[kU];
+    fetch(0);
+    for (int u = 0; u < kU; ++u) next[u] = stats[min(r0 + 32 * u + static_cast<int>(n), r1 - 1)];
+    land(0);
     __syncthreads();
     uint32_t b = 0;
-    for (int r = r0; r < r1; r += 32, b ^= 1) {
-        if (r + 32 < r1) stage(r + 32, b ^ 1);
-        f32x16 s = {};
-        for (int x = 0; x < Q::kRegs; ++x)
-            for (int z = kTerms - 1; z >= 0; --z) {
-                const uint32_t piece = 2 * x + half;
-                const u32x4 y = *reinterpret_cast<const u32x4*>(
-                    lds[b] + z * kTermBytes + (n * kPieces + (piece ^ (n % (kPieces < 16 ? kPieces : 16)))) * 16);
-                if constexpr (CT == PKV_F32) {
-                    for (int e = 0; e < 4; ++e)
-                        s = __builtin_amdgcn_mfma_f32_32x32x2f32(__uint_as_float(k[x][e]), __uint_as_float(y[e]), s, 0, 0, 0);
-                } else {
-                    s = mma32<MT>(k[x], y, s);
-                }
-            }
-        const float mc = s_stat[b][n][0], inv = s_stat[b][n][1];
-        const int pos = sp.first + (r + static_cast<int>(n)) / G;
-        if (all_visible(a, sp.first + r / G, sp.first + min(r + 31, r1 - 1) / G, s0, s0 + 31) && r + 32 <= r1) {
-            for (int x = 0; x < 16; ++x)
-                w[x] = __builtin_fmaf(__builtin_amdgcn_exp2f(__builtin_fmaf(s[x], a.scale2, mc)), inv, w[x]);
-        } else {
-            for (int x = 0; x < 16; ++x)
-                if (r + static_cast<int>(n) < r1 && inv != 0.0f && visible(a, pos, s0 + row32(x, half)))
-                    w[x] = __builtin_fmaf(__builtin_amdgcn_exp2f(__builtin_fmaf(s[x], a.scale2, mc)), inv, w[x]);
+    At top = {i0, 0};                        // of row r
+    for (int r = r0; r < r1; r += kRows, b ^= 1) {
+        for (int u = 0; u < kU; ++u) now[u] = next[u];
+        if (r + kRows < r1) {
+            fetch(b ^ 1);
+            for (int u = 0; u < kU; ++u) next[u] = stats[min(r + kRows + 32 * u + static_cast<int>(n), r1 - 1)];
         }
+        for (int u = 0; u < kU; ++u) {
+            const int ru = r + 32 * u;
+            if (ru >= r1) break;
+            f32x16 s = {};
+            for (int x = 0; x < Q::kRegs; ++x)
+                for (int z = kTerms - 1; z >= 0; --z) {
+                    const u32x4 y = *reinterpret_cast<const u32x4*>(lds[b] + z * kTermBytes +
+                                                                    St::key_at(32 * u + n, 2 * x + half));
+                    if constexpr (CT == PKV_F32) {
+                        for (int e = 0; e < 4; ++e)
+                            s = __builtin_amdgcn_mfma_f32_32x32x2f32(__uint_as_float(k[x][e]), __uint_as_float(y[e]), s,
+                                                                     0, 0, 0);
+                    } else {
+                        s = mma32<MT>(k[x], y, s);
+                    }
+                }
+            const float mc = now[u][0], inv = now[u][1];
+            // positions of the piece's rows, from above (the last one's a little late)
+            const int pa = sp.first + top.i + (kU > 1 && u ? 32 / G : 0), pb = sp.first + top.i + (32 * u + 31 + G) / G;
+            if (ru + 32 <= r1 && all_visible(a, pa, pb, s0, s0 + 31)) {
+                for (int x = 0; x < 16; ++x)
+                    sum[x] = __builtin_fmaf(__builtin_amdgcn_exp2f(__builtin_fmaf(s[x], a.scale2, mc)), inv, sum[x]);
+            } else {
+                const int pos = sp.first + (ru + static_cast<int>(n)) / G;
+                const bool in = ru + static_cast<int>(n) < r1 && inv != 0.0f;
+                for (int x = 0; x < 16; ++x)
+                    if (in && visible(a, pos, s0 + row32(x, half)))
+                        sum[x] = __builtin_fmaf(__builtin_amdgcn_exp2f(__builtin_fmaf(s[x], a.scale2, mc)), inv, sum[x]);
+            }
+        }
+        top = step(top, adv_i, adv_g);
+        if (r + kRows < r1) land(b ^ 1);
         __syncthreads();
     }
-    for (int x = 0; x < 16; ++x)
-        for (int y = 16; y; y >>= 1) w[x] += __shfl_xor(w[x], y);
-    float* out = a.weights + c * a.w_copy + h * a.w_head;
+    float total = 0.0f;                      // lane n < 16 of a half: register n's slot
     for (int x = 0; x < 16; ++x) {
-        const int j = s0 + row32(x, half);
-        if (n == 0 && j < high && (!a.window || j >= sp.first - static_cast<int64_t>(a.window) + 1 || static_cast<uint32_t>(j) < a.sinks))
-            out[j] += w[x];
+        for (int y = 16; y; y >>= 1) sum[x] += __shfl_xor(sum[x], y);
+        total = n == static_cast<uint32_t>(x) ? sum[x] : total;
     }
+    const int j = s0 + row32(static_cast<int>(n), half);
+    if (n < 16 && j < high && (!a.window || j >= sp.first - static_cast<int64_t>(a.window) + 1 || static_cast<uint32_t>(j) < a.sinks))
+        a.weights[c * a.w_copy + h * a.w_head + j] += total;
 }
 
 // ------------------------------------------------------------ the 4-bit cache
@@ -1312,7 +1396,7 @@ int attend_typed(AttendDev a, uint8_t* ws, hipStream_t st) {
     const Plan p = plan_of(a, D, CT);
     const Partial part{reinterpret_cast<float*>(ws), reinterpret_cast<float*>(ws + p.ml),
                        reinterpret_cast<float*>(ws + p.logits), p.splits, p.ld, p.rows};
-    const uint32_t heads = a.copies * a.heads, outs = (heads * a.nq * a.group + 3) / 4;
+    const uint32_t heads = a.copies * a.heads, outs = heads * a.nq * a.group;
     if (a.nq * a.group <= kDecodeRows) {
         if (a.weights) decode_kernel<CT, QT, D, true><<<heads * p.splits, 256, 0, st>>>(a, part);
         else decode_kernel<CT, QT, D, false><<<heads * p.splits, 256, 0, st>>>(a, part);
