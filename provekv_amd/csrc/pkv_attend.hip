@@ -52,6 +52,19 @@ __device__ inline bool visible(const AttendDev& a, int pos, int j) {
     return j <= pos && (!a.window || static_cast<uint32_t>(pos - j) < a.window || static_cast<uint32_t>(j) < a.sinks);
 }
 
+// x combined with the lane 32 or 16 away, by lane swaps (a shuffle goes through LDS).
+template <class F>
+__device__ inline float across32(float x, F f) {
+    const auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+    return f(__uint_as_float(r[0]), __uint_as_float(r[1]));
+}
+template <class F>
+__device__ inline float across16(float x, F f) {
+    const auto r = __builtin_amdgcn_permlane16_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+    return f(__uint_as_float(r[0]), __uint_as_float(r[1]));
+}
+__device__ inline float larger(float a, float b) { return fmaxf(a, b); }
+
 __device__ inline float wave_sum(float x) {
     for (int o = 32; o; o >>= 1) x += __shfl_xor(x, o);
     return x;
@@ -332,8 +345,7 @@ __global__ __launch_bounds__(256, 2) void decode_kernel(AttendDev a, Partial par
         float top = fmaxf(fmaxf(sc[0][0], sc[0][1]), fmaxf(sc[0][2], sc[0][3]));
         for (int u = 1; u < kSub; ++u)
             top = fmaxf(top, fmaxf(fmaxf(sc[u][0], sc[u][1]), fmaxf(sc[u][2], sc[u][3])));
-        top = fmaxf(top, __shfl_xor(top, 16));
-        top = fmaxf(top, __shfl_xor(top, 32));
+        top = across32(across16(top, larger), larger);
         const bool grow = m == -kInf ? top > -kInf : (top - m) * a.scale2 > 8.0f;
         if (__any(grow)) {
             const float mn = fmaxf(m, top);
@@ -450,6 +462,8 @@ __device__ inline void join_splits(const float* ml, uint32_t splits, uint32_t ro
 // weights of few rows, then, a workgroup's rows of softmax statistics against
 // the stored logits, four slots a thread.  blockIdx.x < outs: rows of all
 // copies x heads; else 1,024 slots.
+//
+// (Many rows have at most 16 shares and are joined by join_rows_kernel.)
 template <int QT, int D>
 __global__ __launch_bounds__(256) void join_kernel(AttendDev a, Partial part, uint32_t outs) {
     using T = typename Elem<QT>::T;
@@ -482,15 +496,9 @@ __global__ __launch_bounds__(256) void join_kernel(AttendDev a, Partial part, ui
             for (int e = 0; e < 4; ++e) y[e] = static_cast<T>(sum == 0.0f ? 0.0f : o[e] / sum);
             *reinterpret_cast<T4*>(out + d) = y;
         }
-        if (threadIdx.x == 0) {
-            if (a.lse)
-                a.lse[(static_cast<uint64_t>(c) * a.heads * a.group + h * a.group + g) * a.nq + i] =
-                    sum == 0.0f ? -kInf : (mu * a.scale2 + log2f(sum)) * kLn2;
-            if (a.stats) {
-                a.stats[2 * (static_cast<uint64_t>(ch) * all + r)] = -mu * a.scale2;
-                a.stats[2 * (static_cast<uint64_t>(ch) * all + r) + 1] = sum == 0.0f ? 0.0f : 1.0f / sum;
-            }
-        }
+        if (a.lse && threadIdx.x == 0)
+            a.lse[(static_cast<uint64_t>(c) * a.heads * a.group + h * a.group + g) * a.nq + i] =
+                sum == 0.0f ? -kInf : (mu * a.scale2 + log2f(sum)) * kLn2;
         return;
     }
     const uint32_t chunks = (a.max_len + 1023) / 1024;
@@ -828,7 +836,7 @@ __global__ __launch_bounds__(256, (query_terms(CT, QT) * D >= 256 ? 1 : 2)) void
                 float top = sc[0][0];
                 for (int u = 0; u < kU; ++u)
                     for (int x = 0; x < 16; ++x) top = fmaxf(top, sc[u][x]);
-                top = fmaxf(top, __shfl_xor(top, 32));
+                top = across32(top, larger);
                 const bool grow = m == -kInf ? top > -kInf : (top - m) * a.scale2 > 8.0f;
                 if (__any(grow)) {   // as in decode_kernel
                     const float mn = fmaxf(m, top);
@@ -952,6 +960,42 @@ __global__ __launch_bounds__(256, (query_terms(CT, QT) * D >= 256 ? 1 : 2)) void
     return;
 }
 
+// rows_kernel's shares joined: D / 4 lanes a row.
+template <int QT, int D>
+__global__ __launch_bounds__(256) void join_rows_kernel(AttendDev a, Partial part) {
+    using T = typename Elem<QT>::T;
+    typedef T T4 __attribute__((ext_vector_type(4)));
+    constexpr uint32_t kLanes = D / 4, kRows = 256 / kLanes;
+    const uint32_t all = a.nq * a.group, blocks = (all + kRows - 1) / kRows, ch = blockIdx.x / blocks;
+    const uint32_t r = blockIdx.x % blocks * kRows + threadIdx.x / kLanes, d = threadIdx.x % kLanes * 4;
+    const uint32_t c = ch / a.heads, h = ch % a.heads, i = r / a.group, g = r % a.group;
+    if (static_cast<int>(i) >= span(a, c).rows || r >= all) return;
+    const uint64_t at = static_cast<uint64_t>(ch) * part.splits * part.rows + r;
+    float top = -kInf, sum = 0.0f;
+    for (uint32_t s = 0; s < part.splits; ++s) top = fmaxf(top, part.ml[2 * (at + static_cast<uint64_t>(part.rows) * s)]);
+    const float mu = top == -kInf ? 0.0f : top;
+    f32x4 o = {};
+    for (uint32_t s = 0; s < part.splits; ++s) {
+        const uint64_t x = at + static_cast<uint64_t>(part.rows) * s;
+        const f32x4 p = *reinterpret_cast<const f32x4*>(part.o + x * D + d);
+        const float ms = part.ml[2 * x], f = ms == top || ms == -kInf ? 1.0f : exp2f((ms - mu) * a.scale2);
+        sum += part.ml[2 * x + 1] * f;       // without a largest logit: 0, or NaN from NaN logits
+        if (ms != -kInf) o += p * f;
+    }
+    T4 y;
+    for (int e = 0; e < 4; ++e) y[e] = static_cast<T>(sum == 0.0f ? 0.0f : o[e] / sum);
+    *reinterpret_cast<T4*>(reinterpret_cast<T*>(a.out) + c * a.o_copy + i * a.o_row + (h * a.group + g) * a.o_head + d) = y;
+    if (d == 0) {
+        if (a.lse)
+            a.lse[(static_cast<uint64_t>(c) * a.heads * a.group + h * a.group + g) * a.nq + i] =
+                sum == 0.0f ? -kInf : (mu * a.scale2 + log2f(sum)) * kLn2;
+        if (a.stats) {
+            a.stats[2 * (static_cast<uint64_t>(ch) * all + r)] = -mu * a.scale2;
+            a.stats[2 * (static_cast<uint64_t>(ch) * all + r) + 1] = sum == 0.0f ? 0.0f : 1.0f / sum;
+        }
+    }
+}
+
 // Accumulated weights of many rows: 32 slots a wave, its keys held in registers
 // as the S^T operand, all rows that can see them streamed through LDS (four
 // waves share them) 64 at a time (queries of more than one term: 32), straight
@@ -959,8 +1003,15 @@ __global__ __launch_bounds__(256, (query_terms(CT, QT) * D >= 256 ? 1 : 2)) void
 // wave, so sums have one order.  S^T, one multiply-add, one exponential and one
 // more multiply-add a logit: half of rows_kernel's matrix work, its softmax
 // work without maximum and rounding.
+//
+// With few blocks of slots their rows are cut into shares as well (splits > 1),
+// whose sums go to `shares` [split][copy][kv head][ld] for add_weights_kernel.
+struct Shares {
+    float* sums;
+    uint32_t splits, ld;
+};
 template <int CT, int QT, int D>
-__global__ __launch_bounds__(256, 2) void weights_kernel(AttendDev a) {
+__global__ __launch_bounds__(256, 2) void weights_kernel(AttendDev a, Shares shares) {
     using T = typename Elem<QT>::T;
     using Q = Query<CT, QT, D>;
     using St = Stage<CT, D>;
@@ -971,8 +1022,10 @@ __global__ __launch_bounds__(256, 2) void weights_kernel(AttendDev a) {
     const uint32_t lane = threadIdx.x % 64, wave = __builtin_amdgcn_readfirstlane(threadIdx.x / 64);
     const uint32_t n = lane % 32, half = lane / 32, heads = a.copies * a.heads;
     const uint32_t ch = blockIdx.x % heads, c = ch / a.heads, h = ch % a.heads;
+    const uint32_t split = blockIdx.x / heads % shares.splits;
     const Span sp = span(a, c);
-    const int G = static_cast<int>(a.group), b0 = static_cast<int>(blockIdx.x / heads) * 128, s0 = b0 + 32 * static_cast<int>(wave);
+    const int G = static_cast<int>(a.group), b0 = static_cast<int>(blockIdx.x / heads / shares.splits) * 128;
+    const int s0 = b0 + 32 * static_cast<int>(wave);
     const int high = sp.first + sp.rows;                 // slots below it are seen by the last row or hidden by its window
     if (b0 >= high || sp.rows == 0) return;
     // rows i0 .. i1 see something of b0 .. b0 + 127
@@ -982,7 +1035,8 @@ __global__ __launch_bounds__(256, 2) void weights_kernel(AttendDev a) {
                               : static_cast<int64_t>(b0) + 126 + a.window - sp.first;
     const int i1 = static_cast<int>(min(reach, static_cast<int64_t>(sp.rows - 1)));
     if (i0 > i1) return;
-    const int r0 = i0 * G, r1 = i1 * G + G;
+    const int per = ((i1 - i0 + 1) * G + kRows * static_cast<int>(shares.splits) - 1) / (kRows * static_cast<int>(shares.splits)) * kRows;
+    const int r0 = i0 * G + static_cast<int>(split) * per, r1 = min(r0 + per, i1 * G + G);   // may be none
 
     // the wave's keys as operand A: slot n, channels as Query
     u32x4 k[Q::kRegs];
@@ -1020,7 +1074,7 @@ __global__ __launch_bounds__(256, 2) void weights_kernel(AttendDev a) {
     At here[kMoves];
     for (int x = 0; x < kMoves; ++x) {
         const int row = static_cast<int>(mine) + kMoveStep * x;
-        here[x] = At{i0 + row / G, row % G};
+        here[x] = At{(r0 + row) / G, (r0 + row) % G};
     }
     const int adv_i = kRows / G, adv_g = kRows % G;
     u32x4 w[kTerms == 1 ? 1 : kMoves];      // a multi-term query on its way (f16: 8 values; f32: the first half)
@@ -1069,12 +1123,14 @@ __global__ __launch_bounds__(256, 2) void weights_kernel(AttendDev a) {
     typedef float f32x2u __attribute__((ext_vector_type(2)));
     const f32x2u* stats = reinterpret_cast<const f32x2u*>(a.stats) + ch * all;
     f32x2u next[kU], now[kU];
-    fetch(0);
-    for (int u = 0; u < kU; ++u) next[u] = stats[min(r0 + 32 * u + static_cast<int>(n), r1 - 1)];
-    land(0);
+    if (r0 < r1) {
+        fetch(0);
+        for (int u = 0; u < kU; ++u) next[u] = stats[min(r0 + 32 * u + static_cast<int>(n), r1 - 1)];
+        land(0);
+    }
     __syncthreads();
     uint32_t b = 0;
-    At top = {i0, 0};                        // of row r
+    At top = {r0 / G, r0 % G};               // of row r
     for (int r = r0; r < r1; r += kRows, b ^= 1) {
         for (int u = 0; u < kU; ++u) now[u] = next[u];
         if (r + kRows < r1) {
@@ -1121,8 +1177,20 @@ __global__ __launch_bounds__(256, 2) void weights_kernel(AttendDev a) {
         total = n == static_cast<uint32_t>(x) ? sum[x] : total;
     }
     const int j = s0 + row32(static_cast<int>(n), half);
-    if (n < 16 && j < high && (!a.window || j >= sp.first - static_cast<int64_t>(a.window) + 1 || static_cast<uint32_t>(j) < a.sinks))
-        a.weights[c * a.w_copy + h * a.w_head + j] += total;
+    if (n >= 16 || !any_visible(a, tiles_of(a, sp.first, high - 1, 1), j)) return;
+    if (shares.splits == 1) a.weights[c * a.w_copy + h * a.w_head + j] += total;
+    else shares.sums[(static_cast<uint64_t>(split) * heads + ch) * shares.ld + j] = total;
+}
+
+// The shares of every slot that some row sees, in their order.
+__global__ __launch_bounds__(256) void add_weights_kernel(AttendDev a, Shares shares, uint32_t blocks) {
+    const uint32_t heads = a.copies * a.heads, ch = blockIdx.x / blocks, c = ch / a.heads, h = ch % a.heads;
+    const int j = static_cast<int>(blockIdx.x % blocks * 256 + threadIdx.x);
+    const Span sp = span(a, c);
+    if (!sp.rows || !any_visible(a, tiles_of(a, sp.first, sp.first + sp.rows - 1, 1), j)) return;
+    float sum = 0.0f;
+    for (uint32_t s = 0; s < shares.splits; ++s) sum += shares.sums[(static_cast<uint64_t>(s) * heads + ch) * shares.ld + j];
+    a.weights[c * a.w_copy + h * a.w_head + j] += sum;
 }
 
 // ------------------------------------------------------------ the 4-bit cache
@@ -1365,7 +1433,8 @@ constexpr uint32_t kDecodeRows = 16;   // rows x group that decode_kernel takes
 // workgroups) while a share has work for its waves.
 struct Plan {
     uint32_t row_tiles, splits, rows, ld;
-    uint64_t ml, logits, stats, bytes;   // offsets in the workspace (partial outputs first), all of it
+    uint32_t w_splits, w_ld;             // shares of the rows in weights_kernel
+    uint64_t ml, logits, stats, shares, bytes;   // offsets in the workspace (partial outputs first), all of it
 };
 Plan plan_of(const AttendDev& a, uint32_t dim, int cache_dtype) {
     Plan p{};
@@ -1379,15 +1448,40 @@ Plan plan_of(const AttendDev& a, uint32_t dim, int cache_dtype) {
     if (a.window)
         most = std::min<uint64_t>(most, static_cast<uint64_t>(a.window) + std::min<uint64_t>(a.nq, p.rows) + a.sinks + 2 * step);
     const uint64_t tiles = (most + step - 1) / step, groups = heads * p.row_tiles;
-    // few rows: 768 workgroups are three a CU, every wave of a share has a tile; many rows: two a CU, four tiles a share
-    const uint64_t want = few ? (768 + groups - 1) / groups : 512 / groups;
-    p.splits = static_cast<uint32_t>(std::max<uint64_t>(1, std::min<uint64_t>(want, tiles / 4)));
+    if (few) {
+        // 768 workgroups are three a CU; every wave of a share has a tile
+        p.splits = static_cast<uint32_t>(std::max<uint64_t>(1, std::min<uint64_t>((768 + groups - 1) / groups, tiles / 4)));
+    } else {
+        // The least of rounds x tiles a share: as many workgroups as fit run at the speed of one (2 us a tile), and
+        // a share costs four tiles' time for its start and end, and the passage of its outputs through memory.
+        const uint64_t fit = 256 * (dim == 64 && cache_dtype != PKV_FP4 ? 3 : 2);
+        uint64_t least = ~0ull;
+        for (uint32_t n = 1; n <= 16 && (n == 1 || n * 4 <= tiles); ++n) {
+            const uint64_t rounds = (groups * n + fit - 1) / fit;
+            const uint64_t cost = rounds * ((tiles + n - 1) / n + (n == 1 ? 2 : 4)) +
+                                  (n == 1 ? 0 : heads * all * dim * 8 * n / 8000000);
+            if (cost < least) {
+                least = cost;
+                p.splits = n;
+            }
+        }
+    }
     const bool parts = few || p.splits > 1;
     p.ld = few && a.weights ? (a.max_len + 31) / 32 * 32 + 4 : 0;
     p.ml = parts ? round256(heads * p.splits * p.rows * dim * 4) : 0;
     p.logits = p.ml + (parts ? round256(heads * p.splits * p.rows * 8) : 0);
     p.stats = p.logits + round256(4 * heads * all * p.ld);
-    p.bytes = p.stats + (!few && a.weights ? round256(8 * heads * all) : 0);
+    p.shares = p.stats + (!few && a.weights ? round256(8 * heads * all) : 0);
+    p.w_splits = 1;
+    p.w_ld = (a.max_len + 127) / 128 * 128;
+    if (!few && a.weights) {
+        // blocks of 128 slots that some row sees; three workgroups a CU, at least 256 rows each
+        uint64_t seen = a.max_len;
+        if (a.window) seen = std::min<uint64_t>(seen, static_cast<uint64_t>(a.window) + a.nq + a.sinks + 256);
+        const uint64_t blocks = (seen + 127) / 128 * heads;
+        p.w_splits = static_cast<uint32_t>(std::max<uint64_t>(1, std::min<uint64_t>(768 / blocks, all / 256)));
+    }
+    p.bytes = p.shares + (p.w_splits > 1 ? round256(4ull * heads * p.w_splits * p.w_ld) : 0);
     return p;
 }
 
@@ -1406,8 +1500,14 @@ int attend_typed(AttendDev a, uint8_t* ws, hipStream_t st) {
     }
     a.stats = a.weights ? reinterpret_cast<float*>(ws + p.stats) : nullptr;
     rows_kernel<CT, QT, D><<<heads * p.row_tiles * p.splits, 256, 0, st>>>(a, part, p.row_tiles);
-    if (p.splits > 1) join_kernel<QT, D><<<outs, 256, 0, st>>>(a, part, outs);
-    if (a.weights) weights_kernel<CT, QT, D><<<(a.max_len + 127) / 128 * heads, 256, 0, st>>>(a);
+    constexpr uint32_t kJoin = 1024 / D;     // rows of a workgroup
+    if (p.splits > 1) join_rows_kernel<QT, D><<<(a.nq * a.group + kJoin - 1) / kJoin * heads, 256, 0, st>>>(a, part);
+    if (a.weights) {
+        const Shares shares{reinterpret_cast<float*>(ws + p.shares), p.w_splits, p.w_ld};
+        weights_kernel<CT, QT, D><<<p.w_ld / 128 * heads * p.w_splits, 256, 0, st>>>(a, shares);
+        const uint32_t blocks = (a.max_len + 255) / 256;
+        if (p.w_splits > 1) add_weights_kernel<<<blocks * heads, 256, 0, st>>>(a, shares, blocks);
+    }
     return hipGetLastError();
 }
 
