@@ -1287,91 +1287,135 @@ __device__ inline uint32_t weight_key(float w) {
     return u & 0x80000000u ? ~u : u | 0x80000000u;
 }
 
-constexpr int kSelect = 1024;   // threads of select_kernel
+constexpr int kSelect = 1024, kWaves = kSelect / 64;   // threads of select_kernel
+constexpr int kHeld = 32;                              // weights a lane holds: 32,768 a workgroup
 
-// Inclusive prefix sum over the workgroup, in thread order.
-__device__ inline uint32_t block_scan(uint32_t x, uint32_t* tmp) {
-    const uint32_t lane = threadIdx.x % 64, wave = threadIdx.x / 64;
+// The bin that holds the want-th largest key and how many lie above it, by the
+// first wave: four bins a lane, counted from the top.
+__device__ inline void find_bin(const uint32_t* hist, uint32_t want, uint32_t* found) {
+    const uint32_t lane = threadIdx.x;
+    uint32_t h[4], s = 0;
+    for (int x = 0; x < 4; ++x) s += h[x] = hist[4 * lane + x];
+    uint32_t up = s;                                   // of this lane's bins and all above
     for (int o = 1; o < 64; o <<= 1) {
-        const uint32_t y = __shfl_up(x, o);
-        if (lane >= static_cast<uint32_t>(o)) x += y;
+        const uint32_t y = __shfl_down(up, o);
+        if (lane + o < 64) up += y;
     }
-    __syncthreads();
-    if (lane == 63) tmp[wave] = x;
-    __syncthreads();
-    for (uint32_t w = 0; w < wave; ++w) x += tmp[w];
-    return x;
+    uint32_t above = up - s;
+    if (above < want && want <= up) {
+        int x = 3;
+        while (above + h[x] < want) above += h[x--];
+        found[0] = 4 * lane + x;
+        found[1] = above;
+    }
 }
 
-// One workgroup per (head, layer, copy): the budget's border among the middle
-// slots by four passes over 8 bits of the key, then the kept slots in order.
+// One workgroup per (head, layer, copy): the border among the middle slots by
+// four passes over 8 bits of the key, then the kept slots in order.  Each wave
+// has a run of slots, so that two counts a wave place every slot; up to 32,768
+// slots are read once and held in registers.  The counts' LDS atomics are taken
+// together where lanes share the first lane's bin (many weights are 0).
 __global__ __launch_bounds__(kSelect) void select_kernel(EvictDev a) {
     const uint32_t h = blockIdx.x % a.heads, cl = blockIdx.x / a.heads, l = cl % a.layers, c = cl / a.layers;
     const uint32_t n = min(max(a.lens[c], 0), static_cast<int>(a.slots));
     const float* w = a.w + c * a.ws[0] + l * a.ws[1] + h * a.ws[2];
     float* wo = a.w_out + c * a.os[0] + l * a.os[1] + h * a.os[2];
     int32_t* kept = a.kept + static_cast<uint64_t>(blockIdx.x) * a.budget;
-    const uint32_t keep = min(n, a.budget), t = threadIdx.x;
-    __shared__ uint32_t hist[256], tmp[16], found[2];
+    const uint32_t keep = min(n, a.budget), t = threadIdx.x, lane = t % 64, wave = t / 64;
+    __shared__ uint32_t hist[256], sures[kWaves], ties[kWaves], found[2];
     if (l == 0 && h == 0 && t == 0) a.new_lens[c] = static_cast<int32_t>(keep);
-    if (n <= a.budget) {
-        for (uint32_t j = t; j < a.budget; j += kSelect) kept[j] = j < n ? static_cast<int32_t>(j) : -1;
-    } else {
-        const uint32_t lo = a.sinks, hi = n - a.recent;
-        uint32_t want = a.budget - a.sinks - a.recent;   // of the middle; < hi - lo
-        uint32_t prefix = 0, mask = 0;
-        // the key of the want-th largest: its bits from the top, 8 at a time
-        for (int shift = 24; shift >= 0 && want; shift -= 8) {
-            if (t < 256) hist[t] = 0;
-            __syncthreads();
-            for (uint32_t j = lo + t; j < hi; j += kSelect) {
-                const uint32_t k = weight_key(w[j]);
-                if ((k & mask) == prefix) atomicAdd(&hist[k >> shift & 255], 1u);
-            }
-            __syncthreads();
-            if (t == 0) {
-                uint32_t above = 0;
-                int b = 255;
-                while (above + hist[b] < want) above += hist[b--];
-                found[0] = b;
-                found[1] = above;
-            }
-            __syncthreads();
-            prefix |= found[0] << shift;
-            mask |= 255u << shift;
-            want -= found[1];
-            __syncthreads();
+    // the wave's slots: `run` from `from` on, 64 a step
+    const uint32_t run = (n + kSelect - 1) / kSelect * 64, from = wave * run, to = min(from + run, n);
+    const bool held = n <= kSelect * kHeld, all = n <= a.budget;
+    const uint32_t lo = all ? 0 : a.sinks, hi = all ? 0 : n - a.recent;
+    // the key of a middle slot; 0, below every weight's, for the others: they
+    // only add to the lowest bin, behind everything that is looked for
+    auto key_of = [&](uint32_t j, float x) { return j >= lo && j < hi ? weight_key(x) : 0u; };
+    float mine[kHeld];
+    uint32_t key[kHeld];
+    if (held)
+#pragma unroll
+        for (int x = 0; x < kHeld; ++x) {
+            const uint32_t j = from + 64 * x + lane;
+            mine[x] = j < to ? w[j] : 0.0f;
+            key[x] = j < to ? key_of(j, mine[x]) : 0;
         }
-        // kept: protected slots, keys above the border, and the first `want` at it
-        const bool any = mask != 0;
-        uint32_t done = 0, ties = 0;
-        for (uint32_t j0 = 0; j0 < n; j0 += kSelect) {
-            const uint32_t j = j0 + t;
-            const bool in = j < n, mid = in && j >= lo && j < hi;
-            const uint32_t k = mid ? weight_key(w[j]) : 0;
-            const bool tie = mid && any && k == prefix;
-            const uint32_t before = block_scan(tie, tmp);
-            if (t == kSelect - 1) found[0] = before;
-            const bool take = in && (!mid || (any && (k > prefix || (tie && ties + before <= want))));
-            const uint32_t at = block_scan(take, tmp);
-            if (t == kSelect - 1) found[1] = at;
-            if (take) kept[done + at - 1] = static_cast<int32_t>(j);
-            __syncthreads();
-            ties += found[0];
-            done += found[1];
-            __syncthreads();
+    // f(slot, weight, key, there) for every step of the wave's slots
+    auto each = [&](auto f) {
+        if (held) {
+#pragma unroll
+            for (int x = 0; x < kHeld; ++x) {
+                if (from + 64 * x >= to) break;
+                f(from + 64 * x + lane, mine[x], key[x], from + 64 * x + lane < to);
+            }
+        } else {
+            for (uint32_t j0 = from; j0 < to; j0 += 64) {
+                const bool in = j0 + lane < to;
+                const float x = in ? w[j0 + lane] : 0.0f;
+                f(j0 + lane, x, in ? key_of(j0 + lane, x) : 0, in);
+            }
         }
+    };
+    uint32_t want = all ? 0 : a.budget - a.sinks - a.recent;   // of the middle; < hi - lo
+    uint32_t prefix = 0, mask = 0;
+    for (int shift = 24; shift >= 0 && want; shift -= 8) {
+        if (t < 256) hist[t] = 0;
+        __syncthreads();
+        each([&](uint32_t, float, uint32_t k, bool) {
+            const uint32_t bin = k >> shift & 255;
+            const bool count = (k & mask) == prefix;
+            const uint64_t any = __ballot(count);
+            if (!any) return;
+            const uint32_t one = __builtin_ctzll(any), first = __builtin_amdgcn_readlane(bin, one);
+            const uint64_t same = __ballot(count && bin == first);
+            if (lane == one) atomicAdd(&hist[first], static_cast<uint32_t>(__popcll(same)));
+            if (count && bin != first) atomicAdd(&hist[bin], 1u);
+        });
+        __syncthreads();
+        if (wave == 0) find_bin(hist, want, found);
+        __syncthreads();
+        prefix |= found[0] << shift;
+        mask |= 255u << shift;
+        want -= found[1];
     }
-    // the kept slots' weights, in steps: every read of a step comes before its
-    // writes, and a later step's sources lie behind everything written
+    // kept: protected slots and keys above the border (sure), and the first `want` at it
+    const uint32_t above = mask ? prefix : ~0u;
+    auto sure = [&](uint32_t j, uint32_t k, bool in) { return k > above || (in && (j < lo || j >= hi)); };
+    auto tie = [&](uint32_t k) { return mask && k == prefix; };
+    uint32_t ns = 0, nt = 0;
+    each([&](uint32_t j, float, uint32_t k, bool in) {
+        ns += __popcll(__ballot(sure(j, k, in)));
+        nt += __popcll(__ballot(tie(k)));
+    });
+    if (lane == 0) { sures[wave] = ns; ties[wave] = nt; }
     __syncthreads();
-    __threadfence_block();
-    for (uint32_t j0 = 0; j0 < keep; j0 += kSelect) {
-        const uint32_t j = j0 + t;
-        const float x = j < keep ? w[kept[j]] : 0.0f;
+    ns = nt = 0;
+    for (uint32_t x = 0; x < wave; ++x) { ns += sures[x]; nt += ties[x]; }
+    const uint64_t below = (1ull << lane) - 1;
+    // held weights are all read by now: their places may be written
+    each([&](uint32_t j, float x, uint32_t k, bool in) {
+        const bool s = sure(j, k, in), e = tie(k);
+        const uint64_t bs = __ballot(s), be = __ballot(e);
+        const uint32_t ps = ns + __popcll(bs & below), pe = nt + __popcll(be & below);
+        if (s || (e && pe < want)) {
+            const uint32_t at = ps + min(pe, want);
+            kept[at] = static_cast<int32_t>(j);
+            if (held) wo[at] = x;
+        }
+        ns += __popcll(bs);
+        nt += __popcll(be);
+    });
+    for (uint32_t j = keep + t; j < a.budget; j += kSelect) kept[j] = -1;
+    if (!held) {
+        // in steps: every read of a step comes before its writes, and a later step's sources lie behind them
         __syncthreads();
-        if (j < keep) wo[j] = x;
-        __syncthreads();
+        for (uint32_t j0 = 0; j0 < keep; j0 += kSelect) {
+            const uint32_t j = j0 + t;
+            const float x = j < keep ? w[kept[j]] : 0.0f;
+            __syncthreads();
+            if (j < keep) wo[j] = x;
+            __syncthreads();
+        }
     }
     for (uint32_t j = keep + t; j < a.into_slots; j += kSelect) wo[j] = 0.0f;
 }
@@ -1379,48 +1423,81 @@ __global__ __launch_bounds__(kSelect) void select_kernel(EvictDev a) {
 template <int DT>
 __device__ inline uint64_t elem_byte(uint64_t e) { return DT == PKV_FP4 ? e / 2 : DT == PKV_F32 ? e * 4 : e * 2; }
 
-// Kept rows to their new slots, one workgroup per (head, layer, copy) and side
-// (blockIdx.y), pieces of 16 bytes; in place by the same order as the weights.
-template <int DT, int D>
-__global__ __launch_bounds__(256) void move_kernel(EvictDev a) {
-    constexpr uint32_t kBytes = DT == PKV_FP4 ? D / 2 : DT == PKV_F32 ? D * 4 : D * 2;
-    constexpr uint32_t kLanes = kBytes / 16, kRows = 256 / kLanes;
-    const uint32_t h = blockIdx.x % a.heads, cl = blockIdx.x / a.heads, l = cl % a.layers, c = cl / a.layers;
+// Kept rows to their new slots, in pieces of 16 bytes, four rows' at a time
+// (4-bit caches: the scale bytes with the first piece).
+//   into other memory  a workgroup takes kBatch rows of one side of a (copy,
+//                      layer, head); bound by the rows' bytes
+//   in place           a workgroup takes a column of at most 64 bytes of all
+//                      rows, in order: a step's rows are read before it writes
+//                      (a barrier), and rows read later lie behind everything
+//                      it writes, so the next step's reads are already under
+//                      way; columns do not meet.
+template <int DT, int D, bool IN_PLACE>
+struct Move {
+    static constexpr uint32_t kBytes = DT == PKV_FP4 ? D / 2 : DT == PKV_F32 ? D * 4 : D * 2;
+    static constexpr uint32_t kPieces = IN_PLACE && kBytes > 64 ? 4 : kBytes / 16, kColumns = kBytes / 16 / kPieces;
+    static constexpr uint32_t kHold = IN_PLACE ? 8 : 4, kStep = 256 / kPieces, kBatch = kStep * kHold;
+    u32x4 x[kHold];
+    uint32_t s[DT == PKV_FP4 ? kHold : 1];
+    // rows j0 + row, + kStep, .. below `keep`
+    __device__ void read(const EvictDev& a, const uint8_t* src, const uint8_t* scales, uint64_t from, const int32_t* kept,
+                         uint32_t j0, uint32_t keep, uint32_t piece) {
+#pragma unroll
+        for (uint32_t k = 0; k < kHold; ++k) {
+            const uint32_t j = j0 + k * kStep;
+            const uint64_t e = from + static_cast<uint64_t>(j < keep ? kept[j] : 0) * a.kv.slot;   // slot 0: read, not written
+            x[k] = *reinterpret_cast<const u32x4*>(src + elem_byte<DT>(e) + 16 * piece);
+            if constexpr (DT == PKV_FP4)
+                s[k] = D == 64 ? *reinterpret_cast<const uint16_t*>(scales + e / 32)
+                               : *reinterpret_cast<const uint32_t*>(scales + e / 32);
+        }
+    }
+    __device__ void write(const EvictDev& a, uint8_t* dst, uint8_t* scales, uint64_t to, uint32_t j0, uint32_t keep,
+                          uint32_t piece) const {
+#pragma unroll
+        for (uint32_t k = 0; k < kHold; ++k) {
+            const uint32_t j = j0 + k * kStep;
+            if (j >= keep) continue;
+            const uint64_t e = to + static_cast<uint64_t>(j) * a.into.slot;
+            *reinterpret_cast<u32x4*>(dst + elem_byte<DT>(e) + 16 * piece) = x[k];
+            if constexpr (DT == PKV_FP4)
+                if (piece == 0) {
+                    if constexpr (D == 64) *reinterpret_cast<uint16_t*>(scales + e / 32) = static_cast<uint16_t>(s[k]);
+                    else *reinterpret_cast<uint32_t*>(scales + e / 32) = s[k];
+                }
+        }
+    }
+};
+
+template <int DT, int D, bool IN_PLACE>
+__global__ __launch_bounds__(256) void move_kernel(EvictDev a, uint32_t batches) {
+    using M = Move<DT, D, IN_PLACE>;
+    const uint32_t per = IN_PLACE ? M::kColumns : batches, part = blockIdx.x % per, set = blockIdx.x / per / 2;
+    const bool values = blockIdx.x / per % 2;
+    const uint32_t h = set % a.heads, cl = set / a.heads, l = cl % a.layers, c = cl / a.layers;
     const uint32_t n = min(max(a.lens[c], 0), static_cast<int>(a.slots)), keep = min(n, a.budget);
-    const int32_t* kept = a.kept + static_cast<uint64_t>(blockIdx.x) * a.budget;
-    const uint8_t* src = blockIdx.y ? a.kv.v : a.kv.k;
-    uint8_t* dst = const_cast<uint8_t*>(blockIdx.y ? a.into.v : a.into.k);
-    const uint8_t* ssc = blockIdx.y ? a.kv.vs : a.kv.ks;
-    uint8_t* dsc = const_cast<uint8_t*>(blockIdx.y ? a.into.vs : a.into.ks);
+    const int32_t* kept = a.kept + static_cast<uint64_t>(set) * a.budget;
+    const uint8_t *src = values ? a.kv.v : a.kv.k, *ssc = values ? a.kv.vs : a.kv.ks;
+    uint8_t *dst = const_cast<uint8_t*>(values ? a.into.v : a.into.k);
+    uint8_t* dsc = const_cast<uint8_t*>(values ? a.into.vs : a.into.ks);
     const uint64_t from = c * a.kv.copy + l * a.kv.layer + h * a.kv.head;
     const uint64_t to = c * a.into.copy + l * a.into.layer + h * a.into.head;
-    const uint32_t sub = threadIdx.x % kLanes, row = threadIdx.x / kLanes;
-    for (uint32_t j0 = 0; j0 < keep; j0 += kRows) {
-        const uint32_t j = j0 + row;
-        const bool in = j < keep;
-        uint4 x{};
-        uint32_t sc = 0;
-        if (in) {
-            const uint64_t e = from + static_cast<uint64_t>(kept[j]) * a.kv.slot;
-            x = *reinterpret_cast<const uint4*>(src + elem_byte<DT>(e) + 16 * sub);
-            if constexpr (DT == PKV_FP4) {
-                if (sub == 0)
-                    sc = D == 64 ? *reinterpret_cast<const uint16_t*>(ssc + e / 32)
-                                 : *reinterpret_cast<const uint32_t*>(ssc + e / 32);
-            }
+    const uint32_t row = threadIdx.x / M::kPieces, piece = threadIdx.x % M::kPieces + (IN_PLACE ? part * M::kPieces : 0);
+    if constexpr (!IN_PLACE) {
+        M m;
+        m.read(a, src, ssc, from, kept, part * M::kBatch + row, keep, piece);
+        m.write(a, dst, dsc, to, part * M::kBatch + row, keep, piece);
+    } else {
+        if (n <= a.budget) return;             // every slot stays where it is
+        M m, next;
+        m.read(a, src, ssc, from, kept, row, keep, piece);
+        for (uint32_t j0 = 0; j0 < keep; j0 += M::kBatch) {
+            next.read(a, src, ssc, from, kept, j0 + M::kBatch + row, keep, piece);
+            __builtin_amdgcn_s_waitcnt(0);     // this step's rows have been read ..
+            __syncthreads();                   // .. by every wave
+            m.write(a, dst, dsc, to, j0 + row, keep, piece);
+            m = next;
         }
-        __syncthreads();
-        if (in) {
-            const uint64_t e = to + static_cast<uint64_t>(j) * a.into.slot;
-            *reinterpret_cast<uint4*>(dst + elem_byte<DT>(e) + 16 * sub) = x;
-            if constexpr (DT == PKV_FP4) {
-                if (sub == 0) {
-                    if constexpr (D == 64) *reinterpret_cast<uint16_t*>(dsc + e / 32) = static_cast<uint16_t>(sc);
-                    else *reinterpret_cast<uint32_t*>(dsc + e / 32) = sc;
-                }
-            }
-        }
-        __syncthreads();
     }
 }
 
@@ -1552,22 +1629,26 @@ int launch_attend(const AttendDev& a, uint32_t dim, int cache_dtype, int dtype, 
 int launch_fp4_store(const RowsDev& r, uint32_t dim, int dtype, void* stream) { PKV_ROWS_LAUNCH(fp4_store_kernel) }
 int launch_fp4_load(const RowsDev& r, uint32_t dim, int dtype, void* stream) { PKV_ROWS_LAUNCH(fp4_load_kernel) }
 
-template <int DT>
-static void move_dim(const EvictDev& e, uint32_t dim, dim3 grid, hipStream_t st) {
-    if (dim == 64) move_kernel<DT, 64><<<grid, 256, 0, st>>>(e);
-    else move_kernel<DT, 128><<<grid, 256, 0, st>>>(e);
+template <int DT, int D>
+static int move_typed(const EvictDev& e, hipStream_t st) {
+    const uint64_t sets = static_cast<uint64_t>(e.copies) * e.layers * e.heads;
+    if (e.in_place) {
+        move_kernel<DT, D, true><<<static_cast<uint32_t>(sets * 2 * Move<DT, D, true>::kColumns), 256, 0, st>>>(e, 0);
+    } else {
+        const uint32_t most = std::min(e.budget, e.slots), rows = Move<DT, D, false>::kBatch;
+        const uint32_t batches = (most + rows - 1) / rows;
+        move_kernel<DT, D, false><<<static_cast<uint32_t>(sets * 2 * batches), 256, 0, st>>>(e, batches);
+    }
+    return hipGetLastError();
 }
 
 int launch_evict(const EvictDev& e, uint32_t dim, int dtype, void* stream) {
     hipStream_t st = static_cast<hipStream_t>(stream);
-    const uint32_t sets = e.copies * e.layers * e.heads;
-    select_kernel<<<sets, kSelect, 0, st>>>(e);
-    const dim3 grid(sets, 2);
-    if (dtype == PKV_F32) move_dim<PKV_F32>(e, dim, grid, st);
-    else if (dtype == PKV_BF16) move_dim<PKV_BF16>(e, dim, grid, st);
-    else if (dtype == PKV_F16) move_dim<PKV_F16>(e, dim, grid, st);
-    else move_dim<PKV_FP4>(e, dim, grid, st);
-    return hipGetLastError();
+    select_kernel<<<e.copies * e.layers * e.heads, kSelect, 0, st>>>(e);
+    if (dtype == PKV_F32) return dim == 64 ? move_typed<PKV_F32, 64>(e, st) : move_typed<PKV_F32, 128>(e, st);
+    if (dtype == PKV_BF16) return dim == 64 ? move_typed<PKV_BF16, 64>(e, st) : move_typed<PKV_BF16, 128>(e, st);
+    if (dtype == PKV_F16) return dim == 64 ? move_typed<PKV_F16, 64>(e, st) : move_typed<PKV_F16, 128>(e, st);
+    return dim == 64 ? move_typed<PKV_FP4, 64>(e, st) : move_typed<PKV_FP4, 128>(e, st);
 }
 
 }  // namespace pkv
