@@ -1313,8 +1313,9 @@ __device__ inline void find_bin(const uint32_t* hist, uint32_t want, uint32_t* f
 // One workgroup per (head, layer, copy): the border among the middle slots by
 // four passes over 8 bits of the key, then the kept slots in order.  Each wave
 // has a run of slots, so that two counts a wave place every slot; up to 32,768
-// slots are read once and held in registers.  The counts' LDS atomics are taken
-// together where lanes share the first lane's bin (many weights are 0).
+// slots are read once and held in registers.  A bin has 16 counts, by lane: the
+// high bytes of weights are nearly all the same, and 64 lanes adding to one
+// word would take their turns.
 __global__ __launch_bounds__(kSelect) void select_kernel(EvictDev a) {
     const uint32_t h = blockIdx.x % a.heads, cl = blockIdx.x / a.heads, l = cl % a.layers, c = cl / a.layers;
     const uint32_t n = min(max(a.lens[c], 0), static_cast<int>(a.slots));
@@ -1322,7 +1323,10 @@ __global__ __launch_bounds__(kSelect) void select_kernel(EvictDev a) {
     float* wo = a.w_out + c * a.os[0] + l * a.os[1] + h * a.os[2];
     int32_t* kept = a.kept + static_cast<uint64_t>(blockIdx.x) * a.budget;
     const uint32_t keep = min(n, a.budget), t = threadIdx.x, lane = t % 64, wave = t / 64;
-    __shared__ uint32_t hist[256], sures[kWaves], ties[kWaves], found[2];
+    constexpr uint32_t kCopies = 16;
+    __shared__ __align__(16) uint32_t hist[256 * kCopies];
+    __shared__ uint32_t total[256], sures[kWaves], ties[kWaves], found[2];
+    static_assert(256 * kCopies == 4 * kSelect, "four counts a thread");
     if (l == 0 && h == 0 && t == 0) a.new_lens[c] = static_cast<int32_t>(keep);
     // the wave's slots: `run` from `from` on, 64 a step
     const uint32_t run = (n + kSelect - 1) / kSelect * 64, from = wave * run, to = min(from + run, n);
@@ -1359,20 +1363,19 @@ __global__ __launch_bounds__(kSelect) void select_kernel(EvictDev a) {
     uint32_t want = all ? 0 : a.budget - a.sinks - a.recent;   // of the middle; < hi - lo
     uint32_t prefix = 0, mask = 0;
     for (int shift = 24; shift >= 0 && want; shift -= 8) {
-        if (t < 256) hist[t] = 0;
+        *reinterpret_cast<u32x4*>(&hist[4 * t]) = u32x4{};
         __syncthreads();
         each([&](uint32_t, float, uint32_t k, bool) {
-            const uint32_t bin = k >> shift & 255;
-            const bool count = (k & mask) == prefix;
-            const uint64_t any = __ballot(count);
-            if (!any) return;
-            const uint32_t one = __builtin_ctzll(any), first = __builtin_amdgcn_readlane(bin, one);
-            const uint64_t same = __ballot(count && bin == first);
-            if (lane == one) atomicAdd(&hist[first], static_cast<uint32_t>(__popcll(same)));
-            if (count && bin != first) atomicAdd(&hist[bin], 1u);
+            if ((k & mask) == prefix) atomicAdd(&hist[(k >> shift & 255) * kCopies + lane % kCopies], 1u);
         });
         __syncthreads();
-        if (wave == 0) find_bin(hist, want, found);
+        const u32x4 four = *reinterpret_cast<const u32x4*>(&hist[4 * t]);
+        uint32_t sum = four[0] + four[1] + four[2] + four[3];
+        sum += __shfl_xor(sum, 1);
+        sum += __shfl_xor(sum, 2);
+        if (t % 4 == 0) total[t / 4] = sum;
+        __syncthreads();
+        if (wave == 0) find_bin(total, want, found);
         __syncthreads();
         prefix |= found[0] << shift;
         mask |= 255u << shift;
