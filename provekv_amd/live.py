@@ -22,9 +22,14 @@ from . import _lib as L
 from .device import device_context
 
 
+_TYPES: dict = {}
+
+
 def _rows_dtype(t):
-    import torch
-    return {torch.float32: L.DT_F32, torch.bfloat16: L.DT_BF16, torch.float16: L.DT_F16}.get(t)
+    if not _TYPES:
+        import torch
+        _TYPES.update({torch.float32: L.DT_F32, torch.bfloat16: L.DT_BF16, torch.float16: L.DT_F16})
+    return _TYPES.get(t)
 
 
 def _strides(t) -> list:
@@ -38,30 +43,54 @@ def _fits(t) -> bool:
     return t.stride(-1) == 1 and t.data_ptr() % 16 == 0 and all(s % unit == 0 for s in _strides(t)[:-1])
 
 
+def _like(t):
+    """What a call's struct depends on in a tensor besides its address."""
+    return None if t is None else (t.shape, t.dtype, t.stride())
+
+
+_NO_GUARD = contextlib.nullcontext()
+
+
 class LiveCache:
     """What a cache of [copies][layers][K|V][heads][tokens][dim] rows does on
     the device.  A subclass has copies, layers, heads, tokens, dim, device and
     _pointers(): (dtype, bytes of an element or None for 4-bit codes, keys,
-    values, key scales, value scales)."""
+    values, key scales, value scales, elements of the whole memory)."""
 
     # ------------------------------------------------------------ the call's frame
-    def _frame(self, stream):
+    def _frame(self, dev, stream):
         """(context, stream handle, guard): the guard makes the cache's device
         and the stream current, so that what a call allocates belongs to it."""
         import torch
-        dev = self.device
         if dev.type != "cuda":
             raise ValueError("the cache is not on a GPU")
-        index = dev.index if dev.index is not None else torch.cuda.current_device()
-        if stream is None:
-            guard = contextlib.nullcontext() if index == torch.cuda.current_device() else torch.cuda.device(index)
-            return device_context(index), torch.cuda.current_stream(index).cuda_stream, guard
-        if stream.device_index != index:
-            raise ValueError("the stream belongs to another device than the cache")
-        return device_context(index), stream.cuda_stream, torch.cuda.stream(stream)
+        index, now = dev.index, torch.cuda.current_device()
+        if index is None:
+            index = now
+        if stream is not None:
+            if stream.device_index != index:
+                raise ValueError("the stream belongs to another device than the cache")
+            return device_context(index), stream.cuda_stream, torch.cuda.stream(stream)
+        raw = getattr(torch._C, "_cuda_getCurrentRawStream", None)   # a Stream object costs as much as a launch
+        handle = raw(index) if raw is not None else torch.cuda.current_stream(index).cuda_stream
+        return device_context(index), handle, _NO_GUARD if index == now else torch.cuda.device(index)
+
+    def _plan(self, key, make):
+        """A copy of the call's struct for `key`: checked and filled once (the
+        caches' addresses are part of the key), then only the tensors'
+        addresses change from call to call."""
+        plans = self.__dict__.setdefault("_plans", {})
+        got = plans.get(key)
+        if got is None:
+            got = make()
+            if len(plans) >= 256:
+                plans.clear()
+            plans[key] = got
+        op, extra = got
+        return type(op).from_buffer_copy(op), extra
 
     def _view(self, layer=None) -> "L.KvView":
-        dtype, size, k, v, ks, vs = self._pointers()
+        dtype, size, k, v, ks, vs, elems = self._pointers()
         side = self.heads * self.tokens * self.dim
         per_layer, first = 2 * side, 0
         if layer is not None:
@@ -72,7 +101,9 @@ class LiveCache:
             k, v, ks, vs = k + first // 2, v + first // 2, ks + first // 32, vs + first // 32
         else:
             k, v = k + first * size, v + first * size
-        elems = self.copies * self.layers * per_layer - side - first
+        elems -= side + first
+        if elems < 0:
+            raise ValueError("the cache's memory is smaller than its shape")
         return L.KvView(k, v, ks or None, vs or None, self.layers * per_layer, per_layer, self.tokens * self.dim,
                         self.dim, elems, self.copies, 1 if layer is not None else self.layers, self.heads,
                         self.tokens, self.dim, dtype)
@@ -86,10 +117,11 @@ class LiveCache:
             raise ValueError(f"{name} must be a contiguous int32 tensor of {self.copies} on the cache's device")
         return x
 
-    def _on_device(self, **tensors):
-        for name, t in tensors.items():
-            if t is not None and t.device != self.device:
-                raise ValueError(f"{name} is on {t.device}, the cache on {self.device}")
+    @staticmethod
+    def _on_device(dev, *tensors):
+        for t in tensors:
+            if t is not None and t.device != dev:
+                raise ValueError(f"a tensor is on {t.device}, the cache on {dev}")
 
     # ------------------------------------------------------------ attention
     def attend(self, layer: int, q, lens, q_lens=None, window: int = 0, sinks: int = 0, scale: float | None = None,
@@ -110,58 +142,83 @@ class LiveCache:
         sum of exponentials.  max_len: no length is above it (an int `lens`
         says so itself); sizes the launch."""
         import torch
-        dtype = _rows_dtype(q.dtype)
-        if dtype is None or (not isinstance(self, FourBitKVCache) and self.buf.dtype != q.dtype):
-            raise TypeError("q must have the cache's dtype (float32, bfloat16 or float16 over a 4-bit cache)")
-        if q.dim() != 4 or q.shape[0] != self.copies or q.shape[3] != self.dim:
-            raise ValueError(f"q must be [{self.copies}, rows, query heads, {self.dim}]")
+        dev = self.device
+        self._on_device(dev, q, weights, lse, out)
         if q.requires_grad and torch.is_grad_enabled():
             raise ValueError("attend has no backward pass: detach q or call it under torch.no_grad()")
-        self._on_device(q=q, weights=weights, lse=lse, out=out)
-        rows, heads = q.shape[1], q.shape[2]
-        if not heads or heads % self.heads:
-            raise ValueError(f"{heads} query heads over {self.heads} heads")
-        if window < 0 or sinks < 0:
-            raise ValueError("window and sinks are not negative")
-        ctx, handle, guard = self._frame(stream)
+        by_tensor = isinstance(lens, torch.Tensor)
+        if max_len is None:
+            max_len = self.tokens if by_tensor else min(max(int(lens), 1), self.tokens)
+
+        def make():
+            return self._attend_op(layer, q, window, sinks, scale, weights, lse, out, max_len, q_lens is not None)
+
+        key = (0, layer, q.shape, q.dtype, window, sinks, scale, max_len, self._address(), q_lens is None, _like(weights),
+               _like(lse), _like(out))
+        op, (need, rows_of) = self._plan(key, make)
+        ctx, handle, guard = self._frame(dev, stream)
         with guard:
-            if max_len is None:
-                max_len = self.tokens if isinstance(lens, torch.Tensor) else min(max(int(lens), 1), self.tokens)
-            if not 1 <= max_len <= self.tokens:
-                raise ValueError(f"max_len is 1 .. {self.tokens}")
             lens = self._words(lens, "lens")
-            q_lens = None if q_lens is None else self._words(q_lens, "q_lens")
             if not _fits(q):
                 q = q.contiguous()
                 if q.data_ptr() % 16:
                     q = q.clone()
             if out is None:
                 # rows behind q_lens are nobody's: 0 rather than whatever the memory held
-                out = (torch.empty if q_lens is None else torch.zeros)(q.shape, dtype=q.dtype, device=q.device)
-            elif out.shape != q.shape or out.dtype != q.dtype or not _fits(out):
-                raise ValueError("out must have q's shape and dtype, rows of 16-byte pieces")
-            qs, os = _strides(q), _strides(out)
-            op = L.AttendOp(self._view(layer), q.data_ptr(), out.data_ptr(), qs[0], qs[1], qs[2], os[0], os[1], os[2],
-                            lens.data_ptr(), None if q_lens is None else q_lens.data_ptr(), None, None, 0, 0, None, 0,
-                            1.0 / math.sqrt(self.dim) if scale is None else scale, dtype, heads, rows, max_len,
-                            min(window, 0xffffffff), min(sinks, 0xffffffff), 0)
+                out = (torch.empty if q_lens is None else torch.zeros)(q.shape, dtype=q.dtype, device=dev)
+            s = q.stride()
+            op.q_copy_stride, op.q_row_stride, op.q_head_stride = (n if m else 0 for n, m in zip(s, rows_of))
+            op.d_q, op.d_out, op.d_lens = q.data_ptr(), out.data_ptr(), lens.data_ptr()
+            if q_lens is not None:
+                q_lens = self._words(q_lens, "q_lens")
+                op.d_q_lens = q_lens.data_ptr()
             if weights is not None:
-                if weights.dtype != torch.float32 or weights.shape != (self.copies, self.heads, self.tokens) or \
-                        weights.stride(2) != 1:
-                    raise ValueError(f"weights must be float32 [{self.copies}, {self.heads}, {self.tokens}], "
-                                     "slots contiguous")
-                ws = _strides(weights)
-                op.d_weights, op.weight_copy_stride, op.weight_head_stride = weights.data_ptr(), ws[0], ws[1]
+                op.d_weights = weights.data_ptr()
             if lse is not None:
-                if lse.dtype != torch.float32 or lse.shape != (self.copies, heads, rows) or not lse.is_contiguous():
-                    raise ValueError(f"lse must be a contiguous float32 [{self.copies}, {heads}, {rows}]")
                 op.d_lse = lse.data_ptr()
-            need = L.lib().pkv_attend_workspace(C.byref(op))
             if need:
-                work = torch.empty(need, dtype=torch.uint8, device=q.device)
-                op.d_workspace, op.workspace_bytes = work.data_ptr(), need
-            L.check(L.lib().pkv_attend(ctx.ptr, C.byref(op), handle), "pkv_attend")
+                work = torch.empty(need, dtype=torch.uint8, device=dev)
+                op.d_workspace = work.data_ptr()
+            rc = L.lib().pkv_attend(ctx.ptr, C.byref(op), handle)
+            if rc:
+                L.check(rc, "pkv_attend")
         return out
+
+    def _attend_op(self, layer, q, window, sinks, scale, weights, lse, out, max_len, ragged):
+        """The call's struct but for the addresses and q's strides, and
+        (workspace bytes, which of q's strides count)."""
+        import torch
+        dtype = _rows_dtype(q.dtype)
+        if dtype is None or (not isinstance(self, FourBitKVCache) and self.buf.dtype != q.dtype):
+            raise TypeError("q must have the cache's dtype (float32, bfloat16 or float16 over a 4-bit cache)")
+        if q.dim() != 4 or q.shape[0] != self.copies or q.shape[3] != self.dim:
+            raise ValueError(f"q must be [{self.copies}, rows, query heads, {self.dim}]")
+        rows, heads = q.shape[1], q.shape[2]
+        if not heads or heads % self.heads:
+            raise ValueError(f"{heads} query heads over {self.heads} heads")
+        if window < 0 or sinks < 0:
+            raise ValueError("window and sinks are not negative")
+        if not 1 <= max_len <= self.tokens:
+            raise ValueError(f"max_len is 1 .. {self.tokens}")
+        if out is not None and (out.shape != q.shape or out.dtype != q.dtype or not _fits(out)):
+            raise ValueError("out must have q's shape and dtype, rows of 16-byte pieces")
+        # a new out is contiguous
+        os = _strides(out) if out is not None else [rows * heads * self.dim, heads * self.dim, self.dim]
+        op = L.AttendOp(self._view(layer), None, None, 0, 0, 0, os[0], os[1], os[2], None, None, None, None, 0, 0, None, 0,
+                        1.0 / math.sqrt(self.dim) if scale is None else scale, dtype, heads, rows, max_len,
+                        min(window, 0xffffffff), min(sinks, 0xffffffff), 0)
+        if weights is not None:
+            if weights.dtype != torch.float32 or weights.shape != (self.copies, self.heads, self.tokens) or \
+                    weights.stride(2) != 1:
+                raise ValueError(f"weights must be float32 [{self.copies}, {self.heads}, {self.tokens}], "
+                                 "slots contiguous")
+            ws = _strides(weights)
+            op.d_weights, op.weight_copy_stride, op.weight_head_stride = weights.data_ptr(), ws[0], ws[1]
+        if lse is not None and (lse.dtype != torch.float32 or lse.shape != (self.copies, heads, rows) or
+                                not lse.is_contiguous()):
+            raise ValueError(f"lse must be a contiguous float32 [{self.copies}, {heads}, {rows}]")
+        op.workspace_bytes = L.lib().pkv_attend_workspace(C.byref(op))
+        return op, (op.workspace_bytes, [n > 1 for n in q.shape[:3]])
 
     # ------------------------------------------------------------ eviction
     def evict(self, lens, weights, budget: int, sinks: int = 0, recent: int = 0, layer: int | None = None, into=None,
@@ -180,33 +237,42 @@ class LiveCache:
         new tensor of `into`'s slots otherwise.  An all-layer call takes one
         length per copy for all layers."""
         import torch
-        to = self if into is None else into
-        if type(to)._kind(to) != type(self)._kind(self) or (to.copies, to.layers, to.heads, to.dim) != \
-                (self.copies, self.layers, self.heads, self.dim):
-            raise ValueError("into must be a cache of the same kind, copies, layers, heads and dim")
-        if to.device != self.device:
-            raise ValueError("into is on another device")
-        if budget < 1 or sinks < 0 or recent < 0 or sinks + recent > budget:
-            raise ValueError("the budget holds at least one slot, the sinks and the recent slots")
-        if to.tokens < min(budget, self.tokens):
-            raise ValueError(f"into has {to.tokens} slots, the budget is {budget}")
+        to, dev = self if into is None else into, self.device
         lead = (self.copies, self.layers, self.heads) if layer is None else (self.copies, self.heads)
-        if weights.dtype != torch.float32 or weights.shape != (*lead, self.tokens) or weights.stride(-1) != 1:
-            raise ValueError(f"weights must be float32 {[*lead, self.tokens]}, slots contiguous")
-        self._on_device(weights=weights)
-        ctx, handle, guard = self._frame(stream)
+        if to.device != dev:
+            raise ValueError("into is on another device")
+        self._on_device(dev, weights)
+
+        def make():
+            if to._kind() != self._kind() or (to.copies, to.layers, to.heads, to.dim) != \
+                    (self.copies, self.layers, self.heads, self.dim):
+                raise ValueError("into must be a cache of the same kind, copies, layers, heads and dim")
+            if budget < 1 or sinks < 0 or recent < 0 or sinks + recent > budget:
+                raise ValueError("the budget holds at least one slot, the sinks and the recent slots")
+            if to.tokens < min(budget, self.tokens):
+                raise ValueError(f"into has {to.tokens} slots, the budget is {budget}")
+            if weights.dtype != torch.float32 or weights.shape != (*lead, self.tokens) or weights.stride(-1) != 1:
+                raise ValueError(f"weights must be float32 {[*lead, self.tokens]}, slots contiguous")
+            op = L.EvictOp(self._view(layer), to._view(layer))
+            out = _strides(weights)
+            if into is not None:   # contiguous
+                out = [math.prod(lead[k + 1:]) * to.tokens for k in range(len(lead))]
+            for dst, s in ((op.weight_strides, _strides(weights)), (op.out_strides, out)):
+                dst[:] = s[:3] if layer is None else (s[0], 0, s[1])
+            op.budget, op.sinks, op.recent = budget, sinks, recent
+            return op, None
+
+        key = (1, layer, budget, sinks, recent, self._address(), None if into is None else (to._address(), to.copies, to.layers, to.heads, to.tokens, to.dim),
+               _like(weights))
+        op, _ = self._plan(key, make)
+        ctx, handle, guard = self._frame(dev, stream)
         with guard:
             lens = self._words(lens, "lens")
             new_lens = torch.empty_like(lens)
-            kept = torch.empty((*lead, budget), dtype=torch.int32, device=self.device)
-            packed = weights if into is None else torch.empty((*lead, to.tokens), dtype=torch.float32,
-                                                              device=self.device)
-            op = L.EvictOp(self._view(layer), to._view(layer), lens.data_ptr(), new_lens.data_ptr(), kept.data_ptr(),
-                           weights.data_ptr(), packed.data_ptr())
-            for dst, t in ((op.weight_strides, weights), (op.out_strides, packed)):
-                s = _strides(t)
-                dst[:] = s[:3] if layer is None else (s[0], 0, s[1])
-            op.budget, op.sinks, op.recent = budget, sinks, recent
+            kept = torch.empty((*lead, budget), dtype=torch.int32, device=dev)
+            packed = weights if into is None else torch.empty((*lead, to.tokens), dtype=torch.float32, device=dev)
+            op.d_lens, op.d_new_lens, op.d_kept = lens.data_ptr(), new_lens.data_ptr(), kept.data_ptr()
+            op.d_weights, op.d_weights_out = weights.data_ptr(), packed.data_ptr()
             L.check(L.lib().pkv_evict(ctx.ptr, C.byref(op), handle), "pkv_evict")
         if layer is None:
             filled = min(self._seq_len, budget)
@@ -215,6 +281,10 @@ class LiveCache:
 
     def _kind(self):
         return self._pointers()[0]
+
+    def _address(self):
+        """Where the cache's memory is (and what it holds)."""
+        return self._pointers()
 
 
 class FourBitKVCache(LiveCache):
@@ -260,19 +330,31 @@ class FourBitKVCache(LiveCache):
     def _pointers(self):
         side = self.heads * self.tokens * self.dim
         c, s = self.codes.data_ptr(), self.scales.data_ptr()
-        return L.DT_FP4, None, c, c + side // 2, s, s + side // 32
+        return L.DT_FP4, None, c, c + side // 2, s, s + side // 32, min(2 * self.codes.numel(), 32 * self.scales.numel())
 
     # ------------------------------------------------------------ rows in and out
-    def _rows_op(self, keys, values, first, counts, layer):
+    def _rows(self, entry, keys, values, first, counts, layer, dev, stream_frame):
+        """One store or load of tensors that fit; returns what must outlive the launch."""
         some = keys if keys is not None else values
-        ks = _strides(some)
-        ks = ks if layer is None else [ks[0], 0, *ks[1:]]
+
+        def make():
+            ks = _strides(some)
+            ks = ks if layer is None else [ks[0], 0, *ks[1:]]
+            return L.RowsOp(self._view(layer), None, None, ks[0], ks[1], ks[2], ks[3], None, None,
+                            _rows_dtype(some.dtype), some.shape[-2]), None
+
+        op, _ = self._plan((2, layer, self._address(), _like(some)), make)
+        ctx, handle = stream_frame
         first = self._words(first, "first")
-        counts = None if counts is None else self._words(counts, "counts")
-        op = L.RowsOp(self._view(layer), None if keys is None else keys.data_ptr(),
-                      None if values is None else values.data_ptr(), ks[0], ks[1], ks[2], ks[3], first.data_ptr(),
-                      None if counts is None else counts.data_ptr(), _rows_dtype(some.dtype), some.shape[-2])
-        return op, (first, counts)   # the words live until the launch
+        op.d_first = first.data_ptr()
+        if counts is not None:
+            counts = self._words(counts, "counts")
+            op.d_counts = counts.data_ptr()
+        if keys is not None:
+            op.d_keys = keys.data_ptr()
+        if values is not None:
+            op.d_values = values.data_ptr()
+        L.check(getattr(L.lib(), entry)(ctx.ptr, C.byref(op), handle), entry)
 
     def store(self, keys, values, first, layer: int | None = None, counts=None, stream=None) -> None:
         """Put rows [copies, layers, heads, rows, dim] of float32, bfloat16 or
@@ -294,14 +376,15 @@ class FourBitKVCache(LiveCache):
                 raise TypeError("keys and values are both float32, bfloat16 or float16")
             if t.shape != (*lead, some.shape[-2], self.dim):
                 raise ValueError(f"keys and values must be {[*lead, 'rows', self.dim]}")
-        self._on_device(keys=keys, values=values)
-        ctx, handle, guard = self._frame(stream)
+        dev = self.device
+        self._on_device(dev, keys, values)
+        ctx, handle, guard = self._frame(dev, stream)
         with guard:
-            if not all(t is None or (_fits(t) and _strides(t) == _strides(some)) for t in (keys, values)):
+            if not _fits(some) or (values is not None and values is not some and
+                                   (values.stride() != some.stride() or values.data_ptr() % 16)):
                 keys, values = (None if t is None else t.contiguous() for t in (keys, values))
                 keys, values = (t if t is None or t.data_ptr() % 16 == 0 else t.clone() for t in (keys, values))
-            op, _words = self._rows_op(keys, values, first, counts, layer)
-            L.check(L.lib().pkv_fp4_store(ctx.ptr, C.byref(op), handle), "pkv_fp4_store")
+            self._rows("pkv_fp4_store", keys, values, first, counts, layer, dev, (ctx, handle))
 
     def load(self, first, rows: int, layer: int | None = None, dtype=None, counts=None, stream=None):
         """The values that the slots first[c] .. first[c] + rows - 1 stand for:
@@ -315,11 +398,11 @@ class FourBitKVCache(LiveCache):
         if rows < 0:
             raise ValueError("rows is not negative")
         lead = (self.copies, self.layers, self.heads) if layer is None else (self.copies, self.heads)
-        ctx, handle, guard = self._frame(stream)
+        dev = self.device
+        ctx, handle, guard = self._frame(dev, stream)
         with guard:
-            keys, values = (torch.empty((*lead, rows, self.dim), dtype=dtype, device=self.device) for _ in range(2))
-            op, _words = self._rows_op(keys, values, first, counts, layer)
-            L.check(L.lib().pkv_fp4_load(ctx.ptr, C.byref(op), handle), "pkv_fp4_load")
+            keys, values = (torch.empty((*lead, rows, self.dim), dtype=dtype, device=dev) for _ in range(2))
+            self._rows("pkv_fp4_load", keys, values, first, counts, layer, dev, (ctx, handle))
         return keys, values
 
     # ------------------------------------------------------------ CacheTarget

@@ -22,7 +22,7 @@ import numpy as np
 
 from . import _lib as L
 from .device import SEG_DTYPE
-from .live import FourBitKVCache, LiveCache  # noqa: F401
+from .live import FourBitKVCache, LiveCache, _rows_dtype  # noqa: F401
 
 
 def read_fb2_n_blocks(payload: bytes):
@@ -104,12 +104,12 @@ class DeviceKVCache(LiveCache):
         return self
 
     def _pointers(self):
-        import torch
-        dts = {torch.float32: L.DT_F32, torch.bfloat16: L.DT_BF16, torch.float16: L.DT_F16}
-        if self.buf.dtype not in dts:
+        buf = self.buf
+        dtype = _rows_dtype(buf.dtype)
+        if dtype is None:
             raise TypeError("a cache is float32, bfloat16 or float16")
-        p, side = self.buf.data_ptr(), self.heads * self.tokens * self.dim
-        return dts[self.buf.dtype], self.buf.element_size(), p, p + side * self.buf.element_size(), 0, 0
+        p, size = buf.data_ptr(), buf.element_size()
+        return dtype, size, p, p + self.heads * self.tokens * self.dim * size, 0, 0, buf.numel()
 
     @property
     def device(self):
