@@ -39,6 +39,8 @@ def _strides(t) -> list:
 
 def _fits(t) -> bool:
     """Rows of 16-byte pieces, as the kernels read and write them."""
+    if t.is_contiguous() and t.shape[-1] % 8 == 0:
+        return t.data_ptr() % 16 == 0
     unit = 16 // t.element_size()
     return t.stride(-1) == 1 and t.data_ptr() % 16 == 0 and all(s % unit == 0 for s in _strides(t)[:-1])
 
@@ -146,29 +148,26 @@ class LiveCache:
         self._on_device(dev, q, weights, lse, out)
         if q.requires_grad and torch.is_grad_enabled():
             raise ValueError("attend has no backward pass: detach q or call it under torch.no_grad()")
-        by_tensor = isinstance(lens, torch.Tensor)
         if max_len is None:
-            max_len = self.tokens if by_tensor else min(max(int(lens), 1), self.tokens)
+            max_len = self.tokens if isinstance(lens, torch.Tensor) else min(max(int(lens), 1), self.tokens)
 
-        def make():
-            return self._attend_op(layer, q, window, sinks, scale, weights, lse, out, max_len, q_lens is not None)
+        def plan(q):
+            return self._plan((0, layer, _like(q), window, sinks, scale, max_len, self._address(), _like(weights),
+                               _like(lse), _like(out)),
+                              lambda: self._attend_op(layer, q, window, sinks, scale, weights, lse, out, max_len))
 
-        key = (0, layer, q.shape, q.dtype, window, sinks, scale, max_len, self._address(), q_lens is None, _like(weights),
-               _like(lse), _like(out))
-        op, (need, rows_of) = self._plan(key, make)
+        op, (need, fits) = plan(q)
         ctx, handle, guard = self._frame(dev, stream)
         with guard:
+            if not fits or q.data_ptr() % 16:
+                q = q.clone(memory_format=torch.contiguous_format)
+                op, (need, _) = plan(q)
             lens = self._words(lens, "lens")
-            if not _fits(q):
-                q = q.contiguous()
-                if q.data_ptr() % 16:
-                    q = q.clone()
+            op.d_lens = lens.data_ptr()
             if out is None:
                 # rows behind q_lens are nobody's: 0 rather than whatever the memory held
                 out = (torch.empty if q_lens is None else torch.zeros)(q.shape, dtype=q.dtype, device=dev)
-            s = q.stride()
-            op.q_copy_stride, op.q_row_stride, op.q_head_stride = (n if m else 0 for n, m in zip(s, rows_of))
-            op.d_q, op.d_out, op.d_lens = q.data_ptr(), out.data_ptr(), lens.data_ptr()
+            op.d_q, op.d_out = q.data_ptr(), out.data_ptr()
             if q_lens is not None:
                 q_lens = self._words(q_lens, "q_lens")
                 op.d_q_lens = q_lens.data_ptr()
@@ -184,9 +183,9 @@ class LiveCache:
                 L.check(rc, "pkv_attend")
         return out
 
-    def _attend_op(self, layer, q, window, sinks, scale, weights, lse, out, max_len, ragged):
-        """The call's struct but for the addresses and q's strides, and
-        (workspace bytes, which of q's strides count)."""
+    def _attend_op(self, layer, q, window, sinks, scale, weights, lse, out, max_len):
+        """The call's struct but for the addresses, its workspace bytes, and
+        whether q's strides are the kernels' (if not, the call copies it)."""
         import torch
         dtype = _rows_dtype(q.dtype)
         if dtype is None or (not isinstance(self, FourBitKVCache) and self.buf.dtype != q.dtype):
@@ -204,7 +203,8 @@ class LiveCache:
             raise ValueError("out must have q's shape and dtype, rows of 16-byte pieces")
         # a new out is contiguous
         os = _strides(out) if out is not None else [rows * heads * self.dim, heads * self.dim, self.dim]
-        op = L.AttendOp(self._view(layer), None, None, 0, 0, 0, os[0], os[1], os[2], None, None, None, None, 0, 0, None, 0,
+        qs = _strides(q)
+        op = L.AttendOp(self._view(layer), None, None, qs[0], qs[1], qs[2], os[0], os[1], os[2], None, None, None, None, 0, 0, None, 0,
                         1.0 / math.sqrt(self.dim) if scale is None else scale, dtype, heads, rows, max_len,
                         min(window, 0xffffffff), min(sinks, 0xffffffff), 0)
         if weights is not None:
@@ -218,7 +218,8 @@ class LiveCache:
                                 not lse.is_contiguous()):
             raise ValueError(f"lse must be a contiguous float32 [{self.copies}, {heads}, {rows}]")
         op.workspace_bytes = L.lib().pkv_attend_workspace(C.byref(op))
-        return op, (op.workspace_bytes, [n > 1 for n in q.shape[:3]])
+        unit = 16 // q.element_size()
+        return op, (op.workspace_bytes, q.stride(3) == 1 and all(n % unit == 0 for n in qs[:3]))
 
     # ------------------------------------------------------------ eviction
     def evict(self, lens, weights, budget: int, sinks: int = 0, recent: int = 0, layer: int | None = None, into=None,
