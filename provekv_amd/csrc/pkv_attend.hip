@@ -302,10 +302,11 @@ __global__ __launch_bounds__(256, 2) void decode_kernel(AttendDev a, Partial par
 
     float m = -kInf, l = 0.0f;
     f32x4 o[kO] = {};
-    for (int t = t0 + static_cast<int>(wave); t < t1; t += 4) {
+    auto fetch = [&](Tile& x, int t) {   // past the last tile: the last again, unused
+        x.load(kp, vp, ksp, vsp, a.kv.slot, tl.slot(min(t, t1 - 1), Tile::kStep), tl.high - 1, lane);
+    };
+    auto work = [&](Tile& x, int t) {
         const int slot = tl.slot(t, Tile::kStep);
-        Tile x;
-        x.load(kp, vp, ksp, vsp, a.kv.slot, slot, tl.high - 1, lane);
         // logits
         f32x4 sc[kSub] = {};
         for (int u = 0; u < kSub; ++u)
@@ -406,6 +407,19 @@ __global__ __launch_bounds__(256, 2) void decode_kernel(AttendDev a, Partial par
             }
         } else {
             gather(o, x);
+        }
+    };
+    // two tiles in turn: one is on its way while the other is worked on
+    const int first = t0 + static_cast<int>(wave);
+    if (first < t1) {
+        Tile even, odd;
+        fetch(even, first);
+        for (int t = first; t < t1; t += 8) {
+            fetch(odd, t + 4);
+            work(even, t);
+            if (t + 4 >= t1) break;
+            fetch(even, t + 8);
+            work(odd, t + 4);
         }
     }
     l += __shfl_xor(l, 16);
