@@ -135,6 +135,7 @@ AttendDev attend_dev(const pkv_attend_op& op) {
     a.max_len = op.max_len ? op.max_len : op.cache.slots;
     a.window = op.window;
     a.sinks = op.sinks;
+    a.reach = op.window ? std::min(op.window, 0x80000000u) : 0x80000000u;
     a.scale2 = static_cast<float>(static_cast<double>(op.scale) * 1.4426950408889634074);
     return a;
 }

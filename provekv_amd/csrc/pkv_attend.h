@@ -29,6 +29,7 @@ struct AttendDev {
     uint64_t w_copy, w_head;
     float* stats;          // (max logit * scale * log2 e, 1 / sum) of [copy][kv head][row i * group + g]
     uint32_t copies, heads, group, nq, max_len, window, sinks;
+    uint32_t reach;        // window, 2^31 at most and where there is none: a row sees slots less than this behind it
     float scale2;          // scale * log2 e
 };
 

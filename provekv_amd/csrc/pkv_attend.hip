@@ -48,8 +48,10 @@ __device__ inline Span span(const AttendDev& a, uint32_t c) {
     s.first = s.len - s.rows;
     return s;
 }
+// The row at `pos` sees slot j (reach: the window, or 2^31 for none).
+__device__ inline bool in_reach(const AttendDev& a, int pos, int j) { return static_cast<uint32_t>(pos - j) < a.reach; }
 __device__ inline bool visible(const AttendDev& a, int pos, int j) {
-    return j <= pos && (!a.window || static_cast<uint32_t>(pos - j) < a.window || static_cast<uint32_t>(j) < a.sinks);
+    return in_reach(a, pos, j) | ((j <= pos) & (static_cast<uint32_t>(j) < a.sinks));   // no branches
 }
 
 // x combined with the lane 32 or 16 away, by lane swaps (a shuffle goes through LDS).
@@ -155,7 +157,7 @@ __device__ inline Tiles tiles_of(const AttendDev& a, int pos0, int pos1, int ste
 }
 // Every row between pos0 and pos1 sees all of lo .. hi.
 __device__ inline bool all_visible(const AttendDev& a, int pos0, int pos1, int lo, int hi) {
-    return hi <= pos0 && (!a.window || static_cast<uint32_t>(pos1 - lo) < a.window || static_cast<uint32_t>(hi) < a.sinks);
+    return hi <= pos0 && (in_reach(a, pos1, lo) || static_cast<uint32_t>(hi) < a.sinks);
 }
 // Some row of the tile list's rows sees slot j.
 __device__ inline bool any_visible(const AttendDev& a, const Tiles& t, int j) {
@@ -755,7 +757,9 @@ __device__ inline f32x16 logits32(const uint8_t* lds, int u, const Query<CT, QT,
     return s;
 }
 
-constexpr uint32_t kRowTile = 128;   // query rows (rows x group of one KV head) of a workgroup
+// Query rows (rows x group of one KV head) of a workgroup whose waves share
+// every tile's slots `ks` ways.
+constexpr uint32_t row_tile(int ks) { return 128u / ks; }
 
 // Query rows in tiles of 128, 32 a wave, against tiles of 64 slots (f32: 32)
 // staged through LDS in two buffers, one barrier a tile:
@@ -773,16 +777,19 @@ constexpr uint32_t kRowTile = 128;   // query rows (rows x group of one KV head)
 // slot.  The loop does not look for those: an output that is not finite sends
 // the workgroup through it again, with infinities and NaN taken out of the
 // staged values and each added afterwards to the rows that see it.
-template <int CT, int QT, int D>
+template <int CT, int QT, int D, int KS>
 __global__ __launch_bounds__(256, (query_terms(CT, QT) * D >= 256 ? 1 : 2)) void rows_kernel(AttendDev a, Partial part,
                                                                                         uint32_t row_tiles) {
     __shared__ __align__(16) uint8_t lds[2 * Stage<CT, D>::kBytes];
     using T = typename Elem<QT>::T;
     using St = Stage<CT, D>;
-    constexpr int MT = mat_type(CT), kU = St::kSlots / 32, kO = D / 32;
+    constexpr int MT = mat_type(CT), kU = St::kSlots / 32 / KS, kO = D / 32;   // kU: 32-slot pieces a wave takes of a tile
     constexpr int NP = CT == PKV_FP4 ? query_terms(CT, QT) : 1;
-    const uint32_t lane = threadIdx.x % 64, wave = __builtin_amdgcn_readfirstlane(threadIdx.x / 64);
+    constexpr uint32_t kRowTile = row_tile(KS);
+    const uint32_t lane = threadIdx.x % 64, wave_id = __builtin_amdgcn_readfirstlane(threadIdx.x / 64);
     const uint32_t n = lane % 32, half = lane / 32;
+    const uint32_t wave = wave_id % (4 / KS);                     // its 32 rows
+    const int share = static_cast<int>(wave_id / (4 / KS)) * 32 * kU;   // its slots of a tile: share .. + 32 kU
     // heads fastest, so that a head's workgroups share an XCD's L2 where the heads are a multiple of 8; row tiles
     // from the last, whose rows see most
     const uint32_t heads = a.copies * a.heads;
@@ -821,7 +828,8 @@ __global__ __launch_bounds__(256, (query_terms(CT, QT) * D >= 256 ? 1 : 2)) void
     };
     // no row of the wave sees any of the tile
     auto skip = [&](int slot) {
-        return slot >= wt.high || (slot + St::kSlots <= wt.low && static_cast<uint32_t>(slot) >= a.sinks);
+        return slot + share >= wt.high ||
+               (slot + share + 32 * kU <= wt.low && static_cast<uint32_t>(slot + share) >= a.sinks);
     };
     for (bool clean = false;; clean = true) {
         m = -kInf;
@@ -842,11 +850,20 @@ __global__ __launch_bounds__(256, (query_terms(CT, QT) * D >= 256 ? 1 : 2)) void
             }
             if (!skip(slot)) {
                 f32x16 sc[kU];
-                for (int u = 0; u < kU; ++u) sc[u] = logits32<CT, QT, D>(buf, u, q, lane);
-                if (!all_visible(a, wpos0, wpos1, slot, slot + St::kSlots - 1))
-                    for (int u = 0; u < kU; ++u)
-                        for (int x = 0; x < 16; ++x)
-                            if (!visible(a, pos, slot + 32 * u + row32(x, half))) sc[u][x] = -kInf;
+                const int mine = slot + share;
+                for (int u = 0; u < kU; ++u) sc[u] = logits32<CT, QT, D>(buf + share * St::kRow, u, q, lane);
+                if (!all_visible(a, wpos0, wpos1, mine, mine + 32 * kU - 1)) {
+                    const int off = pos - mine - 4 * static_cast<int>(half);   // less the register's place: how far back
+                    if (static_cast<uint32_t>(mine) >= a.sinks) {
+                        for (int u = 0; u < kU; ++u)
+                            for (int x = 0; x < 16; ++x)
+                                if (!in_reach(a, off, 32 * u + row32(x, 0))) sc[u][x] = -kInf;
+                    } else {
+                        for (int u = 0; u < kU; ++u)
+                            for (int x = 0; x < 16; ++x)
+                                if (!visible(a, pos, mine + 32 * u + row32(x, half))) sc[u][x] = -kInf;
+                    }
+                }
                 float top = sc[0][0];
                 for (int u = 0; u < kU; ++u)
                     for (int x = 0; x < 16; ++x) top = fmaxf(top, sc[u][x]);
@@ -884,7 +901,7 @@ __global__ __launch_bounds__(256, (query_terms(CT, QT) * D >= 256 ? 1 : 2)) void
                                 pt[k] = u32x4{pack_term<MT>(p[0], p[1]), pack_term<MT>(p[2], p[3]),
                                               pack_term<MT>(p[4], p[5]), pack_term<MT>(p[6], p[7])};
                             for (int e = 0; e < kO; ++e) {
-                                const u32x4 v = St::values16(buf, 32 * u + 16 * y, e, lane);
+                                const u32x4 v = St::values16(buf + share * St::kRow, 32 * u + 16 * y, e, lane);
                                 for (int k = NP - 1; k >= 0; --k) o[e] = mma32<MT>(v, pt[k], o[e]);
                             }
                         }
@@ -914,7 +931,7 @@ __global__ __launch_bounds__(256, (query_terms(CT, QT) * D >= 256 ? 1 : 2)) void
             st.land(buf);
             __syncthreads();
 #pragma unroll 1
-            for (int j = 0; j < St::kSlots; ++j) {
+            for (int j = share; j < share + 32 * kU; ++j) {
                 const bool sees = visible(a, pos, slot + j);
                 if (!__any(sees)) continue;
                 uint32_t hf = half;
@@ -938,6 +955,24 @@ __global__ __launch_bounds__(256, (query_terms(CT, QT) * D >= 256 ? 1 : 2)) void
         break;
     }
     l += __shfl_xor(l, 32);
+    if constexpr (KS > 1) {
+        // the other share of the slots joins the first: [row block][o, m, l][lane]
+        float* to = reinterpret_cast<float*>(lds) + wave * (16 * kO + 2) * 64 + lane;
+        if (share) {
+            for (int x = 0; x < 16 * kO; ++x) to[x * 64] = o[x / 16][x % 16];
+            to[16 * kO * 64] = m;
+            to[(16 * kO + 1) * 64] = l;
+        }
+        __syncthreads();
+        if (share) return;
+        const float m2 = to[16 * kO * 64], l2 = to[(16 * kO + 1) * 64], top = fmaxf(m, m2);
+        // a share without a largest logit has o = 0 and the sum 0, or NaN from NaN logits
+        const float f = m == top || m == -kInf ? 1.0f : exp2f((m - top) * a.scale2);
+        const float f2 = m2 == top || m2 == -kInf ? 1.0f : exp2f((m2 - top) * a.scale2);
+        m = top;
+        l = l * f + l2 * f2;
+        for (int x = 0; x < 16 * kO; ++x) o[x / 16][x % 16] = o[x / 16][x % 16] * f + to[x * 64] * f2;
+    }
     if (!real) return;
     const uint64_t all = static_cast<uint64_t>(a.nq) * a.group;
     if (part.splits > 1) {
@@ -1010,6 +1045,16 @@ __global__ __launch_bounds__(256) void join_rows_kernel(AttendDev a, Partial par
     }
 }
 
+// left[0 .. N) = the half of left[0 .. 2N) that the lane keeps (upper: the
+// second) and the lane across's share of it.
+template <int CTRL, int N>
+__device__ inline void hand_over(float (&left)[16], bool upper) {
+    for (int x = 0; x < N; ++x) {
+        const float keep = upper ? left[x + N] : left[x], give = upper ? left[x] : left[x + N];
+        left[x] = keep + __uint_as_float(__builtin_amdgcn_update_dpp(0u, __float_as_uint(give), CTRL, 15, 15, true));
+    }
+}
+
 // Accumulated weights of many rows: 32 slots a wave, its keys held in registers
 // as the S^T operand, all rows that can see them streamed through LDS (four
 // waves share them) 64 at a time (queries of more than one term: 32), straight
@@ -1038,10 +1083,12 @@ __global__ __launch_bounds__(256, 2) void weights_kernel(AttendDev a, Shares sha
     const uint32_t ch = blockIdx.x % heads, c = ch / a.heads, h = ch % a.heads;
     const uint32_t split = blockIdx.x / heads % shares.splits;
     const Span sp = span(a, c);
-    const int G = static_cast<int>(a.group), b0 = static_cast<int>(blockIdx.x / heads / shares.splits) * 128;
-    const int s0 = b0 + 32 * static_cast<int>(wave);
-    const int high = sp.first + sp.rows;                 // slots below it are seen by the last row or hidden by its window
-    if (b0 >= high || sp.rows == 0) return;
+    // the grid's blocks are those that some row sees, the first ones and those of the window, of this copy's length
+    const Tiles tl = tiles_of(a, sp.first, sp.rows ? sp.first + sp.rows - 1 : -1, 128);
+    const int block = static_cast<int>(blockIdx.x / heads / shares.splits);
+    if (block >= tl.count) return;
+    const int G = static_cast<int>(a.group), b0 = tl.slot(block, 128), s0 = b0 + 32 * static_cast<int>(wave);
+    const int high = tl.high;
     // rows i0 .. i1 see something of b0 .. b0 + 127
     const int i0 = max(b0 - sp.first, 0);
     const int64_t reach = !a.window || static_cast<uint32_t>(b0) < a.sinks
@@ -1069,35 +1116,42 @@ __global__ __launch_bounds__(256, 2) void weights_kernel(AttendDev a, Shares sha
     const uint64_t all = static_cast<uint64_t>(a.nq) * a.group;
     const T* qp = reinterpret_cast<const T*>(a.q) + c * a.q_copy + static_cast<uint64_t>(h) * a.group * a.q_head;
     const uint32_t at = static_cast<uint32_t>(reinterpret_cast<uintptr_t>((LdsByte*)&lds[0][0]));
-    // Row that this thread fetches a piece of, as (row, head of the group); steps of rows without dividing again.
+    // Rows that this thread fetches a piece of: (row, head of the group) and where it is; a step of kRows rows without
+    // dividing or multiplying again.
     struct At {
         int i, g;
+        const T* p;
     };
-    auto step = [&](At x, int rows_i, int rows_g) {
-        x.i += rows_i;
-        x.g += rows_g;
+    const int adv_i = kRows / G, adv_g = kRows % G;
+    const int64_t adv = static_cast<int64_t>(adv_i) * a.q_row + static_cast<int64_t>(adv_g) * a.q_head;
+    const int64_t wrap = static_cast<int64_t>(a.q_row) - static_cast<int64_t>(G) * a.q_head;
+    auto step = [&](At x) {
+        x.i += adv_i;
+        x.g += adv_g;
+        x.p += adv;
         if (x.g >= G) {
             x.g -= G;
             ++x.i;
+            x.p += wrap;
         }
         return x;
     };
+    const T* last_row = qp + static_cast<uint64_t>(i1) * a.q_row + static_cast<uint64_t>(G - 1) * a.q_head;
     constexpr int kCopies = kRows * St::kRow / 4096, kStep = St::kCopyStep;
     const uint32_t mine = kTerms == 1 ? St::kCopyRows * wave + lane / kPieces : threadIdx.x / kPieces;
     constexpr int kMoves = kTerms == 1 ? kCopies : kRows * kPieces / 256, kMoveStep = kTerms == 1 ? kStep : 256 / kPieces;
     At here[kMoves];
     for (int x = 0; x < kMoves; ++x) {
         const int row = static_cast<int>(mine) + kMoveStep * x;
-        here[x] = At{(r0 + row) / G, (r0 + row) % G};
+        const int i = (r0 + row) / G, g = (r0 + row) % G;
+        here[x] = At{i, g, qp + static_cast<uint64_t>(i) * a.q_row + static_cast<uint64_t>(g) * a.q_head};
     }
-    const int adv_i = kRows / G, adv_g = kRows % G;
     u32x4 w[kTerms == 1 ? 1 : kMoves];      // a multi-term query on its way (f16: 8 values; f32: the first half)
     u32x4 w2[QT == PKV_F32 && kTerms > 1 ? kMoves : 1];
     auto fetch = [&](uint32_t b) {
         const uint32_t piece = (kTerms == 1 ? lane : threadIdx.x) % kPieces;
         for (int x = 0; x < kMoves; ++x) {
-            const At r = here[x].i <= i1 ? here[x] : At{i1, G - 1};
-            const T* p = qp + static_cast<uint64_t>(r.i) * a.q_row + static_cast<uint64_t>(r.g) * a.q_head;
+            const T* p = here[x].i <= i1 ? here[x].p : last_row;
             if constexpr (kTerms == 1) {
                 const uint32_t row = mine + kStep * x;
                 copy_row_to_lds(at + b * kTermBytes + (kStep * x + St::kCopyRows * wave) * St::kRow,
@@ -1106,7 +1160,7 @@ __global__ __launch_bounds__(256, 2) void weights_kernel(AttendDev a, Shares sha
                 w[x] = reinterpret_cast<const u32x4*>(p + 8 * piece)[0];
                 if constexpr (QT == PKV_F32) w2[x] = reinterpret_cast<const u32x4*>(p + 8 * piece)[1];
             }
-            here[x] = step(here[x], adv_i, adv_g);
+            here[x] = step(here[x]);
         }
     };
     auto land = [&](uint32_t b) {
@@ -1144,7 +1198,7 @@ __global__ __launch_bounds__(256, 2) void weights_kernel(AttendDev a, Shares sha
     }
     __syncthreads();
     uint32_t b = 0;
-    At top = {r0 / G, r0 % G};               // of row r
+    At top = {r0 / G, r0 % G, qp};           // of row r
     for (int r = r0; r < r1; r += kRows, b ^= 1) {
         for (int u = 0; u < kU; ++u) now[u] = next[u];
         if (r + kRows < r1) {
@@ -1154,6 +1208,10 @@ __global__ __launch_bounds__(256, 2) void weights_kernel(AttendDev a, Shares sha
         for (int u = 0; u < kU; ++u) {
             const int ru = r + 32 * u;
             if (ru >= r1) break;
+            // positions of the piece's rows, from below and above
+            const int pa = sp.first + top.i + (kU > 1 && u ? 32 / G : 0), pb = sp.first + top.i + (32 * u + 31 + G) / G;
+            // none of them sees any of the wave's slots
+            if (pb < s0 || (pa > s0 + 31 && !in_reach(a, pa, s0 + 31) && static_cast<uint32_t>(s0) >= a.sinks)) continue;
             f32x16 s = {};
             for (int x = 0; x < Q::kRegs; ++x)
                 for (int z = kTerms - 1; z >= 0; --z) {
@@ -1168,30 +1226,37 @@ __global__ __launch_bounds__(256, 2) void weights_kernel(AttendDev a, Shares sha
                     }
                 }
             const float mc = now[u][0], inv = now[u][1];
-            // positions of the piece's rows, from above (the last one's a little late)
-            const int pa = sp.first + top.i + (kU > 1 && u ? 32 / G : 0), pb = sp.first + top.i + (32 * u + 31 + G) / G;
             if (ru + 32 <= r1 && all_visible(a, pa, pb, s0, s0 + 31)) {
                 for (int x = 0; x < 16; ++x)
                     sum[x] = __builtin_fmaf(__builtin_amdgcn_exp2f(__builtin_fmaf(s[x], a.scale2, mc)), inv, sum[x]);
             } else {
                 const int pos = sp.first + (ru + static_cast<int>(n)) / G;
-                const bool in = ru + static_cast<int>(n) < r1 && inv != 0.0f;
-                for (int x = 0; x < 16; ++x)
-                    if (in && visible(a, pos, s0 + row32(x, half)))
-                        sum[x] = __builtin_fmaf(__builtin_amdgcn_exp2f(__builtin_fmaf(s[x], a.scale2, mc)), inv, sum[x]);
+                const bool in = (ru + static_cast<int>(n) < r1) & (inv != 0.0f);
+                const bool sink = static_cast<uint32_t>(s0) < a.sinks;
+                const int off = in ? pos - s0 - 4 * static_cast<int>(half) : -1;   // less the register's place: how far back
+                for (int x = 0; x < 16; ++x) {
+                    const float more = __builtin_fmaf(__builtin_amdgcn_exp2f(__builtin_fmaf(s[x], a.scale2, mc)), inv, sum[x]);
+                    bool see = in_reach(a, off, row32(x, 0));
+                    if (sink) see = in & visible(a, pos, s0 + row32(x, half));
+                    sum[x] = see ? more : sum[x];
+                }
             }
         }
-        top = step(top, adv_i, adv_g);
+        top = step(top);
         if (r + kRows < r1) land(b ^ 1);
         __syncthreads();
     }
-    float total = 0.0f;                      // lane n < 16 of a half: register n's slot
-    for (int x = 0; x < 16; ++x) {
-        for (int y = 16; y; y >>= 1) sum[x] += __shfl_xor(sum[x], y);
-        total = n == static_cast<uint32_t>(x) ? sum[x] : total;
-    }
+    // Register n % 16 summed over the half's 32 lanes: each step hands half of the registers to the lane across and
+    // keeps the other half, 16 to 1 over 16 lanes, then the other 16.
+    float left[16];
+    for (int x = 0; x < 16; ++x) left[x] = sum[x];
+    hand_over<0x140, 8>(left, n & 8);        // row_mirror
+    hand_over<0x141, 4>(left, n & 4);        // row_half_mirror
+    hand_over<0x1b, 2>(left, n & 2);         // quad_perm 3 2 1 0
+    hand_over<0xb1, 1>(left, n & 1);         // quad_perm 1 0 3 2
+    const float total = across16(left[0], [](float x, float y) { return x + y; });
     const int j = s0 + row32(static_cast<int>(n), half);
-    if (n >= 16 || !any_visible(a, tiles_of(a, sp.first, high - 1, 1), j)) return;
+    if (n >= 16 || !any_visible(a, tl, j)) return;
     if (shares.splits == 1) a.weights[c * a.w_copy + h * a.w_head + j] += total;
     else shares.sums[(static_cast<uint64_t>(split) * heads + ch) * shares.ld + j] = total;
 }
@@ -1527,36 +1592,51 @@ constexpr uint32_t kDecodeRows = 16;   // rows x group that decode_kernel takes
 // workgroups) while a share has work for its waves.
 struct Plan {
     uint32_t row_tiles, splits, rows, ld;
-    uint32_t w_splits, w_ld;             // shares of the rows in weights_kernel
+    int ks;                              // rows_kernel: shares of a tile's slots among a workgroup's waves
+    uint32_t w_blocks, w_splits, w_ld;   // weights_kernel: blocks of slots, shares of the rows
     uint64_t ml, logits, stats, shares, bytes;   // offsets in the workspace (partial outputs first), all of it
 };
+constexpr uint64_t kHalf = 6;
 Plan plan_of(const AttendDev& a, uint32_t dim, int cache_dtype) {
     Plan p{};
     const uint64_t all = static_cast<uint64_t>(a.nq) * a.group, heads = static_cast<uint64_t>(a.copies) * a.heads;
     const bool few = all <= kDecodeRows;
     const uint32_t step = (few ? 32 : 64) / (cache_dtype == PKV_F32 ? 2 : 1);
-    p.row_tiles = few ? 1 : static_cast<uint32_t>((all + kRowTile - 1) / kRowTile);
-    p.rows = few ? kDecodeRows : p.row_tiles * kRowTile;
-    // slots that a row tile can see: all, or the window, the rows before its last and the sinks, each up to a tile more
-    uint64_t most = a.max_len;
-    if (a.window)
-        most = std::min<uint64_t>(most, static_cast<uint64_t>(a.window) + std::min<uint64_t>(a.nq, p.rows) + a.sinks + 2 * step);
-    const uint64_t tiles = (most + step - 1) / step, groups = heads * p.row_tiles;
+    // tiles of slots that a tile of `rows` rows can see: all, or the window, the rows before its last and the sinks, each up
+    // to a tile more
+    auto tiles_for = [&](uint32_t rows) {
+        uint64_t most = a.max_len;
+        if (a.window)
+            most = std::min<uint64_t>(most, static_cast<uint64_t>(a.window) + std::min<uint64_t>(a.nq, rows) + a.sinks + 2 * step);
+        return (most + step - 1) / step;
+    };
+    p.ks = 1;
     if (few) {
         // 768 workgroups are three a CU; every wave of a share has a tile
-        p.splits = static_cast<uint32_t>(std::max<uint64_t>(1, std::min<uint64_t>((768 + groups - 1) / groups, tiles / 4)));
+        p.row_tiles = 1;
+        p.rows = kDecodeRows;
+        p.splits = static_cast<uint32_t>(std::max<uint64_t>(
+            1, std::min<uint64_t>((768 + heads - 1) / heads, tiles_for(kDecodeRows) / 4)));
     } else {
-        // The least of rounds x tiles a share: as many workgroups as fit run at the speed of one (2 us a tile), and
-        // a share costs four tiles' time for its start and end, and the passage of its outputs through memory.
+        // The least time, in tenths of the 2 us that a tile takes a workgroup of 128 rows (64 rows: kHalf): as many
+        // workgroups as fit run at the speed of one, and a share costs four tiles' time for its start and end, and the
+        // passage of its outputs through memory.
         const uint64_t fit = 256 * (dim == 64 && cache_dtype != PKV_FP4 ? 3 : 2);
         uint64_t least = ~0ull;
-        for (uint32_t n = 1; n <= 16 && (n == 1 || n * 4 <= tiles); ++n) {
-            const uint64_t rounds = (groups * n + fit - 1) / fit;
-            const uint64_t cost = rounds * ((tiles + n - 1) / n + (n == 1 ? 2 : 4)) +
-                                  (n == 1 ? 0 : heads * all * dim * 8 * n / 8000000);
-            if (cost < least) {
-                least = cost;
-                p.splits = n;
+        for (int ks = 1; ks <= (cache_dtype == PKV_F32 ? 1 : 2); ++ks) {
+            const uint32_t rt = row_tile(ks), row_tiles = static_cast<uint32_t>((all + rt - 1) / rt);
+            const uint64_t groups = heads * row_tiles, tiles = tiles_for(rt);
+            for (uint32_t n = 1; n <= 16 && (n == 1 || n * 4 <= tiles); ++n) {
+                const uint64_t rounds = (groups * n + fit - 1) / fit;
+                const uint64_t cost = rounds * ((tiles + n - 1) / n + (n == 1 ? 2 : 4)) * (ks == 1 ? 10 : kHalf) +
+                                      (n == 1 ? 0 : heads * all * dim * 8 * n / 800000);
+                if (cost < least) {
+                    least = cost;
+                    p.splits = n;
+                    p.ks = ks;
+                    p.row_tiles = row_tiles;
+                    p.rows = row_tiles * rt;
+                }
             }
         }
     }
@@ -1569,11 +1649,13 @@ Plan plan_of(const AttendDev& a, uint32_t dim, int cache_dtype) {
     p.w_splits = 1;
     p.w_ld = (a.max_len + 127) / 128 * 128;
     if (!few && a.weights) {
-        // blocks of 128 slots that some row sees; three workgroups a CU, at least 256 rows each
-        uint64_t seen = a.max_len;
-        if (a.window) seen = std::min<uint64_t>(seen, static_cast<uint64_t>(a.window) + a.nq + a.sinks + 256);
-        const uint64_t blocks = (seen + 127) / 128 * heads;
-        p.w_splits = static_cast<uint32_t>(std::max<uint64_t>(1, std::min<uint64_t>(768 / blocks, all / 256)));
+        // blocks of 128 slots that some row sees, one more for the window's first; eight workgroups a CU, since they see
+        // very different numbers of rows, of at least 256 rows each
+        p.w_blocks = p.w_ld / 128;
+        if (a.window)
+            p.w_blocks = static_cast<uint32_t>(std::min<uint64_t>(
+                p.w_blocks, (static_cast<uint64_t>(a.window) + a.nq + 126) / 128 + 1 + (static_cast<uint64_t>(a.sinks) + 127) / 128));
+        p.w_splits = static_cast<uint32_t>(std::max<uint64_t>(1, std::min<uint64_t>(2048 / (p.w_blocks * heads), all / 256)));
     }
     p.bytes = p.shares + (p.w_splits > 1 ? round256(4ull * heads * p.w_splits * p.w_ld) : 0);
     return p;
@@ -1593,12 +1675,15 @@ int attend_typed(AttendDev a, uint8_t* ws, hipStream_t st) {
         return hipGetLastError();
     }
     a.stats = a.weights ? reinterpret_cast<float*>(ws + p.stats) : nullptr;
-    rows_kernel<CT, QT, D><<<heads * p.row_tiles * p.splits, 256, 0, st>>>(a, part, p.row_tiles);
+    if constexpr (CT != PKV_F32) {
+        if (p.ks == 2) rows_kernel<CT, QT, D, 2><<<heads * p.row_tiles * p.splits, 256, 0, st>>>(a, part, p.row_tiles);
+    }
+    if (p.ks == 1) rows_kernel<CT, QT, D, 1><<<heads * p.row_tiles * p.splits, 256, 0, st>>>(a, part, p.row_tiles);
     constexpr uint32_t kJoin = 1024 / D;     // rows of a workgroup
     if (p.splits > 1) join_rows_kernel<QT, D><<<(a.nq * a.group + kJoin - 1) / kJoin * heads, 256, 0, st>>>(a, part);
     if (a.weights) {
         const Shares shares{reinterpret_cast<float*>(ws + p.shares), p.w_splits, p.w_ld};
-        weights_kernel<CT, QT, D><<<p.w_ld / 128 * heads * p.w_splits, 256, 0, st>>>(a, shares);
+        weights_kernel<CT, QT, D><<<p.w_blocks * heads * p.w_splits, 256, 0, st>>>(a, shares);
         const uint32_t blocks = (a.max_len + 255) / 256;
         if (p.w_splits > 1) add_weights_kernel<<<blocks * heads, 256, 0, st>>>(a, shares, blocks);
     }
