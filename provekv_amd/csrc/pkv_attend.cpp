@@ -144,7 +144,10 @@ int check_rows(const pkv_rows_op& op, bool store) {
     const int rc = check_view(op.cache, store);
     if (rc) return rc;
     if (op.cache.dtype != PKV_FP4 || op.dtype < PKV_F32 || op.dtype > PKV_F16) return PKV_ERR_INVALID_ARG;
-    if (op.rows > kMaxCount / 2 || !op.d_first || !aligned(op.d_first, 4) || !aligned(op.d_counts, 4))
+    if (op.rows > kMaxCount / 2 || !op.d_first ||
+        static_cast<U128>(op.cache.copies) * op.cache.layers * op.cache.heads * op.rows > 0xffffffffu)
+        return PKV_ERR_INVALID_ARG;
+    if (!aligned(op.d_first, 4) || !aligned(op.d_counts, 4))
         return PKV_ERR_INVALID_ARG;
     if (!aligned(op.d_keys, 16) || !aligned(op.d_values, 16)) return PKV_ERR_INVALID_ARG;
     const uint64_t unit = 16 / elem_bytes(op.dtype);
