@@ -102,20 +102,6 @@ KvDev dev(const pkv_kv_view& v) {
             v.d_value_scales, v.copy_stride, v.layer_stride, v.head_stride, v.slot_stride};
 }
 
-// What pkv_attend_workspace looks at.
-int check_attend_shape(const pkv_attend_op& op) {
-    const pkv_kv_view& v = op.cache;
-    if (v.dim != 64 && v.dim != 128) return PKV_ERR_UNSUPPORTED;
-    if (v.dtype < PKV_F32 || v.dtype > PKV_FP4 || op.dtype < PKV_F32 || op.dtype > PKV_F16)
-        return PKV_ERR_INVALID_ARG;
-    if (v.dtype != PKV_FP4 && op.dtype != v.dtype) return PKV_ERR_INVALID_ARG;
-    if (v.layers != 1 || !v.copies || !v.heads || !v.slots || v.slots > kMaxCount / 2 || op.max_len > v.slots)
-        return PKV_ERR_INVALID_ARG;
-    if (!op.q_heads || op.q_heads % v.heads || op.reserved) return PKV_ERR_INVALID_ARG;
-    if (static_cast<U128>(v.copies) * op.q_heads * std::max(op.nq, 1u) > kMaxCount) return PKV_ERR_INVALID_ARG;
-    return PKV_OK;
-}
-
 AttendDev attend_dev(const pkv_attend_op& op) {
     AttendDev a{};
     a.kv = dev(op.cache);
@@ -138,6 +124,22 @@ AttendDev attend_dev(const pkv_attend_op& op) {
     a.reach = op.window ? std::min(op.window, 0x80000000u) : 0x80000000u;
     a.scale2 = static_cast<float>(static_cast<double>(op.scale) * 1.4426950408889634074);
     return a;
+}
+
+// What pkv_attend_workspace looks at.
+int check_attend_shape(const pkv_attend_op& op) {
+    const pkv_kv_view& v = op.cache;
+    if (v.dim != 64 && v.dim != 128) return PKV_ERR_UNSUPPORTED;
+    if (v.dtype < PKV_F32 || v.dtype > PKV_FP4 || op.dtype < PKV_F32 || op.dtype > PKV_F16)
+        return PKV_ERR_INVALID_ARG;
+    if (v.dtype != PKV_FP4 && op.dtype != v.dtype) return PKV_ERR_INVALID_ARG;
+    if (v.layers != 1 || !v.copies || !v.heads || !v.slots || v.slots > kMaxCount / 2 || op.max_len > v.slots)
+        return PKV_ERR_INVALID_ARG;
+    if (!op.q_heads || op.q_heads % v.heads || op.reserved) return PKV_ERR_INVALID_ARG;
+    if (op.nq > kMaxCount / 2 || static_cast<U128>(v.copies) * op.q_heads * std::max(op.nq, 1u) > kMaxCount)
+        return PKV_ERR_INVALID_ARG;
+    if (op.nq && !attend_fits(attend_dev(op), v.dim, v.dtype)) return PKV_ERR_INVALID_ARG;
+    return PKV_OK;
 }
 
 int check_rows(const pkv_rows_op& op, bool store) {
@@ -221,7 +223,7 @@ int pkv_attend(pkv_ctx* ctx, const pkv_attend_op* op, void* stream) {
     int rc = check_attend_shape(*op);
     if (!rc) rc = check_view(op->cache, false);
     if (rc) return rc;
-    if (!std::isfinite(op->scale) || !(op->scale > 0.0f)) return PKV_ERR_INVALID_ARG;
+    if (!(op->scale > 0.0f) || !std::isfinite(attend_dev(*op).scale2)) return PKV_ERR_INVALID_ARG;
     if (!op->d_lens || !aligned(op->d_lens, 4) || !aligned(op->d_q_lens, 4) || !aligned(op->d_lse, 4) ||
         !aligned(op->d_weights, 4))
         return PKV_ERR_INVALID_ARG;
@@ -296,6 +298,7 @@ int pkv_evict(pkv_ctx* ctx, const pkv_evict_op* op, void* stream) {
     e.copies = c.copies; e.layers = c.layers; e.heads = c.heads; e.slots = c.slots; e.into_slots = t.slots;
     e.budget = op->budget; e.sinks = op->sinks; e.recent = op->recent;
     e.in_place = in_place;
+    if (!evict_fits(e)) return PKV_ERR_INVALID_ARG;
     OnDevice dv(ctx_device(ctx));
     if (dv.rc) return dv.rc;
     return hip_rc(launch_evict(e, c.dim, c.dtype, stream));

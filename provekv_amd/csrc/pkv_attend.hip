@@ -102,6 +102,15 @@ __device__ inline uint32_t pack_term(float& a, float& b) {
     }
 }
 
+// The same for a query's values: what an infinity or NaN leaves is 0, so that
+// the terms' products sum to what the value's own would.
+__device__ inline uint32_t pack_query_term(float& a, float& b) {
+    const uint32_t h = pack_term<PKV_BF16>(a, b);
+    if ((h & 0x7f80u) == 0x7f80u) a = 0.0f;
+    if ((h >> 16 & 0x7f80u) == 0x7f80u) b = 0.0f;
+    return h;
+}
+
 // Two 16-bit values that hold an infinity or NaN.
 template <int MT>
 __device__ inline bool nonfinite2(uint32_t x) {
@@ -280,7 +289,7 @@ __global__ __launch_bounds__(256, 2) void decode_kernel(AttendDev a, Partial par
             for (int w = 0; w < 4; ++w) {
                 float x = real ? static_cast<float>(qp[d + 2 * w]) : 0.0f;
                 float y = real ? static_cast<float>(qp[d + 2 * w + 1]) : 0.0f;
-                for (int n = 0; n < NQ; ++n) q[n][s][w] = pack_term<PKV_BF16>(x, y);
+                for (int n = 0; n < NQ; ++n) q[n][s][w] = pack_query_term(x, y);
             }
         }
     }
@@ -571,7 +580,7 @@ struct Query {
                 for (int w = 0; w < 4; ++w) {
                     float x = real ? static_cast<float>(p[d + 2 * w]) : 0.0f;
                     float y = real ? static_cast<float>(p[d + 2 * w + 1]) : 0.0f;
-                    for (int n = 0; n < kTerms; ++n) q[n][s][w] = pack_term<PKV_BF16>(x, y);
+                    for (int n = 0; n < kTerms; ++n) q[n][s][w] = pack_query_term(x, y);
                 }
             }
         }
@@ -1170,7 +1179,7 @@ __global__ __launch_bounds__(256, 2) void weights_kernel(AttendDev a, Shares sha
                         f0 = static_cast<float>(f[0]);
                         f1 = static_cast<float>(f[1]);
                     }
-                    for (int z = 0; z < kTerms; ++z) y[z][e] = pack_term<PKV_BF16>(f0, f1);
+                    for (int z = 0; z < kTerms; ++z) y[z][e] = pack_query_term(f0, f1);
                 }
                 for (int z = 0; z < kTerms; ++z) *reinterpret_cast<u32x4*>(lds[b] + z * kTermBytes + to) = y[z];
             }
@@ -1622,7 +1631,7 @@ Plan plan_of(const AttendDev& a, uint32_t dim, int cache_dtype) {
     if (few) {
         // 768 workgroups are three a CU; every wave of a share has a tile
         p.row_tiles = 1;
-        p.rows = kDecodeRows;
+        p.rows = static_cast<uint32_t>(all);
         p.splits = static_cast<uint32_t>(std::max<uint64_t>(
             1, std::min<uint64_t>((768 + heads - 1) / heads, tiles_for(kDecodeRows) / 4)));
     } else {
@@ -1705,6 +1714,15 @@ int attend_dim(const AttendDev& a, uint32_t dim, uint8_t* ws, hipStream_t st) {
 
 }  // namespace
 
+// Every launch's threads along x stay below 2^32.
+bool attend_fits(const AttendDev& a, uint32_t dim, int cache_dtype) {
+    const Plan p = plan_of(a, dim, cache_dtype);
+    const uint64_t heads = static_cast<uint64_t>(a.copies) * a.heads, all = static_cast<uint64_t>(a.nq) * a.group;
+    const uint64_t most = std::max<uint64_t>({heads * p.splits * p.row_tiles, heads * all + heads * ((a.max_len + 1023ull) / 1024),
+                                    heads * p.w_blocks * p.w_splits, heads * ((a.max_len + 255ull) / 256)});
+    return most < 1u << 24;
+}
+
 uint64_t attend_workspace(const AttendDev& a, uint32_t dim, int cache_dtype, int) {
     return plan_of(a, dim, cache_dtype).bytes;
 }
@@ -1752,6 +1770,12 @@ static int move_typed(const EvictDev& e, hipStream_t st) {
         move_kernel<DT, D, false><<<static_cast<uint32_t>(sets * 2 * batches), 256, 0, st>>>(e, batches);
     }
     return hipGetLastError();
+}
+
+bool evict_fits(const EvictDev& e) {
+    const uint64_t sets = static_cast<uint64_t>(e.copies) * e.layers * e.heads;
+    // select_kernel: 1,024 threads a set; move_kernel: at most 8 columns, or 32 rows a workgroup, of two sides
+    return sets < 1u << 22 && sets * 2 * std::max<uint64_t>(8, (std::min(e.budget, e.slots) + 31ull) / 32) < 1u << 24;
 }
 
 int launch_evict(const EvictDev& e, uint32_t dim, int dtype, void* stream) {

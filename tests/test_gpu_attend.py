@@ -322,3 +322,94 @@ def test_offsets_past_32_bits(ctx):
     ref = R.attend(q[2:, :, 7:].double(), x[:1].unsqueeze(1), x[1:].unsqueeze(1), [700], [2], 600, 0, 1 / math.sqrt(D))
     err = (out[2:, :, 7:].cpu().double() - ref["out"]).abs()
     assert (err <= R.out_bound(ref, BF16)).all() and not out[:2].any()
+
+
+@pytest.mark.parametrize("kind,dtype", KINDS, ids=KIND_IDS)
+@pytest.mark.parametrize("D", [64, 128])
+@pytest.mark.parametrize("n,G,heads,T,window", [(1, 128, 1, 300, 0), (3, 40, 1, 130, 64), (700, 1, 1, 1500, 256),
+                                               (300, 4, 5, 700, 0), (90, 2, 12, 1300, 0)])
+def test_wide_groups_and_many_rows(ctx, n, G, heads, T, window, kind, dtype, D):
+    """Row tiles of both kinds, shares of slots and of rows, weights on top."""
+    cache, k, v = make(kind, dtype, 2, heads, T, D, seed=20)
+    w = torch.zeros(2, heads, T, device="cuda")
+    lens, ql = [T, T - T // 3], [n, n - n // 4]
+    q = torch.randn(2, n, heads * G, D, generator=torch.Generator().manual_seed(2)).to(dtype)
+    lens_d, ql_d = (torch.tensor(x, dtype=torch.int32, device="cuda") for x in (lens, ql))
+    out = cache.attend(0, q.cuda(), lens_d, q_lens=ql_d, window=window, sinks=3, weights=w)
+    some = [0, 1, n // 2, n - n // 4 - 1]           # the plain form of a few rows; all rows' weights add up to their number
+    for c in range(2):
+        for i in sorted({i for i in some if i < ql[c]}):
+            ref = R.attend(q[c:c + 1, i:i + 1].double(), k[c:c + 1], v[c:c + 1], [lens[c] - ql[c] + i + 1], [1], window, 3,
+                           1 / math.sqrt(D))
+            err = (out[c:c + 1, i:i + 1].cpu().double() - ref["out"]).abs() - R.out_bound(ref, dtype)
+            assert not (err > 0).any() and not torch.isnan(err).any(), (c, i, float(err.max()))
+        total = w[c].sum(-1).cpu().double()
+        assert ((total - ql[c] * G).abs() <= ql[c] * G * 2.0 ** -14).all()
+        assert not out[c, ql[c]:].any()
+
+
+@pytest.mark.parametrize("n", [1, 40])
+def test_many_heads(ctx, n):
+    """Thousands of copies x heads."""
+    cache, k, v = make("plain", BF16, 300, 16, 33, 64, seed=21)
+    q = torch.randn(300, n, 16, 64, generator=torch.Generator().manual_seed(3)).to(BF16)
+    out = cache.attend(0, q.cuda(), 33)
+    for c, h in ((0, 0), (150, 7), (299, 15)):
+        ref = R.attend(q[c:c + 1, :, h:h + 1].double(), k[c:c + 1, h:h + 1], v[c:c + 1, h:h + 1], [33], [n], 0, 0, 0.125)
+        assert ((out[c:c + 1, :, h:h + 1].cpu().double() - ref["out"]).abs() <= R.out_bound(ref, BF16)).all()
+
+
+@pytest.mark.parametrize("dtype", [F32, F16], ids=["f32", "f16"])
+@pytest.mark.parametrize("n", [1, 40])
+def test_infinite_query_over_4_bits(ctx, n, dtype):
+    """A query of several terms with an infinity: logits are +inf or -inf as the
+    keys' signs have it -- all +inf gives NaN, all -inf an empty row."""
+    from provekv_amd.pool import FourBitKVCache
+    cache = FourBitKVCache(1, 1, 70, 64)
+    x = torch.ones(1, 1, 1, 70, 64)
+    cache.store(x.cuda(), x.cuda(), 0)
+    q = torch.zeros(1, n, 2, 64)
+    q[:, :, 0, 3], q[:, :, 1, 3] = math.inf, -math.inf
+    out = cache.attend(0, q.to(dtype).cuda(), 70)
+    assert torch.isnan(out[:, :, 0]).all() and not out[:, :, 1].any()
+
+
+def test_uninitialised_memory_behind_the_length(ctx):
+    """A cache allocated and not cleared, filled slot by slot: NaN patterns
+    behind the length never matter, for any row count."""
+    from provekv_amd.pool import DeviceKVCache
+    T, D = 300, 64
+    for dtype in (BF16, F16, F32):
+        cache = DeviceKVCache.over(torch.full((1, 1, 2, 2, T, D), math.nan, dtype=dtype, device="cuda"))
+        x = torch.randn(2, 2, T, D, generator=torch.Generator().manual_seed(4)).to(dtype)
+        for length in (1, 31, 64, 65, 255):
+            cache.buf[0, 0, :, :, :length] = x[:, :, :length].cuda()
+            for n in (1, 5, 20, 64, length):
+                if n > length:
+                    continue
+                run(cache, dtype, x[0:1].double(), x[1:2].double(), [length], n, 2, seed=length + n)
+
+
+def test_other_device_and_stream_refused(ctx):
+    cache, _, _ = make("plain", BF16, 1, 1, 8, 64)
+    q = torch.zeros(1, 1, 1, 64, dtype=BF16)
+    with pytest.raises(ValueError):
+        cache.attend(0, q, 8)
+    with pytest.raises(ValueError):
+        cache.attend(0, q.cuda(), torch.tensor([8], dtype=torch.int32))
+    with pytest.raises(ValueError):
+        cache.attend(0, q.cuda(), torch.tensor([8], device="cuda"))            # int64
+    with pytest.raises(ValueError):
+        cache.attend(0, q.cuda(), 8, out=q.cuda()[..., :32])
+    with pytest.raises(ValueError):
+        cache.attend(0, q.cuda(), 8, max_len=9)
+    with pytest.raises(ValueError):
+        cache.attend(0, q.cuda(), 8, weights=torch.zeros(1, 1, 9, device="cuda"))
+    with pytest.raises(IndexError):
+        cache.attend(1, q.cuda(), 8)
+    from provekv_amd._lib import PkvError
+    x = q.cuda()
+    with pytest.raises(PkvError):
+        cache.attend(0, x, 8, out=x)
+    with pytest.raises(PkvError):
+        cache.attend(0, x, 8, scale=0.0)

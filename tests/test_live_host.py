@@ -83,7 +83,7 @@ def child_attend(lib, L, ctx, launches):
         ("d_workspace", None, INVALID), ("d_workspace", WORK + 64, INVALID), ("workspace_bytes", 0, CAPACITY),
         ("scale", 0.0, INVALID), ("scale", -1.0, INVALID), ("scale", float("nan"), INVALID),
         ("scale", float("inf"), INVALID), ("dtype", 2, INVALID), ("dtype", 3, INVALID), ("dtype", -1, INVALID),
-        ("q_heads", 0, INVALID), ("q_heads", 3, INVALID), ("q_heads", 1, INVALID), ("nq", 0x7fffffff, INVALID),
+        ("q_heads", 0, INVALID), ("q_heads", 3, INVALID), ("q_heads", 1, INVALID), ("nq", 0x7fffffff, INVALID), ("nq", 1 << 30, INVALID), ("scale", 3e38, INVALID),
         ("max_len", 101, INVALID), ("reserved", 1, INVALID), ("cache.d_key_scales", KS, INVALID)]
     each(call, lambda: attend_op(L), common)
     each(call, lambda: attend_op(L, 3, 1), [
@@ -99,6 +99,12 @@ def child_attend(lib, L, ctx, launches):
     assert size and call(op) == CAPACITY
     op.q_heads = 3
     assert lib.pkv_attend_workspace(C.byref(op)) == 0 and lib.pkv_attend_workspace(None) == 0
+    # more workgroups than a launch holds
+    op = attend_op(L, n=1, G=1)
+    op.cache.heads = op.q_heads = 1 << 24
+    op.cache.head_stride, op.q_head_stride, op.out_head_stride, op.d_weights = 0, 0, 64, None
+    op.out_copy_stride = 1 << 30
+    assert call(op) == INVALID and lib.pkv_attend_workspace(C.byref(op)) == 0
     each(call, lambda: attend_op(L), [("d_q_lens", None, OK), ("d_lse", None, OK), ("d_weights", None, OK),
                                       ("max_len", 100, OK), ("window", 2 ** 32 - 1, OK), ("sinks", 2 ** 32 - 1, OK),
                                       ("cache.copy_stride", 0, OK), ("q_head_stride", 0, OK)])
@@ -131,6 +137,10 @@ def child_rows(lib, L, ctx, launches):
         op = rows_op(L)
         op.d_keys = op.d_values = None
         assert call(op) == OK and launches() == before
+        op = rows_op(L)
+        op.rows = 1 << 29
+        op.copy_stride, op.layer_stride, op.head_stride = 1 << 40, 1 << 38, 1 << 36
+        assert call(op) == INVALID and launches() == before
         each(call, lambda: rows_op(L), [("d_keys", None, OK), ("d_values", None, OK), ("d_counts", None, OK)])
 
 
@@ -171,6 +181,16 @@ def child_evict(lib, L, ctx, launches):
     assert call(op) == INVALID and launches() == before
     op = evict_op(L, in_place=True)
     op.cache.copy_stride = op.into.copy_stride = 0
+    assert call(op) == INVALID
+    op = evict_op(L)
+    op.cache.heads = op.into.heads = 1 << 20
+    op.cache.elems = op.into.elems = 1 << 60
+    op.cache.head_stride, op.cache.layer_stride, op.cache.copy_stride = 0, 0, 0
+    op.into.head_stride, op.into.layer_stride, op.into.copy_stride = 1 << 16, 1 << 40, 1 << 44
+    op.into.d_keys, op.into.d_values = 1 << 50, 1 << 58
+    op.out_strides[2], op.out_strides[1], op.out_strides[0] = 40, 1 << 30, 1 << 34
+    op.weight_strides[0] = op.weight_strides[1] = op.weight_strides[2] = 0
+    op.d_weights_out = 1 << 59
     assert call(op) == INVALID
 
 
