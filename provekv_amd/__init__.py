@@ -7,7 +7,9 @@ Layers (bottom up):
   * ``device``: context / profiles / segment tables over torch device tensors;
   * ``codec``: the proveKV plugin surface (KVecCodec, TurboQuantAdapter,
     FibQuantAdapter with encode_batch_compact / decode_batch_compact);
-  * ``pool``: the batched two-tier pool + shell build and rehydrate.
+  * ``pool``: the batched two-tier pool + shell build and rehydrate;
+  * ``live``: attention over a rehydrated cache, the cache held in 4 bits, and
+    eviction by accumulated attention weight.
 """
 from ._lib import PkvError  # noqa: F401
 

@@ -173,9 +173,17 @@ __device__ inline bool any_visible(const AttendDev& a, const Tiles& t, int j) {
 //                 i of a group reads channels 8i .. of its 4 (x 2) slots and
 //                 v_perm gathers each channel across them; channel order
 //                 along M is free again, so O^T tile e holds channels 8m + e.
-// Bound by the cache's bytes: 32 slots cost a wave 16 + 32 matrix
-// instructions at head_dim 128 against 16 KB of bf16, a sixth of the time HBM
-// needs for them.
+// Bound by the cache's bytes: 32 slots cost a wave 8 + 16 matrix instructions at
+// head_dim 128 against 16 KB of bf16.  Weights go into the second product as
+// two terms of a 16-bit type (f32 queries over 4-bit codes: three), which the
+// bytes hide.  Measured: 4 x 32,768 slots of 8 heads of 128, four query heads
+// each, bf16: 104 us, 5.0 TB/s (114 with the loads in front of their own tile's
+// work instead of the one before); 8 x 930 slots of 32 heads of 64, f32: 22 us,
+// 5.5 TB/s; the former in 4 bits: 31 us, 4.4 TB/s, where unpacking (a
+// conversion per two channels and a permute per four) takes about as long as
+// the bytes.  Tried and worse: offsets of whole tiles kept in registers and
+// scale bytes of neighbouring slots in one read (4 bits: 34 us, more registers
+// and one wave a SIMD less at head_dim 64).
 template <int CT, int D>
 struct SlotTile {
     static constexpr int kSub = CT == PKV_F32 ? 1 : 2;        // 16-slot pieces
@@ -564,7 +572,7 @@ __device__ inline f32x16 mma32(u32x4 a, u32x4 b, f32x16 c) {
 __device__ constexpr int row32(int r, int half) { return 8 * (r / 4) + 4 * half + r % 4; }
 
 // The query of one row as matrix operands, a lane half its half of every 16
-// channels (f32: of every 8): channel_of(s, half) onwards, 16 bytes a register.
+// channels (f32: of every 8), 16 bytes a register.
 template <int CT, int QT, int D>
 struct Query {
     using T = typename Elem<QT>::T;
@@ -767,9 +775,16 @@ constexpr uint32_t row_tile(int ks) { return 128u / ks; }
 // Weights of a 16-bit call are rounded once to its type (half a step of the
 // output's own rounding for each, independent, so the output's error grows by
 // less than half); over 4-bit codes they are as many bf16 terms as the query.
-// Bound, at head_dim 128, by the softmax's vector instructions beside the
-// matrix instructions (16 exponentials' 16 cycles each per 8 + 8 matrix
-// instructions of 32) -- see the table of measurements.
+// Bound at head_dim 128 by the matrix cores (a tile is 32 matrix instructions of
+// 32 cycles a wave) together with the softmax beside them (32 exponentials of
+// 16 cycles, about 180 other vector instructions).  Measured: 8,192 causal rows
+// of 32 query heads of 128, bf16: 566 us, 971 TFLOP/s, where a library's square
+// product of 8,192 reaches 1,216; a tile takes a workgroup 2.0 us alone on a CU
+// and 2.2 beside another, so that calls with few workgroups are bound by that
+// latency.  With tiles held in registers on their way to LDS it took 1.93 ms:
+// what no longer fitted was reloaded behind the prefetch.
+// KS 2: a workgroup has 64 rows and two waves share a tile's slots (1.1 us a
+// tile), for calls whose 128-row tiles would not fill the chip.
 //
 // A weight 0 times an infinity or NaN would be NaN in rows that do not see the
 // slot.  The loop does not look for those: an output that is not finite sends
@@ -1059,7 +1074,9 @@ __device__ inline void hand_over(float (&left)[16], bool upper) {
 // from memory while the rows before are worked on; every slot belongs to one
 // wave, so sums have one order.  S^T, one multiply-add, one exponential and one
 // more multiply-add a logit: half of rows_kernel's matrix work, its softmax
-// work without maximum and rounding.
+// work without maximum and rounding; bound by those vector instructions.
+// Measured: 3 x 701 rows of 24 query heads of 64, window 1,024, f16: 26 us (89
+// with rows read when they were needed, 48 with half as many shares).
 //
 // With few blocks of slots their rows are cut into shares as well (splits > 1),
 // whose sums go to `shares` [split][copy][kv head][ld] for add_weights_kernel.
@@ -1411,7 +1428,9 @@ __device__ inline void find_bin(const uint32_t* hist, uint32_t want, uint32_t* f
 // has a run of slots, so that two counts a wave place every slot; up to 32,768
 // slots are read once and held in registers.  A bin has 16 counts, by lane: the
 // high bytes of weights are nearly all the same, and 64 lanes adding to one
-// word would take their turns.
+// word would take their turns.  Bound by its instructions: six passes over 32
+// weights a lane.  64 heads of 32,768 slots: 45 us (65 with one count a bin),
+// 256 heads of 1,024: 10 us (43 with a serial search of the bins).
 __global__ __launch_bounds__(kSelect) void select_kernel(EvictDev a) {
     const uint32_t h = blockIdx.x % a.heads, cl = blockIdx.x / a.heads, l = cl % a.layers, c = cl / a.layers;
     const uint32_t n = min(max(a.lens[c], 0), static_cast<int>(a.slots));
@@ -1525,7 +1544,8 @@ __device__ inline uint64_t elem_byte(uint64_t e) { return DT == PKV_FP4 ? e / 2 
 // Kept rows to their new slots, in pieces of 16 bytes, four rows' at a time
 // (4-bit caches: the scale bytes with the first piece).
 //   into other memory  a workgroup takes kBatch rows of one side of a (copy,
-//                      layer, head); bound by the rows' bytes
+//                      layer, head); bound by the rows' bytes (8,192 of 32,768
+//                      rows of 64 heads of 128, bf16: 107 us, 5.0 TB/s)
 //   in place           a workgroup takes a column of at most 64 bytes of all
 //                      rows, in order: a step's rows are read before it writes
 //                      (a barrier), and rows read later lie behind everything
@@ -1604,9 +1624,9 @@ uint64_t round256(uint64_t x) { return (x + 255) & ~255ull; }
 
 constexpr uint32_t kDecodeRows = 16;   // rows x group that decode_kernel takes
 
-// How a call is cut: row tiles (one of at most 16 rows, or tiles of 128) times
-// `splits` shares of the slots, so that the chip is full (kFew / kMany
-// workgroups) while a share has work for its waves.
+// How a call is cut: row tiles (one of at most 16 rows, or tiles of 128 or 64)
+// times `splits` shares of the slots, so that the chip is full while a share has
+// work for its waves.
 struct Plan {
     uint32_t row_tiles, splits, rows, ld;
     int ks;                              // rows_kernel: shares of a tile's slots among a workgroup's waves
