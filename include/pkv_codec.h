@@ -515,7 +515,7 @@ int pkv_turbo_score_batch(pkv_ctx* ctx, const pkv_profile* prof, const uint8_t* 
  *     dim with one scale byte b, standing for code value * 2^(b - 127); b = 255
  *     makes the block NaN.  d_keys / d_values are the codes (byte = element /
  *     2), d_key_scales / d_value_scales the scale bytes (byte = element / 32),
- *     16- and 4-byte aligned, strides a multiple of dim. */
+ *     aligned to 16 bytes and to dim / 32, strides a multiple of dim. */
 typedef struct pkv_kv_view {
     void* d_keys;
     void* d_values;

@@ -81,7 +81,9 @@ int check_view(const pkv_kv_view& v, bool written) {
     uint64_t unit = 16 / elem_bytes(v.dtype);
     if (v.dtype == PKV_FP4) {
         unit = v.dim;
-        if (!v.d_key_scales || !v.d_value_scales || !aligned(v.d_key_scales, 4) || !aligned(v.d_value_scales, 4))
+        // a row's scale bytes are read as one word of dim / 32 bytes
+        if (!v.d_key_scales || !v.d_value_scales || !aligned(v.d_key_scales, v.dim / 32) ||
+            !aligned(v.d_value_scales, v.dim / 32))
             return PKV_ERR_INVALID_ARG;
     } else if (v.d_key_scales || v.d_value_scales) {
         return PKV_ERR_INVALID_ARG;

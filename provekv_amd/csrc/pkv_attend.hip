@@ -897,6 +897,8 @@ __global__ __launch_bounds__(256, (query_terms(CT, QT) * D >= 256 ? 1 : 2)) void
                         sc[u][x] = __builtin_amdgcn_exp2f(__builtin_fmaf(sc[u][x], a.scale2, -mc));
                         l += sc[u][x];
                     }
+                // ahead of the other workgroup's softmax while the matrix cores have work: 573 -> 565 us (8,192 rows)
+                __builtin_amdgcn_s_setprio(1);
                 for (int u = 0; u < kU; ++u) {
                     if constexpr (CT == PKV_F32) {
                         for (int x = 0; x < 16; ++x)
@@ -921,6 +923,7 @@ __global__ __launch_bounds__(256, (query_terms(CT, QT) * D >= 256 ? 1 : 2)) void
                     }
                 }
             }
+            __builtin_amdgcn_s_setprio(0);
             if (t + 1 < t1) st.land(lds + ((t + 1 - t0) & 1) * St::kBytes);
             __syncthreads();
         }

@@ -348,6 +348,15 @@ def test_wide_groups_and_many_rows(ctx, n, G, heads, T, window, kind, dtype, D):
         assert not out[c, ql[c]:].any()
 
 
+@pytest.mark.parametrize("kind,dtype", KINDS, ids=KIND_IDS)
+@pytest.mark.parametrize("D", [64, 128])
+@pytest.mark.parametrize("n", [1, 21])
+def test_odd_heads_and_slots(ctx, n, kind, dtype, D):
+    """Odd heads x slots: the values' scale bytes start at any row's boundary."""
+    cache, k, v = make(kind, dtype, 3, 3, 47, D, seed=22, layers=3)
+    run(cache, dtype, k, v, [47, 13, 46], n, 2, layer=2, window=9, sinks=1)
+
+
 @pytest.mark.parametrize("n", [1, 40])
 def test_many_heads(ctx, n):
     """Thousands of copies x heads."""

@@ -79,6 +79,13 @@ def test_evict(ctx, T, budget, sinks, recent, coarse, in_place, D, kind):
     check(cache, weights(3, 2, 2, T, T + budget, coarse), lens, budget, sinks, recent, in_place, extra=T % 3)
 
 
+@pytest.mark.parametrize("kind", KINDS, ids=IDS)
+@pytest.mark.parametrize("D", [64, 128])
+@pytest.mark.parametrize("in_place", [True, False], ids=["in-place", "into"])
+def test_odd_heads_and_slots(ctx, in_place, D, kind):
+    check(make(kind, 2, 3, 3, 77, D, seed=9), weights(2, 3, 3, 77, 4, True), [77, 60], 31, 1, 3, in_place)
+
+
 @pytest.mark.parametrize("in_place", [True, False], ids=["in-place", "into"])
 def test_weights_of_every_kind(ctx, in_place):
     """Zeros of both signs, equal, negative, subnormal, infinite and NaN weights."""

@@ -54,6 +54,19 @@ def test_store_load(ctx, n, D, dtype):
         assert not cache.codes[c, :, :, :, rest.cuda()].any() and not cache.scales[c, :, :, :, rest.cuda()].any()
 
 
+@pytest.mark.parametrize("D", [64, 128])
+def test_odd_heads_and_slots(ctx, D):
+    from provekv_amd.pool import FourBitKVCache
+    cache = FourBitKVCache(3, 3, 11, D, copies=2)
+    x = torch.randn(2, 2, 3, 3, 5, D, generator=torch.Generator().manual_seed(1))
+    cache.store(x[0].cuda(), x[1].cuda(), 6)
+    keys, values = cache.load(6, 5, dtype=torch.float32)
+    want = R.fp4_round(x).float()
+    assert R.same(keys, want[0]) and R.same(values, want[1])
+    one, _ = cache.load(6, 5, layer=1, dtype=torch.float32)
+    assert R.same(one, want[0][:, 1])
+
+
 @pytest.mark.parametrize("dtype", DTYPES, ids=IDS)
 def test_no_value_is_off_by_more_than_half_a_step(ctx, dtype):
     from provekv_amd.pool import FourBitKVCache
