@@ -115,6 +115,7 @@ def test_long(ctx, n, G, kind, dtype):
 def test_few_rows_long(ctx, kind, dtype):
     cache, k, v = make(kind, dtype, 1, 1, 5000, 64, seed=7)
     run(cache, dtype, k, v, [5000], 24, 2)
+    run(cache, dtype, k, v, [5000], 3, 16, scale=0.5)
     run(cache, dtype, k, v, [4999], 9, 1, window=3000, sinks=4)
 
 
