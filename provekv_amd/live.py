@@ -78,9 +78,9 @@ class LiveCache:
         return device_context(index), handle, _NO_GUARD if index == now else torch.cuda.device(index)
 
     def _plan(self, key, make):
-        """A copy of the call's struct for `key`: checked and filled once (the
-        caches' addresses are part of the key), then only the tensors'
-        addresses change from call to call."""
+        """A copy of the call's struct for `key`, checked and filled once with
+        what shapes, strides and types decide; every call sets its own
+        addresses, those of the cache too."""
         plans = self.__dict__.setdefault("_plans", {})
         got = plans.get(key)
         if got is None:
@@ -92,23 +92,31 @@ class LiveCache:
         return type(op).from_buffer_copy(op), extra
 
     def _view(self, layer=None) -> "L.KvView":
-        dtype, size, k, v, ks, vs, elems = self._pointers()
+        """The cache, or one layer of it."""
+        memory = self._pointers()
+        dtype, elems = memory[0], memory[6]
         side = self.heads * self.tokens * self.dim
-        per_layer, first = 2 * side, 0
-        if layer is not None:
-            if not 0 <= layer < self.layers:
-                raise IndexError(f"layer {layer} outside the cache")
-            first = layer * per_layer
-        if dtype == L.DT_FP4:
-            k, v, ks, vs = k + first // 2, v + first // 2, ks + first // 32, vs + first // 32
-        else:
-            k, v = k + first * size, v + first * size
-        elems -= side + first
+        per_layer = 2 * side
+        if layer is not None and not 0 <= layer < self.layers:
+            raise IndexError(f"layer {layer} outside the cache")
+        elems -= side + (layer or 0) * per_layer
         if elems < 0:
             raise ValueError("the cache's memory is smaller than its shape")
-        return L.KvView(k, v, ks or None, vs or None, self.layers * per_layer, per_layer, self.tokens * self.dim,
+        view = L.KvView(None, None, None, None, self.layers * per_layer, per_layer, self.tokens * self.dim,
                         self.dim, elems, self.copies, 1 if layer is not None else self.layers, self.heads,
                         self.tokens, self.dim, dtype)
+        self._point(view, layer, memory)
+        return view
+
+    def _point(self, view, layer, memory) -> None:
+        """The addresses of a view, as the cache's memory is now."""
+        _, size, k, v, ks, vs, _ = memory
+        first = (layer or 0) * 2 * self.heads * self.tokens * self.dim
+        if size is None:
+            view.d_keys, view.d_values = k + first // 2, v + first // 2
+            view.d_key_scales, view.d_value_scales = ks + first // 32, vs + first // 32
+        else:
+            view.d_keys, view.d_values = k + first * size, v + first * size
 
     def _words(self, x, name: str):
         """int32 device words, one per copy."""
@@ -151,8 +159,10 @@ class LiveCache:
         if max_len is None:
             max_len = self.tokens if isinstance(lens, torch.Tensor) else min(max(int(lens), 1), self.tokens)
 
+        memory = self._pointers()
+
         def plan(q):
-            return self._plan((0, layer, _like(q), window, sinks, scale, max_len, self._address(), _like(weights),
+            return self._plan((0, layer, _like(q), window, sinks, scale, max_len, memory[0], memory[6], _like(weights),
                                _like(lse), _like(out)),
                               lambda: self._attend_op(layer, q, window, sinks, scale, weights, lse, out, max_len))
 
@@ -167,6 +177,7 @@ class LiveCache:
             if out is None:
                 # rows behind q_lens are nobody's: 0 rather than whatever the memory held
                 out = (torch.empty if q_lens is None else torch.zeros)(q.shape, dtype=q.dtype, device=dev)
+            self._point(op.cache, layer, memory)
             op.d_q, op.d_out = q.data_ptr(), out.data_ptr()
             if q_lens is not None:
                 q_lens = self._words(q_lens, "q_lens")
@@ -240,12 +251,14 @@ class LiveCache:
         import torch
         to, dev = self if into is None else into, self.device
         lead = (self.copies, self.layers, self.heads) if layer is None else (self.copies, self.heads)
+        memory = self._pointers()
+        room = memory if into is None else to._pointers()
         if to.device != dev:
             raise ValueError("into is on another device")
         self._on_device(dev, weights)
 
         def make():
-            if to._kind() != self._kind() or (to.copies, to.layers, to.heads, to.dim) != \
+            if room[0] != memory[0] or (to.copies, to.layers, to.heads, to.dim) != \
                     (self.copies, self.layers, self.heads, self.dim):
                 raise ValueError("into must be a cache of the same kind, copies, layers, heads and dim")
             if budget < 1 or sinks < 0 or recent < 0 or sinks + recent > budget:
@@ -263,8 +276,8 @@ class LiveCache:
             op.budget, op.sinks, op.recent = budget, sinks, recent
             return op, None
 
-        key = (1, layer, budget, sinks, recent, self._address(), None if into is None else (to._address(), to.copies, to.layers, to.heads, to.tokens, to.dim),
-               _like(weights))
+        key = (1, layer, budget, sinks, recent, memory[0], memory[6], _like(weights),
+               None if into is None else (room[0], room[6], to.copies, to.layers, to.heads, to.tokens, to.dim))
         op, _ = self._plan(key, make)
         ctx, handle, guard = self._frame(dev, stream)
         with guard:
@@ -272,6 +285,8 @@ class LiveCache:
             new_lens = torch.empty_like(lens)
             kept = torch.empty((*lead, budget), dtype=torch.int32, device=dev)
             packed = weights if into is None else torch.empty((*lead, to.tokens), dtype=torch.float32, device=dev)
+            self._point(op.cache, layer, memory)
+            to._point(op.into, layer, room)
             op.d_lens, op.d_new_lens, op.d_kept = lens.data_ptr(), new_lens.data_ptr(), kept.data_ptr()
             op.d_weights, op.d_weights_out = weights.data_ptr(), packed.data_ptr()
             L.check(L.lib().pkv_evict(ctx.ptr, C.byref(op), handle), "pkv_evict")
@@ -279,13 +294,6 @@ class LiveCache:
             filled = min(self._seq_len, budget)
             to._seq_len = filled if into is None else max(to._seq_len, filled)
         return kept, new_lens, packed
-
-    def _kind(self):
-        return self._pointers()[0]
-
-    def _address(self):
-        """Where the cache's memory is (and what it holds)."""
-        return self._pointers()
 
 
 class FourBitKVCache(LiveCache):
@@ -344,7 +352,9 @@ class FourBitKVCache(LiveCache):
             return L.RowsOp(self._view(layer), None, None, ks[0], ks[1], ks[2], ks[3], None, None,
                             _rows_dtype(some.dtype), some.shape[-2]), None
 
-        op, _ = self._plan((2, layer, self._address(), _like(some)), make)
+        memory = self._pointers()
+        op, _ = self._plan((2, layer, memory[6], _like(some)), make)
+        self._point(op.cache, layer, memory)
         ctx, handle = stream_frame
         first = self._words(first, "first")
         op.d_first = first.data_ptr()

@@ -144,3 +144,25 @@ def test_captured_step(ctx):
         assert R.same(captured[2], eager[2]) and R.same(captured[0].codes, eager[0].codes)
         for c, m in enumerate(want[1][1].tolist()):
             assert R.same(captured[1].codes[c, :, :, :, :m], eager[1].codes[c, :, :, :, :m])
+
+
+@pytest.mark.parametrize("layer", [0, 1])
+def test_memory_exchanged(ctx, layer):
+    """A cache whose tensors are exchanged for others of the same shape is read where they are now."""
+    from provekv_amd.pool import DeviceKVCache, FourBitKVCache
+    g = torch.Generator(device="cuda").manual_seed(9)
+    q = torch.randn(2, 3, 4, D, device="cuda", generator=g).bfloat16()
+    cache, four = DeviceKVCache(2, 2, 70, D, dtype=torch.bfloat16, copies=2), FourBitKVCache(2, 2, 70, D, copies=2)
+    for step in range(2):
+        buf = torch.randn(2, 2, 2, 2, 70, D, device="cuda", generator=g).bfloat16()
+        cache.buf = buf
+        four.codes, four.scales = torch.zeros_like(four.codes), torch.zeros_like(four.scales)
+        four.store(buf[:, :, 0], buf[:, :, 1], 0)
+        for one in (cache, four):
+            k, v = values_of(one)
+            weights = torch.zeros(2, 2, 70, device="cuda")
+            check(one, (k, v), layer, q, [70, 70], one.attend(layer, q, 70, weights=weights), 0, 0)
+            into = type(one)(2, 2, 20, D, copies=2) if one is four else type(one)(2, 2, 20, D, dtype=buf.dtype, copies=2)
+            kept, _, _ = one.evict(70, weights, 20, layer=layer, into=into)
+            at = kept.cpu().long()[..., None].expand(-1, -1, -1, D)
+            assert R.same(values_of(into)[0][:, layer], k[:, layer].gather(2, at))
