@@ -553,6 +553,15 @@ typedef struct pkv_kv_view {
  *   d_workspace  pkv_attend_workspace(op) bytes, 256-byte aligned, used until
  *            the call's work on `stream` is done; calls that may run at the
  *            same time need one each (a captured graph holds on to its own)
+ * Sizes: copies * q_heads * nq is at most 2^30, and every launch stays below 2^24
+ * workgroups, so that a call is refused (PKV_ERR_INVALID_ARG) when, with R = nq *
+ * q_heads / heads rows of a KV head,
+ *   R <= 16: copies * q_heads * nq (with d_weights and copies * heads *
+ *            ceil(max_len / 1024) added), or
+ *   R > 16:  copies * heads * the tiles of 64 to 128 of the R rows, or with
+ *            d_weights copies * heads * ceil(max_len / 128) (with a window, of
+ *            the slots it reaches)
+ * is 2^24 or more.
  * Logits, softmax and sums are held in 32 bits.  Asynchronous on `stream`; the
  * call can be captured. */
 typedef struct pkv_attend_op {

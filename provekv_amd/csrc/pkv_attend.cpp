@@ -67,6 +67,7 @@ bool overlap(const void* a, uint64_t an, const void* b, uint64_t bn) {
 }
 
 constexpr uint32_t kMaxCount = 0x7fffffffu;
+constexpr uint32_t kMaxRows = 1u << 30;   // query rows of all copies and query heads
 // Elements from a slot to the next: a kernel's tile of 64 slots stays within
 // 32-bit offsets of its first.
 constexpr uint64_t kMaxSlotStride = 1u << 22;
@@ -138,7 +139,8 @@ int check_attend_shape(const pkv_attend_op& op) {
     if (v.layers != 1 || !v.copies || !v.heads || !v.slots || v.slots > kMaxCount / 2 || op.max_len > v.slots)
         return PKV_ERR_INVALID_ARG;
     if (!op.q_heads || op.q_heads % v.heads || op.reserved) return PKV_ERR_INVALID_ARG;
-    if (op.nq > kMaxCount / 2 || static_cast<U128>(v.copies) * op.q_heads * std::max(op.nq, 1u) > kMaxCount)
+    // a head's rows and some tiles more are counted in 31 bits
+    if (op.nq > kMaxCount / 2 || static_cast<U128>(v.copies) * op.q_heads * std::max(op.nq, 1u) > kMaxRows)
         return PKV_ERR_INVALID_ARG;
     if (op.nq && !attend_fits(attend_dev(op), v.dim, v.dtype)) return PKV_ERR_INVALID_ARG;
     return PKV_OK;

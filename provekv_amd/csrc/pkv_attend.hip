@@ -1029,12 +1029,13 @@ __global__ __launch_bounds__(256, (query_terms(CT, QT) * D >= 256 ? 1 : 2)) void
     return;
 }
 
-// rows_kernel's shares joined: D / 4 lanes a row.
+// rows_kernel's shares joined: D / 4 lanes a row, this many rows a workgroup.
+constexpr uint32_t join_rows(uint32_t dim) { return 1024 / dim; }
 template <int QT, int D>
 __global__ __launch_bounds__(256) void join_rows_kernel(AttendDev a, Partial part) {
     using T = typename Elem<QT>::T;
     typedef T T4 __attribute__((ext_vector_type(4)));
-    constexpr uint32_t kLanes = D / 4, kRows = 256 / kLanes;
+    constexpr uint32_t kLanes = D / 4, kRows = join_rows(D);
     const uint32_t all = a.nq * a.group, blocks = (all + kRows - 1) / kRows, ch = blockIdx.x / blocks;
     const uint32_t r = blockIdx.x % blocks * kRows + threadIdx.x / kLanes, d = threadIdx.x % kLanes * 4;
     const uint32_t c = ch / a.heads, h = ch % a.heads, i = r / a.group, g = r % a.group;
@@ -1727,7 +1728,7 @@ int attend_typed(AttendDev a, uint8_t* ws, hipStream_t st) {
     if (p.ks == 1) rows_kernel<CT, QT, D, 1><<<heads * p.row_tiles * p.splits, 256, 0, st>>>(a, part, p.row_tiles);
     // a workgroup a row reads its shares side by side, D / 4 lanes a row one after the other; whole calls on 32,768
     // slots: 1,024 rows 42 us against 61, 4,096 rows 93 and 93, 8,192 rows (16,384 slots) 93 against 87
-    constexpr uint32_t kJoin = 1024 / D;     // rows of a workgroup
+    constexpr uint32_t kJoin = join_rows(D);
     if (p.splits > 1 && outs <= kJoinRows) join_kernel<QT, D><<<outs, 256, 0, st>>>(a, part, outs);
     else if (p.splits > 1) join_rows_kernel<QT, D><<<(a.nq * a.group + kJoin - 1) / kJoin * heads, 256, 0, st>>>(a, part);
     if (a.weights) {
@@ -1746,12 +1747,19 @@ int attend_dim(const AttendDev& a, uint32_t dim, uint8_t* ws, hipStream_t st) {
 
 }  // namespace
 
-// Every launch's threads along x stay below 2^32.
+// The launches of attend_typed: threads along x stay below 2^32.
 bool attend_fits(const AttendDev& a, uint32_t dim, int cache_dtype) {
     const Plan p = plan_of(a, dim, cache_dtype);
     const uint64_t heads = static_cast<uint64_t>(a.copies) * a.heads, all = static_cast<uint64_t>(a.nq) * a.group;
-    const uint64_t most = std::max<uint64_t>({heads * p.splits * p.row_tiles, heads * all + heads * ((a.max_len + 1023ull) / 1024),
-                                    heads * p.w_blocks * p.w_splits, heads * ((a.max_len + 255ull) / 256)});
+    uint64_t most = heads * p.splits * p.row_tiles;
+    if (all <= kDecodeRows) {
+        most = std::max<uint64_t>(most, heads * all + (a.weights ? heads * ((a.max_len + 1023ull) / 1024) : 0));
+    } else {
+        const uint64_t join = join_rows(dim);
+        if (p.splits > 1) most = std::max(most, heads * (heads * all <= kJoinRows ? all : (all + join - 1) / join));
+        if (a.weights) most = std::max(most, heads * p.w_blocks * p.w_splits);
+        if (p.w_splits > 1) most = std::max<uint64_t>(most, heads * ((a.max_len + 255ull) / 256));
+    }
     return most < 1u << 24;
 }
 
