@@ -631,6 +631,10 @@ int pkv_fp4_load(pkv_ctx* ctx, const pkv_rows_op* op, void* stream);
  *                 slots' weights, then 0 up to into.slots; may be d_weights
  *                 with its strides (in place)
  * sinks + recent <= budget, budget >= 1, into.slots >= min(budget, slots).
+ * copies * layers * heads stays below 2^22, and 2 * copies * layers * heads * n
+ * below 2^24, with n the 64-byte pieces of a row (at least 1) in place, the
+ * pieces of 16 KiB of min(budget, slots) rows into other memory; else
+ * PKV_ERR_INVALID_ARG.
  * Asynchronous on `stream`; the call can be captured. */
 typedef struct pkv_evict_op {
     pkv_kv_view cache;

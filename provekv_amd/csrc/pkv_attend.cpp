@@ -302,7 +302,7 @@ int pkv_evict(pkv_ctx* ctx, const pkv_evict_op* op, void* stream) {
     e.copies = c.copies; e.layers = c.layers; e.heads = c.heads; e.slots = c.slots; e.into_slots = t.slots;
     e.budget = op->budget; e.sinks = op->sinks; e.recent = op->recent;
     e.in_place = in_place;
-    if (!evict_fits(e)) return PKV_ERR_INVALID_ARG;
+    if (!evict_fits(e, c.dim, c.dtype)) return PKV_ERR_INVALID_ARG;
     OnDevice dv(ctx_device(ctx));
     if (dv.rc) return dv.rc;
     return hip_rc(launch_evict(e, c.dim, c.dtype, stream));

@@ -58,7 +58,7 @@ struct EvictDev {
 // Launchers (pkv_attend.hip); a hipError_t as int.  dim 64 or 128.
 uint64_t attend_workspace(const AttendDev& a, uint32_t dim, int cache_dtype, int dtype);
 bool attend_fits(const AttendDev& a, uint32_t dim, int cache_dtype);   // the launches are within the device's limits
-bool evict_fits(const EvictDev& e);
+bool evict_fits(const EvictDev& e, uint32_t dim, int dtype);
 int launch_attend(const AttendDev& a, uint32_t dim, int cache_dtype, int dtype, uint8_t* workspace, void* stream);
 int launch_fp4_store(const RowsDev& r, uint32_t dim, int dtype, void* stream);
 int launch_fp4_load(const RowsDev& r, uint32_t dim, int dtype, void* stream);

@@ -1799,23 +1799,34 @@ int launch_fp4_load(const RowsDev& r, uint32_t dim, int dtype, void* stream) {
     return launch_rows(r, dim, dtype, false, static_cast<hipStream_t>(stream));
 }
 
+// Workgroups that move a call's rows: for each side of a (copy, layer, head) a
+// column of all rows in place, else kBatch rows.
+template <int DT>
+static uint64_t move_blocks(const EvictDev& e, uint32_t dim) {
+    const uint64_t sides = 2ull * e.copies * e.layers * e.heads;
+    if (e.in_place) return sides * (dim == 64 ? Move<DT, 64, true>::kColumns : Move<DT, 128, true>::kColumns);
+    const uint32_t rows = dim == 64 ? Move<DT, 64, false>::kBatch : Move<DT, 128, false>::kBatch;
+    return sides * ((std::min(e.budget, e.slots) + rows - 1) / rows);
+}
+static uint64_t move_blocks(const EvictDev& e, uint32_t dim, int dtype) {
+    if (dtype == PKV_F32) return move_blocks<PKV_F32>(e, dim);
+    if (dtype == PKV_FP4) return move_blocks<PKV_FP4>(e, dim);
+    return move_blocks<PKV_BF16>(e, dim);   // f16 rows are as long
+}
+
 template <int DT, int D>
 static int move_typed(const EvictDev& e, hipStream_t st) {
-    const uint64_t sets = static_cast<uint64_t>(e.copies) * e.layers * e.heads;
-    if (e.in_place) {
-        move_kernel<DT, D, true><<<static_cast<uint32_t>(sets * 2 * Move<DT, D, true>::kColumns), 256, 0, st>>>(e, 0);
-    } else {
-        const uint32_t most = std::min(e.budget, e.slots), rows = Move<DT, D, false>::kBatch;
-        const uint32_t batches = (most + rows - 1) / rows;
-        move_kernel<DT, D, false><<<static_cast<uint32_t>(sets * 2 * batches), 256, 0, st>>>(e, batches);
-    }
+    const uint64_t blocks = move_blocks<DT>(e, D);
+    const uint32_t grid = static_cast<uint32_t>(blocks);
+    if (e.in_place) move_kernel<DT, D, true><<<grid, 256, 0, st>>>(e, 0);
+    else move_kernel<DT, D, false><<<grid, 256, 0, st>>>(e, static_cast<uint32_t>(blocks / (2ull * e.copies * e.layers * e.heads)));
     return hipGetLastError();
 }
 
-bool evict_fits(const EvictDev& e) {
+// The launches of launch_evict: threads along x stay below 2^32 (select_kernel: 1,024 threads a set).
+bool evict_fits(const EvictDev& e, uint32_t dim, int dtype) {
     const uint64_t sets = static_cast<uint64_t>(e.copies) * e.layers * e.heads;
-    // select_kernel: 1,024 threads a set; move_kernel: at most 8 columns, or 32 rows a workgroup, of two sides
-    return sets < 1u << 22 && sets * 2 * std::max<uint64_t>(8, (std::min(e.budget, e.slots) + 31ull) / 32) < 1u << 24;
+    return sets < 1u << 22 && move_blocks(e, dim, dtype) < 1u << 24;
 }
 
 int launch_evict(const EvictDev& e, uint32_t dim, int dtype, void* stream) {

@@ -8,12 +8,12 @@ import sys
 
 import pytest
 
-from test_live_host import INVALID, OK, attend_op, stub  # noqa: F401
+from test_live_host import INVALID, OK, attend_op, evict_op, stub  # noqa: F401
 
 HERE = os.path.dirname(os.path.abspath(__file__))
 
 
-@pytest.mark.parametrize("name", ["attend"])
+@pytest.mark.parametrize("name", ["attend", "evict"])
 def test_limits(stub, name):  # noqa: F811
     r = subprocess.run([sys.executable, os.path.abspath(__file__), stub, name], capture_output=True, text=True,
                        timeout=120, env={**os.environ, "PYTHONPATH": os.pathsep.join((os.path.dirname(HERE), HERE))})
@@ -66,6 +66,52 @@ def child_attend(lib, L, ctx, launches):
     # .. and with weights blocks of 128 slots, no more than a window's
     assert call(1, most // 8, most // 8, 17, 1024, True) and not call(1, most // 7, most // 7, 17, 1024, True)
     assert call(1, most // 8, most // 8, 17, 100000, True, window=100)
+
+
+def evict(L, dtype, dim, heads, budget, in_place):
+    """One copy and layer of `heads` heads, rows a head apart."""
+    op = evict_op(L, dtype, in_place)
+    slots = budget + 10
+    for v in (op.cache, op.into):
+        v.copies = v.layers = 1
+        v.heads, v.slots, v.dim, v.slot_stride, v.head_stride = heads, slots, dim, dim, slots * dim
+        v.elems = heads * slots * dim
+    op.cache.d_keys, op.cache.d_values = 1 << 50, 1 << 51
+    op.into.d_keys, op.into.d_values = (1 << 50, 1 << 51) if in_place else (1 << 52, 1 << 53)
+    if dtype == 3:
+        op.cache.d_key_scales, op.cache.d_value_scales = 1 << 54, 1 << 55
+        op.into.d_key_scales, op.into.d_value_scales = (1 << 54, 1 << 55) if in_place else (1 << 56, 1 << 57)
+    op.d_weights = 1 << 58
+    op.d_weights_out = 1 << (58 if in_place else 59)
+    op.weight_strides[2] = op.out_strides[2] = slots
+    op.budget, op.sinks, op.recent = budget, 0, 0
+    return op
+
+
+def child_evict(lib, L, ctx, launches):
+    def call(*args):
+        op = evict(L, *args)
+        n = launches()
+        rc = lib.pkv_evict(ctx, C.byref(op), None)
+        assert rc in (OK, INVALID) and (launches() > n) == (rc == OK), rc
+        return rc == OK
+
+    most = (1 << 24) - 1
+    for dtype, size in ((0, 4), (1, 2), (2, 2), (3, 0.5)):
+        for dim in (64, 128):
+            row = int(dim * size)
+            # in place: columns of 64 bytes of both sides, whatever the budget
+            sets = min((1 << 22) - 1, most // (2 * max(row // 64, 1)))
+            for budget in (1, 4096):
+                assert call(dtype, dim, sets, budget, True) and not call(dtype, dim, sets + 1, budget, True)
+            # into other memory: 16 KiB of rows
+            rows = (1 << 14) // row
+            assert call(dtype, dim, (1 << 22) - 1, rows, False) and not call(dtype, dim, 1 << 22, rows, False)
+            for blocks in (7, 100):
+                sets = most // (2 * blocks)
+                assert call(dtype, dim, sets, rows * blocks, False)
+                assert not call(dtype, dim, sets + 1, rows * blocks, False)
+                assert not call(dtype, dim, sets, rows * blocks + 1, False)
 
 
 if __name__ == "__main__":
