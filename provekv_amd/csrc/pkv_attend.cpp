@@ -126,6 +126,7 @@ AttendDev attend_dev(const pkv_attend_op& op) {
     a.sinks = op.sinks;
     a.reach = op.window ? std::min(op.window, 0x80000000u) : 0x80000000u;
     a.scale2 = static_cast<float>(static_cast<double>(op.scale) * 1.4426950408889634074);
+    a.lift = op.cache.dtype == PKV_F16 ? 11.0f : 0.0f;
     return a;
 }
 

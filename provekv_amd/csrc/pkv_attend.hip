@@ -136,6 +136,26 @@ __device__ inline uint32_t finite_or_0(uint32_t x) {
     return x;
 }
 
+// Softmax weights are held as 2^(s * scale2 + base), base = lift - (largest
+// logit) * scale2 when it was last set: up to kLag behind the largest logit seen
+// since, so that sums are rescaled seldom; +inf before the first logit.  A
+// share's base goes with its sums, exact as it was used.
+//
+// lift: f16 ends at 2^-24, so that weights up to 1 would lose all below 2^-25,
+// and a long cache's sum with them.  Weights up to 2^(11 + 4) use its top
+// instead: full precision down to 2^-25 of the largest, the end at 2^-36.
+template <int MT> constexpr float kLag = MT == PKV_F16 ? 4.0f : 8.0f;
+// The base with a row's logits up to `top` seen as well.
+__device__ inline float lower_base(const AttendDev& a, float base, float top) {
+    return fminf(base, __builtin_fmaf(-top, a.scale2, a.lift));
+}
+// Of the weights of a share with `base` when they join those of a lower one.
+__device__ inline float joined(float low, float base) { return base == low ? 1.0f : exp2f(low - base); }
+// Log of the sum of exponentials.
+__device__ inline float lse_of(const AttendDev& a, float base, float sum) {
+    return sum == 0.0f ? -kInf : (log2f(sum * exp2f(-a.lift)) + (a.lift - base)) * kLn2;
+}
+
 // The slots that the rows of a tile see, as tiles of `step` slots: [0, first)
 // with the always-visible slots, then [second, second + count - first).
 struct Tiles {
@@ -260,7 +280,7 @@ struct SlotTile {
 
 struct Partial {
     float* o;        // [copy][kv head][split][rows][D]
-    float* ml;       // [copy][kv head][split][rows][2]: largest logit (unscaled), sum
+    float* ml;       // [copy][kv head][split][rows][2]: base, sum of the weights
     float* logits;   // [copy][kv head][rows x group][ld], unscaled (few rows)
     uint32_t splits, ld, rows;
 };
@@ -302,13 +322,13 @@ __global__ __launch_bounds__(256, 2) void decode_kernel(AttendDev a, Partial par
         }
     }
 
-    const uint64_t base = c * a.kv.copy + h * a.kv.head;
-    const uint64_t byte = CT == PKV_FP4 ? base / 2 : CT == PKV_F32 ? base * 4 : base * 2;
+    const uint64_t head = c * a.kv.copy + h * a.kv.head;
+    const uint64_t byte = CT == PKV_FP4 ? head / 2 : CT == PKV_F32 ? head * 4 : head * 2;
     const uint8_t *kp = a.kv.k + byte, *vp = a.kv.v + byte;
-    const uint8_t *ksp = CT == PKV_FP4 ? a.kv.ks + base / 32 : nullptr;
-    const uint8_t *vsp = CT == PKV_FP4 ? a.kv.vs + base / 32 : nullptr;
+    const uint8_t *ksp = CT == PKV_FP4 ? a.kv.ks + head / 32 : nullptr;
+    const uint8_t *vsp = CT == PKV_FP4 ? a.kv.vs + head / 32 : nullptr;
 
-    float m = -kInf, l = 0.0f;
+    float base = kInf, l = 0.0f;
     f32x4 o[kO] = {};
     auto fetch = [&](Tile& x, int t) {   // past the last tile: the last again, unused
         x.load(kp, vp, ksp, vsp, a.kv.slot, tl.slot(min(t, t1 - 1), Tile::kStep), tl.high - 1, lane);
@@ -349,27 +369,24 @@ __global__ __launch_bounds__(256, 2) void decode_kernel(AttendDev a, Partial par
                         }
                 }
         }
-        // running maximum; rescaled only when it grows by more than 2^8 (weights
-        // stay below 2^8 times the largest, exact all the same)
         float top = fmaxf(fmaxf(sc[0][0], sc[0][1]), fmaxf(sc[0][2], sc[0][3]));
         for (int u = 1; u < kSub; ++u)
             top = fmaxf(top, fmaxf(fmaxf(sc[u][0], sc[u][1]), fmaxf(sc[u][2], sc[u][3])));
         top = across32(across16(top, larger), larger);
-        const bool grow = m == -kInf ? top > -kInf : (top - m) * a.scale2 > 8.0f;
-        if (__any(grow)) {
-            const float mn = fmaxf(m, top);
-            const float f = m == -kInf ? 1.0f : exp2f((m - mn) * a.scale2);
-            if (mn > m) {
+        if (__any(__builtin_fmaf(top, a.scale2, base) > a.lift + kLag<MT>)) {
+            const float low = lower_base(a, base, top);
+            const float f = base == kInf ? 1.0f : exp2f(low - base);
+            if (low < base) {
                 l *= f;
                 for (int e = 0; e < kO; ++e) o[e] *= f;
-                m = mn;
+                base = low;
             }
         }
-        const float mc = m == -kInf ? 0.0f : m * a.scale2;
+        const float from = base == kInf ? 0.0f : base;
         float p[kSub][4];
         for (int u = 0; u < kSub; ++u)
             for (int j = 0; j < 4; ++j) {
-                p[u][j] = __builtin_amdgcn_exp2f(__builtin_fmaf(sc[u][j], a.scale2, -mc));
+                p[u][j] = __builtin_amdgcn_exp2f(__builtin_fmaf(sc[u][j], a.scale2, from));
                 l += p[u][j];
             }
         // weighted values
@@ -434,53 +451,50 @@ __global__ __launch_bounds__(256, 2) void decode_kernel(AttendDev a, Partial par
     l += __shfl_xor(l, 32);
 
     // the four waves' shares joined; channel of o[e][r]: see SlotTile
-    __shared__ float so[4][16][D + 4], sm[4][16], sl[4][16];
+    __shared__ float so[4][16][D + 4], sb[4][16], sl[4][16];
     for (int r = 0; r < 4; ++r)
         for (int e = 0; e < kO; ++e) {
             const int w = 4 * g + r;
             const int d = CT == PKV_F32 ? 64 * (e / 4) + 4 * w + e % 4 : kO * w + e;
             so[wave][row][d] = o[e][r];
         }
-    if (g == 0) { sm[wave][row] = m; sl[wave][row] = l; }
+    if (g == 0) { sb[wave][row] = base; sl[wave][row] = l; }
     __syncthreads();
     for (uint32_t x = threadIdx.x; x < static_cast<uint32_t>(R) * (D / 4); x += 256) {
         const uint32_t r = x / (D / 4), d = x % (D / 4) * 4;
-        const float top = fmaxf(fmaxf(sm[0][r], sm[1][r]), fmaxf(sm[2][r], sm[3][r])), mu = top == -kInf ? 0.0f : top;
+        const float low = fminf(fminf(sb[0][r], sb[1][r]), fminf(sb[2][r], sb[3][r]));
         float sum = 0.0f;
         f32x4 acc = {};
         for (int w = 0; w < 4; ++w) {
-            const float f = sm[w][r] == -kInf ? 0.0f : sm[w][r] == mu ? 1.0f : exp2f((sm[w][r] - mu) * a.scale2);
+            const float f = joined(low, sb[w][r]);
             sum += sl[w][r] * f;
-            if (f != 0.0f) acc += *reinterpret_cast<const f32x4*>(&so[w][r][d]) * f;
+            acc += *reinterpret_cast<const f32x4*>(&so[w][r][d]) * f;
         }
         const uint64_t at = (static_cast<uint64_t>(ch) * part.splits + split) * part.rows + r;
         *reinterpret_cast<f32x4*>(part.o + at * D + d) = acc;
         if (d == 0) {
-            part.ml[2 * at] = top;
+            part.ml[2 * at] = low;
             part.ml[2 * at + 1] = sum;
         }
     }
 }
 
-// The splits of a row joined: largest logit and the sum under it.
-__device__ inline void join_splits(const float* ml, uint32_t splits, uint32_t rows, float scale2, uint32_t lane,
-                                   float* mu, float* sum) {
+// The splits of a row joined: the lowest base and the sum under it (a share
+// without a logit has the sum 0, or NaN from NaN logits).
+__device__ inline void join_splits(const float* ml, uint32_t splits, uint32_t rows, uint32_t lane, float* base,
+                                   float* sum) {
     const uint64_t step = 2ull * rows;
-    float top = -kInf;
-    for (uint32_t s = lane; s < splits; s += 64) top = fmaxf(top, ml[step * s]);
-    for (int x = 32; x; x >>= 1) top = fmaxf(top, __shfl_xor(top, x));
+    float low = kInf;
+    for (uint32_t s = lane; s < splits; s += 64) low = fminf(low, ml[step * s]);
+    for (int x = 32; x; x >>= 1) low = fminf(low, __shfl_xor(low, x));
     float l = 0.0f;
-    for (uint32_t s = lane; s < splits; s += 64) {
-        // a share without a largest logit holds the sum 0, or NaN from NaN logits
-        const float ms = ml[step * s];
-        l += ml[step * s + 1] * (ms == top || ms == -kInf ? 1.0f : exp2f((ms - top) * scale2));
-    }
+    for (uint32_t s = lane; s < splits; s += 64) l += ml[step * s + 1] * joined(low, ml[step * s]);
     *sum = wave_sum(l);
-    *mu = top == -kInf ? 0.0f : top;
+    *base = low;
 }
 
-// The splits' shares joined, a workgroup a row: every wave the row's largest
-// logit and sum, then 1024 / D shares at a time, 4 channels a thread.  With
+// The splits' shares joined, a workgroup a row: every wave the row's base
+// and sum, then 1024 / D shares at a time, 4 channels a thread.  With
 // weights of few rows, then, a workgroup's rows of softmax statistics against
 // the stored logits, four slots a thread.  blockIdx.x < outs: rows of all
 // copies x heads; else 1,024 slots.
@@ -495,15 +509,12 @@ __global__ __launch_bounds__(256) void join_kernel(AttendDev a, Partial part, ui
         const uint64_t at = static_cast<uint64_t>(ch) * part.splits * part.rows + r;
         constexpr uint32_t kLanes = D / 4, kShares = 256 / kLanes;
         const uint32_t first = threadIdx.x / kLanes, d = threadIdx.x % kLanes * 4;
-        float mu, sum;
-        join_splits(part.ml + 2 * at, part.splits, part.rows, a.scale2, lane, &mu, &sum);
+        float base, sum;
+        join_splits(part.ml + 2 * at, part.splits, part.rows, lane, &base, &sum);
         f32x4 o = {};
         for (uint32_t s = first; s < part.splits; s += kShares) {
             const uint64_t x = at + static_cast<uint64_t>(part.rows) * s;
-            const float ms = part.ml[2 * x];
-            const f32x4 p = *reinterpret_cast<const f32x4*>(part.o + x * D + d);
-            const float f = ms == mu ? 1.0f : exp2f((ms - mu) * a.scale2);
-            if (ms != -kInf) o += p * f;
+            o += *reinterpret_cast<const f32x4*>(part.o + x * D + d) * joined(base, part.ml[2 * x]);
         }
         __shared__ f32x4 so[256];
         so[threadIdx.x] = o;
@@ -518,10 +529,9 @@ __global__ __launch_bounds__(256) void join_kernel(AttendDev a, Partial part, ui
         }
         if (threadIdx.x == 0) {
             if (a.lse)
-                a.lse[(static_cast<uint64_t>(c) * a.heads * a.group + h * a.group + g) * a.nq + i] =
-                    sum == 0.0f ? -kInf : (mu * a.scale2 + log2f(sum)) * kLn2;
+                a.lse[(static_cast<uint64_t>(c) * a.heads * a.group + h * a.group + g) * a.nq + i] = lse_of(a, base, sum);
             if (a.stats) {
-                a.stats[2 * (static_cast<uint64_t>(ch) * all + r)] = -mu * a.scale2;
+                a.stats[2 * (static_cast<uint64_t>(ch) * all + r)] = sum == 0.0f ? 0.0f : base;
                 a.stats[2 * (static_cast<uint64_t>(ch) * all + r) + 1] = sum == 0.0f ? 0.0f : 1.0f / sum;
             }
         }
@@ -535,11 +545,11 @@ __global__ __launch_bounds__(256) void join_kernel(AttendDev a, Partial part, ui
     if (j0 >= tl.high || (j0 + 1023 < tl.low && static_cast<uint32_t>(j0) >= a.sinks)) return;
     __shared__ float st[16][2];
     for (int r = wave; r < rows; r += 4) {
-        float mu, sum;
-        join_splits(part.ml + 2 * (static_cast<uint64_t>(ch) * part.splits * part.rows + r), part.splits, part.rows,
-                    a.scale2, lane, &mu, &sum);
+        float base, sum;
+        join_splits(part.ml + 2 * (static_cast<uint64_t>(ch) * part.splits * part.rows + r), part.splits, part.rows, lane,
+                    &base, &sum);
         if (lane == 0) {
-            st[r][0] = -mu * a.scale2;
+            st[r][0] = base;
             st[r][1] = sum == 0.0f ? 0.0f : 1.0f / sum;
         }
     }
@@ -830,14 +840,14 @@ __global__ __launch_bounds__(256, (query_terms(CT, QT) * D >= 256 ? 1 : 2)) void
     q.load(reinterpret_cast<const T*>(a.q) + c * a.q_copy + qi * a.q_row + (h * a.group + (real ? r : last) % G) * a.q_head,
            real, half);
 
-    const uint64_t base = c * a.kv.copy + h * a.kv.head;
-    const uint64_t byte = CT == PKV_FP4 ? base / 2 : CT == PKV_F32 ? base * 4 : base * 2;
+    const uint64_t head = c * a.kv.copy + h * a.kv.head;
+    const uint64_t byte = CT == PKV_FP4 ? head / 2 : CT == PKV_F32 ? head * 4 : head * 2;
     const uint8_t *kp = a.kv.k + byte, *vp = a.kv.v + byte;
-    const uint8_t *ksp = CT == PKV_FP4 ? a.kv.ks + base / 32 : nullptr;
-    const uint8_t *vsp = CT == PKV_FP4 ? a.kv.vs + base / 32 : nullptr;
+    const uint8_t *ksp = CT == PKV_FP4 ? a.kv.ks + head / 32 : nullptr;
+    const uint8_t *vsp = CT == PKV_FP4 ? a.kv.vs + head / 32 : nullptr;
 
     const uint32_t at = static_cast<uint32_t>(reinterpret_cast<uintptr_t>((LdsByte*)lds));
-    float m, l;
+    float base, l;
     f32x16 o[kO];
     St st;
     auto fetch = [&](int t) {
@@ -849,7 +859,7 @@ __global__ __launch_bounds__(256, (query_terms(CT, QT) * D >= 256 ? 1 : 2)) void
                (slot + share + 32 * kU <= wt.low && static_cast<uint32_t>(slot + share) >= a.sinks);
     };
     for (bool clean = false;; clean = true) {
-        m = -kInf;
+        base = kInf;
         l = 0.0f;
         for (int e = 0; e < kO; ++e) o[e] = f32x16{};
         if (t0 < t1) {
@@ -885,20 +895,19 @@ __global__ __launch_bounds__(256, (query_terms(CT, QT) * D >= 256 ? 1 : 2)) void
                 for (int u = 0; u < kU; ++u)
                     for (int x = 0; x < 16; ++x) top = fmaxf(top, sc[u][x]);
                 top = across32(top, larger);
-                const bool grow = m == -kInf ? top > -kInf : (top - m) * a.scale2 > 8.0f;
-                if (__any(grow)) {   // as in decode_kernel
-                    const float mn = fmaxf(m, top);
-                    const float f = m == -kInf ? 1.0f : exp2f((m - mn) * a.scale2);
-                    if (mn > m) {
+                if (__any(__builtin_fmaf(top, a.scale2, base) > a.lift + kLag<MT>)) {
+                    const float low = lower_base(a, base, top);
+                    const float f = base == kInf ? 1.0f : exp2f(low - base);
+                    if (low < base) {
                         l *= f;
                         for (int e = 0; e < kO; ++e) o[e] *= f;
-                        m = mn;
+                        base = low;
                     }
                 }
-                const float mc = m == -kInf ? 0.0f : m * a.scale2;
+                const float from = base == kInf ? 0.0f : base;
                 for (int u = 0; u < kU; ++u)
                     for (int x = 0; x < 16; ++x) {
-                        sc[u][x] = __builtin_amdgcn_exp2f(__builtin_fmaf(sc[u][x], a.scale2, -mc));
+                        sc[u][x] = __builtin_amdgcn_exp2f(__builtin_fmaf(sc[u][x], a.scale2, from));
                         l += sc[u][x];
                     }
                 // ahead of the other workgroup's softmax while the matrix cores have work: 573 -> 565 us (8,192 rows)
@@ -938,7 +947,7 @@ __global__ __launch_bounds__(256, (query_terms(CT, QT) * D >= 256 ? 1 : 2)) void
             if (!__syncthreads_or(odd && real)) break;
             continue;
         }
-        const float mc = m == -kInf ? 0.0f : m * a.scale2;
+        const float from = base == kInf ? 0.0f : base;
 #pragma unroll 1
         for (int t = t0; t < t1; ++t) {
             const int slot = tl.slot(t, St::kSlots);
@@ -963,7 +972,7 @@ __global__ __launch_bounds__(256, (query_terms(CT, QT) * D >= 256 ? 1 : 2)) void
                         for (int y = 0; y < Query<CT, QT, D>::kTerms; ++y) dot += dot_word<MT>(k[w], q.q[y][x][w]);
                 }
                 dot += __shfl_xor(dot, 32);
-                const float p = __builtin_amdgcn_exp2f(__builtin_fmaf(dot, a.scale2, -mc));
+                const float p = __builtin_amdgcn_exp2f(__builtin_fmaf(dot, a.scale2, from));
                 for (int e = 0; e < kO; ++e)
                     for (int x = 0; x < 16; ++x) {
                         const float v = St::value(buf, j, 32 * e + row32(x, hf));
@@ -976,21 +985,18 @@ __global__ __launch_bounds__(256, (query_terms(CT, QT) * D >= 256 ? 1 : 2)) void
     }
     l += __shfl_xor(l, 32);
     if constexpr (KS > 1) {
-        // the other share of the slots joins the first: [row block][o, m, l][lane]
+        // the other share of the slots joins the first: [row block][o, base, l][lane]
         float* to = reinterpret_cast<float*>(lds) + wave * (16 * kO + 2) * 64 + lane;
         if (share) {
             for (int x = 0; x < 16 * kO; ++x) to[x * 64] = o[x / 16][x % 16];
-            to[16 * kO * 64] = m;
+            to[16 * kO * 64] = base;
             to[(16 * kO + 1) * 64] = l;
         }
         __syncthreads();
         if (share) return;
-        const float m2 = to[16 * kO * 64], l2 = to[(16 * kO + 1) * 64], top = fmaxf(m, m2);
-        // a share without a largest logit has o = 0 and the sum 0, or NaN from NaN logits
-        const float f = m == top || m == -kInf ? 1.0f : exp2f((m - top) * a.scale2);
-        const float f2 = m2 == top || m2 == -kInf ? 1.0f : exp2f((m2 - top) * a.scale2);
-        m = top;
-        l = l * f + l2 * f2;
+        const float base2 = to[16 * kO * 64], low = fminf(base, base2), f = joined(low, base), f2 = joined(low, base2);
+        base = low;
+        l = l * f + to[(16 * kO + 1) * 64] * f2;
         for (int x = 0; x < 16 * kO; ++x) o[x / 16][x % 16] = o[x / 16][x % 16] * f + to[x * 64] * f2;
     }
     if (!real) return;
@@ -1002,12 +1008,12 @@ __global__ __launch_bounds__(256, (query_terms(CT, QT) * D >= 256 ? 1 : 2)) void
                 *reinterpret_cast<f32x4*>(part.o + at * D + 32 * e + 8 * x + 4 * half) =
                     f32x4{o[e][4 * x], o[e][4 * x + 1], o[e][4 * x + 2], o[e][4 * x + 3]};
         if (half == 0) {
-            part.ml[2 * at] = m;
+            part.ml[2 * at] = base;
             part.ml[2 * at + 1] = l;
         }
         return;
     }
-    const float inv = l == 0.0f ? 0.0f : 1.0f / l, mu = m == -kInf ? 0.0f : m;
+    const float inv = l == 0.0f ? 0.0f : 1.0f / l;
     const uint32_t g = static_cast<uint32_t>(r % G);
     T* out = reinterpret_cast<T*>(a.out) + c * a.o_copy + qi * a.o_row + (h * a.group + g) * a.o_head;
     for (int e = 0; e < kO; ++e)
@@ -1019,10 +1025,9 @@ __global__ __launch_bounds__(256, (query_terms(CT, QT) * D >= 256 ? 1 : 2)) void
         }
     if (half == 0) {
         if (a.lse)
-            a.lse[(static_cast<uint64_t>(c) * a.heads * a.group + h * a.group + g) * a.nq + qi] =
-                l == 0.0f ? -kInf : (mu * a.scale2 + log2f(l)) * kLn2;
+            a.lse[(static_cast<uint64_t>(c) * a.heads * a.group + h * a.group + g) * a.nq + qi] = lse_of(a, base, l);
         if (a.stats) {
-            a.stats[2 * (ch * all + r)] = -mu * a.scale2;
+            a.stats[2 * (ch * all + r)] = l == 0.0f ? 0.0f : base;
             a.stats[2 * (ch * all + r) + 1] = inv;
         }
     }
@@ -1041,26 +1046,23 @@ __global__ __launch_bounds__(256) void join_rows_kernel(AttendDev a, Partial par
     const uint32_t c = ch / a.heads, h = ch % a.heads, i = r / a.group, g = r % a.group;
     if (static_cast<int>(i) >= span(a, c).rows || r >= all) return;
     const uint64_t at = static_cast<uint64_t>(ch) * part.splits * part.rows + r;
-    float top = -kInf, sum = 0.0f;
-    for (uint32_t s = 0; s < part.splits; ++s) top = fmaxf(top, part.ml[2 * (at + static_cast<uint64_t>(part.rows) * s)]);
-    const float mu = top == -kInf ? 0.0f : top;
+    float base = kInf, sum = 0.0f;
+    for (uint32_t s = 0; s < part.splits; ++s) base = fminf(base, part.ml[2 * (at + static_cast<uint64_t>(part.rows) * s)]);
     f32x4 o = {};
     for (uint32_t s = 0; s < part.splits; ++s) {
         const uint64_t x = at + static_cast<uint64_t>(part.rows) * s;
-        const f32x4 p = *reinterpret_cast<const f32x4*>(part.o + x * D + d);
-        const float ms = part.ml[2 * x], f = ms == top || ms == -kInf ? 1.0f : exp2f((ms - mu) * a.scale2);
-        sum += part.ml[2 * x + 1] * f;       // without a largest logit: 0, or NaN from NaN logits
-        if (ms != -kInf) o += p * f;
+        const float f = joined(base, part.ml[2 * x]);
+        sum += part.ml[2 * x + 1] * f;
+        o += *reinterpret_cast<const f32x4*>(part.o + x * D + d) * f;
     }
     T4 y;
     for (int e = 0; e < 4; ++e) y[e] = static_cast<T>(sum == 0.0f ? 0.0f : o[e] / sum);
     *reinterpret_cast<T4*>(reinterpret_cast<T*>(a.out) + c * a.o_copy + i * a.o_row + (h * a.group + g) * a.o_head + d) = y;
     if (d == 0) {
         if (a.lse)
-            a.lse[(static_cast<uint64_t>(c) * a.heads * a.group + h * a.group + g) * a.nq + i] =
-                sum == 0.0f ? -kInf : (mu * a.scale2 + log2f(sum)) * kLn2;
+            a.lse[(static_cast<uint64_t>(c) * a.heads * a.group + h * a.group + g) * a.nq + i] = lse_of(a, base, sum);
         if (a.stats) {
-            a.stats[2 * (static_cast<uint64_t>(ch) * all + r)] = -mu * a.scale2;
+            a.stats[2 * (static_cast<uint64_t>(ch) * all + r)] = sum == 0.0f ? 0.0f : base;
             a.stats[2 * (static_cast<uint64_t>(ch) * all + r) + 1] = sum == 0.0f ? 0.0f : 1.0f / sum;
         }
     }

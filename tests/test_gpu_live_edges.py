@@ -34,3 +34,31 @@ def test_millions_of_rows(ctx, copies, G, n):
     total = w.double().sum((1, 2)).cpu()
     assert ((total - n * G).abs() <= n * G * 2.0 ** -14).all()
     assert R.same(w[0], w[-1])
+
+
+@pytest.mark.parametrize("gap", [17.0, 17.5])
+@pytest.mark.parametrize("n,G", [(1, 1), (3, 4), (40, 1), (150, 1)])
+def test_f16_small_weights_of_many_slots(ctx, n, G, gap):
+    """A first slot `gap` nats ahead of all others, whose value is small: the
+    others' weights, 2^-24.5 and 2^-25.2 of its own, are what the output is.
+    They are rounded at 2^11 times their size (pkv_attend.hip): half a step,
+    2^-11 of them, or 2^-25 for those below 2^-14, here 2^-10 of them at most
+    (2^-14.3 is the smallest).  No part of the bound grows with the slots."""
+    from provekv_amd.pool import DeviceKVCache
+    C, H, T, D = 96, 8, 4096, 64          # as many heads as fill the chip: a row is not split over many workgroups
+    cache = DeviceKVCache(1, H, T, D, dtype=F16, copies=C)
+    v = (32 + 32 * torch.rand(T, D, generator=torch.Generator().manual_seed(1))).to(F16)
+    v[0] = 0
+    cache.buf[:, 0, 0, :, 0, 5] = gap
+    cache.buf[:, 0, 1] = v.cuda()
+    q = torch.zeros(C, n, H * G, D, dtype=F16)
+    q[..., 5] = 1.0
+    out = cache.attend(0, q.cuda(), torch.full((C,), T, dtype=torch.int32, device="cuda"), scale=1.0).cpu().double()
+    k = torch.zeros(1, 1, T, D, dtype=torch.float64)
+    k[..., 0, 5] = gap
+    ref = R.attend(q[:1, :, :1].double(), k, v.double().view(1, 1, T, D), [T], [n], 0, 0, 1.0)
+    h, u = 2.0 ** -11, 2.0 ** -24
+    rel = 2 * ref["dev"].unsqueeze(-1) * u + 4 * (T + 16) * u + 2 * h
+    bound = h * ref["out"] + rel * ref["mass"]
+    err = (out - ref["out"]).abs() - bound
+    assert not (err > 0).any() and not torch.isnan(err).any(), float(((out - ref["out"]).abs() / ref["out"]).max())
