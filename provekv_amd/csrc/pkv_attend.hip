@@ -144,6 +144,9 @@ __device__ inline uint32_t finite_or_0(uint32_t x) {
 // lift: f16 ends at 2^-24, so that weights up to 1 would lose all below 2^-25,
 // and a long cache's sum with them.  Weights up to 2^(11 + 4) use its top
 // instead: full precision down to 2^-25 of the largest, the end at 2^-36.
+// Other types have f32's exponents, whose end a sum of weighted values could
+// pass where their mean does not: a lift of 2^-8 over the slots keeps the sum
+// below the largest value (the host sets it).
 template <int MT> constexpr float kLag = MT == PKV_F16 ? 4.0f : 8.0f;
 // The base with a row's logits up to `top` seen as well.
 __device__ inline float lower_base(const AttendDev& a, float base, float top) {

@@ -11,6 +11,21 @@ pytestmark = pytest.mark.gpu
 F32, BF16, F16 = torch.float32, torch.bfloat16, torch.float16
 
 
+def held(kind, dtype, x, copies):
+    """(cache of `copies` times the rows x [1, 1, 2, heads, slots, dim], keys and
+    values as it holds them in f64)"""
+    from provekv_amd.pool import DeviceKVCache, FourBitKVCache
+    if kind == "plain":
+        cache = DeviceKVCache.over(x.to(dtype).cuda().repeat(copies, 1, 1, 1, 1, 1))
+        full = x.to(dtype).double()
+    else:
+        cache = FourBitKVCache(1, *x.shape[3:], copies=copies)
+        x = x.cuda().expand(copies, -1, -1, -1, -1, -1)
+        cache.store(x[:, :, 0], x[:, :, 1], 0)
+        full = R.fp4_values(cache.codes[:1], cache.scales[:1])
+    return cache, full[:, 0, 0], full[:, 0, 1]
+
+
 @pytest.mark.parametrize("copies,G,n", [(64, 32, 8192), (2, 128, 65537)])
 def test_millions_of_rows(ctx, copies, G, n):
     """copies x query heads x rows of 2^24 and past it, with weights: prompts of
@@ -62,3 +77,27 @@ def test_f16_small_weights_of_many_slots(ctx, n, G, gap):
     bound = h * ref["out"] + rel * ref["mass"]
     err = (out - ref["out"]).abs() - bound
     assert not (err > 0).any() and not torch.isnan(err).any(), float(((out - ref["out"]).abs() / ref["out"]).max())
+
+
+@pytest.mark.parametrize("kind,dtype", [("plain", F32), ("plain", BF16), ("fp4", F32), ("fp4", BF16)],
+                         ids=["f32", "bf16", "fp4-f32", "fp4-bf16"])
+@pytest.mark.parametrize("D", [64, 128])
+@pytest.mark.parametrize("n,G,copies", [(1, 1, 1), (1, 1, 400), (5, 3, 2), (40, 1, 2), (40, 1, 400), (300, 2, 1)])
+def test_values_near_the_types_largest(ctx, n, G, copies, D, kind, dtype):
+    """Means of values up to 2^126: sums over thousands of slots, before they are
+    divided, stay finite."""
+    T = 3000
+    x = torch.randn(1, 1, 2, 1, T, D, generator=torch.Generator().manual_seed(2))
+    x[:, :, 1] = (0.25 + 0.75 * torch.rand(x[:, :, 1].shape, generator=torch.Generator().manual_seed(3))) * 2.0 ** 126
+    cache, k, v = held(kind, dtype, x, copies)
+    q = torch.randn(1, n, G, D, generator=torch.Generator().manual_seed(4)).to(dtype)
+    w = torch.zeros(copies, 1, T, device="cuda")
+    lse = torch.zeros(copies, G, n, device="cuda")
+    out = cache.attend(0, q.cuda().expand(copies, -1, -1, -1), T, weights=w, lse=lse)
+    ref = R.attend(q.double(), k, v, [T], [n], 0, 0, 1 / math.sqrt(D))
+    for c in {0, copies - 1}:
+        err = (out[c:c + 1].cpu().double() - ref["out"]).abs()
+        assert (err <= R.out_bound(ref, dtype)).all()
+        assert ((lse[c:c + 1].cpu().double() - ref["lse"]).abs() <= R.lse_bound(ref)).all()
+        err = (w[c:c + 1].cpu().double() - ref["weights"]).abs()
+        assert (err <= R.weights_bound(ref, torch.zeros(1, 1, T), n * G)).all()
