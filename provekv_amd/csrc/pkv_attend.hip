@@ -275,6 +275,30 @@ struct SlotTile {
             for (int t = 0; t < kSub; ++t)
                 for (int j = 0; j < 4; ++j) v[t][j][0] = expand(v[t][j][0][0], vs[t][j]);
     }
+    // Infinities and NaN among slot j of piece t's values to 0; true if the lane had any.
+    __device__ bool clean(int t, int j) {
+        bool odd = false;
+        for (int q = 0; q < kVRegs; ++q)
+            for (int w = 0; w < 4; ++w) {
+                uint32_t y = v[t][j][q][w];
+                if constexpr (CT == PKV_F32) y = (y & 0x7f800000u) == 0x7f800000u ? 0 : y;
+                else if (w < kPer / 2) y = finite_or_0<mat_type(CT)>(y);
+                odd |= y != v[t][j][q][w];
+                v[t][j][q][w] = y;
+            }
+        return odd;
+    }
+    // The value that output register (e, r) of lane group g meets, of the row whose bytes are at `p` (scale bytes `sp`).
+    __device__ static float value(const uint8_t* p, const uint8_t* sp, int e, int r, uint32_t g) {
+        const uint32_t d = out_channel(e, r, g);
+        if constexpr (CT == PKV_F32) return reinterpret_cast<const float*>(p)[d];
+        else if constexpr (CT == PKV_FP4)
+            return __uint_as_float(expand(p[d / 2] >> d % 2 * 4, sp[d / 32])[0] << 16);
+        else return static_cast<float>(reinterpret_cast<const typename Elem<CT>::T*>(p)[d]);
+    }
+    __device__ static uint32_t out_channel(int e, int r, uint32_t g) {
+        return CT == PKV_F32 ? 64 * (e / 4) + 4 * (4 * g + r) + e % 4 : kPer * (4 * g + r) + e;
+    }
     // The channel that word `word` of step `s` of a lane's keys starts at (two channels a word, 16-bit types).
     __device__ static uint32_t channel(int s, uint32_t g) {
         return CT == PKV_FP4 ? (D / 4) * g + 8 * s : CT == PKV_F32 ? 16 * s + 4 * g : 32 * s + 8 * g;
@@ -336,7 +360,8 @@ __global__ __launch_bounds__(256, 2) void decode_kernel(AttendDev a, Partial par
     auto fetch = [&](Tile& x, int t) {   // past the last tile: the last again, unused
         x.load(kp, vp, ksp, vsp, a.kv.slot, tl.slot(min(t, t1 - 1), Tile::kStep), tl.high - 1, lane);
     };
-    auto work = [&](Tile& x, int t) {
+    auto work = [&](Tile& x, int t, auto again) {
+        constexpr bool CLEAN = decltype(again)::value;   // infinities and NaN of the values by themselves
         const int slot = tl.slot(t, Tile::kStep);
         // logits
         f32x4 sc[kSub] = {};
@@ -352,26 +377,24 @@ __global__ __launch_bounds__(256, 2) void decode_kernel(AttendDev a, Partial par
                 }
             }
         const bool full = all_visible(a, sp.first, pos1, slot, slot + Tile::kStep - 1);
-        if (LOGITS && real)
+        if (LOGITS && !CLEAN && real)
             for (int u = 0; u < kSub; ++u)
                 *reinterpret_cast<f32x4*>(part.logits + (static_cast<uint64_t>(ch) * a.nq * a.group + row) * part.ld +
                                           slot + 16 * u + 4 * g) = sc[u];
         x.expand_values();
-        bool odd = false;   // a value that must not meet the weight 0 of a row that does not see it
         if (!full) {
             for (int u = 0; u < kSub; ++u)
                 for (int j = 0; j < 4; ++j) {
                     const int key = slot + 16 * u + 4 * static_cast<int>(g) + j;
                     if (!visible(a, pos, key)) sc[u][j] = -kInf;
-                    const bool any = any_visible(a, tl, key);
-                    for (int n = 0; n < Tile::kVRegs; ++n)
-                        for (int w = 0; w < 4; ++w) {
-                            if (!any) x.v[u][j][n][w] = 0;
-                            if constexpr (CT == PKV_F32) odd |= (x.v[u][j][n][w] & 0x7f800000u) == 0x7f800000u;
-                            else if (w < kO / 2) odd |= nonfinite2<MT>(x.v[u][j][n][w]);
-                        }
+                    if (!any_visible(a, tl, key))
+                        for (int n = 0; n < Tile::kVRegs; ++n) x.v[u][j][n] = u32x4{};
                 }
         }
+        bool odd[kSub][4] = {};
+        if constexpr (CLEAN)
+            for (int u = 0; u < kSub; ++u)
+                for (int j = 0; j < 4; ++j) odd[u][j] = x.clean(u, j);
         float top = fmaxf(fmaxf(sc[0][0], sc[0][1]), fmaxf(sc[0][2], sc[0][3]));
         for (int u = 1; u < kSub; ++u)
             top = fmaxf(top, fmaxf(fmaxf(sc[u][0], sc[u][1]), fmaxf(sc[u][2], sc[u][3])));
@@ -393,49 +416,48 @@ __global__ __launch_bounds__(256, 2) void decode_kernel(AttendDev a, Partial par
                 l += p[u][j];
             }
         // weighted values
-        auto gather = [&](f32x4 (&acc)[kO], const Tile& y) {
-            if constexpr (CT == PKV_F32) {
-                for (int j = 0; j < 4; ++j)
-                    for (int n = 0; n < Tile::kVRegs; ++n)
-                        for (int e = 0; e < 4; ++e)
-                            acc[4 * n + e] = __builtin_amdgcn_mfma_f32_16x16x4f32(__uint_as_float(y.v[0][j][n][e]),
-                                                                                  p[0][j], acc[4 * n + e], 0, 0, 0);
-            } else {
-                float r[kSub][4];
-                for (int u = 0; u < kSub; ++u)
-                    for (int j = 0; j < 4; ++j) r[u][j] = p[u][j];
-                u32x4 pt[NP];
-                for (int n = 0; n < NP; ++n)
-                    pt[n] = u32x4{pack_term<MT>(r[0][0], r[0][1]), pack_term<MT>(r[0][2], r[0][3]),
-                                  pack_term<MT>(r[1][0], r[1][1]), pack_term<MT>(r[1][2], r[1][3])};
-                for (int e = 0; e < kO; ++e) {
-                    const uint32_t sel = e % 2 ? 0x07060302u : 0x05040100u;
-                    const u32x4 va = {__builtin_amdgcn_perm(y.v[0][1][0][e / 2], y.v[0][0][0][e / 2], sel),
-                                      __builtin_amdgcn_perm(y.v[0][3][0][e / 2], y.v[0][2][0][e / 2], sel),
-                                      __builtin_amdgcn_perm(y.v[1][1][0][e / 2], y.v[1][0][0][e / 2], sel),
-                                      __builtin_amdgcn_perm(y.v[1][3][0][e / 2], y.v[1][2][0][e / 2], sel)};
-                    for (int n = NP - 1; n >= 0; --n) acc[e] = mma16<MT>(va, pt[n], acc[e]);
-                }
-            }
-        };
-        if (__builtin_expect(__any(odd) && sp.rows > 1, 0)) {
-            // an infinity or NaN in a slot that only some rows see: each query
-            // row by itself, with the slots it does not see cleared
-            for (int i = 0; i < sp.rows; ++i) {
-                Tile y = x;
-                for (int u = 0; u < kSub; ++u)
-                    for (int j = 0; j < 4; ++j)
-                        if (!visible(a, sp.first + i, slot + 16 * u + 4 * static_cast<int>(g) + j))
-                            for (int n = 0; n < Tile::kVRegs; ++n) y.v[u][j][n] = u32x4{};
-                f32x4 acc[kO];
-                for (int e = 0; e < kO; ++e) acc[e] = o[e];
-                gather(acc, y);
-                if (qi == i)
-                    for (int e = 0; e < kO; ++e) o[e] = acc[e];
-            }
+        if constexpr (CT == PKV_F32) {
+            for (int j = 0; j < 4; ++j)
+                for (int n = 0; n < Tile::kVRegs; ++n)
+                    for (int e = 0; e < 4; ++e)
+                        o[4 * n + e] = __builtin_amdgcn_mfma_f32_16x16x4f32(__uint_as_float(x.v[0][j][n][e]), p[0][j],
+                                                                            o[4 * n + e], 0, 0, 0);
         } else {
-            gather(o, x);
+            float r[kSub][4];
+            for (int u = 0; u < kSub; ++u)
+                for (int j = 0; j < 4; ++j) r[u][j] = p[u][j];
+            u32x4 pt[NP];
+            for (int n = 0; n < NP; ++n)
+                pt[n] = u32x4{pack_term<MT>(r[0][0], r[0][1]), pack_term<MT>(r[0][2], r[0][3]),
+                              pack_term<MT>(r[1][0], r[1][1]), pack_term<MT>(r[1][2], r[1][3])};
+            for (int e = 0; e < kO; ++e) {
+                const uint32_t sel = e % 2 ? 0x07060302u : 0x05040100u;
+                const u32x4 va = {__builtin_amdgcn_perm(x.v[0][1][0][e / 2], x.v[0][0][0][e / 2], sel),
+                                  __builtin_amdgcn_perm(x.v[0][3][0][e / 2], x.v[0][2][0][e / 2], sel),
+                                  __builtin_amdgcn_perm(x.v[1][1][0][e / 2], x.v[1][0][0][e / 2], sel),
+                                  __builtin_amdgcn_perm(x.v[1][3][0][e / 2], x.v[1][2][0][e / 2], sel)};
+                for (int n = NP - 1; n >= 0; --n) o[e] = mma16<MT>(va, pt[n], o[e]);
+            }
         }
+        if constexpr (CLEAN)
+            for (int u = 0; u < kSub; ++u)
+                for (int j = 0; j < 4; ++j) {
+                    const uint64_t has = __ballot(odd[u][j]);
+#pragma unroll 1
+                    for (uint32_t g2 = 0; g2 < 4; ++g2) {
+                        if (!(has >> 16 * g2 & 0xffff)) continue;
+                        const int key = slot + 16 * u + 4 * static_cast<int>(g2) + j;
+                        const bool sees = real && visible(a, pos, key);
+                        const float w = __shfl(p[u][j], static_cast<int>(16 * g2 + row));
+                        const uint64_t at = static_cast<uint64_t>(key) * a.kv.slot;
+                        const uint8_t* vr = vp + (CT == PKV_FP4 ? at / 2 : CT == PKV_F32 ? at * 4 : at * 2);
+                        for (int e = 0; e < kO; ++e)
+                            for (int r = 0; r < 4; ++r) {
+                                const float v = Tile::value(vr, CT == PKV_FP4 ? vsp + at / 32 : nullptr, e, r, g);
+                                if (sees && (__float_as_uint(v) & 0x7f800000u) == 0x7f800000u) o[e][r] += w * v;
+                            }
+                    }
+                }
     };
     // two tiles in turn: one is on its way while the other is worked on
     const int first = t0 + static_cast<int>(wave);
@@ -444,22 +466,36 @@ __global__ __launch_bounds__(256, 2) void decode_kernel(AttendDev a, Partial par
         fetch(even, first);
         for (int t = first; t < t1; t += 8) {
             fetch(odd, t + 4);
-            work(even, t);
+            work(even, t, std::false_type());
             if (t + 4 >= t1) break;
             fetch(even, t + 8);
-            work(odd, t + 4);
+            work(odd, t + 4, std::false_type());
+        }
+        // An infinity or NaN among the values: a row that does not see it has met it with the weight 0, and the terms
+        // of a weight that does see it may be 0 or negative.  Again, with those values taken out of the products and
+        // each added to the rows that see it.
+        bool bad = false;
+        for (int e = 0; e < kO; ++e)
+            for (int r = 0; r < 4; ++r) bad |= (__float_as_uint(o[e][r]) & 0x7f800000u) == 0x7f800000u;
+        if (__builtin_expect(__any(bad && real), 0)) {
+            base = kInf;
+            l = 0.0f;
+            for (int e = 0; e < kO; ++e) o[e] = f32x4{};
+#pragma unroll 1
+            for (int t = first; t < t1; t += 4) {
+                fetch(even, t);
+                work(even, t, std::true_type());
+            }
         }
     }
     l += __shfl_xor(l, 16);
     l += __shfl_xor(l, 32);
 
-    // the four waves' shares joined; channel of o[e][r]: see SlotTile
+    // the four waves' shares joined
     __shared__ float so[4][16][D + 4], sb[4][16], sl[4][16];
     for (int r = 0; r < 4; ++r)
         for (int e = 0; e < kO; ++e) {
-            const int w = 4 * g + r;
-            const int d = CT == PKV_F32 ? 64 * (e / 4) + 4 * w + e % 4 : kO * w + e;
-            so[wave][row][d] = o[e][r];
+            so[wave][row][Tile::out_channel(e, r, g)] = o[e][r];
         }
     if (g == 0) { sb[wave][row] = base; sl[wave][row] = l; }
     __syncthreads();

@@ -101,3 +101,36 @@ def test_values_near_the_types_largest(ctx, n, G, copies, D, kind, dtype):
         assert ((lse[c:c + 1].cpu().double() - ref["lse"]).abs() <= R.lse_bound(ref)).all()
         err = (w[c:c + 1].cpu().double() - ref["weights"]).abs()
         assert (err <= R.weights_bound(ref, torch.zeros(1, 1, T), n * G)).all()
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16, F16], ids=["f32", "bf16", "f16"])
+@pytest.mark.parametrize("D", [64, 128])
+@pytest.mark.parametrize("window", [0, 40])
+@pytest.mark.parametrize("n,G,T", [(1, 1, 60), (1, 4, 3000), (4, 2, 300), (16, 1, 300), (17, 1, 300), (140, 2, 400)])
+def test_infinite_values_keep_their_sign(ctx, n, G, T, window, D, dtype):
+    """sum w_j v_j with infinities among the values that a row sees: inf with
+    their sign, NaN where both signs meet or a NaN is among them, and the other
+    channels and rows as with 0 in those places."""
+    x = torch.randn(1, 1, 2, 2, T, D, generator=torch.Generator().manual_seed(5))
+    bad = [(3, 1, math.inf), (3, 7, -math.inf), (T // 2, D - 1, -math.inf), (T - 1 - n // 2, 1, math.inf),
+           (T - 1 - n // 2, 7, math.inf), (T - 1 - n // 3, 33, math.inf), (T - 1, 34, -math.inf), (T - 9, 40, math.nan)]
+    for slot, d, _ in bad:
+        x[0, 0, 1, :, slot, d] = 0
+    cache, k, v = held("plain", dtype, x, 1)
+    q = (0.2 * torch.randn(1, n, 2 * G, D, generator=torch.Generator().manual_seed(6))).to(dtype)
+    ref = R.attend(q.double(), k, v, [T], [n], window, 2, 1 / math.sqrt(D))
+    for slot, d, value in bad:
+        cache.buf[0, 0, 1, 1, slot, d] = value        # the second head's
+    lse = torch.zeros(1, 2 * G, n, device="cuda")
+    got = cache.attend(0, q.cuda(), T, window=window, sinks=2, lse=lse).cpu().double()
+    want = ref["out"].clone()
+    for i in range(n):
+        see = R.seen(T - n + i, T, window, 2)
+        for slot, d, value in bad:
+            if see[slot]:
+                want[0, i, G:, d] += value
+    assert R.same(torch.isnan(got), torch.isnan(want)) and R.same(got.isposinf(), want.isposinf())
+    assert R.same(got.isneginf(), want.isneginf())
+    fin = torch.isfinite(want)
+    assert ((got - want).abs()[fin] <= R.out_bound(ref, dtype)[fin]).all()
+    assert ((lse.cpu().double() - ref["lse"]).abs() <= R.lse_bound(ref)).all()
