@@ -126,11 +126,6 @@ AttendDev attend_dev(const pkv_attend_op& op) {
     a.sinks = op.sinks;
     a.reach = op.window ? std::min(op.window, 0x80000000u) : 0x80000000u;
     a.scale2 = static_cast<float>(static_cast<double>(op.scale) * 1.4426950408889634074);
-    // f16: see kLag in pkv_attend.hip.  Else 2^-8 (the lag) over the slots, so that a sum of weighted values is at most the
-    // largest value: with weights up to 2^8 it could pass the type's end where the mean does not
-    int bits = 0;
-    while (bits < 31 && 1ull << bits < a.max_len) ++bits;
-    a.lift = op.cache.dtype == PKV_F16 ? 11.0f : -8.0f - static_cast<float>(bits);
     return a;
 }
 

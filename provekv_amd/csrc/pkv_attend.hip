@@ -136,27 +136,39 @@ __device__ inline uint32_t finite_or_0(uint32_t x) {
     return x;
 }
 
-// Softmax weights are held as 2^(s * scale2 + base), base = lift - (largest
-// logit) * scale2 when it was last set: up to kLag behind the largest logit seen
-// since, so that sums are rescaled seldom; +inf before the first logit.  A
-// share's base goes with its sums, exact as it was used.
+// Softmax weights are held as 2^(s * scale2 + base).  base is an integer, kLift -
+// (largest logit) * scale2 rounded up when it was last set: the largest logit
+// may since have grown by up to 2^kLag, so that sums are rescaled seldom, and
+// rescaling and joining multiply by powers of two, without an error.  +inf
+// before the first logit.  A share's base goes with its sums.
 //
-// lift: f16 ends at 2^-24, so that weights up to 1 would lose all below 2^-25,
-// and a long cache's sum with them.  Weights up to 2^(11 + 4) use its top
-// instead: full precision down to 2^-25 of the largest, the end at 2^-36.
-// Other types have f32's exponents, whose end a sum of weighted values could
-// pass where their mean does not: a lift of 2^-8 over the slots keeps the sum
-// below the largest value (the host sets it).
+// f16 ends at 2^-24, so that weights up to 1 would lose all below 2^-25, and a
+// long cache's sum with them.  Weights up to 2^(11 + 4) use its top instead:
+// full precision down to 2^-25 of the largest, the end at 2^-36.
 template <int MT> constexpr float kLag = MT == PKV_F16 ? 4.0f : 8.0f;
+template <int MT> constexpr float kLift = MT == PKV_F16 ? 11.0f : 0.0f;
+// Weighted values are summed before they are divided, and the sum can pass the
+// end of f32 (and bf16) where the mean does not.  The output is then not finite,
+// and the pass that looks for infinities among the values scales the weights by
+// 2^-kDown, the lag over 2^30 slots and more (decode_kernel), or a further one
+// does (rows_kernel); f16 values are far from it.
+// Shares that are joined are scaled by their number at most.
+template <int MT> constexpr int kDown = MT == PKV_F16 ? 0 : 40;
+constexpr int kJoinDown = 10;           // shares of a row: up to 768
+// 2^x, x an integer, +-inf or NaN (0).
+__device__ inline float power(float x) { return __builtin_ldexpf(1.0f, static_cast<int>(fmaxf(x, -1000.0f))); }
 // The base with a row's logits up to `top` seen as well.
-__device__ inline float lower_base(const AttendDev& a, float base, float top) {
-    return fminf(base, __builtin_fmaf(-top, a.scale2, a.lift));
+__device__ inline float lower_base(const AttendDev& a, float lift, float base, float top) {
+    return fminf(base, lift - floorf(top * a.scale2));
 }
-// Of the weights of a share with `base` when they join those of a lower one.
-__device__ inline float joined(float low, float base) { return base == low ? 1.0f : exp2f(low - base); }
-// Log of the sum of exponentials.
-__device__ inline float lse_of(const AttendDev& a, float base, float sum) {
-    return sum == 0.0f ? -kInf : (log2f(sum * exp2f(-a.lift)) + (a.lift - base)) * kLn2;
+// Log of the sum of exponentials, and a row's (base, factor): weight = 2^(s * scale2 + base) * factor.  An empty row: -inf, 0.
+__device__ inline float lse_of(float base, float sum) {
+    if (sum == 0.0f) return -kInf;
+    return (log2f(__builtin_amdgcn_frexp_mantf(sum)) + (static_cast<float>(__builtin_amdgcn_frexp_expf(sum)) - base)) * kLn2;
+}
+__device__ inline void stats_of(float base, float sum, float* stats) {
+    stats[0] = sum == 0.0f ? 0.0f : base - static_cast<float>(__builtin_amdgcn_frexp_expf(sum));
+    stats[1] = sum == 0.0f ? 0.0f : 1.0f / __builtin_amdgcn_frexp_mantf(sum);
 }
 
 // The slots that the rows of a tile see, as tiles of `step` slots: [0, first)
@@ -399,9 +411,8 @@ __global__ __launch_bounds__(256, 2) void decode_kernel(AttendDev a, Partial par
         for (int u = 1; u < kSub; ++u)
             top = fmaxf(top, fmaxf(fmaxf(sc[u][0], sc[u][1]), fmaxf(sc[u][2], sc[u][3])));
         top = across32(across16(top, larger), larger);
-        if (__any(__builtin_fmaf(top, a.scale2, base) > a.lift + kLag<MT>)) {
-            const float low = lower_base(a, base, top);
-            const float f = base == kInf ? 1.0f : exp2f(low - base);
+        if (__any(__builtin_fmaf(top, a.scale2, base) > kLift<MT> + kLag<MT>)) {
+            const float low = lower_base(a, kLift<MT>, base, top), f = power(low - base);
             if (low < base) {
                 l *= f;
                 for (int e = 0; e < kO; ++e) o[e] *= f;
@@ -413,6 +424,7 @@ __global__ __launch_bounds__(256, 2) void decode_kernel(AttendDev a, Partial par
         for (int u = 0; u < kSub; ++u)
             for (int j = 0; j < 4; ++j) {
                 p[u][j] = __builtin_amdgcn_exp2f(__builtin_fmaf(sc[u][j], a.scale2, from));
+                if (CLEAN) p[u][j] *= power(-kDown<MT>);
                 l += p[u][j];
             }
         // weighted values
@@ -473,7 +485,7 @@ __global__ __launch_bounds__(256, 2) void decode_kernel(AttendDev a, Partial par
         }
         // An infinity or NaN among the values: a row that does not see it has met it with the weight 0, and the terms
         // of a weight that does see it may be 0 or negative.  Again, with those values taken out of the products and
-        // each added to the rows that see it.
+        // each added to the rows that see it; or a sum past the type's end: see kDown.
         bool bad = false;
         for (int e = 0; e < kO; ++e)
             for (int r = 0; r < 4; ++r) bad |= (__float_as_uint(o[e][r]) & 0x7f800000u) == 0x7f800000u;
@@ -486,6 +498,7 @@ __global__ __launch_bounds__(256, 2) void decode_kernel(AttendDev a, Partial par
                 fetch(even, t);
                 work(even, t, std::true_type());
             }
+            base -= kDown<MT>;
         }
     }
     l += __shfl_xor(l, 16);
@@ -505,14 +518,14 @@ __global__ __launch_bounds__(256, 2) void decode_kernel(AttendDev a, Partial par
         float sum = 0.0f;
         f32x4 acc = {};
         for (int w = 0; w < 4; ++w) {
-            const float f = joined(low, sb[w][r]);
+            const float f = power(low - 2 - sb[w][r]);
             sum += sl[w][r] * f;
             acc += *reinterpret_cast<const f32x4*>(&so[w][r][d]) * f;
         }
         const uint64_t at = (static_cast<uint64_t>(ch) * part.splits + split) * part.rows + r;
         *reinterpret_cast<f32x4*>(part.o + at * D + d) = acc;
         if (d == 0) {
-            part.ml[2 * at] = low;
+            part.ml[2 * at] = low - 2;
             part.ml[2 * at + 1] = sum;
         }
     }
@@ -527,7 +540,8 @@ __device__ inline void join_splits(const float* ml, uint32_t splits, uint32_t ro
     for (uint32_t s = lane; s < splits; s += 64) low = fminf(low, ml[step * s]);
     for (int x = 32; x; x >>= 1) low = fminf(low, __shfl_xor(low, x));
     float l = 0.0f;
-    for (uint32_t s = lane; s < splits; s += 64) l += ml[step * s + 1] * joined(low, ml[step * s]);
+    low -= kJoinDown;
+    for (uint32_t s = lane; s < splits; s += 64) l += ml[step * s + 1] * power(low - ml[step * s]);
     *sum = wave_sum(l);
     *base = low;
 }
@@ -553,7 +567,7 @@ __global__ __launch_bounds__(256) void join_kernel(AttendDev a, Partial part, ui
         f32x4 o = {};
         for (uint32_t s = first; s < part.splits; s += kShares) {
             const uint64_t x = at + static_cast<uint64_t>(part.rows) * s;
-            o += *reinterpret_cast<const f32x4*>(part.o + x * D + d) * joined(base, part.ml[2 * x]);
+            o += *reinterpret_cast<const f32x4*>(part.o + x * D + d) * power(base - part.ml[2 * x]);
         }
         __shared__ f32x4 so[256];
         so[threadIdx.x] = o;
@@ -568,11 +582,8 @@ __global__ __launch_bounds__(256) void join_kernel(AttendDev a, Partial part, ui
         }
         if (threadIdx.x == 0) {
             if (a.lse)
-                a.lse[(static_cast<uint64_t>(c) * a.heads * a.group + h * a.group + g) * a.nq + i] = lse_of(a, base, sum);
-            if (a.stats) {
-                a.stats[2 * (static_cast<uint64_t>(ch) * all + r)] = sum == 0.0f ? 0.0f : base;
-                a.stats[2 * (static_cast<uint64_t>(ch) * all + r) + 1] = sum == 0.0f ? 0.0f : 1.0f / sum;
-            }
+                a.lse[(static_cast<uint64_t>(c) * a.heads * a.group + h * a.group + g) * a.nq + i] = lse_of(base, sum);
+            if (a.stats) stats_of(base, sum, a.stats + 2 * (static_cast<uint64_t>(ch) * all + r));
         }
         return;
     }
@@ -587,10 +598,7 @@ __global__ __launch_bounds__(256) void join_kernel(AttendDev a, Partial part, ui
         float base, sum;
         join_splits(part.ml + 2 * (static_cast<uint64_t>(ch) * part.splits * part.rows + r), part.splits, part.rows, lane,
                     &base, &sum);
-        if (lane == 0) {
-            st[r][0] = base;
-            st[r][1] = sum == 0.0f ? 0.0f : 1.0f / sum;
-        }
+        if (lane == 0) stats_of(base, sum, st[r]);
     }
     __syncthreads();
     const int j = j0 + 4 * static_cast<int>(threadIdx.x);
@@ -842,7 +850,9 @@ constexpr uint32_t row_tile(int ks) { return 128u / ks; }
 // A weight 0 times an infinity or NaN would be NaN in rows that do not see the
 // slot.  The loop does not look for those: an output that is not finite sends
 // the workgroup through it again, with infinities and NaN taken out of the
-// staged values and each added afterwards to the rows that see it.
+// staged values and each added afterwards to the rows that see it.  Where the
+// sums of finite values are not finite either, a third time with smaller
+// weights (kDown).
 template <int CT, int QT, int D, int KS>
 __global__ __launch_bounds__(256, (query_terms(CT, QT) * D >= 256 ? 1 : 2)) void rows_kernel(AttendDev a, Partial part,
                                                                                         uint32_t row_tiles) {
@@ -897,7 +907,8 @@ __global__ __launch_bounds__(256, (query_terms(CT, QT) * D >= 256 ? 1 : 2)) void
         return slot + share >= wt.high ||
                (slot + share + 32 * kU <= wt.low && static_cast<uint32_t>(slot + share) >= a.sinks);
     };
-    for (bool clean = false;; clean = true) {
+    float lift = kLift<MT>;
+    for (int pass = 0;; ++pass) {
         base = kInf;
         l = 0.0f;
         for (int e = 0; e < kO; ++e) o[e] = f32x16{};
@@ -910,7 +921,7 @@ __global__ __launch_bounds__(256, (query_terms(CT, QT) * D >= 256 ? 1 : 2)) void
             uint8_t* buf = lds + ((t - t0) & 1) * St::kBytes;
             if (t + 1 < t1) fetch(t + 1);
             const int slot = tl.slot(t, St::kSlots);
-            if (__builtin_expect(clean, 0)) {
+            if (__builtin_expect(pass, 0)) {
                 St::clean(buf);
                 __syncthreads();
             }
@@ -934,9 +945,8 @@ __global__ __launch_bounds__(256, (query_terms(CT, QT) * D >= 256 ? 1 : 2)) void
                 for (int u = 0; u < kU; ++u)
                     for (int x = 0; x < 16; ++x) top = fmaxf(top, sc[u][x]);
                 top = across32(top, larger);
-                if (__any(__builtin_fmaf(top, a.scale2, base) > a.lift + kLag<MT>)) {
-                    const float low = lower_base(a, base, top);
-                    const float f = base == kInf ? 1.0f : exp2f(low - base);
+                if (__any(__builtin_fmaf(top, a.scale2, base) > lift + kLag<MT>)) {
+                    const float low = lower_base(a, lift, base, top), f = power(low - base);
                     if (low < base) {
                         l *= f;
                         for (int e = 0; e < kO; ++e) o[e] *= f;
@@ -979,12 +989,19 @@ __global__ __launch_bounds__(256, (query_terms(CT, QT) * D >= 256 ? 1 : 2)) void
             if (t + 1 < t1) st.land(lds + ((t + 1 - t0) & 1) * St::kBytes);
             __syncthreads();
         }
-        if (!clean) {
+        if (pass < 2) {
             bool odd = false;
             for (int e = 0; e < kO; ++e)
                 for (int x = 0; x < 16; ++x) odd |= (__float_as_uint(o[e][x]) & 0x7f800000u) == 0x7f800000u;
-            if (!__syncthreads_or(odd && real)) break;
-            continue;
+            // with the values finite, from a NaN among the logits, as the weights' sum, or past the type's end
+            if (pass) odd &= !__builtin_isnan(across32(l, [](float x, float y) { return x + y; }));
+            const bool again = __syncthreads_or(odd && real);
+            if (!pass && !again) break;
+            if (!pass) continue;
+            if (again && kDown<MT>) {
+                lift -= kDown<MT>;
+                continue;
+            }
         }
         const float from = base == kInf ? 0.0f : base;
 #pragma unroll 1
@@ -1033,7 +1050,7 @@ __global__ __launch_bounds__(256, (query_terms(CT, QT) * D >= 256 ? 1 : 2)) void
         }
         __syncthreads();
         if (share) return;
-        const float base2 = to[16 * kO * 64], low = fminf(base, base2), f = joined(low, base), f2 = joined(low, base2);
+        const float base2 = to[16 * kO * 64], low = fminf(base, base2) - 1, f = power(low - base), f2 = power(low - base2);
         base = low;
         l = l * f + to[(16 * kO + 1) * 64] * f2;
         for (int x = 0; x < 16 * kO; ++x) o[x / 16][x % 16] = o[x / 16][x % 16] * f + to[x * 64] * f2;
@@ -1064,11 +1081,8 @@ __global__ __launch_bounds__(256, (query_terms(CT, QT) * D >= 256 ? 1 : 2)) void
         }
     if (half == 0) {
         if (a.lse)
-            a.lse[(static_cast<uint64_t>(c) * a.heads * a.group + h * a.group + g) * a.nq + qi] = lse_of(a, base, l);
-        if (a.stats) {
-            a.stats[2 * (ch * all + r)] = l == 0.0f ? 0.0f : base;
-            a.stats[2 * (ch * all + r) + 1] = inv;
-        }
+            a.lse[(static_cast<uint64_t>(c) * a.heads * a.group + h * a.group + g) * a.nq + qi] = lse_of(base, l);
+        if (a.stats) stats_of(base, l, a.stats + 2 * (ch * all + r));
     }
     return;
 }
@@ -1087,10 +1101,11 @@ __global__ __launch_bounds__(256) void join_rows_kernel(AttendDev a, Partial par
     const uint64_t at = static_cast<uint64_t>(ch) * part.splits * part.rows + r;
     float base = kInf, sum = 0.0f;
     for (uint32_t s = 0; s < part.splits; ++s) base = fminf(base, part.ml[2 * (at + static_cast<uint64_t>(part.rows) * s)]);
+    base -= kJoinDown;
     f32x4 o = {};
     for (uint32_t s = 0; s < part.splits; ++s) {
         const uint64_t x = at + static_cast<uint64_t>(part.rows) * s;
-        const float f = joined(base, part.ml[2 * x]);
+        const float f = power(base - part.ml[2 * x]);
         sum += part.ml[2 * x + 1] * f;
         o += *reinterpret_cast<const f32x4*>(part.o + x * D + d) * f;
     }
@@ -1099,11 +1114,8 @@ __global__ __launch_bounds__(256) void join_rows_kernel(AttendDev a, Partial par
     *reinterpret_cast<T4*>(reinterpret_cast<T*>(a.out) + c * a.o_copy + i * a.o_row + (h * a.group + g) * a.o_head + d) = y;
     if (d == 0) {
         if (a.lse)
-            a.lse[(static_cast<uint64_t>(c) * a.heads * a.group + h * a.group + g) * a.nq + i] = lse_of(a, base, sum);
-        if (a.stats) {
-            a.stats[2 * (static_cast<uint64_t>(ch) * all + r)] = sum == 0.0f ? 0.0f : base;
-            a.stats[2 * (static_cast<uint64_t>(ch) * all + r) + 1] = sum == 0.0f ? 0.0f : 1.0f / sum;
-        }
+            a.lse[(static_cast<uint64_t>(c) * a.heads * a.group + h * a.group + g) * a.nq + i] = lse_of(base, sum);
+        if (a.stats) stats_of(base, sum, a.stats + 2 * (static_cast<uint64_t>(ch) * all + r));
     }
 }
 

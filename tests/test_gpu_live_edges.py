@@ -134,3 +134,43 @@ def test_infinite_values_keep_their_sign(ctx, n, G, T, window, D, dtype):
     fin = torch.isfinite(want)
     assert ((got - want).abs()[fin] <= R.out_bound(ref, dtype)[fin]).all()
     assert ((lse.cpu().double() - ref["lse"]).abs() <= R.lse_bound(ref)).all()
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16, F16], ids=["f32", "bf16", "f16"])
+@pytest.mark.parametrize("n,T", [(1, 28), (3, 27), (40, 60), (200, 62)])
+def test_same_bits_whatever_the_launch_is_sized_by(ctx, n, T, dtype):
+    """Calls that are cut alike give the same bits for any max_len and capacity."""
+    from provekv_amd.pool import DeviceKVCache
+    x = torch.randn(1, 1, 2, 2, T, 64, generator=torch.Generator().manual_seed(7)).to(dtype).cuda()
+    q = torch.randn(1, n, 4, 64, generator=torch.Generator().manual_seed(8)).to(dtype).cuda()
+    lens = torch.tensor([T], dtype=torch.int32, device="cuda")
+    first = None
+    for room, max_len in ((T, T), (T + 1, T), (2 * T, T), (2 * T, None)):
+        buf = torch.zeros(1, 1, 2, 2, room, 64, dtype=dtype, device="cuda")
+        buf[:, :, :, :, :T] = x
+        cache = DeviceKVCache.over(buf)
+        w, lse = torch.zeros(1, 2, room, device="cuda"), torch.zeros(1, 4, n, device="cuda")
+        got = [cache.attend(0, q, lens, weights=w, lse=lse, max_len=max_len), lse, w[:, :, :T]]
+        first = first or got
+        for a, b in zip(got, first):
+            assert R.same(a, b)
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16], ids=["f32", "bf16"])
+@pytest.mark.parametrize("n,G", [(1, 1), (7, 2), (40, 1), (300, 1)])
+def test_infinite_and_large_values_together(ctx, n, G, dtype):
+    T, D = 3000, 64
+    x = torch.randn(1, 1, 2, 1, T, D, generator=torch.Generator().manual_seed(9))
+    x[:, :, 1] = (0.25 + 0.75 * torch.rand(x[:, :, 1].shape, generator=torch.Generator().manual_seed(3))) * 2.0 ** 126
+    x[0, 0, 1, 0, 11, 5] = x[0, 0, 1, 0, T - 1, 9] = 0
+    cache, k, v = held("plain", dtype, x, 1)
+    q = (0.2 * torch.randn(1, n, G, D, generator=torch.Generator().manual_seed(4))).to(dtype)
+    ref = R.attend(q.double(), k, v, [T], [n], 0, 0, 1 / math.sqrt(D))
+    cache.buf[0, 0, 1, 0, 11, 5], cache.buf[0, 0, 1, 0, T - 1, 9] = -math.inf, math.inf
+    got = cache.attend(0, q.cuda(), T).cpu().double()
+    want = ref["out"].clone()
+    want[..., 5] = -math.inf
+    want[0, n - 1, :, 9] = math.inf
+    assert R.same(got.isposinf(), want.isposinf()) and R.same(got.isneginf(), want.isneginf())
+    fin = torch.isfinite(want)
+    assert ((got - want).abs()[fin] <= R.out_bound(ref, dtype)[fin]).all()
