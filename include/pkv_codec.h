@@ -562,8 +562,12 @@ typedef struct pkv_kv_view {
  *            d_weights copies * heads * ceil(max_len / 128) (with a window, of
  *            the slots it reaches)
  * is 2^24 or more.
- * Logits, softmax and sums are held in 32 bits.  Asynchronous on `stream`; the
- * call can be captured. */
+ * Logits, the softmax's sums and outputs' sums are held in 32 bits.  Weights meet
+ * the values as two or more terms of a 16-bit type (f32 caches: as they are);
+ * with more than 16 rows of a KV head over a 16-bit cache, or of bf16 queries
+ * over 4 bits, as one: rounded to the type, which adds to the output's own
+ * rounding at most half a step of the type times sum w_j |v_j|.  Asynchronous on
+ * `stream`; the call can be captured. */
 typedef struct pkv_attend_op {
     pkv_kv_view cache;
     const void* d_q;
