@@ -156,8 +156,11 @@ class LiveCache:
         self._on_device(dev, q, weights, lse, out)
         if q.requires_grad and torch.is_grad_enabled():
             raise ValueError("attend has no backward pass: detach q or call it under torch.no_grad()")
+        sized = None      # by an int length: the call's own, so that a loop over lengths keeps one struct
         if max_len is None:
-            max_len = self.tokens if isinstance(lens, torch.Tensor) else min(max(int(lens), 1), self.tokens)
+            max_len = self.tokens
+            if not isinstance(lens, torch.Tensor):
+                sized = min(max(int(lens), 1), self.tokens)
 
         memory = self._pointers()
 
@@ -186,6 +189,9 @@ class LiveCache:
                 op.d_weights = weights.data_ptr()
             if lse is not None:
                 op.d_lse = lse.data_ptr()
+            if sized is not None:
+                op.max_len = sized
+                need = op.workspace_bytes = L.lib().pkv_attend_workspace(C.byref(op))
             if need:
                 work = torch.empty(need, dtype=torch.uint8, device=dev)
                 op.d_workspace = work.data_ptr()

@@ -174,3 +174,17 @@ def test_infinite_and_large_values_together(ctx, n, G, dtype):
     assert R.same(got.isposinf(), want.isposinf()) and R.same(got.isneginf(), want.isneginf())
     fin = torch.isfinite(want)
     assert ((got - want).abs()[fin] <= R.out_bound(ref, dtype)[fin]).all()
+
+
+@pytest.mark.parametrize("n", [1, 20])
+def test_int_lengths_are_the_launch_s_size(ctx, n):
+    """A loop over int lengths gives what length tensors of that max_len give."""
+    x = torch.randn(1, 1, 2, 2, 5000, 64, generator=torch.Generator().manual_seed(10))
+    cache, _, _ = held("plain", BF16, x, 2)
+    q = torch.randn(2, n, 4, 64, generator=torch.Generator().manual_seed(11)).to(BF16).cuda()
+    for length in (0, 1, 100, 129, 1000, 4097, 5000, 6000):
+        w, w2 = torch.zeros(2, 2, 2, 5000, device="cuda")
+        got = cache.attend(0, q, length, weights=w)
+        d = torch.full((2,), length, dtype=torch.int32, device="cuda")
+        want = cache.attend(0, q, d, weights=w2, max_len=min(max(length, 1), 5000))
+        assert R.same(got, want) and R.same(w, w2)
