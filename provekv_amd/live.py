@@ -128,6 +128,17 @@ class LiveCache:
         return x
 
     @staticmethod
+    def _served(t, call: str):
+        """No gradient or tangent of t is lost without a word."""
+        import torch
+        if t is None:
+            return
+        if t.requires_grad and torch.is_grad_enabled():
+            raise ValueError(f"{call} has no backward pass: detach its tensors or call it under torch.no_grad()")
+        if torch.autograd.forward_ad.unpack_dual(t).tangent is not None:
+            raise ValueError(f"{call} has no forward-mode derivative: give it the primal of a dual tensor")
+
+    @staticmethod
     def _on_device(dev, *tensors):
         for t in tensors:
             if t is not None and t.device != dev:
@@ -154,8 +165,7 @@ class LiveCache:
         import torch
         dev = self.device
         self._on_device(dev, q, weights, lse, out)
-        if q.requires_grad and torch.is_grad_enabled():
-            raise ValueError("attend has no backward pass: detach q or call it under torch.no_grad()")
+        self._served(q, "attend")
         sized = None      # by an int length: the call's own, so that a loop over lengths keeps one struct
         if max_len is None:
             max_len = self.tokens
@@ -393,6 +403,7 @@ class FourBitKVCache(LiveCache):
                 raise TypeError("keys and values are both float32, bfloat16 or float16")
             if t.shape != (*lead, some.shape[-2], self.dim):
                 raise ValueError(f"keys and values must be {[*lead, 'rows', self.dim]}")
+            self._served(t, "store")
         dev = self.device
         self._on_device(dev, keys, values)
         ctx, handle, guard = self._frame(dev, stream)
