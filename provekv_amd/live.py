@@ -308,7 +308,7 @@ class LiveCache:
             L.check(L.lib().pkv_evict(ctx.ptr, C.byref(op), handle), "pkv_evict")
         if layer is None:
             filled = min(self._seq_len, budget)
-            to._seq_len = filled if into is None else max(to._seq_len, filled)
+            to._seq_len = filled if to is self else max(to._seq_len, filled)
         return kept, new_lens, packed
 
 
