@@ -136,11 +136,10 @@ __device__ inline uint32_t finite_or_0(uint32_t x) {
     return x;
 }
 
-// Softmax weights are held as 2^(s * scale2 + base).  base is an integer, kLift -
-// (largest logit) * scale2 rounded up when it was last set: the largest logit
-// may since have grown by up to 2^kLag, so that sums are rescaled seldom, and
-// rescaling and joining multiply by powers of two, without an error.  +inf
-// before the first logit.  A share's base goes with its sums.
+// Softmax weights are held as 2^(s * scale2 + base), base = kLift - (largest
+// logit) * scale2 when it was last set: the largest logit may since have grown
+// by up to 2^kLag, so that sums are rescaled seldom.  +inf before the first
+// logit.  A share's base goes with its sums, as it was used.
 //
 // f16 ends at 2^-24, so that weights up to 1 would lose all below 2^-25, and a
 // long cache's sum with them.  Weights up to 2^(11 + 4) use its top instead:
@@ -151,24 +150,24 @@ template <int MT> constexpr float kLift = MT == PKV_F16 ? 11.0f : 0.0f;
 // end of f32 (and bf16) where the mean does not.  The output is then not finite,
 // and the pass that looks for infinities among the values scales the weights by
 // 2^-kDown, the lag over 2^30 slots and more (decode_kernel), or a further one
-// does (rows_kernel); f16 values are far from it.
-// Shares that are joined are scaled by their number at most.
+// does (rows_kernel); f16 values are far from it.  Shares' outputs are stored
+// 2^-kPartDown as large and joined 2^-kJoinDown, by as many shares as there can be.
 template <int MT> constexpr int kDown = MT == PKV_F16 ? 0 : 40;
+constexpr int kPartDown = 2;            // decode_kernel's four waves
 constexpr int kJoinDown = 10;           // shares of a row: up to 768
-// 2^x, x an integer, +-inf or NaN (0).
-__device__ inline float power(float x) { return __builtin_ldexpf(1.0f, static_cast<int>(fmaxf(x, -1000.0f))); }
+constexpr float power(int x) { return x < 0 ? 0.5f * power(x + 1) : x ? 2.0f * power(x - 1) : 1.0f; }
+template <int X> constexpr float kPower = power(X);   // 2^X
 // The base with a row's logits up to `top` seen as well.
 __device__ inline float lower_base(const AttendDev& a, float lift, float base, float top) {
-    return fminf(base, lift - floorf(top * a.scale2));
+    return fminf(base, __builtin_fmaf(-top, a.scale2, lift));
 }
+// Of the weights with `base` when they join those of a lower one.
+__device__ inline float joined(float low, float base) { return base == low ? 1.0f : exp2f(low - base); }
 // Log of the sum of exponentials, and a row's (base, factor): weight = 2^(s * scale2 + base) * factor.  An empty row: -inf, 0.
-__device__ inline float lse_of(float base, float sum) {
-    if (sum == 0.0f) return -kInf;
-    return (log2f(__builtin_amdgcn_frexp_mantf(sum)) + (static_cast<float>(__builtin_amdgcn_frexp_expf(sum)) - base)) * kLn2;
-}
+__device__ inline float lse_of(float base, float sum) { return sum == 0.0f ? -kInf : (log2f(sum) - base) * kLn2; }
 __device__ inline void stats_of(float base, float sum, float* stats) {
-    stats[0] = sum == 0.0f ? 0.0f : base - static_cast<float>(__builtin_amdgcn_frexp_expf(sum));
-    stats[1] = sum == 0.0f ? 0.0f : 1.0f / __builtin_amdgcn_frexp_mantf(sum);
+    stats[0] = sum == 0.0f ? 0.0f : base;
+    stats[1] = sum == 0.0f ? 0.0f : 1.0f / sum;
 }
 
 // The slots that the rows of a tile see, as tiles of `step` slots: [0, first)
@@ -412,7 +411,7 @@ __global__ __launch_bounds__(256, 2) void decode_kernel(AttendDev a, Partial par
             top = fmaxf(top, fmaxf(fmaxf(sc[u][0], sc[u][1]), fmaxf(sc[u][2], sc[u][3])));
         top = across32(across16(top, larger), larger);
         if (__any(__builtin_fmaf(top, a.scale2, base) > kLift<MT> + kLag<MT>)) {
-            const float low = lower_base(a, kLift<MT>, base, top), f = power(low - base);
+            const float low = lower_base(a, kLift<MT>, base, top), f = joined(low, base);
             if (low < base) {
                 l *= f;
                 for (int e = 0; e < kO; ++e) o[e] *= f;
@@ -424,7 +423,7 @@ __global__ __launch_bounds__(256, 2) void decode_kernel(AttendDev a, Partial par
         for (int u = 0; u < kSub; ++u)
             for (int j = 0; j < 4; ++j) {
                 p[u][j] = __builtin_amdgcn_exp2f(__builtin_fmaf(sc[u][j], a.scale2, from));
-                if (CLEAN) p[u][j] *= power(-kDown<MT>);
+                if constexpr (CLEAN) p[u][j] *= kPower<-kDown<MT>>;
                 l += p[u][j];
             }
         // weighted values
@@ -498,7 +497,15 @@ __global__ __launch_bounds__(256, 2) void decode_kernel(AttendDev a, Partial par
                 fetch(even, t);
                 work(even, t, std::true_type());
             }
-            base -= kDown<MT>;
+            bool past = false;   // back, unless it does not fit
+            for (int e = 0; e < kO; ++e)
+                for (int r = 0; r < 4; ++r) past |= fabsf(o[e][r]) < kInf && !(fabsf(o[e][r]) * kPower<kDown<MT>> < kInf);
+            if (__any(past && real)) {
+                base -= kDown<MT>;
+            } else {
+                for (int e = 0; e < kO; ++e) o[e] *= kPower<kDown<MT>>;
+                l *= kPower<kDown<MT>>;
+            }
         }
     }
     l += __shfl_xor(l, 16);
@@ -518,14 +525,14 @@ __global__ __launch_bounds__(256, 2) void decode_kernel(AttendDev a, Partial par
         float sum = 0.0f;
         f32x4 acc = {};
         for (int w = 0; w < 4; ++w) {
-            const float f = power(low - 2 - sb[w][r]);
+            const float f = joined(low, sb[w][r]);
             sum += sl[w][r] * f;
-            acc += *reinterpret_cast<const f32x4*>(&so[w][r][d]) * f;
+            acc += *reinterpret_cast<const f32x4*>(&so[w][r][d]) * (f * kPower<-kPartDown>);
         }
         const uint64_t at = (static_cast<uint64_t>(ch) * part.splits + split) * part.rows + r;
         *reinterpret_cast<f32x4*>(part.o + at * D + d) = acc;
         if (d == 0) {
-            part.ml[2 * at] = low - 2;
+            part.ml[2 * at] = low;
             part.ml[2 * at + 1] = sum;
         }
     }
@@ -540,8 +547,7 @@ __device__ inline void join_splits(const float* ml, uint32_t splits, uint32_t ro
     for (uint32_t s = lane; s < splits; s += 64) low = fminf(low, ml[step * s]);
     for (int x = 32; x; x >>= 1) low = fminf(low, __shfl_xor(low, x));
     float l = 0.0f;
-    low -= kJoinDown;
-    for (uint32_t s = lane; s < splits; s += 64) l += ml[step * s + 1] * power(low - ml[step * s]);
+    for (uint32_t s = lane; s < splits; s += 64) l += ml[step * s + 1] * joined(low, ml[step * s]);
     *sum = wave_sum(l);
     *base = low;
 }
@@ -567,7 +573,7 @@ __global__ __launch_bounds__(256) void join_kernel(AttendDev a, Partial part, ui
         f32x4 o = {};
         for (uint32_t s = first; s < part.splits; s += kShares) {
             const uint64_t x = at + static_cast<uint64_t>(part.rows) * s;
-            o += *reinterpret_cast<const f32x4*>(part.o + x * D + d) * power(base - part.ml[2 * x]);
+            o += *reinterpret_cast<const f32x4*>(part.o + x * D + d) * (joined(base, part.ml[2 * x]) * kPower<-kJoinDown>);
         }
         __shared__ f32x4 so[256];
         so[threadIdx.x] = o;
@@ -577,7 +583,7 @@ __global__ __launch_bounds__(256) void join_kernel(AttendDev a, Partial part, ui
             T* out = reinterpret_cast<T*>(a.out) + c * a.o_copy + i * a.o_row + (h * a.group + g) * a.o_head;
             typedef T T4 __attribute__((ext_vector_type(4)));
             T4 y;
-            for (int e = 0; e < 4; ++e) y[e] = static_cast<T>(sum == 0.0f ? 0.0f : o[e] / sum);
+            for (int e = 0; e < 4; ++e) y[e] = static_cast<T>(sum == 0.0f ? 0.0f : o[e] / (sum * kPower<-kPartDown - kJoinDown>));
             *reinterpret_cast<T4*>(out + d) = y;
         }
         if (threadIdx.x == 0) {
@@ -837,10 +843,10 @@ constexpr uint32_t row_tile(int ks) { return 128u / ks; }
 // of the unrounded ones: a weight is off by up to half a step, so the output by
 // up to half a step of sum w |v| beside its own rounding -- twice that rounding
 // where one slot has nearly all the weight (measured at 64 rows on 2,048 slots
-// of 128, logits of deviation 4: 1.2 half steps in bf16 and 1.4 in f16 against
-// 0.98 and 0.93 of decode_kernel's), 1.07 to 1.4 times in the mean square.  A
-// second term costs half as much matrix work again, and a sum of the rounded
-// weights for the output's divisor (1.0 and 0.9 half steps, the mean square of
+// of 128, logits of deviation 4: 1.2 half steps of sum w |v| in bf16 against
+// 0.98 of decode_kernel's, 0.9 in f16 for both), 1.01 to 1.4 times in the mean
+// square.  A second term costs half as much matrix work again, and a sum of the
+// rounded weights for the output's divisor (0.97 half steps, the mean square of
 // even weights as before) 2.5 % of a prompt's time.  Over 4-bit codes weights
 // are as many bf16 terms as the query, one for bf16 queries.
 // Bound at head_dim 128 by the matrix cores (a tile is 32 matrix instructions of
@@ -953,7 +959,7 @@ __global__ __launch_bounds__(256, (query_terms(CT, QT) * D >= 256 ? 1 : 2)) void
                     for (int x = 0; x < 16; ++x) top = fmaxf(top, sc[u][x]);
                 top = across32(top, larger);
                 if (__any(__builtin_fmaf(top, a.scale2, base) > lift + kLag<MT>)) {
-                    const float low = lower_base(a, lift, base, top), f = power(low - base);
+                    const float low = lower_base(a, lift, base, top), f = joined(low, base);
                     if (low < base) {
                         l *= f;
                         for (int e = 0; e < kO; ++e) o[e] *= f;
@@ -1047,6 +1053,7 @@ __global__ __launch_bounds__(256, (query_terms(CT, QT) * D >= 256 ? 1 : 2)) void
         break;
     }
     l += __shfl_xor(l, 32);
+    constexpr int kShared = KS > 1 ? 1 : 0;   // outputs are 2^-kShared as large from here on
     if constexpr (KS > 1) {
         // the other share of the slots joins the first: [row block][o, base, l][lane]
         float* to = reinterpret_cast<float*>(lds) + wave * (16 * kO + 2) * 64 + lane;
@@ -1057,10 +1064,11 @@ __global__ __launch_bounds__(256, (query_terms(CT, QT) * D >= 256 ? 1 : 2)) void
         }
         __syncthreads();
         if (share) return;
-        const float base2 = to[16 * kO * 64], low = fminf(base, base2) - 1, f = power(low - base), f2 = power(low - base2);
+        const float base2 = to[16 * kO * 64], low = fminf(base, base2);
+        const float f = joined(low, base), f2 = joined(low, base2), of = f * kPower<-kShared>, of2 = f2 * kPower<-kShared>;
         base = low;
         l = l * f + to[(16 * kO + 1) * 64] * f2;
-        for (int x = 0; x < 16 * kO; ++x) o[x / 16][x % 16] = o[x / 16][x % 16] * f + to[x * 64] * f2;
+        for (int x = 0; x < 16 * kO; ++x) o[x / 16][x % 16] = o[x / 16][x % 16] * of + to[x * 64] * of2;
     }
     if (!real) return;
     const uint64_t all = static_cast<uint64_t>(a.nq) * a.group;
@@ -1069,14 +1077,14 @@ __global__ __launch_bounds__(256, (query_terms(CT, QT) * D >= 256 ? 1 : 2)) void
         for (int e = 0; e < kO; ++e)
             for (int x = 0; x < 4; ++x)
                 *reinterpret_cast<f32x4*>(part.o + at * D + 32 * e + 8 * x + 4 * half) =
-                    f32x4{o[e][4 * x], o[e][4 * x + 1], o[e][4 * x + 2], o[e][4 * x + 3]};
+                    f32x4{o[e][4 * x], o[e][4 * x + 1], o[e][4 * x + 2], o[e][4 * x + 3]} * kPower<kShared - kPartDown>;
         if (half == 0) {
             part.ml[2 * at] = base;
             part.ml[2 * at + 1] = l;
         }
         return;
     }
-    const float inv = l == 0.0f ? 0.0f : 1.0f / l;
+    const float inv = l == 0.0f ? 0.0f : 1.0f / l * kPower<kShared>;
     const uint32_t g = static_cast<uint32_t>(r % G);
     T* out = reinterpret_cast<T*>(a.out) + c * a.o_copy + qi * a.o_row + (h * a.group + g) * a.o_head;
     for (int e = 0; e < kO; ++e)
@@ -1108,16 +1116,15 @@ __global__ __launch_bounds__(256) void join_rows_kernel(AttendDev a, Partial par
     const uint64_t at = static_cast<uint64_t>(ch) * part.splits * part.rows + r;
     float base = kInf, sum = 0.0f;
     for (uint32_t s = 0; s < part.splits; ++s) base = fminf(base, part.ml[2 * (at + static_cast<uint64_t>(part.rows) * s)]);
-    base -= kJoinDown;
     f32x4 o = {};
     for (uint32_t s = 0; s < part.splits; ++s) {
         const uint64_t x = at + static_cast<uint64_t>(part.rows) * s;
-        const float f = power(base - part.ml[2 * x]);
+        const float f = joined(base, part.ml[2 * x]);
         sum += part.ml[2 * x + 1] * f;
-        o += *reinterpret_cast<const f32x4*>(part.o + x * D + d) * f;
+        o += *reinterpret_cast<const f32x4*>(part.o + x * D + d) * (f * kPower<-kJoinDown>);
     }
     T4 y;
-    for (int e = 0; e < 4; ++e) y[e] = static_cast<T>(sum == 0.0f ? 0.0f : o[e] / sum);
+    for (int e = 0; e < 4; ++e) y[e] = static_cast<T>(sum == 0.0f ? 0.0f : o[e] / (sum * kPower<-kPartDown - kJoinDown>));
     *reinterpret_cast<T4*>(reinterpret_cast<T*>(a.out) + c * a.o_copy + i * a.o_row + (h * a.group + g) * a.o_head + d) = y;
     if (d == 0) {
         if (a.lse)

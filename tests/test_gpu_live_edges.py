@@ -188,3 +188,48 @@ def test_int_lengths_are_the_launch_s_size(ctx, n):
         d = torch.full((2,), length, dtype=torch.int32, device="cuda")
         want = cache.attend(0, q, d, weights=w2, max_len=min(max(length, 1), 5000))
         assert R.same(got, want) and R.same(w, w2)
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16, F16], ids=["f32", "bf16", "f16"])
+@pytest.mark.parametrize("n", [1, 5, 40])
+@pytest.mark.parametrize("power", [20, 24, 25, 26, 27])
+def test_huge_logits(ctx, n, power, dtype):
+    """A slot ahead by 2^20 .. 2^27 (in powers of two), where 32 bits hold an
+    exponent to whole numbers and less: its value, and an lse within the logit's
+    own rounding."""
+    from provekv_amd.pool import DeviceKVCache
+    C, H, T, D = 4, 16, 200, 64
+    cache = DeviceKVCache(1, H, T, D, dtype=dtype, copies=C)
+    g = torch.Generator().manual_seed(power)
+    v = torch.randn(C, H, T, D, generator=g).to(dtype)
+    cache.buf[:, 0, 1] = v.cuda()
+    ahead = (2.0 ** (power - 13) * 0.69 * (0.5 + 0.5 * torch.rand(C, H, generator=g))).to(dtype)
+    cache.buf[:, 0, 0, :, 7, 3] = ahead.cuda()
+    q = torch.zeros(C, n, H, D, dtype=dtype)
+    q[..., 3] = 8192.0
+    lse = torch.zeros(C, H, n, device="cuda")
+    w = torch.zeros(C, H, T, device="cuda")
+    out = cache.attend(0, q.cuda(), T, scale=1.0, lse=lse, weights=w).cpu()
+    # the only weight: 2^r with r what rounding the logit's exponent to 24 bits leaves (up to 2^-4 at 2^20), the sum as
+    # well; of many rows it is rounded to the type, h at most, and the output once more: (1 + h)^2
+    want, h = v[:, :, 7].unsqueeze(1).double(), R.HALF[dtype]
+    assert ((out.double() - want).abs() <= want.abs() * ((1 + h) ** 2 - 1 if n > 16 else h) + want.abs() * 2.0 ** -20).all()
+    top = 8192.0 * ahead.double().unsqueeze(-1)
+    assert ((lse.cpu().double() - top).abs() <= 4 * top * 2.0 ** -24).all()
+    assert ((w.cpu().double()[:, :, 7] - n).abs() <= n * 2.0 ** -20).all()
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16, F16], ids=["f32", "bf16", "f16"])
+@pytest.mark.parametrize("n", [1, 9, 40, 300])
+def test_a_single_slot_gives_its_value(ctx, n, dtype):
+    """A window of 1: every weight is 2^r / 2^r with r below 2^-18 (logits under
+    2^6), which the types hold as 1; the value comes back as it was."""
+    x = torch.randn(1, 1, 2, 3, 333, 64, generator=torch.Generator().manual_seed(12))
+    cache, k, v = held("plain", dtype, x, 1)
+    q = torch.randn(1, n, 6, 64, generator=torch.Generator().manual_seed(13)).to(dtype).cuda()
+    w = torch.zeros(1, 3, 333, device="cuda")
+    out = cache.attend(0, q, 333, window=1, weights=w).cpu().double()
+    want = v[0, :, 333 - n:].permute(1, 0, 2).repeat_interleave(2, 1)
+    err = (out[0] - want).abs()
+    assert R.same(out[0], want) if dtype != F32 else (err <= want.abs() * 2.0 ** -17).all()
+    assert ((w.cpu()[0, :, 333 - n:] - 2).abs() <= 2.0 ** -17).all() and not w[0, :, :333 - n].any()
