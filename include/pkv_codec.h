@@ -515,7 +515,11 @@ int pkv_turbo_score_batch(pkv_ctx* ctx, const pkv_profile* prof, const uint8_t* 
  *     dim with one scale byte b, standing for code value * 2^(b - 127); b = 255
  *     makes the block NaN.  d_keys / d_values are the codes (byte = element /
  *     2), d_key_scales / d_value_scales the scale bytes (byte = element / 32),
- *     aligned to 16 bytes and to dim / 32, strides a multiple of dim. */
+ *     aligned to 16 bytes and to dim / 32, strides a multiple of dim.
+ *
+ * What a call writes overlaps nothing else that it is given, except where it
+ * says so (checked for out and q, for the two caches of an eviction, for its
+ * weights and lengths; the rest is the caller's). */
 typedef struct pkv_kv_view {
     void* d_keys;
     void* d_values;
@@ -625,7 +629,8 @@ int pkv_fp4_load(pkv_ctx* ctx, const pkv_rows_op* op, void* stream);
  * - recent with the largest weight are kept (equal weights: the lower slot; a
  * NaN counts as -inf).  Kept rows go to slots 0, 1, .. of `into` in their
  * order: of the same memory and strides as `cache` (in place), or of memory
- * that does not overlap it.  Slots of `into` behind them keep what they held.
+ * apart from it, each side from its first row's start to its last row's end.
+ * Slots of `into` behind them keep what they held.
  *   d_kept        int32 [copies][layers][heads][budget]: kept slots ascending,
  *                 then -1
  *   d_new_lens    int32 [copies]: min(n, budget); not d_lens

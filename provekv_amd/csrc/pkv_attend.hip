@@ -212,8 +212,8 @@ __device__ inline bool any_visible(const AttendDev& a, const Tiles& t, int j) {
 // two terms of a 16-bit type (f32 queries over 4-bit codes: three), which the
 // bytes hide.  Measured: 4 x 32,768 slots of 8 heads of 128, four query heads
 // each, bf16: 104 us, 5.0 TB/s (114 with the loads in front of their own tile's
-// work instead of the one before); 8 x 930 slots of 32 heads of 64, f32: 22 us,
-// 5.5 TB/s; the former in 4 bits: 31 us, 4.4 TB/s, where unpacking (a
+// work instead of the one before); 8 x 930 slots of 32 heads of 64, f32: 23 us,
+// 5.4 TB/s; the former in 4 bits: 29 us, 4.7 TB/s, where unpacking (a
 // conversion per two channels and a permute per four) takes about as long as
 // the bytes.  Tried and worse: offsets of whole tiles kept in registers and
 // scale bytes of neighbouring slots in one read (4 bits: 34 us, more registers
@@ -851,8 +851,8 @@ constexpr uint32_t row_tile(int ks) { return 128u / ks; }
 // are as many bf16 terms as the query, one for bf16 queries.
 // Bound at head_dim 128 by the matrix cores (a tile is 32 matrix instructions of
 // 32 cycles a wave) together with the softmax beside them (32 exponentials of
-// 16 cycles, about 180 other vector instructions).  Measured: 8,192 causal rows
-// of 32 query heads of 128, bf16: 566 us, 971 TFLOP/s, where a library's square
+// 16 cycles, about 160 other vector instructions).  Measured: 8,192 causal rows
+// of 32 query heads of 128, bf16: 555 us, 990 TFLOP/s, where a library's square
 // product of 8,192 reaches 1,216; a tile takes a workgroup 2.0 us alone on a CU
 // and 2.2 beside another, so that calls with few workgroups are bound by that
 // latency.  With tiles held in registers on their way to LDS it took 1.93 ms:
@@ -1149,9 +1149,11 @@ __device__ inline void hand_over(float (&left)[16], bool upper) {
 // from memory while the rows before are worked on; every slot belongs to one
 // wave, so sums have one order.  S^T, one multiply-add, one exponential and one
 // more multiply-add a logit: half of rows_kernel's matrix work, its softmax
-// work without maximum and rounding; bound by those vector instructions.
-// Measured: 3 x 701 rows of 24 query heads of 64, window 1,024, f16: 26 us (89
-// with rows read when they were needed, 48 with half as many shares).
+// work without maximum and rounding.  Measured: 3 x 701 rows of 24 query heads of
+// 64, window 1,024, f16: 26 us (89 with rows read when they were needed, 48 with
+// half as many shares), of which those vector instructions are about 6: bound by
+// the latency of a step (copies drained and a barrier every 64 rows, about five
+// steps a workgroup).
 //
 // With few blocks of slots their rows are cut into shares as well (splits > 1),
 // whose sums go to `shares` [split][copy][kv head][ld] for add_weights_kernel.

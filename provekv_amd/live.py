@@ -161,7 +161,10 @@ class LiveCache:
         weight, summed over the rows and the query heads of its head, is
         added.  lse: float32 [copies, query heads, rows], the rows' log of the
         sum of exponentials.  max_len: no length is above it (an int `lens`
-        says so itself); sizes the launch."""
+        says so itself); sizes the launch.
+
+        A q that carries a gradient or a tangent is refused: there is no
+        derivative."""
         import torch
         dev = self.device
         self._on_device(dev, q, weights, lse, out)
@@ -391,7 +394,8 @@ class FourBitKVCache(LiveCache):
         A row whose slot is outside the cache is not stored.  Each block of 32
         values takes the smallest power-of-two scale that keeps the largest
         within 7 steps, each value its nearest code; a block with an infinity
-        or NaN becomes NaN."""
+        or NaN becomes NaN.  Rows that carry a gradient or a tangent are
+        refused, as by `attend`."""
         lead = (self.copies, self.layers, self.heads) if layer is None else (self.copies, self.heads)
         some = keys if keys is not None else values
         if some is None:
