@@ -164,7 +164,10 @@ __device__ inline float lower_base(const AttendDev& a, float lift, float base, f
 // Of the weights with `base` when they join those of a lower one.
 __device__ inline float joined(float low, float base) { return base == low ? 1.0f : exp2f(low - base); }
 // Log of the sum of exponentials, and a row's (base, factor): weight = 2^(s * scale2 + base) * factor.  An empty row: -inf, 0.
-__device__ inline float lse_of(float base, float sum) { return sum == 0.0f ? -kInf : (log2f(sum) - base) * kLn2; }
+__device__ inline float lse_of(float base, float sum) {   // exponents by themselves: sums of one lift or another
+    if (sum == 0.0f) return -kInf;
+    return (log2f(__builtin_amdgcn_frexp_mantf(sum)) + (static_cast<float>(__builtin_amdgcn_frexp_expf(sum)) - base)) * kLn2;
+}
 __device__ inline void stats_of(float base, float sum, float* stats) {
     stats[0] = sum == 0.0f ? 0.0f : base;
     stats[1] = sum == 0.0f ? 0.0f : 1.0f / sum;
@@ -459,7 +462,9 @@ __global__ __launch_bounds__(256, 2) void decode_kernel(AttendDev a, Partial par
                         if (!(has >> 16 * g2 & 0xffff)) continue;
                         const int key = slot + 16 * u + 4 * static_cast<int>(g2) + j;
                         const bool sees = real && visible(a, pos, key);
-                        const float w = __shfl(p[u][j], static_cast<int>(16 * g2 + row));
+                        // not scaled down: that could make it 0
+                        const float w = __shfl(__builtin_amdgcn_exp2f(__builtin_fmaf(sc[u][j], a.scale2, from)),
+                                               static_cast<int>(16 * g2 + row));
                         const uint64_t at = static_cast<uint64_t>(key) * a.kv.slot;
                         const uint8_t* vr = vp + (CT == PKV_FP4 ? at / 2 : CT == PKV_F32 ? at * 4 : at * 2);
                         for (int e = 0; e < kO; ++e)
@@ -1016,7 +1021,7 @@ __global__ __launch_bounds__(256, (query_terms(CT, QT) * D >= 256 ? 1 : 2)) void
                 continue;
             }
         }
-        const float from = base == kInf ? 0.0f : base;
+        const float from = base == kInf ? 0.0f : base + (kLift<MT> - lift);   // not scaled down: that could make a weight 0
 #pragma unroll 1
         for (int t = t0; t < t1; ++t) {
             const int slot = tl.slot(t, St::kSlots);

@@ -233,3 +233,31 @@ def test_a_single_slot_gives_its_value(ctx, n, dtype):
     err = (out[0] - want).abs()
     assert R.same(out[0], want) if dtype != F32 else (err <= want.abs() * 2.0 ** -17).all()
     assert ((w.cpu()[0, :, 333 - n:] - 2).abs() <= 2.0 ** -17).all() and not w[0, :, :333 - n].any()
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16, F16], ids=["f32", "bf16", "f16"])
+@pytest.mark.parametrize("big", [False, True], ids=["", "large-values"])
+@pytest.mark.parametrize("at", [0, 150])
+@pytest.mark.parametrize("n,G", [(1, 1), (5, 2), (40, 1), (200, 1)])
+def test_infinite_value_of_a_small_weight(ctx, n, G, at, big, dtype):
+    """80 nats behind: a weight of 2^-115 still makes an infinity, and the rest
+    is the slot ahead, also where the other values' sums pass the type's end
+    (other weights: 2^-115 each, 300 of them below half a step)."""
+    from provekv_amd.pool import DeviceKVCache
+    if big and dtype == F16:
+        return
+    T, D = 300 + n, 64
+    cache = DeviceKVCache(1, 2, T, D, dtype=dtype)
+    cache.buf[:, 0, 0, :, at, 3] = 80.0
+    cache.buf[:, 0, 1] = 2.0 ** 127 if big else 3.0
+    cache.buf[:, 0, 1, :, 70, 9] = -math.inf
+    q = torch.zeros(1, n, 2 * G, D, dtype=dtype)
+    q[..., 3] = 1.0
+    if big:      # more slots as far ahead, so that their values' sum is past the end
+        cache.buf[:, 0, 0, :, at:at + 20, 3] = 80.0
+    out = cache.attend(0, q.cuda(), T, scale=1.0).cpu().double()
+    want = torch.full_like(out, 2.0 ** 127 if big else 3.0)
+    want[..., 9] = -math.inf
+    fin = torch.isfinite(want)
+    assert R.same(out.isneginf(), want.isneginf())
+    assert ((out - want).abs()[fin] <= want.abs()[fin] * (R.HALF[dtype] + 2.0 ** -18)).all()
