@@ -135,7 +135,8 @@ class LiveCache:
             return
         if t.requires_grad and torch.is_grad_enabled():
             raise ValueError(f"{call} has no backward pass: detach its tensors or call it under torch.no_grad()")
-        if torch.autograd.forward_ad.unpack_dual(t).tangent is not None:
+        fwd = torch.autograd.forward_ad     # outside of any level nothing has a tangent
+        if getattr(fwd, "_current_level", 0) >= 0 and fwd.unpack_dual(t).tangent is not None:
             raise ValueError(f"{call} has no forward-mode derivative: give it the primal of a dual tensor")
 
     @staticmethod
