@@ -27,7 +27,7 @@ struct AttendDev {
     float* lse;
     float* weights;
     uint64_t w_copy, w_head;
-    float* stats;          // (base, factor) of [copy][kv head][row i * group + g]: weight = 2^(s * scale2 + base) * factor
+    float* stats;          // [copy][kv head][row i * group + g] (base, factor): weight 2^(s * scale2 + base) * factor
     uint32_t copies, heads, group, nq, max_len, window, sinks;
     uint32_t reach;        // window, 2^31 at most and where there is none: a row sees slots less than this behind it
     float scale2;          // scale * log2 e

@@ -163,10 +163,12 @@ __device__ inline float lower_base(const AttendDev& a, float lift, float base, f
 }
 // Of the weights with `base` when they join those of a lower one.
 __device__ inline float joined(float low, float base) { return base == low ? 1.0f : exp2f(low - base); }
-// Log of the sum of exponentials, and a row's (base, factor): weight = 2^(s * scale2 + base) * factor.  An empty row: -inf, 0.
+// Log of the sum of exponentials, and a row's (base, factor): weight = 2^(s *
+// scale2 + base) * factor.  An empty row: -inf, 0.
 __device__ inline float lse_of(float base, float sum) {   // exponents by themselves: sums of one lift or another
     if (sum == 0.0f) return -kInf;
-    return (log2f(__builtin_amdgcn_frexp_mantf(sum)) + (static_cast<float>(__builtin_amdgcn_frexp_expf(sum)) - base)) * kLn2;
+    const float e = static_cast<float>(__builtin_amdgcn_frexp_expf(sum));
+    return (log2f(__builtin_amdgcn_frexp_mantf(sum)) + (e - base)) * kLn2;
 }
 __device__ inline void stats_of(float base, float sum, float* stats) {
     stats[0] = sum == 0.0f ? 0.0f : base;
@@ -302,7 +304,7 @@ struct SlotTile {
             }
         return odd;
     }
-    // The value that output register (e, r) of lane group g meets, of the row whose bytes are at `p` (scale bytes `sp`).
+    // The value that output register (e, r) of lane group g meets, of the row whose bytes are at `p` (scales `sp`).
     __device__ static float value(const uint8_t* p, const uint8_t* sp, int e, int r, uint32_t g) {
         const uint32_t d = out_channel(e, r, g);
         if constexpr (CT == PKV_F32) return reinterpret_cast<const float*>(p)[d];
@@ -504,7 +506,8 @@ __global__ __launch_bounds__(256, 2) void decode_kernel(AttendDev a, Partial par
             }
             bool past = false;   // back, unless it does not fit
             for (int e = 0; e < kO; ++e)
-                for (int r = 0; r < 4; ++r) past |= fabsf(o[e][r]) < kInf && !(fabsf(o[e][r]) * kPower<kDown<MT>> < kInf);
+                for (int r = 0; r < 4; ++r)
+                    past |= fabsf(o[e][r]) < kInf && !(fabsf(o[e][r]) * kPower<kDown<MT>> < kInf);
             if (__any(past && real)) {
                 base -= kDown<MT>;
             } else {
@@ -578,7 +581,8 @@ __global__ __launch_bounds__(256) void join_kernel(AttendDev a, Partial part, ui
         f32x4 o = {};
         for (uint32_t s = first; s < part.splits; s += kShares) {
             const uint64_t x = at + static_cast<uint64_t>(part.rows) * s;
-            o += *reinterpret_cast<const f32x4*>(part.o + x * D + d) * (joined(base, part.ml[2 * x]) * kPower<-kJoinDown>);
+            const float f = joined(base, part.ml[2 * x]) * kPower<-kJoinDown>;
+            o += *reinterpret_cast<const f32x4*>(part.o + x * D + d) * f;
         }
         __shared__ f32x4 so[256];
         so[threadIdx.x] = o;
@@ -588,7 +592,8 @@ __global__ __launch_bounds__(256) void join_kernel(AttendDev a, Partial part, ui
             T* out = reinterpret_cast<T*>(a.out) + c * a.o_copy + i * a.o_row + (h * a.group + g) * a.o_head;
             typedef T T4 __attribute__((ext_vector_type(4)));
             T4 y;
-            for (int e = 0; e < 4; ++e) y[e] = static_cast<T>(sum == 0.0f ? 0.0f : o[e] / (sum * kPower<-kPartDown - kJoinDown>));
+            const float div = sum * kPower<-kPartDown - kJoinDown>;
+            for (int e = 0; e < 4; ++e) y[e] = static_cast<T>(sum == 0.0f ? 0.0f : o[e] / div);
             *reinterpret_cast<T4*>(out + d) = y;
         }
         if (threadIdx.x == 0) {
@@ -607,8 +612,8 @@ __global__ __launch_bounds__(256) void join_kernel(AttendDev a, Partial part, ui
     __shared__ float st[16][2];
     for (int r = wave; r < rows; r += 4) {
         float base, sum;
-        join_splits(part.ml + 2 * (static_cast<uint64_t>(ch) * part.splits * part.rows + r), part.splits, part.rows, lane,
-                    &base, &sum);
+        join_splits(part.ml + 2 * (static_cast<uint64_t>(ch) * part.splits * part.rows + r), part.splits, part.rows,
+                    lane, &base, &sum);
         if (lane == 0) stats_of(base, sum, st[r]);
     }
     __syncthreads();
@@ -1021,7 +1026,8 @@ __global__ __launch_bounds__(256, (query_terms(CT, QT) * D >= 256 ? 1 : 2)) void
                 continue;
             }
         }
-        const float from = base == kInf ? 0.0f : base + (kLift<MT> - lift);   // not scaled down: that could make a weight 0
+        // not scaled down: that could make a weight 0
+        const float from = base == kInf ? 0.0f : base + (kLift<MT> - lift);
 #pragma unroll 1
         for (int t = t0; t < t1; ++t) {
             const int slot = tl.slot(t, St::kSlots);
@@ -1070,7 +1076,8 @@ __global__ __launch_bounds__(256, (query_terms(CT, QT) * D >= 256 ? 1 : 2)) void
         __syncthreads();
         if (share) return;
         const float base2 = to[16 * kO * 64], low = fminf(base, base2);
-        const float f = joined(low, base), f2 = joined(low, base2), of = f * kPower<-kShared>, of2 = f2 * kPower<-kShared>;
+        const float f = joined(low, base), f2 = joined(low, base2);
+        const float of = f * kPower<-kShared>, of2 = f2 * kPower<-kShared>;
         base = low;
         l = l * f + to[(16 * kO + 1) * 64] * f2;
         for (int x = 0; x < 16 * kO; ++x) o[x / 16][x % 16] = o[x / 16][x % 16] * of + to[x * 64] * of2;
@@ -1120,7 +1127,8 @@ __global__ __launch_bounds__(256) void join_rows_kernel(AttendDev a, Partial par
     if (static_cast<int>(i) >= span(a, c).rows || r >= all) return;
     const uint64_t at = static_cast<uint64_t>(ch) * part.splits * part.rows + r;
     float base = kInf, sum = 0.0f;
-    for (uint32_t s = 0; s < part.splits; ++s) base = fminf(base, part.ml[2 * (at + static_cast<uint64_t>(part.rows) * s)]);
+    for (uint32_t s = 0; s < part.splits; ++s)
+        base = fminf(base, part.ml[2 * (at + static_cast<uint64_t>(part.rows) * s)]);
     f32x4 o = {};
     for (uint32_t s = 0; s < part.splits; ++s) {
         const uint64_t x = at + static_cast<uint64_t>(part.rows) * s;
@@ -1129,7 +1137,8 @@ __global__ __launch_bounds__(256) void join_rows_kernel(AttendDev a, Partial par
         o += *reinterpret_cast<const f32x4*>(part.o + x * D + d) * (f * kPower<-kJoinDown>);
     }
     T4 y;
-    for (int e = 0; e < 4; ++e) y[e] = static_cast<T>(sum == 0.0f ? 0.0f : o[e] / (sum * kPower<-kPartDown - kJoinDown>));
+    const float div = sum * kPower<-kPartDown - kJoinDown>;
+    for (int e = 0; e < 4; ++e) y[e] = static_cast<T>(sum == 0.0f ? 0.0f : o[e] / div);
     *reinterpret_cast<T4*>(reinterpret_cast<T*>(a.out) + c * a.o_copy + i * a.o_row + (h * a.group + g) * a.o_head + d) = y;
     if (d == 0) {
         if (a.lse)
@@ -1890,10 +1899,9 @@ static uint64_t move_blocks(const EvictDev& e, uint32_t dim, int dtype) {
 
 template <int DT, int D>
 static int move_typed(const EvictDev& e, hipStream_t st) {
-    const uint64_t blocks = move_blocks<DT>(e, D);
-    const uint32_t grid = static_cast<uint32_t>(blocks);
+    const uint32_t grid = static_cast<uint32_t>(move_blocks<DT>(e, D));
     if (e.in_place) move_kernel<DT, D, true><<<grid, 256, 0, st>>>(e, 0);
-    else move_kernel<DT, D, false><<<grid, 256, 0, st>>>(e, static_cast<uint32_t>(blocks / (2ull * e.copies * e.layers * e.heads)));
+    else move_kernel<DT, D, false><<<grid, 256, 0, st>>>(e, grid / (2 * e.copies * e.layers * e.heads));
     return hipGetLastError();
 }
 

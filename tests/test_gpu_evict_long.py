@@ -30,8 +30,9 @@ def test_filled_length(ctx):
     (70001, 5000, 0, 0, True), (70001, 40000, 7, 20000, False), (70001, 69999, 2, 1, True)])
 def test_long(ctx, T, budget, sinks, recent, coarse, in_place, kind):
     """One copy past the registers, one within them, in one launch."""
-    check(make(kind, 2, 1, 2, T, 64, seed=T), weights(2, 1, 2, T, budget, coarse), [T, min(T, 32768) - 5], budget, sinks,
-          recent, in_place, extra=3)
+    lens = [T, min(T, 32768) - 5]
+    check(make(kind, 2, 1, 2, T, 64, seed=T), weights(2, 1, 2, T, budget, coarse), lens, budget, sinks, recent, in_place,
+          extra=3)
 
 
 @pytest.mark.parametrize("in_place", [True, False], ids=["in-place", "into"])

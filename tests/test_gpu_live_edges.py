@@ -33,13 +33,13 @@ def test_millions_of_rows(ctx, copies, G, n):
     from provekv_amd.pool import DeviceKVCache
     T, D, window = n, 64, 40
     assert copies * G * n >= 1 << 24
-    x = torch.randn(1, 1, 2, 1, T, D, generator=torch.Generator().manual_seed(1)).to(BF16).expand(copies, -1, -1, -1, -1, -1)
-    cache = DeviceKVCache.over(x.contiguous().cuda())
+    x = torch.randn(1, 1, 2, 1, T, D, generator=torch.Generator().manual_seed(1)).to(BF16)
+    cache = DeviceKVCache.over(x.cuda().repeat(copies, 1, 1, 1, 1, 1))
     q = torch.randn(1, n, 1, D, generator=torch.Generator().manual_seed(2)).to(BF16)
     w = torch.zeros(copies, 1, T, device="cuda")
-    out = cache.attend(0, q.cuda().expand(copies, -1, G, -1), torch.full((copies,), T, dtype=torch.int32, device="cuda"),
-                       window=window, weights=w)
-    x = x[:1].double()
+    lens = torch.full((copies,), T, dtype=torch.int32, device="cuda")
+    out = cache.attend(0, q.cuda().expand(copies, -1, G, -1), lens, window=window, weights=w)
+    x = x.double()
     for i in (0, 1, 127, 128, n // 2, n - 1):
         ref = R.attend(q[:, i:i + 1].double(), x[:, 0, 0], x[:, 0, 1], [i + 1], [1], window, 0, 0.125)
         for c, g in ((0, 0), (copies - 1, G - 1), (copies // 2, 1)):
@@ -213,7 +213,8 @@ def test_huge_logits(ctx, n, power, dtype):
     # the only weight: 2^r with r what rounding the logit's exponent to 24 bits leaves (up to 2^-4 at 2^20), the sum as
     # well; of many rows it is rounded to the type, h at most, and the output once more: (1 + h)^2
     want, h = v[:, :, 7].unsqueeze(1).double(), R.HALF[dtype]
-    assert ((out.double() - want).abs() <= want.abs() * ((1 + h) ** 2 - 1 if n > 16 else h) + want.abs() * 2.0 ** -20).all()
+    rel = ((1 + h) ** 2 - 1 if n > 16 else h) + 2.0 ** -20
+    assert ((out.double() - want).abs() <= want.abs() * rel).all()
     top = 8192.0 * ahead.double().unsqueeze(-1)
     assert ((lse.cpu().double() - top).abs() <= 4 * top * 2.0 ** -24).all()
     assert ((w.cpu().double()[:, :, 7] - n).abs() <= n * 2.0 ** -20).all()

@@ -31,7 +31,8 @@ class Strided:
         else:
             self.parts = [torch.full((*shape, unit), float(fill), dtype=kind, device="cuda")]
             widths = (D,)
-        self.rows = [[p[:, :, :HEADS, side, -w:].permute(0, 2, 1, 3) for p, w in zip(self.parts, widths)] for side in (0, 1)]
+        self.rows = [[p[:, :, :HEADS, side, -w:].permute(0, 2, 1, 3) for p, w in zip(self.parts, widths)]
+                     for side in (0, 1)]
         slot = (HEADS + 1) * 2 * unit
         ptr = [[r.data_ptr() for r in side] for side in self.rows]
         elems = COPIES * T * slot - unit - gap
@@ -135,8 +136,8 @@ def test_evict(ctx, in_place, D, kind):
     kept2, new2 = torch.zeros_like(kept), torch.zeros_like(new)
     slots = T if in_place else budget + 2
     out = w2 if in_place else torch.zeros(COPIES, 1, HEADS, slots, device="cuda")
-    op = L.EvictOp(other.view, target.view, lens.data_ptr(), new2.data_ptr(), kept2.data_ptr(), w2.data_ptr(), out.data_ptr(),
-                   (C.c_uint64 * 3)(HEADS * T, 0, T), (C.c_uint64 * 3)(HEADS * slots, 0, slots), budget, 2, 9, 0)
+    op = L.EvictOp(other.view, target.view, lens.data_ptr(), new2.data_ptr(), kept2.data_ptr(), w2.data_ptr(),
+                   out.data_ptr(), (C.c_uint64 * 3)(HEADS * T, 0, T), (C.c_uint64 * 3)(HEADS * slots, 0, slots), budget, 2, 9, 0)
     assert L.lib().pkv_evict(ctx.ptr, C.byref(op), stream()) == 0
     assert torch.equal(kept2, kept) and torch.equal(new2, new) and torch.equal(out[..., :budget], packed[..., :budget])
     assert not out[..., budget:].any()

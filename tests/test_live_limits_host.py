@@ -57,7 +57,8 @@ def child_attend(lib, L, ctx, launches):
     # up to 16 rows of a head: a workgroup a row joins its shares
     most = (1 << 24) - 1
     assert call(1, most, most, 1, 64, False) and not call(1, most + 1, most + 1, 1, 64, False)
-    assert call(1, most // 4, most // 4 * 4, 1, 64, False) and not call(1, most // 4 + 1, most // 4 * 4 + 4, 1, 64, False)
+    quarter = most // 4
+    assert call(1, quarter, quarter * 4, 1, 64, False) and not call(1, quarter + 1, quarter * 4 + 4, 1, 64, False)
     # .. and 1,024 slots a workgroup with weights
     assert call(1, most // 2, most // 2, 1, 1024, True) and not call(1, most // 2 + 1, most // 2 + 1, 1, 1024, True)
     assert call(1, most // 5, most // 5, 1, 4000, True) and not call(1, most // 5 + 1, most // 5 + 1, 1, 4000, True)
