@@ -75,7 +75,13 @@ int pkv_device_available(void);
 enum pkv_codec_kind { PKV_CODEC_TURBO = 1, PKV_CODEC_FIB = 2 };
 enum pkv_turbo_mode { PKV_TURBO_POLAR_ONLY = 0, PKV_TURBO_POLAR_WITH_QJL = 1 };
 enum pkv_radii_codec { PKV_RADII_F32 = 0, PKV_RADII_LOG_U8 = 1 };
-enum pkv_dtype { PKV_F32 = 0, PKV_BF16 = 1, PKV_F16 = 2, PKV_FP4 = 3 /* cache views (pkv_kv_view) only */ };
+enum pkv_dtype {
+    PKV_F32 = 0,
+    PKV_BF16 = 1,
+    PKV_F16 = 2,
+    PKV_FP4 = 3, /* cache views (pkv_kv_view) only */
+    PKV_FP8 = 4  /* page views (pkv_page_view) only */
+};
 
 /* Replaces TurboQuantizer::new_with_mode (turbo-quant/src/turbo.rs:124-188)
  * as built by TurboQuantAdapter (proveKV/src/codec.rs:249-250): FastHadamard
