@@ -665,6 +665,153 @@ typedef struct pkv_evict_op {
 } pkv_evict_op;
 int pkv_evict(pkv_ctx* ctx, const pkv_evict_op* op, void* stream);
 
+/* ---------------------------------------------------------------- paged caches, packed rows
+ * A KV cache in pages that a table names, so that sequences of any lengths share
+ * a memory, and agents the pages of a common prefix; its rows stored (16 bits,
+ * or 8 with a scale per 32 values) and loaded; attention of packed rows over it;
+ * and attention of whole packed prompts on their own rows.  No counterpart in
+ * the reference.
+ *
+ * Pages: keys and values of `layers` x `pages` x `heads`, each page_slots rows (a
+ * power of two, 16 .. 65,536) of dim (64 or 128) elements.  Row j of (layer l,
+ * page p, head h) starts at element l * layer_stride + p * page_stride + h *
+ * head_stride + j * slot_stride of d_keys and of d_values; elems bounds every
+ * such row's end (checked).  slot_stride is at most 2^22.
+ *   PKV_BF16, PKV_F16: pointers 16-byte aligned, strides a multiple of 16 bytes;
+ *     scale pointers NULL.
+ *   PKV_FP8: OCP MX FP8, a byte a value: e4m3 codes (no infinity; 0x7f and 0xff
+ *     are NaN), blocks of 32 along dim with one scale byte b, standing for code
+ *     value * 2^(b - 127); b = 255 makes the block NaN.  d_keys / d_values are
+ *     the codes, d_key_scales / d_value_scales the scale bytes (byte = element /
+ *     32); all 16-byte aligned, strides a multiple of 16 * dim except
+ *     slot_stride, which is dim. */
+typedef struct pkv_page_view {
+    void* d_keys;
+    void* d_values;
+    uint8_t* d_key_scales;
+    uint8_t* d_value_scales;
+    uint64_t layer_stride, page_stride, head_stride, slot_stride;
+    uint64_t elems;
+    uint32_t layers, pages, heads, page_slots, dim;
+    int32_t dtype;
+} pkv_page_view;
+
+/* Packed rows of `seqs` sequences and the pages they live in.  Sequence s has the
+ * rows starts[s] .. starts[s + 1] - 1 of the packed tensors; with n of them, row
+ * i is its slot len(s) - n + i: the lengths count the rows' own slots.  Slot j is
+ * place j % page_slots of page tables[s][j / page_slots].
+ *   d_tables  (s, e) at s * table_stride + e, int32 device words, table_pages of
+ *             them a sequence.  A word outside 0 .. pages - 1 names no page: its
+ *             slots are not stored to, loaded as 0 and seen by no row
+ *   d_lens    [seqs] int32 device words, taken into 0 .. table_pages * page_slots
+ *             (and max_len)
+ *   d_starts  [seqs + 1] int32 device words, ascending, or NULL: rows / seqs rows
+ *             each (rows is a multiple of seqs)
+ * All are read on the device.  Starts are taken into 0 .. rows; rows before the
+ * first and behind the last sequence are nobody's.  Starts that do not ascend
+ * give no access out of bounds, but which sequence's a row is, is not said. */
+typedef struct pkv_sequences {
+    const int32_t* d_tables;
+    uint64_t table_stride;
+    const int32_t* d_lens;
+    const int32_t* d_starts;
+    uint32_t seqs, table_pages, rows;
+    uint32_t reserved;        /* 0 */
+} pkv_sequences;
+
+/* Rows into and out of pages.  Element (l, r, h, 0) of keys and values at l *
+ * layer_stride + r * row_stride + h * head_stride of a dtype tensor (PKV_F32,
+ * PKV_BF16 or PKV_F16; 16-byte aligned, strides a multiple of 16 bytes).  d_keys
+ * or d_values may be NULL (that side is left alone).
+ *   store: rounded to the pages' type, to nearest even.  PKV_FP8: each block of
+ *     32 takes the smallest scale 2^e with max |x| <= 448 * 2^e, e in -116 ..
+ *     119 (2^-116 so that half the smallest step is a normal number; 2^119 so
+ *     that 448 steps are finite: f32 values past 448 * 2^119 go to it), each
+ *     value the nearest code, half way to the even one; a block that holds an
+ *     infinity or NaN becomes NaN.  A row whose slot is negative, or has no page,
+ *     is not stored.  Two rows must not name the same place of the same page.
+ *   load: the values the pages hold, rounded to dtype (exact in f32, and in bf16
+ *     from PKV_FP8).  A row without a slot or a page, or nobody's, is 0.
+ * layers * ceil(rows / 16) is below 2^24.  Asynchronous on `stream`; the
+ * calls can be captured. */
+typedef struct pkv_paged_rows_op {
+    pkv_page_view pages;
+    pkv_sequences seqs;
+    void* d_keys;             /* read by a store, written by a load */
+    void* d_values;
+    uint64_t layer_stride, row_stride, head_stride;
+    int32_t dtype;
+    uint32_t reserved;        /* 0 */
+} pkv_paged_rows_op;
+int pkv_paged_store(pkv_ctx* ctx, const pkv_paged_rows_op* op, void* stream);
+int pkv_paged_load(pkv_ctx* ctx, const pkv_paged_rows_op* op, void* stream);
+
+/* Attention of packed query rows over one layer's pages (layers == 1): single
+ * tokens, chunks of prompts, or both in one call.  A row at slot p sees slot j as
+ * pkv_attend's: 0 <= j <= p and (window == 0 or p - j < window or j < sinks);
+ * softmax, a row that sees nothing, grouped heads and what hidden slots may hold
+ * as there.
+ *   q, out   element (r, g, 0) at r * row_stride + g * head_stride, of dtype: the
+ *            pages', or for PKV_FP8 PKV_BF16 or PKV_F16; 16-byte aligned, strides
+ *            a multiple of 16 bytes.  Rows that are nobody's are left as they
+ *            were in out, or with clear = 1 become 0
+ *   d_lse    NULL, or f32 [q_heads][rows]: natural log of the sum of exp(s_j)
+ *            (nobody's rows left as they were)
+ *   max_rows no sequence has more rows (0: rows); rows past it are not computed
+ *   max_len  no len(s) is above it (0: table_pages * page_slots).  Both size the
+ *            launch, so tight ones are faster, and a captured graph wants the
+ *            largest its replays use
+ *   d_workspace  pkv_paged_attend_workspace(op) bytes, 256-byte aligned, used
+ *            until the call's work on `stream` is done; calls that may run at the
+ *            same time need one each (a captured graph holds on to its own)
+ * Logits, the softmax's sums and outputs' sums are held in 32 bits.  Weights meet
+ * the values as two terms of a 16-bit type for sequences with up to 16 rows (rows
+ * x query heads of a KV head), and of f16 queries over PKV_FP8; else as one, as
+ * pkv_attend's of many rows.  rows * q_heads is at most 2^30, and every launch
+ * stays below 2^24 workgroups (else PKV_ERR_INVALID_ARG).  Asynchronous on
+ * `stream`; the call can be captured. */
+typedef struct pkv_paged_attend_op {
+    pkv_page_view pages;
+    pkv_sequences seqs;
+    const void* d_q;
+    void* d_out;
+    uint64_t q_row_stride, q_head_stride, out_row_stride, out_head_stride;
+    float* d_lse;
+    void* d_workspace;
+    uint64_t workspace_bytes;
+    float scale;              /* > 0, finite */
+    int32_t dtype;            /* of q and out */
+    uint32_t q_heads, max_rows, max_len, window, sinks;
+    uint32_t clear;           /* 0 or 1 */
+} pkv_paged_attend_op;
+/* Workspace bytes of a call with these shapes (of the pointers only whether
+ * d_starts is NULL counts); 0 for shapes pkv_paged_attend refuses. */
+uint64_t pkv_paged_attend_workspace(const pkv_paged_attend_op* op);
+int pkv_paged_attend(pkv_ctx* ctx, const pkv_paged_attend_op* op, void* stream);
+
+/* Attention of whole prompts on their own packed rows: row i of a sequence sees
+ * that sequence's rows j <= i (and window, sinks as above).  q and out as above,
+ * k and v (r, h, 0) at r * row_stride + h * head_stride; all of one dtype,
+ * PKV_BF16 or PKV_F16.  d_starts as pkv_sequences', not NULL. */
+typedef struct pkv_prompts_op {
+    const void* d_q;
+    const void* d_k;
+    const void* d_v;
+    void* d_out;
+    uint64_t q_row_stride, q_head_stride, k_row_stride, k_head_stride;
+    uint64_t v_row_stride, v_head_stride, out_row_stride, out_head_stride;
+    const int32_t* d_starts;
+    float* d_lse;
+    void* d_workspace;
+    uint64_t workspace_bytes;
+    float scale;              /* > 0, finite */
+    int32_t dtype;
+    uint32_t seqs, rows, heads, q_heads, dim, max_rows, window, sinks;
+    uint32_t clear;           /* 0 or 1 */
+} pkv_prompts_op;
+uint64_t pkv_prompts_workspace(const pkv_prompts_op* op);
+int pkv_prompts(pkv_ctx* ctx, const pkv_prompts_op* op, void* stream);
+
 /* ---------------------------------------------------------------- diagnostics
  * Validation hook, no counterpart in the reference: the encode kernels take
  * their fast decisions from matrix-core approximations and keep them only

@@ -9,7 +9,9 @@ Layers (bottom up):
     FibQuantAdapter with encode_batch_compact / decode_batch_compact);
   * ``pool``: the batched two-tier pool + shell build and rehydrate;
   * ``live``: attention over a rehydrated cache, the cache held in 4 bits, and
-    eviction by accumulated attention weight.
+    eviction by accumulated attention weight;
+  * ``paged``: a cache in pages that a table names (16 or 8 bits), attention of
+    packed rows over it, and attention of whole packed prompts.
 """
 from ._lib import PkvError  # noqa: F401
 

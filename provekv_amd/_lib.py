@@ -39,6 +39,7 @@ DT_F32 = 0
 DT_BF16 = 1
 DT_F16 = 2
 DT_FP4 = 3
+DT_FP8 = 4
 
 # every symbol include/pkv_codec.h declares
 EXPORTS = (
@@ -58,6 +59,8 @@ EXPORTS = (
     "pkv_host_angle_bins", "pkv_host_octant_bins", "pkv_host_logf", "pkv_host_expf", "pkv_host_expf_fused",
     "pkv_host_div255", "pkv_host_f32_stable_rel50", "pkv_code_from_json", "pkv_fib_digests", "pkv_host_blake3",
     "pkv_attend_workspace", "pkv_attend", "pkv_fp4_store", "pkv_fp4_load", "pkv_evict",
+    "pkv_paged_store", "pkv_paged_load", "pkv_paged_attend_workspace", "pkv_paged_attend", "pkv_prompts_workspace",
+    "pkv_prompts",
 )
 
 
@@ -114,6 +117,51 @@ class EvictOp(C.Structure):
                 ("d_kept", C.c_void_p), ("d_weights", C.c_void_p), ("d_weights_out", C.c_void_p),
                 ("weight_strides", C.c_uint64 * 3), ("out_strides", C.c_uint64 * 3), ("budget", C.c_uint32),
                 ("sinks", C.c_uint32), ("recent", C.c_uint32), ("reserved", C.c_uint32)]
+
+
+class PageView(C.Structure):
+    """pkv_page_view"""
+    _fields_ = [("d_keys", C.c_void_p), ("d_values", C.c_void_p), ("d_key_scales", C.c_void_p),
+                ("d_value_scales", C.c_void_p), ("layer_stride", C.c_uint64), ("page_stride", C.c_uint64),
+                ("head_stride", C.c_uint64), ("slot_stride", C.c_uint64), ("elems", C.c_uint64),
+                ("layers", C.c_uint32), ("pages", C.c_uint32), ("heads", C.c_uint32), ("page_slots", C.c_uint32),
+                ("dim", C.c_uint32), ("dtype", C.c_int32)]
+
+
+class Sequences(C.Structure):
+    """pkv_sequences"""
+    _fields_ = [("d_tables", C.c_void_p), ("table_stride", C.c_uint64), ("d_lens", C.c_void_p),
+                ("d_starts", C.c_void_p), ("seqs", C.c_uint32), ("table_pages", C.c_uint32), ("rows", C.c_uint32),
+                ("reserved", C.c_uint32)]
+
+
+class PagedRowsOp(C.Structure):
+    """pkv_paged_rows_op"""
+    _fields_ = [("pages", PageView), ("seqs", Sequences), ("d_keys", C.c_void_p), ("d_values", C.c_void_p),
+                ("layer_stride", C.c_uint64), ("row_stride", C.c_uint64), ("head_stride", C.c_uint64),
+                ("dtype", C.c_int32), ("reserved", C.c_uint32)]
+
+
+class PagedAttendOp(C.Structure):
+    """pkv_paged_attend_op"""
+    _fields_ = [("pages", PageView), ("seqs", Sequences), ("d_q", C.c_void_p), ("d_out", C.c_void_p),
+                ("q_row_stride", C.c_uint64), ("q_head_stride", C.c_uint64), ("out_row_stride", C.c_uint64),
+                ("out_head_stride", C.c_uint64), ("d_lse", C.c_void_p), ("d_workspace", C.c_void_p),
+                ("workspace_bytes", C.c_uint64), ("scale", C.c_float), ("dtype", C.c_int32), ("q_heads", C.c_uint32),
+                ("max_rows", C.c_uint32), ("max_len", C.c_uint32), ("window", C.c_uint32), ("sinks", C.c_uint32),
+                ("clear", C.c_uint32)]
+
+
+class PromptsOp(C.Structure):
+    """pkv_prompts_op"""
+    _fields_ = [("d_q", C.c_void_p), ("d_k", C.c_void_p), ("d_v", C.c_void_p), ("d_out", C.c_void_p),
+                ("q_row_stride", C.c_uint64), ("q_head_stride", C.c_uint64), ("k_row_stride", C.c_uint64),
+                ("k_head_stride", C.c_uint64), ("v_row_stride", C.c_uint64), ("v_head_stride", C.c_uint64),
+                ("out_row_stride", C.c_uint64), ("out_head_stride", C.c_uint64), ("d_starts", C.c_void_p),
+                ("d_lse", C.c_void_p), ("d_workspace", C.c_void_p), ("workspace_bytes", C.c_uint64),
+                ("scale", C.c_float), ("dtype", C.c_int32), ("seqs", C.c_uint32), ("rows", C.c_uint32),
+                ("heads", C.c_uint32), ("q_heads", C.c_uint32), ("dim", C.c_uint32), ("max_rows", C.c_uint32),
+                ("window", C.c_uint32), ("sinks", C.c_uint32), ("clear", C.c_uint32)]
 
 
 class Seg(C.Structure):
@@ -252,6 +300,12 @@ def _declare(L):
         "pkv_fp4_store": ([P, P, P], I32),
         "pkv_fp4_load": ([P, P, P], I32),
         "pkv_evict": ([P, P, P], I32),
+        "pkv_paged_store": ([P, P, P], I32),
+        "pkv_paged_load": ([P, P, P], I32),
+        "pkv_paged_attend_workspace": ([P], U64),
+        "pkv_paged_attend": ([P, P, P], I32),
+        "pkv_prompts_workspace": ([P], U64),
+        "pkv_prompts": ([P, P, P], I32),
     }
     for name, (args, res) in sig.items():
         fn = getattr(L, name)

@@ -53,25 +53,24 @@ def _like(t):
 _NO_GUARD = contextlib.nullcontext()
 
 
-class LiveCache:
-    """What a cache of [copies][layers][K|V][heads][tokens][dim] rows does on
-    the device.  A subclass has copies, layers, heads, tokens, dim, device and
-    _pointers(): (dtype, bytes of an element or None for 4-bit codes, keys,
-    values, key scales, value scales, elements of the whole memory)."""
+class DeviceCalls:
+    """The frame of a call of the library: its device and stream, its kept
+    struct, and what every call refuses.  _what: whose device it is."""
 
-    # ------------------------------------------------------------ the call's frame
+    _what = "the cache"
+
     def _frame(self, dev, stream):
         """(context, stream handle, guard): the guard makes the cache's device
         and the stream current, so that what a call allocates belongs to it."""
         import torch
         if dev.type != "cuda":
-            raise ValueError("the cache is not on a GPU")
+            raise ValueError(f"{self._what} is not on a GPU")
         index, now = dev.index, torch.cuda.current_device()
         if index is None:
             index = now
         if stream is not None:
             if stream.device_index != index:
-                raise ValueError("the stream belongs to another device than the cache")
+                raise ValueError(f"the stream belongs to another device than {self._what}")
             return device_context(index), stream.cuda_stream, torch.cuda.stream(stream)
         raw = getattr(torch._C, "_cuda_getCurrentRawStream", None)   # a Stream object costs as much as a launch
         handle = raw(index) if raw is not None else torch.cuda.current_stream(index).cuda_stream
@@ -90,6 +89,30 @@ class LiveCache:
             plans[key] = got
         op, extra = got
         return type(op).from_buffer_copy(op), extra
+
+    @staticmethod
+    def _served(t, call: str):
+        """No gradient or tangent of t is lost without a word."""
+        import torch
+        if t is None:
+            return
+        if t.requires_grad and torch.is_grad_enabled():
+            raise ValueError(f"{call} has no backward pass: detach its tensors or call it under torch.no_grad()")
+        fwd = torch.autograd.forward_ad     # outside of any level nothing has a tangent
+        if getattr(fwd, "_current_level", 0) >= 0 and fwd.unpack_dual(t).tangent is not None:
+            raise ValueError(f"{call} has no forward-mode derivative: give it the primal of a dual tensor")
+
+    def _on_device(self, dev, *tensors):
+        for t in tensors:
+            if t is not None and t.device != dev:
+                raise ValueError(f"a tensor is on {t.device}, {self._what} on {dev}")
+
+
+class LiveCache(DeviceCalls):
+    """What a cache of [copies][layers][K|V][heads][tokens][dim] rows does on
+    the device.  A subclass has copies, layers, heads, tokens, dim, device and
+    _pointers(): (dtype, bytes of an element or None for 4-bit codes, keys,
+    values, key scales, value scales, elements of the whole memory)."""
 
     def _view(self, layer=None) -> "L.KvView":
         """The cache, or one layer of it."""
@@ -126,24 +149,6 @@ class LiveCache:
         if x.dtype != torch.int32 or x.shape != (self.copies,) or not x.is_contiguous() or x.device != self.device:
             raise ValueError(f"{name} must be a contiguous int32 tensor of {self.copies} on the cache's device")
         return x
-
-    @staticmethod
-    def _served(t, call: str):
-        """No gradient or tangent of t is lost without a word."""
-        import torch
-        if t is None:
-            return
-        if t.requires_grad and torch.is_grad_enabled():
-            raise ValueError(f"{call} has no backward pass: detach its tensors or call it under torch.no_grad()")
-        fwd = torch.autograd.forward_ad     # outside of any level nothing has a tangent
-        if getattr(fwd, "_current_level", 0) >= 0 and fwd.unpack_dual(t).tangent is not None:
-            raise ValueError(f"{call} has no forward-mode derivative: give it the primal of a dual tensor")
-
-    @staticmethod
-    def _on_device(dev, *tensors):
-        for t in tensors:
-            if t is not None and t.device != dev:
-                raise ValueError(f"a tensor is on {t.device}, the cache on {dev}")
 
     # ------------------------------------------------------------ attention
     def attend(self, layer: int, q, lens, q_lens=None, window: int = 0, sinks: int = 0, scale: float | None = None,

@@ -23,6 +23,7 @@ import numpy as np
 from . import _lib as L
 from .device import SEG_DTYPE
 from .live import FourBitKVCache, LiveCache, _rows_dtype  # noqa: F401
+from .paged import PagedKVCache, attend_prompts  # noqa: F401
 
 
 def read_fb2_n_blocks(payload: bytes):
