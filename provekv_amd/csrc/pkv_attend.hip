@@ -462,15 +462,9 @@ __global__ __launch_bounds__(256) void join_kernel(AttendDev a, Partial part, ui
 template <int CT, int D>
 struct Stage : Staged<CT, D> {
     using L = Staged<CT, D>;
-    using L::kRow, L::kPieces, L::kKeyBytes, L::kCopies, L::kCopyRows, L::kCopyStep, L::turn, L::key_at, L::value_at;
+    using L::kRow, L::kPieces, L::kKeyBytes, L::kCopies, L::kCopyRows, L::kCopyStep, L::turn, L::key_at, L::value_at, L::code_slot;
     u32x4 k, v;                                                 // 4-bit codes on their way
     uint32_t ks, vs;
-
-    // The slot that thread t's 4-bit codes belong to, 16 a wave: 16 lanes write 16 different places of the banks.
-    __device__ static uint32_t code_slot(uint32_t t) {
-        const uint32_t i = t % 64;
-        return t / 64 * 16 + (D == 128 ? i / 16 + i / 4 % 4 * 4 : i / 4 % 2 + i / 8 % 2 * 4 + i / 16 % 2 * 2 + i / 32 * 8);
-    }
 
     // Start a tile on its way.  kp, vp, ksp, vsp: slot 0 of the head; slots past `last` read the last one.
     __device__ void fetch(uint32_t lds, const uint8_t* kp, const uint8_t* vp, const uint8_t* ksp, const uint8_t* vsp,

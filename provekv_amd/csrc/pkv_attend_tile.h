@@ -286,6 +286,11 @@ struct Staged {
     __device__ static uint32_t value_at(uint32_t slot, uint32_t piece) {
         return kKeyBytes + slot * kRow + (piece ^ turn(slot, true)) * 16;
     }
+    // The slot that thread t's codes belong to, 16 a wave: 16 lanes write 16 different places of the banks.
+    __device__ static uint32_t code_slot(uint32_t t) {
+        const uint32_t i = t % 64;
+        return t / 64 * 16 + (D == 128 ? i / 16 + i / 4 % 4 * 4 : i / 4 % 2 + i / 8 % 2 * 4 + i / 16 % 2 * 2 + i / 32 * 8);
+    }
     // Operand of O^T += V^T P^T for channels 32 e .. and 16 slots from `slot` on: a lane's channel 32 e + lane % 32,
     // the slots of row32 in its half of them.
     __device__ static u32x4 values16(const uint8_t* lds, uint32_t slot, uint32_t e, uint32_t lane) {

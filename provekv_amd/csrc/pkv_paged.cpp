@@ -59,6 +59,7 @@ uint32_t log2_of(uint32_t x) { return 31 - __builtin_clz(x); }
 
 SeqsDev seqs_dev(const pkv_sequences& s, const pkv_page_view& v) {
     SeqsDev d{};
+    d.paged = true;
     d.tables = s.d_tables;
     d.table = s.table_stride;
     d.lens = s.d_lens;

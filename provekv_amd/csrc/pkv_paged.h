@@ -9,7 +9,8 @@ namespace pkv {
 
 // Packed rows of sequences and where their slots are (pkv_sequences).
 struct SeqsDev {
-    const int32_t* tables;   // null: packed prompts, slot j is the sequence's row j
+    bool paged;              // false: packed prompts, slot j is the sequence's row j
+    const int32_t* tables;
     uint64_t table;          // words from a sequence to the next
     const int32_t* lens;     // null: a sequence's length is its rows
     const int32_t* starts;   // null: `each` rows a sequence

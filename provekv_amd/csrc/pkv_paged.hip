@@ -220,10 +220,458 @@ __device__ void clear_rows(const PagedDev& a, uint32_t block) {
     }
 }
 
+// Four channels of an output row from their weighted sum (`down` times as large
+// as the weights' sum has it), and with the first the row's lse.
+template <int QT>
+__device__ inline void write_row(const PagedDev& a, uint32_t r, uint32_t qh, uint32_t d, f32x4 o, float base, float sum,
+                                 float down) {
+    using T = typename Elem<QT>::T;
+    typedef T T4 __attribute__((ext_vector_type(4)));
+    T4 y;
+    const float div = sum * down;
+    for (int e = 0; e < 4; ++e) y[e] = static_cast<T>(sum == 0.0f ? 0.0f : o[e] / div);
+    *reinterpret_cast<T4*>(reinterpret_cast<T*>(a.out) + static_cast<uint64_t>(r) * a.o_row + qh * a.o_head + d) = y;
+    if (d == 0 && a.lse) a.lse[static_cast<uint64_t>(qh) * a.seq.rows + r] = lse_of(base, sum);
+}
+
+// ------------------------------------------------------------ few rows: split over the slots
+constexpr int kFew = 16;            // rows x group of a KV head that decode_kernel takes
+constexpr int kStep = 32;           // slots of its tiles
+constexpr uint32_t kUnits = 1024;   // units of all heads that it aims at
+constexpr int kLeast = 4;           // tiles of a unit, one a wave
+
+__device__ inline int wave_add(int x) {
+    for (int o = 32; o; o >>= 1) x += __shfl_xor(x, o);
+    return x;
+}
+
+// The tiles that a sequence of few rows has; -1: it has no rows, or more.
+__device__ inline int few_tiles(const PagedDev& a, uint32_t s) {
+    const Seq q = seq_of(a.seq, s, a.max_rows);
+    if (!q.rows || static_cast<int64_t>(q.rows) * a.group > kFew) return -1;
+    return tiles_of(a, q.first, q.first + q.rows - 1, kStep).count;
+}
+
+// A share of a sequence's tiles, as units of about as many tiles for all
+// sequences: all their tiles by the units wanted a head, at least kLeast.  Every
+// workgroup works this out from the lengths, which only the device knows: a lane
+// takes a run of sequences, so up to 64 of them cost one read of their words.
+struct Unit {
+    int seq, share, shares, first;   // first: the sequence's first unit
+};
+__device__ inline bool find_unit(const PagedDev& a, uint32_t u, uint32_t target, uint32_t lane, Unit* o) {
+    const uint32_t per = (a.seq.seqs + 63) / 64, s0 = min(lane * per, a.seq.seqs), s1 = min(s0 + per, a.seq.seqs);
+    int mine = -1;                      // of the run's only sequence
+    float all = 0.0f;
+    for (uint32_t s = s0; s < s1; ++s) {
+        mine = few_tiles(a, s);
+        all += static_cast<float>(max(mine, 0));
+    }
+    all = wave_sum(all);
+    // above the quotient, so that there are no more than target + sequences units whatever the rounding
+    const int size = max(kLeast, static_cast<int>(all * 1.000001f / static_cast<float>(target)) + 1);
+    auto units = [&](int tiles) { return tiles < 0 ? 0 : max(1, (tiles + size - 1) / size); };
+    int n = 0;
+    if (per == 1) n = units(mine);
+    else
+        for (uint32_t s = s0; s < s1; ++s) n += units(few_tiles(a, s));
+    int end = n;
+    for (int x = 1; x < 64; x <<= 1) {
+        const int y = __shfl_up(end, x);
+        if (static_cast<int>(lane) >= x) end += y;
+    }
+    const int want = static_cast<int>(u);
+    const uint32_t at = __popcll(__ballot(end <= want));
+    if (at == 64) return false;
+    int first = __shfl(end - n, static_cast<int>(at));
+    uint32_t s = at * per;
+    for (;; ++s) {
+        n = per == 1 ? __shfl(n, static_cast<int>(at)) : units(few_tiles(a, s));
+        if (want < first + n) break;
+        first += n;
+    }
+    o->seq = __builtin_amdgcn_readfirstlane(s);
+    o->first = __builtin_amdgcn_readfirstlane(first);
+    o->shares = __builtin_amdgcn_readfirstlane(n);
+    o->share = want - o->first;
+    return true;
+}
+
+// Pages of a tile's 16-slot pieces: a lane reads one piece's word.  `last` is the
+// last slot that is read; pieces behind its own take its page.
+__device__ inline int piece_start(int slot, int piece, int last) { return min(slot + 16 * piece, last & ~15); }
+template <int PIECES>
+__device__ inline int read_pages(const SeqsDev& q, const int32_t* table, int slot, int last, uint32_t lane) {
+    return table[static_cast<uint32_t>(piece_start(slot, lane % PIECES, last)) >> q.shift];
+}
+// Bit p: piece p of them is on no page.
+template <int PIECES>
+__device__ inline uint32_t no_page(const SeqsDev& q, int words) {
+    return static_cast<uint32_t>(__ballot(static_cast<uint32_t>(words) >= q.pages)) & ((1u << PIECES) - 1);
+}
+// Elements to the piece that starts at slot `start` (on no page: page 0's, which is not used).
+__device__ inline uint64_t piece_at(const PagedDev& a, int words, int piece, int start, uint64_t head) {
+    const uint32_t p = __builtin_amdgcn_readlane(words, piece);
+    return (p < a.seq.pages ? p : 0) * a.page + head +
+           (static_cast<uint32_t>(start) & ((1u << a.seq.shift) - 1)) * a.k_slot;
+}
+
+// Eight 8-bit codes under one scale to bf16.
+__device__ inline u32x4 expand8(uint32_t lo, uint32_t hi, float s) {
+    return u32x4{__builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(lo, s, false)),
+                 __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(lo, s, true)),
+                 __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(hi, s, false)),
+                 __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(hi, s, true))};
+}
+
+// A wave's tile of 32 slots as matrix operands in registers (two pieces of 16):
+// of the keys a lane holds slot lane % 16 and a quarter of every 32 channels (8
+// bits: a quarter of all), of the values channels kPer (lane % 16) .. of the
+// slots 4 (lane / 16) ..: what decode_kernel's products want, every read of 4 to
+// 16 bytes in line.
+template <int CT, int D>
+struct PageTile {
+    static constexpr bool k8 = CT == PKV_FP8;
+    static constexpr int kKRegs = k8 ? D / 64 : D / 32, kPer = D / 16;
+    typedef typename std::conditional<D == 128, uint32_t, uint16_t>::type ScaleRow;   // of a slot
+    u32x4 k[2][kKRegs], v[2][4];
+    uint32_t ks[2];
+    u32x4 vs[2];
+    uint32_t missing;                   // pieces on no page
+
+    __device__ void load(const PagedDev& a, uint64_t head, int words, int slot, int last, uint32_t lane) {
+        const uint32_t i = lane % 16, g = lane / 16;
+        const uint32_t st = static_cast<uint32_t>(a.k_slot);
+        constexpr uint32_t kSize = k8 ? 1 : 2;
+        missing = no_page<2>(a.seq, words);
+        const uint8_t *kt[2], *vt[2], *kst[2], *vst[2];
+        int room[2];
+        for (int u = 0; u < 2; ++u) {
+            const int start = piece_start(slot, u, last);
+            const uint64_t e = piece_at(a, words, u, start, head);
+            room[u] = last - start;
+            kt[u] = a.k + e * kSize;
+            vt[u] = a.v + e * kSize;
+            if constexpr (k8) { kst[u] = a.ks + e / 32; vst[u] = a.vs + e / 32; }
+        }
+        for (int u = 0; u < 2; ++u) {
+            const uint32_t e = static_cast<uint32_t>(min(static_cast<int>(i), room[u])) * st;
+            for (int s = 0; s < kKRegs; ++s)
+                k[u][s] = *reinterpret_cast<const u32x4*>(kt[u] + (k8 ? e + D / 4 * g + 16 * s : 2 * e + 64 * s + 16 * g));
+            if constexpr (k8) ks[u] = kst[u][e / 32 + (D == 128 ? g : g / 2)];
+        }
+        for (int u = 0; u < 2; ++u) {
+            for (int j = 0; j < 4; ++j) {
+                const uint32_t e = static_cast<uint32_t>(min(static_cast<int>(4 * g) + j, room[u])) * st;
+                if constexpr (k8 && D == 64) v[u][j][0] = *reinterpret_cast<const uint32_t*>(vt[u] + e + 4 * i);
+                else if constexpr (!k8 && D == 128) v[u][j] = *reinterpret_cast<const u32x4*>(vt[u] + 2 * e + 16 * i);
+                else {
+                    const u32x2 x = *reinterpret_cast<const u32x2*>(vt[u] + kSize * e + 8 * i);
+                    v[u][j] = u32x4{x[0], x[1], 0, 0};
+                }
+            }
+            // of the lane group's four slots; slots of the piece past the last: bytes of the page that are not used
+            if constexpr (k8 && D == 128) vs[u] = *reinterpret_cast<const u32x4*>(vst[u] + 16 * g);
+            else if constexpr (k8) {
+                const u32x2 x = *reinterpret_cast<const u32x2*>(vst[u] + 8 * g);
+                vs[u] = u32x4{x[0] & 0xffff, x[0] >> 16, x[1] & 0xffff, x[1] >> 16};
+            }
+        }
+    }
+    // The operand of step s (32 channels) of piece u's logits.
+    __device__ u32x4 keys(int u, int s) const {
+        if constexpr (!k8) return k[u][s];
+        else {
+            const uint32_t lo = k[u][s / 2][s % 2 * 2], hi = k[u][s / 2][s % 2 * 2 + 1];
+            return expand8(lo, hi, block_scale(ks[u]));
+        }
+    }
+    __device__ void expand_values(uint32_t lane) {
+        if constexpr (k8)
+            for (int u = 0; u < 2; ++u)
+                for (int j = 0; j < 4; ++j) {
+                    const uint32_t row = vs[u][j], lo = v[u][j][0], hi = v[u][j][1];
+                    v[u][j] = expand8(lo, hi, block_scale(row >> (lane % 16 / (D == 128 ? 4 : 8) * 8) & 0xff));
+                }
+    }
+    // Infinities and NaN among slot j of piece u's values to 0; true if the lane had any.
+    __device__ bool clean(int u, int j) {
+        bool odd = false;
+        for (int w = 0; w < kPer / 2; ++w) {
+            const uint32_t x = v[u][j][w], y = finite_or_0<mat_type(CT)>(x);
+            odd |= y != x;
+            v[u][j][w] = y;
+        }
+        return odd;
+    }
+    // The channel that the lane's keys of step s start at, and that output register (e, r) of lane group g is.
+    __device__ static uint32_t channel(int s, uint32_t g) { return k8 ? D / 4 * g + 8 * s : 32 * s + 8 * g; }
+    __device__ static uint32_t out_channel(int e, int r, uint32_t g) { return kPer * (4 * g + r) + e; }
+};
+
+// Shares of a unit's or a tile's rows on their way to a join.
+struct PagedPart {
+    float* o;          // [head][unit or tile][..][rows][D]
+    float* ml;         // [..][rows][2]: base, sum of the weights
+    int32_t* plan;     // [sequence][2]: first unit, units (few rows)
+    uint32_t units, target, rows, splits;
+};
+
+// The rows of a sequence of few (rows x group up to 16) against a share of its
+// slots, both products on the matrix cores with nothing staged in LDS:
+//   S^T = K Q^T   A = 16 slots (lane % 16) x 8 channels a lane group (lane /
+//                 16); B = 16 rows (lane % 16).  Any order of the channels will
+//                 do as long as q has the same.  Result: row lane % 16, slots 4
+//                 (lane / 16) + r.
+//   O^T = V^T P^T A wants, for one channel a lane, the slots its lane group has
+//                 in S^T: the softmax's registers are B as they are, v_perm
+//                 gathers each channel across the lane's four (x 2) slots.
+// Weights meet the values as two terms of a 16-bit type, which the bytes hide.
+// The next tile is on its way while one is worked on, and the words of the pages
+// of the one after it, so that no read waits for a page's number.
+template <int CT, int QT, int D>
+__global__ __launch_bounds__(256, 2) void decode_kernel(PagedDev a, PagedPart part) {
+    using T = typename Elem<QT>::T;
+    using Tile = PageTile<CT, D>;
+    constexpr int MT = mat_type(CT), NQ = query_terms(CT, QT), NP = 2, kQ = D / 32, kO = D / 16;
+    const uint32_t work_blocks = a.heads * part.units;
+    if (blockIdx.x >= work_blocks) return clear_rows<QT, D>(a, blockIdx.x - work_blocks);
+    const uint32_t lane = threadIdx.x % 64, wave = __builtin_amdgcn_readfirstlane(threadIdx.x / 64);
+    // heads fastest, so that a head's workgroups share an XCD's L2 (and the pages of a common prefix) where the heads
+    // are a multiple of 8
+    const uint32_t h = blockIdx.x % a.heads, u = blockIdx.x / a.heads;
+    Unit unit;
+    if (!find_unit(a, u, part.target, lane, &unit)) return;
+    if (h == 0 && unit.share == 0 && threadIdx.x == 0) {
+        part.plan[2 * unit.seq] = unit.first;
+        part.plan[2 * unit.seq + 1] = unit.shares;
+    }
+    const Seq sq = seq_of(a.seq, unit.seq, a.max_rows);
+    const uint32_t row = lane % 16, g = lane / 16;
+    const int R = sq.rows * static_cast<int>(a.group), pos1 = sq.first + sq.rows - 1;
+    const bool real = static_cast<int>(row) < R;
+    const int qi = row / a.group, pos = real ? sq.first + qi : -1;
+    const Tiles tl = tiles_of(a, sq.first, pos1, kStep);
+    const int per = (tl.count + unit.shares - 1) / unit.shares;
+    const int t0 = unit.share * per, t1 = min(t0 + per, tl.count);
+    const int32_t* table = a.seq.tables + unit.seq * a.seq.table;
+
+    const T* qp = reinterpret_cast<const T*>(a.q) + static_cast<uint64_t>(sq.row0 + (real ? qi : 0)) * a.q_row +
+                  (h * a.group + (real ? row % a.group : 0)) * a.q_head;
+    u32x4 q[NQ][kQ];
+    for (int s = 0; s < kQ; ++s) {
+        const uint32_t d = Tile::channel(s, g);
+        if constexpr (NQ == 1) {
+            q[0][s] = real ? *reinterpret_cast<const u32x4*>(qp + d) : u32x4{};
+        } else {
+            for (int w = 0; w < 4; ++w) {
+                float x = real ? static_cast<float>(qp[d + 2 * w]) : 0.0f;
+                float y = real ? static_cast<float>(qp[d + 2 * w + 1]) : 0.0f;
+                for (int n = 0; n < NQ; ++n) q[n][s][w] = pack_query_term(x, y);
+            }
+        }
+    }
+
+    const uint64_t head = h * a.k_head;
+    float base = kInf, l = 0.0f;
+    f32x4 o[kO] = {};
+    auto pages = [&](int t) {   // past the last tile: the last's again, unused
+        return read_pages<2>(a.seq, table, tl.slot(min(t, t1 - 1), kStep), tl.high - 1, lane);
+    };
+    auto fetch = [&](Tile& x, int t, int words) {
+        x.load(a, head, words, tl.slot(min(t, t1 - 1), kStep), tl.high - 1, lane);
+    };
+    auto work = [&](Tile& x, int t, auto again) {
+        constexpr bool CLEAN = decltype(again)::value;   // infinities and NaN of the values by themselves
+        const int slot = tl.slot(t, kStep);
+        f32x4 sc[2] = {};
+        for (int p = 0; p < 2; ++p)
+            for (int s = 0; s < kQ; ++s) {
+                const u32x4 ka = x.keys(p, s);
+                for (int n = NQ - 1; n >= 0; --n) sc[p] = mma16<MT>(ka, q[n][s], sc[p]);
+            }
+        x.expand_values(lane);
+        if (x.missing || !all_visible(a, sq.first, pos1, slot, slot + kStep - 1)) {
+            for (int p = 0; p < 2; ++p)
+                for (int j = 0; j < 4; ++j) {
+                    const int key = slot + 16 * p + 4 * static_cast<int>(g) + j;
+                    const bool none = x.missing >> p & 1;
+                    if (none || !visible(a, pos, key)) sc[p][j] = -kInf;
+                    if (none || !any_visible(a, tl, key)) x.v[p][j] = u32x4{};
+                }
+        }
+        bool odd[2][4] = {};
+        if constexpr (CLEAN)
+            for (int p = 0; p < 2; ++p)
+                for (int j = 0; j < 4; ++j) odd[p][j] = x.clean(p, j);
+        float top = fmaxf(fmaxf(sc[0][0], sc[0][1]), fmaxf(sc[0][2], sc[0][3]));
+        top = fmaxf(top, fmaxf(fmaxf(sc[1][0], sc[1][1]), fmaxf(sc[1][2], sc[1][3])));
+        top = across32(across16(top, larger), larger);
+        if (__any(__builtin_fmaf(top, a.scale2, base) > kLift<MT> + kLag<MT>)) {
+            const float low = lower_base(a, kLift<MT>, base, top), f = joined(low, base);
+            if (low < base) {
+                l *= f;
+                for (int e = 0; e < kO; ++e) o[e] *= f;
+                base = low;
+            }
+        }
+        const float from = base == kInf ? 0.0f : base;
+        float p[2][4], r[2][4];
+        for (int x2 = 0; x2 < 2; ++x2)
+            for (int j = 0; j < 4; ++j) {
+                p[x2][j] = __builtin_amdgcn_exp2f(__builtin_fmaf(sc[x2][j], a.scale2, from));
+                if constexpr (CLEAN) p[x2][j] *= kPower<-kDown<MT>>;
+                l += p[x2][j];
+                r[x2][j] = p[x2][j];
+            }
+        u32x4 pt[NP];
+        for (int n = 0; n < NP; ++n)
+            pt[n] = u32x4{pack_term<MT>(r[0][0], r[0][1]), pack_term<MT>(r[0][2], r[0][3]),
+                          pack_term<MT>(r[1][0], r[1][1]), pack_term<MT>(r[1][2], r[1][3])};
+        for (int e = 0; e < kO; ++e) {
+            const uint32_t sel = e % 2 ? 0x07060302u : 0x05040100u;
+            const u32x4 va = {__builtin_amdgcn_perm(x.v[0][1][e / 2], x.v[0][0][e / 2], sel),
+                              __builtin_amdgcn_perm(x.v[0][3][e / 2], x.v[0][2][e / 2], sel),
+                              __builtin_amdgcn_perm(x.v[1][1][e / 2], x.v[1][0][e / 2], sel),
+                              __builtin_amdgcn_perm(x.v[1][3][e / 2], x.v[1][2][e / 2], sel)};
+            for (int n = NP - 1; n >= 0; --n) o[e] = mma16<MT>(va, pt[n], o[e]);
+        }
+        if constexpr (CLEAN)
+            for (int x2 = 0; x2 < 2; ++x2)
+                for (int j = 0; j < 4; ++j) {
+                    const uint64_t has = __ballot(odd[x2][j]);
+#pragma unroll 1
+                    for (uint32_t g2 = 0; g2 < 4; ++g2) {
+                        if (!(has >> 16 * g2 & 0xffff)) continue;
+                        const int key = slot + 16 * x2 + 4 * static_cast<int>(g2) + j;
+                        const bool sees = real && visible(a, pos, key);
+                        // not scaled down: that could make it 0
+                        const float w = __shfl(__builtin_amdgcn_exp2f(__builtin_fmaf(sc[x2][j], a.scale2, from)),
+                                               static_cast<int>(16 * g2 + row));
+                        const int page = page_of(a.seq, unit.seq, min(key, tl.high - 1));
+                        const uint64_t at = (page < 0 ? 0 : page) * a.page + head +
+                                            (static_cast<uint32_t>(key) & ((1u << a.seq.shift) - 1)) * a.k_slot;
+                        for (int e = 0; e < kO; ++e)
+                            for (int r2 = 0; r2 < 4; ++r2) {
+                                const float v = element<CT>(a.v, a.vs, at + Tile::out_channel(e, r2, g));
+                                if (sees && (__float_as_uint(v) & 0x7f800000u) == 0x7f800000u) o[e][r2] += w * v;
+                            }
+                    }
+                }
+    };
+    // two tiles in turn: one is on its way while the other is worked on
+    const int first = t0 + static_cast<int>(wave);
+    if (first < t1) {
+        Tile even, odd;
+        int words = pages(first), next = pages(first + 4);
+        fetch(even, first, words);
+        for (int t = first; t < t1; t += 8) {
+            words = pages(t + 8);
+            fetch(odd, t + 4, next);
+            work(even, t, std::false_type());
+            if (t + 4 >= t1) break;
+            next = pages(t + 12);
+            fetch(even, t + 8, words);
+            work(odd, t + 4, std::false_type());
+        }
+        // An infinity or NaN among the values: a row that does not see it has met it with the weight 0, and the terms
+        // of a weight that does see it may be 0 or negative.  Again, with those values taken out of the products and
+        // each added to the rows that see it; or a sum past the type's end: see kDown.
+        bool bad = false;
+        for (int e = 0; e < kO; ++e)
+            for (int r = 0; r < 4; ++r) bad |= (__float_as_uint(o[e][r]) & 0x7f800000u) == 0x7f800000u;
+        if (__builtin_expect(__any(bad && real), 0)) {
+            base = kInf;
+            l = 0.0f;
+            for (int e = 0; e < kO; ++e) o[e] = f32x4{};
+#pragma unroll 1
+            for (int t = first; t < t1; t += 4) {
+                fetch(even, t, pages(t));
+                work(even, t, std::true_type());
+            }
+            bool past = false;   // back, unless it does not fit
+            for (int e = 0; e < kO; ++e)
+                for (int r = 0; r < 4; ++r)
+                    past |= fabsf(o[e][r]) < kInf && !(fabsf(o[e][r]) * kPower<kDown<MT>> < kInf);
+            if (__any(past && real)) {
+                base -= kDown<MT>;
+            } else {
+                for (int e = 0; e < kO; ++e) o[e] *= kPower<kDown<MT>>;
+                l *= kPower<kDown<MT>>;
+            }
+        }
+    }
+    l += __shfl_xor(l, 16);
+    l += __shfl_xor(l, 32);
+
+    // the four waves' shares joined; a sequence of one unit is done
+    __shared__ float so[4][16][D + 4], sb[4][16], sl[4][16];
+    for (int r = 0; r < 4; ++r)
+        for (int e = 0; e < kO; ++e) so[wave][row][Tile::out_channel(e, r, g)] = o[e][r];
+    if (g == 0) { sb[wave][row] = base; sl[wave][row] = l; }
+    __syncthreads();
+    for (uint32_t x = threadIdx.x; x < static_cast<uint32_t>(R) * (D / 4); x += 256) {
+        const uint32_t r = x / (D / 4), d = x % (D / 4) * 4;
+        const float low = fminf(fminf(sb[0][r], sb[1][r]), fminf(sb[2][r], sb[3][r]));
+        float sum = 0.0f;
+        f32x4 acc = {};
+        for (int w = 0; w < 4; ++w) {
+            const float f = joined(low, sb[w][r]);
+            sum += sl[w][r] * f;
+            acc += *reinterpret_cast<const f32x4*>(&so[w][r][d]) * (f * kPower<-kPartDown>);
+        }
+        if (unit.shares == 1) {
+            write_row<QT>(a, sq.row0 + r / a.group, h * a.group + r % a.group, d, acc, low, sum, kPower<-kPartDown>);
+        } else {
+            const uint64_t at = (static_cast<uint64_t>(h) * part.units + u) * part.rows + r;
+            *reinterpret_cast<f32x4*>(part.o + at * D + d) = acc;
+            if (d == 0) {
+                part.ml[2 * at] = low;
+                part.ml[2 * at + 1] = sum;
+            }
+        }
+    }
+}
+
+// The units of a row joined, a workgroup a row: every wave the row's base and
+// sum, then 1024 / D units at a time, 4 channels a thread.
+template <int QT, int D>
+__global__ __launch_bounds__(256) void join_kernel(PagedDev a, PagedPart part) {
+    const uint32_t lane = threadIdx.x % 64;
+    const uint32_t r = blockIdx.x % part.rows, sh = blockIdx.x / part.rows, s = sh / a.heads, h = sh % a.heads;
+    const Seq q = seq_of(a.seq, s, a.max_rows);
+    const int64_t all = static_cast<int64_t>(q.rows) * a.group;
+    if (r >= all || all > kFew) return;
+    const uint32_t first = part.plan[2 * s], shares = part.plan[2 * s + 1];
+    if (shares == 1) return;
+    const uint64_t at = (static_cast<uint64_t>(h) * part.units + first) * part.rows + r;
+    const float* ml = part.ml + 2 * at;
+    const uint64_t step = 2ull * part.rows;
+    float low = kInf;
+    for (uint32_t x = lane; x < shares; x += 64) low = fminf(low, ml[step * x]);
+    for (int x = 32; x; x >>= 1) low = fminf(low, __shfl_xor(low, x));
+    float sum = 0.0f;
+    for (uint32_t x = lane; x < shares; x += 64) sum += ml[step * x + 1] * joined(low, ml[step * x]);
+    sum = wave_sum(sum);
+    constexpr uint32_t kLanes = D / 4, kShares = 256 / kLanes;
+    const uint32_t mine = threadIdx.x / kLanes, d = threadIdx.x % kLanes * 4;
+    f32x4 o = {};
+    for (uint32_t x = mine; x < shares; x += kShares) {
+        const float f = joined(low, ml[step * x]) * kPower<-kJoinDown>;
+        o += *reinterpret_cast<const f32x4*>(part.o + (at + static_cast<uint64_t>(part.rows) * x) * D + d) * f;
+    }
+    __shared__ f32x4 so[256];
+    so[threadIdx.x] = o;
+    __syncthreads();
+    if (mine) return;
+    for (uint32_t x = 1; x < kShares; ++x) o += so[threadIdx.x + x * kLanes];
+    write_row<QT>(a, q.row0 + r / a.group, h * a.group + r % a.group, d, o, low, sum, kPower<-kPartDown - kJoinDown>);
+}
+
 // A wave a packed row and query head: a slot a lane for the logits, the channels
 // over the lanes for the values, one pass with the running maximum and sum.
 template <int CT, int QT, int D, bool PAGED>
-__global__ __launch_bounds__(256) void row_kernel(PagedDev a, uint32_t work) {
+__global__ __launch_bounds__(256) void row_kernel(PagedDev a, uint32_t work, bool few) {
     using T = typename Elem<QT>::T;
     if (blockIdx.x >= work) return clear_rows<QT, D>(a, blockIdx.x - work);
     __shared__ float sq[4][D];
@@ -234,7 +682,7 @@ __global__ __launch_bounds__(256) void row_kernel(PagedDev a, uint32_t work) {
     if (s < 0) return;
     const Seq q = seq_of(a.seq, s, a.max_rows);
     const int i = static_cast<int>(r) - q.row0;
-    if (i >= q.rows) return;
+    if (i >= q.rows || (few && static_cast<int64_t>(q.rows) * a.group <= kFew)) return;
     const int pos = q.first + i;
     const T* qp = reinterpret_cast<const T*>(a.q) + static_cast<uint64_t>(r) * a.q_row + qh * a.q_head;
     for (uint32_t d = lane; d < D; d += 64) sq[wave][d] = static_cast<float>(qp[d]);
@@ -274,10 +722,50 @@ __global__ __launch_bounds__(256) void row_kernel(PagedDev a, uint32_t work) {
 
 uint32_t clears(const PagedDev& a) { return a.clear && a.seq.starts ? kClear : 0; }
 
+uint64_t round256(uint64_t x) { return (x + 255) & ~255ull; }
+
+// The launches of a call and its workspace.
+struct Plan {
+    bool few, many;                // sequences of few rows are looked for; of more
+    uint32_t units, target, rows;  // decode_kernel: units a head at most, aimed at, rows of one
+    uint64_t ml, plan, bytes;      // offsets in the workspace (partial outputs first), all of it
+};
+Plan plan_of(const PagedDev& a, uint32_t dim) {
+    Plan p{};
+    const uint64_t most = static_cast<uint64_t>(a.max_rows) * a.group;
+    p.few = a.seq.paged && (!a.seq.each || most <= kFew);
+    p.many = !a.seq.paged || most > kFew;
+    if (p.few) {
+        p.rows = static_cast<uint32_t>(std::min<uint64_t>(kFew, most));
+        p.target = (kUnits + a.heads - 1) / a.heads;
+        // tiles that a sequence can have: all, or the window, the rows before its last and the sinks, rounded to tiles apart
+        uint64_t tiles = a.seq.max_len;
+        if (a.window) tiles = std::min<uint64_t>(tiles, static_cast<uint64_t>(a.window) + kFew + a.sinks + 4 * kStep);
+        tiles = (tiles + kStep - 1) / kStep;
+        const uint64_t each = std::max<uint64_t>(1, (tiles + kLeast - 1) / kLeast);
+        p.units = static_cast<uint32_t>(std::min<uint64_t>(static_cast<uint64_t>(a.seq.seqs) + p.target, a.seq.seqs * each));
+        const uint64_t rows = static_cast<uint64_t>(a.heads) * p.units * p.rows;
+        p.ml = round256(rows * dim * 4);
+        p.plan = p.ml + round256(rows * 8);
+        p.bytes = p.plan + round256(8ull * a.seq.seqs);
+    }
+    return p;
+}
+
 template <int CT, int QT, int D, bool PAGED>
-int attend_typed(const PagedDev& a, uint8_t*, hipStream_t st) {
-    const uint32_t work = static_cast<uint32_t>((static_cast<uint64_t>(a.seq.rows) * a.heads * a.group + 3) / 4);
-    row_kernel<CT, QT, D, PAGED><<<work + clears(a), 256, 0, st>>>(a, work);
+int attend_typed(const PagedDev& a, uint8_t* ws, hipStream_t st) {
+    const Plan p = plan_of(a, D);
+    if constexpr (PAGED)
+        if (p.few) {
+            const PagedPart part{reinterpret_cast<float*>(ws), reinterpret_cast<float*>(ws + p.ml),
+                                 reinterpret_cast<int32_t*>(ws + p.plan), p.units, p.target, p.rows, 1};
+            decode_kernel<CT, QT, D><<<a.heads * p.units + clears(a), 256, 0, st>>>(a, part);
+            if (p.units > a.seq.seqs) join_kernel<QT, D><<<a.seq.seqs * a.heads * p.rows, 256, 0, st>>>(a, part);
+        }
+    if (p.many) {
+        const uint32_t work = static_cast<uint32_t>((static_cast<uint64_t>(a.seq.rows) * a.heads * a.group + 3) / 4);
+        row_kernel<CT, QT, D, PAGED><<<work + (p.few ? 0 : clears(a)), 256, 0, st>>>(a, work, p.few);
+    }
     return hipGetLastError();
 }
 template <int CT, int QT, bool PAGED>
@@ -307,15 +795,19 @@ int launch_rows(const PagedRowsDev& r, uint32_t dim, int cache_dtype, int dtype,
 
 }  // namespace
 
-bool paged_fits(const PagedDev& a, uint32_t, int) {
-    return static_cast<uint64_t>(a.seq.rows) * a.heads * a.group < 1u << 26;
+bool paged_fits(const PagedDev& a, uint32_t dim, int) {
+    const Plan p = plan_of(a, dim);
+    uint64_t most = 0;
+    if (p.few)
+        most = std::max(static_cast<uint64_t>(a.heads) * p.units, static_cast<uint64_t>(a.seq.seqs) * a.heads * p.rows);
+    return most < (1u << 24) - kClear && (!p.many || static_cast<uint64_t>(a.seq.rows) * a.heads * a.group < 1u << 25);
 }
 
-uint64_t paged_workspace(const PagedDev&, uint32_t, int) { return 0; }
+uint64_t paged_workspace(const PagedDev& a, uint32_t dim, int) { return plan_of(a, dim).bytes; }
 
 int launch_paged(const PagedDev& a, uint32_t dim, int cache_dtype, int dtype, uint8_t* ws, void* stream) {
     hipStream_t st = static_cast<hipStream_t>(stream);
-    if (!a.seq.tables)
+    if (!a.seq.paged)
         return dtype == PKV_BF16 ? attend_dim<PKV_BF16, PKV_BF16, false>(a, dim, ws, st)
                                  : attend_dim<PKV_F16, PKV_F16, false>(a, dim, ws, st);
     if (cache_dtype == PKV_BF16) return attend_dim<PKV_BF16, PKV_BF16, true>(a, dim, ws, st);
