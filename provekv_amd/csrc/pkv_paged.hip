@@ -175,22 +175,7 @@ __global__ __launch_bounds__(256) void paged_load_kernel(PagedRowsDev a) {
 }
 
 // ------------------------------------------------------------ attention
-// Element offsets of slot j of sequence s, keys and values; false: no page holds it.
-template <bool PAGED>
-__device__ inline bool slot_at(const PagedDev& a, uint32_t s, int row0, uint32_t h, int j, uint64_t* k, uint64_t* v) {
-    uint64_t kj, vj;
-    if constexpr (PAGED) {
-        const int page = page_of(a.seq, s, j);
-        if (page < 0) return false;
-        kj = vj = page * a.page + (static_cast<uint32_t>(j) & ((1u << a.seq.shift) - 1)) * a.k_slot;
-    } else {
-        kj = static_cast<uint64_t>(row0 + j) * a.k_slot;
-        vj = static_cast<uint64_t>(row0 + j) * a.v_slot;
-    }
-    *k = kj + h * a.k_head;
-    *v = vj + h * a.v_head;
-    return true;
-}
+// A cached value.
 template <int CT>
 __device__ inline float element(const uint8_t* p, const uint8_t* scales, uint64_t e) {
     if constexpr (CT == PKV_FP8) {
@@ -239,11 +224,6 @@ constexpr int kFew = 16;            // rows x group of a KV head that decode_ker
 constexpr int kStep = 32;           // slots of its tiles
 constexpr uint32_t kUnits = 1024;   // units of all heads that it aims at
 constexpr int kLeast = 4;           // tiles of a unit, one a wave
-
-__device__ inline int wave_add(int x) {
-    for (int o = 32; o; o >>= 1) x += __shfl_xor(x, o);
-    return x;
-}
 
 // The tiles that a sequence of few rows has; -1: it has no rows, or more.
 __device__ inline int few_tiles(const PagedDev& a, uint32_t s) {
@@ -668,56 +648,385 @@ __global__ __launch_bounds__(256) void join_kernel(PagedDev a, PagedPart part) {
     write_row<QT>(a, q.row0 + r / a.group, h * a.group + r % a.group, d, o, low, sum, kPower<-kPartDown - kJoinDown>);
 }
 
-// A wave a packed row and query head: a slot a lane for the logits, the channels
-// over the lanes for the values, one pass with the running maximum and sum.
-template <int CT, int QT, int D, bool PAGED>
-__global__ __launch_bounds__(256) void row_kernel(PagedDev a, uint32_t work, bool few) {
-    using T = typename Elem<QT>::T;
-    if (blockIdx.x >= work) return clear_rows<QT, D>(a, blockIdx.x - work);
-    __shared__ float sq[4][D];
-    const uint32_t lane = threadIdx.x % 64, wave = threadIdx.x / 64, heads = a.heads * a.group;
-    const uint32_t item = blockIdx.x * 4 + wave, r = item / heads, qh = item % heads, h = qh / a.group;
-    if (r >= a.seq.rows) return;
-    const int s = seq_of_row(a.seq, static_cast<int>(r), lane);
-    if (s < 0) return;
-    const Seq q = seq_of(a.seq, s, a.max_rows);
-    const int i = static_cast<int>(r) - q.row0;
-    if (i >= q.rows || (few && static_cast<int64_t>(q.rows) * a.group <= kFew)) return;
-    const int pos = q.first + i;
-    const T* qp = reinterpret_cast<const T*>(a.q) + static_cast<uint64_t>(r) * a.q_row + qh * a.q_head;
-    for (uint32_t d = lane; d < D; d += 64) sq[wave][d] = static_cast<float>(qp[d]);
-    float top = -kInf, sum = 0.0f, o[D / 64] = {};
-    const Tiles tl = tiles_of(a, pos, pos, 64);
-    for (int t = 0; t < tl.count; ++t) {
-        const int j0 = tl.slot(t, 64), j = j0 + static_cast<int>(lane);
-        uint64_t kj = 0, vj = 0;
-        const bool see = j < tl.high && visible(a, pos, j) && slot_at<PAGED>(a, s, q.row0, h, j, &kj, &vj);
-        float x = -kInf;
-        if (see) {
-            x = 0.0f;
-            for (uint32_t d = 0; d < D; ++d) x += element<CT>(a.k, a.ks, kj + d) * sq[wave][d];
-            x *= a.scale2;
-        }
-        float m = x;
-        for (int y = 32; y; y >>= 1) m = fmaxf(m, __shfl_xor(m, y));
-        m = fmaxf(m, top);
-        const float f = m == -kInf ? 1.0f : exp2f(top - m), w = see && m != -kInf ? exp2f(x - m) : 0.0f;
-        top = m;
-        // o is the mean so far: a sum could pass the end of f32 where the mean does not
-        const float before = sum * f, all = before + wave_sum(w), part = all == 0.0f ? 0.0f : 1.0f / all;
-        sum = all;
-        for (int e = 0; e < D / 64; ++e) o[e] *= before * part;
-        for (int y = 0; y < 64; ++y) {
-            if (!__shfl(static_cast<int>(see), y)) continue;
-            const float wy = __shfl(w, y) * part;
-            const uint64_t at = static_cast<uint64_t>(__shfl(static_cast<unsigned long long>(vj), y));
-            for (int e = 0; e < D / 64; ++e) o[e] += wy * element<CT>(a.v, a.vs, at + 64 * e + lane);
+// ------------------------------------------------------------ many rows: tiles of rows through LDS
+// Row tile u of a head: sequences in order, of each its tiles from the last, whose
+// rows see most.
+struct RowTile {
+    int seq, tile;
+};
+__device__ inline int row_tiles(const PagedDev& a, uint32_t s, int64_t few, int rows) {
+    const int64_t all = static_cast<int64_t>(seq_of(a.seq, s, a.max_rows).rows) * a.group;
+    return all > few ? static_cast<int>((all + rows - 1) / rows) : 0;
+}
+__device__ inline bool find_tile(const PagedDev& a, uint32_t u, int64_t few, int rows, uint32_t lane, RowTile* o) {
+    const uint32_t per = (a.seq.seqs + 63) / 64, s0 = min(lane * per, a.seq.seqs), s1 = min(s0 + per, a.seq.seqs);
+    int n = 0;
+    for (uint32_t s = s0; s < s1; ++s) n += row_tiles(a, s, few, rows);
+    int end = n;
+    for (int x = 1; x < 64; x <<= 1) {
+        const int y = __shfl_up(end, x);
+        if (static_cast<int>(lane) >= x) end += y;
+    }
+    const int want = static_cast<int>(u);
+    const uint32_t at = __popcll(__ballot(end <= want));
+    if (at == 64) return false;
+    int first = __shfl(end - n, static_cast<int>(at));
+    uint32_t s = at * per;
+    for (;; ++s) {
+        n = row_tiles(a, s, few, rows);
+        if (want < first + n) break;
+        first += n;
+    }
+    o->seq = __builtin_amdgcn_readfirstlane(s);
+    o->tile = __builtin_amdgcn_readfirstlane(n - 1 - (want - first));
+    return true;
+}
+
+// Staged's tiles from pages, or (PAGED false) from packed rows.  16-bit rows go
+// from memory to LDS without registers; a wave's 1,024 bytes lie in one page.
+template <int CT, int D, bool PAGED>
+struct PageStage : Staged<CT, D> {
+    using L = Staged<CT, D>;
+    using L::kRow, L::kPieces, L::kKeyBytes, L::kCopies, L::kCopyRows, L::kCopyStep, L::turn, L::key_at, L::value_at, L::code_slot;
+    static constexpr int kHeld = CT == PKV_FP8 ? D / 64 : 1;   // 16 codes a register
+    u32x4 k[kHeld], v[kHeld];                                  // 8-bit codes on their way
+    uint32_t ks, vs;
+
+    // Start a tile on its way.  head: elements to the head's first page (packed rows: kp, vp are its row 0); slots past
+    // `last` read the last one.
+    __device__ void fetch(const PagedDev& a, uint32_t lds, const uint8_t* kp, const uint8_t* vp, uint64_t head, int words,
+                          int slot, int last) {
+        const uint32_t lane = threadIdx.x % 64, wave = __builtin_amdgcn_readfirstlane(threadIdx.x / 64);
+        if constexpr (CT == PKV_FP8) {
+            const int start = piece_start(slot, wave, last);
+            const uint64_t e = piece_at(a, words, wave, start, head) +
+                               static_cast<uint32_t>(min(static_cast<int>(code_slot(threadIdx.x) - 16 * wave), last - start)) * D;
+            const uint32_t b = threadIdx.x % 4;
+            for (int x = 0; x < kHeld; ++x) {
+                k[x] = *reinterpret_cast<const u32x4*>(a.k + e + D / 4 * b + 16 * x);
+                v[x] = *reinterpret_cast<const u32x4*>(a.v + e + D / 4 * b + 16 * x);
+            }
+            ks = a.ks[e / 32 + (D == 128 ? b : b / 2)];
+            vs = a.vs[e / 32 + (D == 128 ? b : b / 2)];
+        } else {
+            // turn() of the row is the same for all of a lane's copies
+            const uint32_t row = kCopyRows * wave + lane / kPieces, piece = lane % kPieces;
+            const uint32_t kc = (piece ^ turn(row, false)) * 16, vc = (piece ^ turn(row, true)) * 16;
+            for (int x = 0; x < kCopies; ++x) {
+                const uint32_t to = lds + (kCopyStep * x + kCopyRows * wave) * kRow;
+                const int j = min(slot + kCopyStep * x + static_cast<int>(row), last);
+                if constexpr (PAGED) {
+                    const int p = (kCopyStep * x + kCopyRows * wave) / 16, start = piece_start(slot, p, last);
+                    const uint64_t e = 2 * piece_at(a, words, p, start, head);
+                    const uint32_t off = static_cast<uint32_t>(j - start) * static_cast<uint32_t>(a.k_slot) * 2;
+                    copy_to_lds(to, a.k + e, off + kc);
+                    copy_to_lds(to + kKeyBytes, a.v + e, off + vc);
+                } else {
+                    const uint32_t i = static_cast<uint32_t>(j - slot);
+                    copy_to_lds(to, kp + 2 * static_cast<uint64_t>(slot) * a.k_slot, 2 * i * static_cast<uint32_t>(a.k_slot) + kc);
+                    copy_to_lds(to + kKeyBytes, vp + 2 * static_cast<uint64_t>(slot) * a.v_slot,
+                                2 * i * static_cast<uint32_t>(a.v_slot) + vc);
+                }
+            }
         }
     }
-    T* out = reinterpret_cast<T*>(a.out) + static_cast<uint64_t>(r) * a.o_row + qh * a.o_head;
-    for (int e = 0; e < D / 64; ++e) out[64 * e + lane] = static_cast<T>(sum == 0.0f ? 0.0f : o[e]);
-    if (lane == 0 && a.lse)
-        a.lse[static_cast<uint64_t>(qh) * a.seq.rows + r] = sum == 0.0f ? -kInf : (top + log2f(sum)) * kLn2;
+    // What fetch started, into LDS (a barrier follows).
+    __device__ void land(uint8_t* lds) {
+        if constexpr (CT == PKV_FP8) {
+            const uint32_t row = code_slot(threadIdx.x), b = threadIdx.x % 4;
+            for (int w = 0; w < D / 32; ++w) {
+                const int r = w / 2, c = w % 2 * 2;
+                const uint32_t k0 = k[r][c], k1 = k[r][c + 1], v0 = v[r][c], v1 = v[r][c + 1];
+                *reinterpret_cast<u32x4*>(lds + key_at(row, b * (D / 32) + w)) = expand8(k0, k1, block_scale(ks));
+                *reinterpret_cast<u32x4*>(lds + value_at(row, b * (D / 32) + w)) = expand8(v0, v1, block_scale(vs));
+            }
+        } else {
+            copies_done();
+        }
+    }
+};
+
+// Rows in tiles of 128, 32 a wave, against tiles of 64 slots staged through LDS
+// in two buffers, one barrier a tile:
+//   S^T = K Q^T (32x32 tiles; a lane holds one query row and half of each
+//   piece's slots), softmax in registers, O^T += V^T P^T with the rounded
+//   weights straight from those registers.
+// Weights are rounded once to the type of the products (f16 queries over 8-bit
+// codes: two bf16 terms), while their sum is that of the unrounded ones.
+// KS 2: a workgroup has 64 rows and two waves share a tile's slots, for calls
+// whose 128-row tiles would not fill the chip.
+//
+// A weight 0 times an infinity or NaN would be NaN in rows that do not see the
+// slot.  The loop does not look for those: an output that is not finite sends
+// the workgroup through it again, with infinities and NaN taken out of the
+// staged values and each added afterwards to the rows that see it.  Where the
+// sums of finite values are not finite either, a third time with smaller
+// weights (kDown).
+template <int CT, int QT, int D, bool PAGED, int KS>
+__global__ __launch_bounds__(256, (query_terms(CT, QT) * D >= 256 ? 1 : 2)) void rows_kernel(PagedDev a, PagedPart part,
+                                                                                            int few) {
+    __shared__ __align__(16) uint8_t lds[2 * Staged<CT, D>::kBytes];
+    using T = typename Elem<QT>::T;
+    using St = PageStage<CT, D, PAGED>;
+    constexpr int MT = mat_type(CT), kU = St::kSlots / 32 / KS, kO = D / 32;   // kU: 32-slot pieces a wave takes of a tile
+    constexpr int NP = query_terms(CT, QT), kRowTile = row_tile(KS);
+    const uint32_t work_blocks = a.heads * part.units * part.splits;
+    if (blockIdx.x >= work_blocks) return clear_rows<QT, D>(a, blockIdx.x - work_blocks);
+    const uint32_t lane = threadIdx.x % 64, wave_id = __builtin_amdgcn_readfirstlane(threadIdx.x / 64);
+    const uint32_t n = lane % 32, half = lane / 32;
+    const uint32_t wave = wave_id % (4 / KS);                     // its 32 rows
+    const int share = static_cast<int>(wave_id / (4 / KS)) * 32 * kU;   // its slots of a tile: share .. + 32 kU
+    // heads fastest, so that a head's workgroups share an XCD's L2 where the heads are a multiple of 8
+    const uint32_t h = blockIdx.x % a.heads, split = blockIdx.x / a.heads % part.splits, u = blockIdx.x / a.heads / part.splits;
+    RowTile rt;
+    if (!find_tile(a, u, few, kRowTile, lane, &rt)) return;
+    const Seq sq = seq_of(a.seq, rt.seq, a.max_rows);
+    const int R = sq.rows * static_cast<int>(a.group), r0 = rt.tile * kRowTile, G = static_cast<int>(a.group);
+    const int last = min(r0 + kRowTile, R) - 1;
+    const int pos0 = sq.first + r0 / G, pos1 = sq.first + last / G;
+    const Tiles tl = tiles_of(a, pos0, pos1, St::kSlots);
+    const int per = (tl.count + static_cast<int>(part.splits) - 1) / static_cast<int>(part.splits);
+    const int t0 = static_cast<int>(split) * per, t1 = min(t0 + per, tl.count);
+
+    const int w0 = r0 + 32 * static_cast<int>(wave), w1 = min(w0 + 31, last), r = w0 + static_cast<int>(n);
+    const bool real = r <= last;
+    const int qi = (real ? r : last) / G, pos = real ? sq.first + qi : -1;
+    const int wpos0 = sq.first + w0 / G, wpos1 = sq.first + w1 / G;   // of the wave's rows (w0 > last: none)
+    const Tiles wt = tiles_of(a, wpos0, w0 <= last ? wpos1 : -1, 1);
+    Query<CT, QT, D> q;
+    q.load(reinterpret_cast<const T*>(a.q) + static_cast<uint64_t>(sq.row0 + qi) * a.q_row +
+               (h * a.group + (real ? r : last) % G) * a.q_head,
+           real, half);
+
+    const uint64_t head = h * a.k_head;
+    const int32_t* table = PAGED ? a.seq.tables + rt.seq * a.seq.table : nullptr;
+    const uint8_t* kp = PAGED ? nullptr : a.k + 2 * (static_cast<uint64_t>(sq.row0) * a.k_slot + head);
+    const uint8_t* vp = PAGED ? nullptr : a.v + 2 * (static_cast<uint64_t>(sq.row0) * a.v_slot + h * a.v_head);
+
+    const uint32_t at = static_cast<uint32_t>(reinterpret_cast<uintptr_t>((LdsByte*)lds));
+    float base, l;
+    f32x16 o[kO];
+    St st;
+    // the words of tile t's pages (past the last: the last's again, unused)
+    auto pages = [&](int t) {
+        if constexpr (!PAGED) return 0;
+        else return read_pages<4>(a.seq, table, tl.slot(min(t, t1 - 1), St::kSlots), tl.high - 1, lane);
+    };
+    auto missing = [&](int words) { return PAGED ? no_page<4>(a.seq, words) : 0u; };
+    auto fetch = [&](int t, int words) {
+        st.fetch(a, at + ((t - t0) & 1) * St::kBytes, kp, vp, head, words, tl.slot(t, St::kSlots), tl.high - 1);
+    };
+    // no row of the wave sees any of the tile
+    auto skip = [&](int slot) {
+        return slot + share >= wt.high ||
+               (slot + share + 32 * kU <= wt.low && static_cast<uint32_t>(slot + share) >= a.sinks);
+    };
+    float lift = kLift<MT>;
+    for (int pass = 0;; ++pass) {
+        base = kInf;
+        l = 0.0f;
+        for (int e = 0; e < kO; ++e) o[e] = f32x16{};
+        int words = 0, next = 0;
+        if (t0 < t1) {
+            words = pages(t0);
+            next = pages(t0 + 1);
+            fetch(t0, words);
+            st.land(lds);
+        }
+        __syncthreads();
+        for (int t = t0; t < t1; ++t) {
+            uint8_t* buf = lds + ((t - t0) & 1) * St::kBytes;
+            const uint32_t none = missing(words) >> share / 16;
+            if (t + 1 < t1) {
+                words = next;
+                next = pages(t + 2);      // ahead of its tile's copies, which wait for it
+                fetch(t + 1, words);
+            }
+            const int slot = tl.slot(t, St::kSlots);
+            if (__builtin_expect(pass, 0)) {
+                St::clean(buf);
+                __syncthreads();
+            }
+            if (!skip(slot)) {
+                f32x16 sc[kU];
+                const int mine = slot + share;
+                for (int p = 0; p < kU; ++p) sc[p] = logits32<CT, QT, D>(buf + share * St::kRow, p, q, lane);
+                if (!all_visible(a, wpos0, wpos1, mine, mine + 32 * kU - 1)) {
+                    const int off = pos - mine - 4 * static_cast<int>(half);   // less the register's place: how far back
+                    if (static_cast<uint32_t>(mine) >= a.sinks) {
+                        for (int p = 0; p < kU; ++p)
+                            for (int x = 0; x < 16; ++x)
+                                if (!in_reach(a, off, 32 * p + row32(x, 0))) sc[p][x] = -kInf;
+                    } else {
+                        for (int p = 0; p < kU; ++p)
+                            for (int x = 0; x < 16; ++x)
+                                if (!visible(a, pos, mine + 32 * p + row32(x, half))) sc[p][x] = -kInf;
+                    }
+                }
+                if (PAGED && none)
+                    for (int p = 0; p < kU; ++p)
+                        for (int x = 0; x < 16; ++x)
+                            if (none >> (2 * p + x / 8) & 1) sc[p][x] = -kInf;
+                float top = sc[0][0];
+                for (int p = 0; p < kU; ++p)
+                    for (int x = 0; x < 16; ++x) top = fmaxf(top, sc[p][x]);
+                top = across32(top, larger);
+                if (__any(__builtin_fmaf(top, a.scale2, base) > lift + kLag<MT>)) {
+                    const float low = lower_base(a, lift, base, top), f = joined(low, base);
+                    if (low < base) {
+                        l *= f;
+                        for (int e = 0; e < kO; ++e) o[e] *= f;
+                        base = low;
+                    }
+                }
+                const float from = base == kInf ? 0.0f : base;
+                for (int p = 0; p < kU; ++p)
+                    for (int x = 0; x < 16; ++x) {
+                        sc[p][x] = __builtin_amdgcn_exp2f(__builtin_fmaf(sc[p][x], a.scale2, from));
+                        l += sc[p][x];
+                    }
+                // ahead of the other workgroup's softmax while the matrix cores have work
+                __builtin_amdgcn_s_setprio(1);
+                for (int p = 0; p < kU; ++p)
+                    for (int y = 0; y < 2; ++y) {
+                        float w[8];
+                        for (int x = 0; x < 8; ++x) w[x] = sc[p][8 * y + x];
+                        u32x4 pt[NP];
+                        for (int k = 0; k < NP; ++k)
+                            pt[k] = u32x4{pack_term<MT>(w[0], w[1]), pack_term<MT>(w[2], w[3]),
+                                          pack_term<MT>(w[4], w[5]), pack_term<MT>(w[6], w[7])};
+                        for (int e = 0; e < kO; ++e) {
+                            const u32x4 v = St::values16(buf + share * St::kRow, 32 * p + 16 * y, e, lane);
+                            for (int k = NP - 1; k >= 0; --k) o[e] = mma32<MT>(v, pt[k], o[e]);
+                        }
+                    }
+            }
+            __builtin_amdgcn_s_setprio(0);
+            if (t + 1 < t1) st.land(lds + ((t + 1 - t0) & 1) * St::kBytes);
+            __syncthreads();
+        }
+        if (pass < 2) {
+            bool odd = false;
+            for (int e = 0; e < kO; ++e)
+                for (int x = 0; x < 16; ++x) odd |= (__float_as_uint(o[e][x]) & 0x7f800000u) == 0x7f800000u;
+            // with the values finite, from a NaN among the logits, as the weights' sum, or past the type's end
+            if (pass) odd &= !__builtin_isnan(across32(l, [](float x, float y) { return x + y; }));
+            const bool again = __syncthreads_or(odd && real);
+            if (!pass && !again) break;
+            if (!pass) continue;
+            if (again && kDown<MT>) {
+                lift -= kDown<MT>;
+                continue;
+            }
+        }
+        // not scaled down: that could make a weight 0
+        const float from = base == kInf ? 0.0f : base + (kLift<MT> - lift);
+#pragma unroll 1
+        for (int t = t0; t < t1; ++t) {
+            const int slot = tl.slot(t, St::kSlots), here = pages(t);
+            const uint32_t none = missing(here);
+            uint8_t* buf = lds + ((t - t0) & 1) * St::kBytes;
+            fetch(t, here);
+            st.land(buf);
+            __syncthreads();
+            if (!__syncthreads_or(St::clean(buf))) continue;
+            fetch(t, here);
+            st.land(buf);
+            __syncthreads();
+#pragma unroll 1
+            for (int j = share; j < share + 32 * kU; ++j) {
+                const bool sees = visible(a, pos, slot + j) && !(none >> j / 16 & 1);
+                if (!__any(sees)) continue;
+                uint32_t hf = half;
+                asm volatile("" : "+v"(hf));   // this rare loop's addresses are not kept over the main one
+                float dot = 0.0f;
+                for (int x = 0; x < Query<CT, QT, D>::kRegs; ++x) {
+                    const u32x4 k = *reinterpret_cast<const u32x4*>(buf + St::key_at(j, 2 * x + hf));
+                    for (int w = 0; w < 4; ++w)
+                        for (int y = 0; y < Query<CT, QT, D>::kTerms; ++y) dot += dot_word<MT>(k[w], q.q[y][x][w]);
+                }
+                dot += __shfl_xor(dot, 32);
+                const float p = __builtin_amdgcn_exp2f(__builtin_fmaf(dot, a.scale2, from));
+                for (int e = 0; e < kO; ++e)
+                    for (int x = 0; x < 16; ++x) {
+                        const float v = St::value(buf, j, 32 * e + row32(x, hf));
+                        if (sees && (__float_as_uint(v) & 0x7f800000u) == 0x7f800000u) o[e][x] += p * v;
+                    }
+            }
+            __syncthreads();
+        }
+        break;
+    }
+    l += __shfl_xor(l, 32);
+    constexpr int kShared = KS > 1 ? 1 : 0;   // outputs are 2^-kShared as large from here on
+    if constexpr (KS > 1) {
+        // the other share of the slots joins the first: [row block][o, base, l][lane]
+        float* to = reinterpret_cast<float*>(lds) + wave * (16 * kO + 2) * 64 + lane;
+        if (share) {
+            for (int x = 0; x < 16 * kO; ++x) to[x * 64] = o[x / 16][x % 16];
+            to[16 * kO * 64] = base;
+            to[(16 * kO + 1) * 64] = l;
+        }
+        __syncthreads();
+        if (share) return;
+        const float base2 = to[16 * kO * 64], low = fminf(base, base2);
+        const float f = joined(low, base), f2 = joined(low, base2);
+        const float of = f * kPower<-kShared>, of2 = f2 * kPower<-kShared>;
+        base = low;
+        l = l * f + to[(16 * kO + 1) * 64] * f2;
+        for (int x = 0; x < 16 * kO; ++x) o[x / 16][x % 16] = o[x / 16][x % 16] * of + to[x * 64] * of2;
+    }
+    if (!real) return;
+    if (part.splits > 1) {
+        const uint64_t to = ((static_cast<uint64_t>(h) * part.units + u) * part.splits + split) * kRowTile + (r - r0);
+        for (int e = 0; e < kO; ++e)
+            for (int x = 0; x < 4; ++x)
+                *reinterpret_cast<f32x4*>(part.o + to * D + 32 * e + 8 * x + 4 * half) =
+                    f32x4{o[e][4 * x], o[e][4 * x + 1], o[e][4 * x + 2], o[e][4 * x + 3]} * kPower<kShared - kPartDown>;
+        if (half == 0) {
+            part.ml[2 * to] = base;
+            part.ml[2 * to + 1] = l;
+        }
+        return;
+    }
+    const float inv = l == 0.0f ? 0.0f : 1.0f / l * kPower<kShared>;
+    const uint32_t qh = h * a.group + static_cast<uint32_t>(r % G);
+    T* out = reinterpret_cast<T*>(a.out) + static_cast<uint64_t>(sq.row0 + qi) * a.o_row + qh * a.o_head;
+    for (int e = 0; e < kO; ++e)
+        for (int x = 0; x < 4; ++x) {
+            typedef T T4 __attribute__((ext_vector_type(4)));
+            T4 y;
+            for (int k = 0; k < 4; ++k) y[k] = static_cast<T>(l == 0.0f ? 0.0f : o[e][4 * x + k] * inv);
+            *reinterpret_cast<T4*>(out + 32 * e + 8 * x + 4 * half) = y;
+        }
+    if (half == 0 && a.lse) a.lse[static_cast<uint64_t>(qh) * a.seq.rows + sq.row0 + qi] = lse_of(base, l);
+}
+
+// rows_kernel's shares joined: D / 4 lanes a row, this many rows a workgroup.
+constexpr uint32_t join_rows(uint32_t dim) { return 1024 / dim; }
+template <int QT, int D>
+__global__ __launch_bounds__(256) void join_rows_kernel(PagedDev a, PagedPart part, int few) {
+    constexpr uint32_t kLanes = D / 4, kRows = join_rows(D);
+    const uint32_t blocks = part.rows / kRows, h = blockIdx.x % a.heads, b = blockIdx.x / a.heads % blocks;
+    const uint32_t u = blockIdx.x / a.heads / blocks;
+    RowTile rt;
+    if (!find_tile(a, u, few, static_cast<int>(part.rows), threadIdx.x % 64, &rt)) return;
+    const Seq sq = seq_of(a.seq, rt.seq, a.max_rows);
+    const uint32_t mine = b * kRows + threadIdx.x / kLanes, d = threadIdx.x % kLanes * 4;
+    const uint32_t r = static_cast<uint32_t>(rt.tile) * part.rows + mine;
+    if (r >= static_cast<uint32_t>(sq.rows) * a.group) return;
+    const uint64_t at = (static_cast<uint64_t>(h) * part.units + u) * part.splits * part.rows + mine;
+    float base = kInf, sum = 0.0f;
+    for (uint32_t s = 0; s < part.splits; ++s)
+        base = fminf(base, part.ml[2 * (at + static_cast<uint64_t>(part.rows) * s)]);
+    f32x4 o = {};
+    for (uint32_t s = 0; s < part.splits; ++s) {
+        const uint64_t x = at + static_cast<uint64_t>(part.rows) * s;
+        const float f = joined(base, part.ml[2 * x]);
+        sum += part.ml[2 * x + 1] * f;
+        o += *reinterpret_cast<const f32x4*>(part.o + x * D + d) * (f * kPower<-kJoinDown>);
+    }
+    write_row<QT>(a, sq.row0 + r / a.group, h * a.group + r % a.group, d, o, base, sum, kPower<-kPartDown - kJoinDown>);
 }
 
 uint32_t clears(const PagedDev& a) { return a.clear && a.seq.starts ? kClear : 0; }
@@ -728,33 +1037,72 @@ uint64_t round256(uint64_t x) { return (x + 255) & ~255ull; }
 struct Plan {
     bool few, many;                // sequences of few rows are looked for; of more
     uint32_t units, target, rows;  // decode_kernel: units a head at most, aimed at, rows of one
-    uint64_t ml, plan, bytes;      // offsets in the workspace (partial outputs first), all of it
+    uint64_t ml, plan;             // offsets in the workspace (partial outputs first)
+    int ks;                        // rows_kernel: shares of a tile's slots among a workgroup's waves
+    uint32_t tiles, splits;        // row tiles a head at most, shares of the slots
+    uint64_t rows_ml, bytes;       // the two kernels follow each other in the same workspace; all of it
 };
-Plan plan_of(const PagedDev& a, uint32_t dim) {
+constexpr uint64_t kHalf = 6;
+constexpr uint32_t kMaxShares = 64;     // of many rows
+Plan plan_of(const PagedDev& a, uint32_t dim, int cache_dtype) {
     Plan p{};
     const uint64_t most = static_cast<uint64_t>(a.max_rows) * a.group;
     p.few = a.seq.paged && (!a.seq.each || most <= kFew);
     p.many = !a.seq.paged || most > kFew;
+    // tiles of `step` slots that `rows` rows can see: all, or the window, the rows before the last and the sinks, rounded
+    // to tiles apart
+    auto tiles_for = [&](uint64_t rows, uint64_t step) {
+        uint64_t slots = a.seq.max_len;
+        if (a.window)
+            slots = std::min<uint64_t>(slots, static_cast<uint64_t>(a.window) + std::min<uint64_t>(a.max_rows, rows) +
+                                                  a.sinks + 4 * step);
+        return (slots + step - 1) / step;
+    };
     if (p.few) {
         p.rows = static_cast<uint32_t>(std::min<uint64_t>(kFew, most));
         p.target = (kUnits + a.heads - 1) / a.heads;
-        // tiles that a sequence can have: all, or the window, the rows before its last and the sinks, rounded to tiles apart
-        uint64_t tiles = a.seq.max_len;
-        if (a.window) tiles = std::min<uint64_t>(tiles, static_cast<uint64_t>(a.window) + kFew + a.sinks + 4 * kStep);
-        tiles = (tiles + kStep - 1) / kStep;
-        const uint64_t each = std::max<uint64_t>(1, (tiles + kLeast - 1) / kLeast);
+        const uint64_t each = std::max<uint64_t>(1, (tiles_for(kFew, kStep) + kLeast - 1) / kLeast);
         p.units = static_cast<uint32_t>(std::min<uint64_t>(static_cast<uint64_t>(a.seq.seqs) + p.target, a.seq.seqs * each));
         const uint64_t rows = static_cast<uint64_t>(a.heads) * p.units * p.rows;
         p.ml = round256(rows * dim * 4);
         p.plan = p.ml + round256(rows * 8);
         p.bytes = p.plan + round256(8ull * a.seq.seqs);
     }
+    if (p.many) {
+        // The least time, in tenths of the 2 us that a tile takes a workgroup of 128 rows (64 rows: kHalf): as many
+        // workgroups as fit run at the speed of one, and a share costs four tiles' time for its start and end, and the
+        // passage of its outputs through memory.
+        const uint64_t fit = 256 * (dim == 64 && cache_dtype != PKV_FP8 ? 3 : 2);
+        uint64_t least = ~0ull;
+        for (int ks = 1; ks <= 2; ++ks) {
+            const uint64_t rt = row_tile(ks);
+            const uint64_t row_tiles = std::min((static_cast<uint64_t>(a.seq.rows) * a.group + rt - 1) / rt + a.seq.seqs,
+                                                a.seq.seqs * ((most + rt - 1) / rt));
+            const uint64_t groups = a.heads * row_tiles, tiles = tiles_for(rt, 64);
+            for (uint32_t n = 1; n <= kMaxShares && (n == 1 || n * 4 <= tiles); ++n) {
+                const uint64_t rounds = (groups * n + fit - 1) / fit;
+                const uint64_t cost = rounds * ((tiles + n - 1) / n + (n == 1 ? 2 : 4)) * (ks == 1 ? 10 : kHalf) +
+                                      (n == 1 ? 0 : groups * rt * dim * 8 * n / 800000);
+                if (cost < least) {
+                    least = cost;
+                    p.splits = n;
+                    p.ks = ks;
+                    p.tiles = static_cast<uint32_t>(row_tiles);
+                }
+            }
+        }
+        if (p.splits > 1) {
+            const uint64_t rows = static_cast<uint64_t>(a.heads) * p.tiles * p.splits * row_tile(p.ks);
+            p.rows_ml = round256(rows * dim * 4);
+            p.bytes = std::max(p.bytes, p.rows_ml + round256(rows * 8));
+        }
+    }
     return p;
 }
 
 template <int CT, int QT, int D, bool PAGED>
 int attend_typed(const PagedDev& a, uint8_t* ws, hipStream_t st) {
-    const Plan p = plan_of(a, D);
+    const Plan p = plan_of(a, D, CT);
     if constexpr (PAGED)
         if (p.few) {
             const PagedPart part{reinterpret_cast<float*>(ws), reinterpret_cast<float*>(ws + p.ml),
@@ -763,8 +1111,14 @@ int attend_typed(const PagedDev& a, uint8_t* ws, hipStream_t st) {
             if (p.units > a.seq.seqs) join_kernel<QT, D><<<a.seq.seqs * a.heads * p.rows, 256, 0, st>>>(a, part);
         }
     if (p.many) {
-        const uint32_t work = static_cast<uint32_t>((static_cast<uint64_t>(a.seq.rows) * a.heads * a.group + 3) / 4);
-        row_kernel<CT, QT, D, PAGED><<<work + (p.few ? 0 : clears(a)), 256, 0, st>>>(a, work, p.few);
+        const PagedPart part{reinterpret_cast<float*>(ws), reinterpret_cast<float*>(ws + p.rows_ml), nullptr, p.tiles, 0,
+                             row_tile(p.ks), p.splits};
+        const int few = PAGED && p.few ? kFew : 0;
+        const uint32_t grid = a.heads * p.tiles * p.splits + (p.few ? 0 : clears(a));
+        if (p.ks == 2) rows_kernel<CT, QT, D, PAGED, 2><<<grid, 256, 0, st>>>(a, part, few);
+        else rows_kernel<CT, QT, D, PAGED, 1><<<grid, 256, 0, st>>>(a, part, few);
+        if (p.splits > 1)
+            join_rows_kernel<QT, D><<<a.heads * p.tiles * (part.rows / join_rows(D)), 256, 0, st>>>(a, part, few);
     }
     return hipGetLastError();
 }
@@ -795,15 +1149,23 @@ int launch_rows(const PagedRowsDev& r, uint32_t dim, int cache_dtype, int dtype,
 
 }  // namespace
 
-bool paged_fits(const PagedDev& a, uint32_t dim, int) {
-    const Plan p = plan_of(a, dim);
-    uint64_t most = 0;
+// The launches of attend_typed: threads along x stay below 2^32.
+bool paged_fits(const PagedDev& a, uint32_t dim, int cache_dtype) {
+    const uint64_t most = static_cast<uint64_t>(a.heads) * (static_cast<uint64_t>(a.seq.rows) * a.group / 64 + a.seq.seqs);
+    if (most >= 1u << 28) return false;     // what plan_of counts in 32 bits
+    const Plan p = plan_of(a, dim, cache_dtype);
+    uint64_t blocks = 0;
     if (p.few)
-        most = std::max(static_cast<uint64_t>(a.heads) * p.units, static_cast<uint64_t>(a.seq.seqs) * a.heads * p.rows);
-    return most < (1u << 24) - kClear && (!p.many || static_cast<uint64_t>(a.seq.rows) * a.heads * a.group < 1u << 25);
+        blocks = std::max(static_cast<uint64_t>(a.heads) * p.units, static_cast<uint64_t>(a.seq.seqs) * a.heads * p.rows);
+    if (p.many) {
+        const uint64_t tiles = static_cast<uint64_t>(a.heads) * p.tiles;
+        blocks = std::max(blocks, tiles * p.splits);
+        if (p.splits > 1) blocks = std::max<uint64_t>(blocks, tiles * (row_tile(p.ks) / join_rows(dim)));
+    }
+    return blocks < (1u << 24) - kClear;
 }
 
-uint64_t paged_workspace(const PagedDev& a, uint32_t dim, int) { return plan_of(a, dim).bytes; }
+uint64_t paged_workspace(const PagedDev& a, uint32_t dim, int cache_dtype) { return plan_of(a, dim, cache_dtype).bytes; }
 
 int launch_paged(const PagedDev& a, uint32_t dim, int cache_dtype, int dtype, uint8_t* ws, void* stream) {
     hipStream_t st = static_cast<hipStream_t>(stream);
