@@ -189,7 +189,7 @@ __device__ inline float element(const uint8_t* p, const uint8_t* scales, uint64_
 // Nobody's rows, before the first sequence's and behind the last's, to 0: the
 // workgroups behind `work`, kClear of them.
 constexpr uint32_t kClear = 64;
-template <int QT, int D>
+template <int QT, int D, int THREADS = 256>
 __device__ void clear_rows(const PagedDev& a, uint32_t block) {
     using T = typename Elem<QT>::T;
     const int rows = static_cast<int>(a.seq.rows), heads = static_cast<int>(a.heads * a.group);
@@ -200,7 +200,7 @@ __device__ void clear_rows(const PagedDev& a, uint32_t block) {
     const int rest = first + rows - last;
     for (int x = static_cast<int>(block); x < rest; x += kClear) {
         T* out = reinterpret_cast<T*>(a.out) + static_cast<uint64_t>(x < first ? x : last + x - first) * a.o_row;
-        for (int y = static_cast<int>(threadIdx.x); y < heads * (D / 8); y += 256)
+        for (int y = static_cast<int>(threadIdx.x); y < heads * (D / 8); y += THREADS)
             *reinterpret_cast<u32x4*>(out + static_cast<uint64_t>(y / (D / 8)) * a.o_head + y % (D / 8) * 8) = u32x4{};
     }
 }
@@ -682,79 +682,145 @@ __device__ inline bool find_tile(const PagedDev& a, uint32_t u, int64_t few, int
     return true;
 }
 
-// Staged's tiles from pages, or (PAGED false) from packed rows.  16-bit rows go
-// from memory to LDS without registers; a wave's 1,024 bytes lie in one page.
+// Staged's tiles from pages, or (PAGED false) from packed rows, a side at a time
+// by the four waves of a group.  16-bit rows go from memory to LDS without
+// registers; a wave's 1,024 bytes lie in one page.
 template <int CT, int D, bool PAGED>
 struct PageStage : Staged<CT, D> {
     using L = Staged<CT, D>;
     using L::kRow, L::kPieces, L::kKeyBytes, L::kCopies, L::kCopyRows, L::kCopyStep, L::turn, L::key_at, L::value_at, L::code_slot;
     static constexpr int kHeld = CT == PKV_FP8 ? D / 64 : 1;   // 16 codes a register
-    u32x4 k[kHeld], v[kHeld];                                  // 8-bit codes on their way
-    uint32_t ks, vs;
+    struct Side {
+        u32x4 codes[kHeld];                                    // 8-bit codes on their way
+        uint32_t scale;
+    };
 
-    // Start a tile on its way.  head: elements to the head's first page (packed rows: kp, vp are its row 0); slots past
-    // `last` read the last one.
-    __device__ void fetch(const PagedDev& a, uint32_t lds, const uint8_t* kp, const uint8_t* vp, uint64_t head, int words,
-                          int slot, int last) {
-        const uint32_t lane = threadIdx.x % 64, wave = __builtin_amdgcn_readfirstlane(threadIdx.x / 64);
+    // A side's copies (16 bits): LDS place of the wave's part, and the lane's offset from the first row that it copies a
+    // piece of.  turn() of the row is the same for all of a lane's copies.
+    struct Copies {
+        uint32_t to, off, stride;
+    };
+    template <bool VALUES>
+    __device__ static Copies copies(const PagedDev& a, uint32_t t) {
+        const uint32_t lane = t % 64, wave = __builtin_amdgcn_readfirstlane(t / 64), row = kCopyRows * wave + lane / kPieces;
+        Copies c;
+        c.stride = 2 * static_cast<uint32_t>(VALUES ? a.v_slot : a.k_slot);
+        c.to = (VALUES ? kKeyBytes : 0) + kCopyRows * wave * kRow;
+        c.off = lane / kPieces * c.stride + (lane % kPieces ^ turn(row, VALUES)) * 16;
+        return c;
+    }
+    // Where the rows that copy x takes of the tile at `slot` start: of the head's pages (rows: the head's packed row 0).
+    template <bool VALUES>
+    __device__ static const uint8_t* copy_from(const PagedDev& a, const uint8_t* rows, uint64_t head, int words, int slot,
+                                               int last, uint32_t stride, int x, uint32_t wave) {
+        const int r = kCopyStep * x + kCopyRows * static_cast<int>(wave);
+        if constexpr (PAGED) {
+            const int start = piece_start(slot, r / 16, last);
+            return (VALUES ? a.v : a.k) + 2 * piece_at(a, words, r / 16, start, head) + r % 16 * stride;
+        } else {
+            return rows + static_cast<uint64_t>(slot + r) * stride;
+        }
+    }
+    // Start a side of a tile on its way to the tile at `lds`.  head: elements to the head's first page; rows: the head's
+    // packed row 0 (PAGED false); slots past `last` read the last one.  t: the thread in its group.
+    template <bool VALUES>
+    __device__ static void fetch(Side& s, const Copies& c, const PagedDev& a, uint32_t lds, const uint8_t* rows,
+                                 uint64_t head, int words, int slot, int last, uint32_t t) {
+        const uint32_t lane = t % 64, wave = __builtin_amdgcn_readfirstlane(t / 64);
+        const uint8_t* from = VALUES ? a.v : a.k;
         if constexpr (CT == PKV_FP8) {
             const int start = piece_start(slot, wave, last);
             const uint64_t e = piece_at(a, words, wave, start, head) +
-                               static_cast<uint32_t>(min(static_cast<int>(code_slot(threadIdx.x) - 16 * wave), last - start)) * D;
-            const uint32_t b = threadIdx.x % 4;
-            for (int x = 0; x < kHeld; ++x) {
-                k[x] = *reinterpret_cast<const u32x4*>(a.k + e + D / 4 * b + 16 * x);
-                v[x] = *reinterpret_cast<const u32x4*>(a.v + e + D / 4 * b + 16 * x);
-            }
-            ks = a.ks[e / 32 + (D == 128 ? b : b / 2)];
-            vs = a.vs[e / 32 + (D == 128 ? b : b / 2)];
+                               static_cast<uint32_t>(min(static_cast<int>(code_slot(t) - 16 * wave), last - start)) * D;
+            const uint32_t b = t % 4;
+            for (int x = 0; x < kHeld; ++x) s.codes[x] = *reinterpret_cast<const u32x4*>(from + e + D / 4 * b + 16 * x);
+            s.scale = (VALUES ? a.vs : a.ks)[e / 32 + (D == 128 ? b : b / 2)];
         } else {
-            // turn() of the row is the same for all of a lane's copies
-            const uint32_t row = kCopyRows * wave + lane / kPieces, piece = lane % kPieces;
-            const uint32_t kc = (piece ^ turn(row, false)) * 16, vc = (piece ^ turn(row, true)) * 16;
+            const int row = kCopyRows * static_cast<int>(wave) + static_cast<int>(lane / kPieces);
             for (int x = 0; x < kCopies; ++x) {
-                const uint32_t to = lds + (kCopyStep * x + kCopyRows * wave) * kRow;
-                const int j = min(slot + kCopyStep * x + static_cast<int>(row), last);
-                if constexpr (PAGED) {
-                    const int p = (kCopyStep * x + kCopyRows * wave) / 16, start = piece_start(slot, p, last);
-                    const uint64_t e = 2 * piece_at(a, words, p, start, head);
-                    const uint32_t off = static_cast<uint32_t>(j - start) * static_cast<uint32_t>(a.k_slot) * 2;
-                    copy_to_lds(to, a.k + e, off + kc);
-                    copy_to_lds(to + kKeyBytes, a.v + e, off + vc);
-                } else {
-                    const uint32_t i = static_cast<uint32_t>(j - slot);
-                    copy_to_lds(to, kp + 2 * static_cast<uint64_t>(slot) * a.k_slot, 2 * i * static_cast<uint32_t>(a.k_slot) + kc);
-                    copy_to_lds(to + kKeyBytes, vp + 2 * static_cast<uint64_t>(slot) * a.v_slot,
-                                2 * i * static_cast<uint32_t>(a.v_slot) + vc);
-                }
+                const uint8_t* at = copy_from<VALUES>(a, rows, head, words, slot, last, c.stride, x, wave);
+                // the piece may start in front of the tile's part, and the row lie in front of copy_from's
+                const int r = kCopyStep * x + row, first = PAGED ? piece_start(slot, r / 16, last) + r % 16 : slot + r;
+                const int32_t back = (min(slot + r, last) - first) * static_cast<int32_t>(c.stride);
+                copy_row_to_lds(lds + c.to + kCopyStep * kRow * x, at + c.off + static_cast<int64_t>(back));
             }
         }
     }
     // What fetch started, into LDS (a barrier follows).
-    __device__ void land(uint8_t* lds) {
+    template <bool VALUES>
+    __device__ static void land(const Side& s, uint8_t* lds, uint32_t t) {
         if constexpr (CT == PKV_FP8) {
-            const uint32_t row = code_slot(threadIdx.x), b = threadIdx.x % 4;
+            const uint32_t row = code_slot(t), b = t % 4;
             for (int w = 0; w < D / 32; ++w) {
-                const int r = w / 2, c = w % 2 * 2;
-                const uint32_t k0 = k[r][c], k1 = k[r][c + 1], v0 = v[r][c], v1 = v[r][c + 1];
-                *reinterpret_cast<u32x4*>(lds + key_at(row, b * (D / 32) + w)) = expand8(k0, k1, block_scale(ks));
-                *reinterpret_cast<u32x4*>(lds + value_at(row, b * (D / 32) + w)) = expand8(v0, v1, block_scale(vs));
+                const uint32_t lo = s.codes[w / 2][w % 2 * 2], hi = s.codes[w / 2][w % 2 * 2 + 1], piece = b * (D / 32) + w;
+                *reinterpret_cast<u32x4*>(lds + (VALUES ? value_at(row, piece) : key_at(row, piece))) =
+                    expand8(lo, hi, block_scale(s.scale));
             }
+            asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
         } else {
             copies_done();
         }
     }
+    // Infinities and NaN among a staged tile's values to 0, by the group's 256 threads; true if this one had any.
+    __device__ static bool clean(uint8_t* lds, uint32_t t) {
+        bool odd = false;
+        for (uint32_t x = t; x < kKeyBytes / 16; x += 256) {
+            u32x4* p = reinterpret_cast<u32x4*>(lds + kKeyBytes) + x;
+            u32x4 w = *p;
+            bool any = false;
+            for (int y = 0; y < 4; ++y) {
+                const uint32_t z = w[y];
+                any |= nonfinite2<mat_type(CT)>(z);
+                w[y] = finite_or_0<mat_type(CT)>(z);
+            }
+            if (any) *p = w;
+            odd |= any;
+        }
+        return odd;
+    }
 };
 
-// Rows in tiles of 128, 32 a wave, against tiles of 64 slots staged through LDS
-// in two buffers, one barrier a tile:
+// copy_to_lds among products, free to pass LDS reads: between two meetings
+// nothing reads what a copy overwrites.  MAYBE: only if `brings`, the same in all
+// lanes, of which all are at work (a branch would part the products).
+template <bool MAYBE>
+__device__ inline void start_copy(uint32_t to, const uint8_t* from, uint32_t offset, int brings) {
+    uint32_t m0;
+    if constexpr (MAYBE)
+        asm volatile("s_mov_b32 %0, m0\n\ts_mov_b32 m0, %1\n\ts_cmp_lg_u32 %4, 0\n\ts_cselect_b64 exec, -1, 0\n\t"
+                     "global_load_lds_dwordx4 %2, %3\n\ts_mov_b64 exec, -1\n\ts_mov_b32 m0, %0"
+                     : "=&s"(m0)
+                     : "s"(to), "v"(offset), "s"(from), "s"(__builtin_amdgcn_readfirstlane(brings))
+                     : "scc");
+    else
+        asm volatile("s_mov_b32 %0, m0\n\ts_mov_b32 m0, %1\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %2, %3\n\ts_mov_b32 m0, %0"
+                     : "=&s"(m0)
+                     : "s"(to), "v"(offset), "s"(from));
+}
+
+// The waves of a workgroup meet; nothing moves across, no copy is waited for.
+__device__ inline void meet() {
+    __builtin_amdgcn_sched_barrier(0);
+    asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
+    __builtin_amdgcn_sched_barrier(0);
+}
+
+// Rows in tiles of 256 (KS 1), 32 a wave, against tiles of 64 slots staged
+// through LDS in two buffers:
 //   S^T = K Q^T (32x32 tiles; a lane holds one query row and half of each
 //   piece's slots), softmax in registers, O^T += V^T P^T with the rounded
 //   weights straight from those registers.
+// The workgroup's waves are two groups of four, one of each on a SIMD, that take
+// turns: while one has the matrix cores, O of the tile before and S of the next,
+// the other has the vector units for its softmax, and they meet between.  Two
+// workgroups of four waves each, which meet nobody, did one after the other (964
+// TFLOP/s for prompts of 8,192, 6,298 and 3,900 rows of 32 heads of 128, with
+// the matrix cores busy 44 % of the cycles and the vector units 47 %).
 // Weights are rounded once to the type of the products (f16 queries over 8-bit
 // codes: two bf16 terms), while their sum is that of the unrounded ones.
-// KS 2: a workgroup has 64 rows and two waves share a tile's slots, for calls
-// whose 128-row tiles would not fill the chip.
+// KS 2, 4: 128, 64 rows; the groups take the slots' tiles in turn, at 4 also two
+// waves of a group the halves of a tile, for calls whose larger row tiles would
+// not fill the chip.
 //
 // A weight 0 times an infinity or NaN would be NaN in rows that do not see the
 // slot.  The loop does not look for those: an output that is not finite sends
@@ -762,20 +828,38 @@ struct PageStage : Staged<CT, D> {
 // staged values and each added afterwards to the rows that see it.  Where the
 // sums of finite values are not finite either, a third time with smaller
 // weights (kDown).
+constexpr int rows_of_tile(int ks) { return 256 / ks; }
+
+// The order of V operands of two reads and K operands of one, PRODUCTS products
+// each: the reads run kAhead operands ahead of the products (left to itself the
+// compiler reads an operand, waits for it and multiplies).
+constexpr int kAhead = 4;
+template <int V, int K, int PRODUCTS>
+__device__ inline void reads_ahead() {
+    auto reads = [](int n) { return n < V ? 2 : n < V + K ? 1 : 0; };
+    static_assert(V + K >= kAhead && (V == 0 || V >= kAhead) && (K == 0 || K >= kAhead), "operands ahead are of one kind");
+    __builtin_amdgcn_sched_group_barrier(0x100, kAhead * (V ? 2 : 1), 0);
+#pragma unroll
+    for (int i = 0; i < V + K; ++i) {
+        __builtin_amdgcn_sched_group_barrier(0x008, PRODUCTS, 0);
+        if (reads(i + kAhead) == 2) __builtin_amdgcn_sched_group_barrier(0x100, 2, 0);
+        if (reads(i + kAhead) == 1) __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);
+    }
+}
 template <int CT, int QT, int D, bool PAGED, int KS>
-__global__ __launch_bounds__(256, (query_terms(CT, QT) * D >= 256 ? 1 : 2)) void rows_kernel(PagedDev a, PagedPart part,
-                                                                                            int few) {
-    __shared__ __align__(16) uint8_t lds[2 * Staged<CT, D>::kBytes];
+__global__ __launch_bounds__(512, 2) void rows_kernel(PagedDev a, PagedPart part, int few) {
     using T = typename Elem<QT>::T;
     using St = PageStage<CT, D, PAGED>;
-    constexpr int MT = mat_type(CT), kU = St::kSlots / 32 / KS, kO = D / 32;   // kU: 32-slot pieces a wave takes of a tile
-    constexpr int NP = query_terms(CT, QT), kRowTile = row_tile(KS);
+    constexpr int MT = mat_type(CT), kU = KS == 4 ? 1 : 2, kO = D / 32;   // kU: 32-slot pieces a wave takes of a tile
+    constexpr int NP = query_terms(CT, QT), kRowTile = rows_of_tile(KS);
+    constexpr bool kTurns = KS > 1;                               // a group has tiles of its own
+    __shared__ __align__(16) uint8_t lds[(kTurns ? 4 : 2) * St::kBytes];   // two tiles a group, or of both
     const uint32_t work_blocks = a.heads * part.units * part.splits;
-    if (blockIdx.x >= work_blocks) return clear_rows<QT, D>(a, blockIdx.x - work_blocks);
+    if (blockIdx.x >= work_blocks) return clear_rows<QT, D, 512>(a, blockIdx.x - work_blocks);
     const uint32_t lane = threadIdx.x % 64, wave_id = __builtin_amdgcn_readfirstlane(threadIdx.x / 64);
-    const uint32_t n = lane % 32, half = lane / 32;
-    const uint32_t wave = wave_id % (4 / KS);                     // its 32 rows
-    const int share = static_cast<int>(wave_id / (4 / KS)) * 32 * kU;   // its slots of a tile: share .. + 32 kU
+    const uint32_t n = lane % 32, half = lane / 32, group = wave_id / 4, gt = threadIdx.x % 256;
+    const uint32_t wave = KS == 1 ? wave_id : wave_id % (8 / KS);         // its 32 rows
+    const int share = KS == 4 ? static_cast<int>(wave_id / 2 % 2) * 32 : 0;   // its slots of a tile: share .. + 32 kU
     // heads fastest, so that a head's workgroups share an XCD's L2 where the heads are a multiple of 8
     const uint32_t h = blockIdx.x % a.heads, split = blockIdx.x / a.heads % part.splits, u = blockIdx.x / a.heads / part.splits;
     RowTile rt;
@@ -787,6 +871,11 @@ __global__ __launch_bounds__(256, (query_terms(CT, QT) * D >= 256 ? 1 : 2)) void
     const Tiles tl = tiles_of(a, pos0, pos1, St::kSlots);
     const int per = (tl.count + static_cast<int>(part.splits) - 1) / static_cast<int>(part.splits);
     const int t0 = static_cast<int>(split) * per, t1 = min(t0 + per, tl.count);
+    // the group's tiles: t0 + first, + step, ..; as many steps for both
+    constexpr int kEvery = kTurns ? 2 : 1;
+    const int first = t0 + (kTurns ? static_cast<int>(group) : 0), steps = max(t1 - t0 + kEvery - 1, 0) / kEvery;
+    auto tile = [&](int i) { return first + kEvery * i; };
+    auto slot_of = [&](int i) { return tl.slot(tile(i), St::kSlots); };
 
     const int w0 = r0 + 32 * static_cast<int>(wave), w1 = min(w0 + 31, last), r = w0 + static_cast<int>(n);
     const bool real = r <= last;
@@ -803,178 +892,318 @@ __global__ __launch_bounds__(256, (query_terms(CT, QT) * D >= 256 ? 1 : 2)) void
     const uint8_t* kp = PAGED ? nullptr : a.k + 2 * (static_cast<uint64_t>(sq.row0) * a.k_slot + head);
     const uint8_t* vp = PAGED ? nullptr : a.v + 2 * (static_cast<uint64_t>(sq.row0) * a.v_slot + h * a.v_head);
 
-    const uint32_t at = static_cast<uint32_t>(reinterpret_cast<uintptr_t>((LdsByte*)lds));
-    float base, l;
-    f32x16 o[kO];
-    St st;
-    // the words of tile t's pages (past the last: the last's again, unused)
-    auto pages = [&](int t) {
+    uint8_t* const mine = lds + (kTurns ? group * 2 * St::kBytes : 0);
+    const bool brings = kTurns || group == 0;      // the group that copies the tiles that this one reads
+    const uint32_t at = static_cast<uint32_t>(reinterpret_cast<uintptr_t>((LdsByte*)mine)), w4 = wave_id % 4;
+    float base = kInf, l = 0.0f;
+    f32x16 o[kO], sc[kU];
+    u32x4 pt[NP][2 * kU];
+    typename St::Side ks, vs;
+    const typename St::Copies kc = St::template copies<false>(a, gt), vc = St::template copies<true>(a, gt);
+    // LDS addresses of the lane's operands in the first tile: keys of slot n, values as Staged::values16 reads them
+    constexpr int kX = D / 16;
+    uint32_t key_read[kX], value_read[kO][2];
+    for (int x = 0; x < kX; ++x) key_read[x] = at + share * St::kRow + St::key_at(n, 2 * x + half);
+    for (int e = 0; e < kO; ++e)
+        for (int y = 0; y < 2; ++y) {
+            const uint32_t s = lane % 16, row = lane / 32 * 4 + s / 4 + 8 * y;
+            value_read[e][y] = at + share * St::kRow + St::value_at(row, 4 * e + lane / 16 % 2 * 2 + s % 4 / 2) + s % 2 * 8;
+        }
+    // the words of step i's pages (past the last tile: the last's again, unused)
+    auto pages = [&](int i) {
         if constexpr (!PAGED) return 0;
-        else return read_pages<4>(a.seq, table, tl.slot(min(t, t1 - 1), St::kSlots), tl.high - 1, lane);
+        else return read_pages<4>(a.seq, table, tl.slot(min(tile(i), t1 - 1), St::kSlots), tl.high - 1, lane);
     };
-    auto missing = [&](int words) { return PAGED ? no_page<4>(a.seq, words) : 0u; };
-    auto fetch = [&](int t, int words) {
-        st.fetch(a, at + ((t - t0) & 1) * St::kBytes, kp, vp, head, words, tl.slot(t, St::kSlots), tl.high - 1);
+    auto there = [&](int i) { return tile(i) < t1; };
+    auto buffer = [&](int i) { return static_cast<uint32_t>(i & 1) * St::kBytes; };
+    auto fetch_keys = [&](int i, int words) {
+        if (brings && there(i))
+            St::template fetch<false>(ks, kc, a, at + buffer(i), kp, head, words, slot_of(i), tl.high - 1, gt);
     };
-    // no row of the wave sees any of the tile
-    auto skip = [&](int slot) {
-        return slot + share >= wt.high ||
-               (slot + share + 32 * kU <= wt.low && static_cast<uint32_t>(slot + share) >= a.sinks);
+    auto fetch_values = [&](int i, int words) {
+        if (brings && there(i))
+            St::template fetch<true>(vs, vc, a, at + buffer(i), vp, head, words, slot_of(i), tl.high - 1, gt);
+    };
+    auto land_keys = [&](int i) { if (brings && there(i)) St::template land<false>(ks, mine + buffer(i), gt); };
+    auto land_values = [&](int i) { if (brings && there(i)) St::template land<true>(vs, mine + buffer(i), gt); };
+    // some row of the wave sees some of step i's tile
+    auto sees = [&](int i) {
+        if (!there(i)) return false;
+        const int slot = slot_of(i) + share;
+        return slot < wt.high && (slot + 32 * kU > wt.low || static_cast<uint32_t>(slot) < a.sinks);
     };
     float lift = kLift<MT>;
-    for (int pass = 0;; ++pass) {
-        base = kInf;
-        l = 0.0f;
-        for (int e = 0; e < kO; ++e) o[e] = f32x16{};
-        int words = 0, next = 0;
-        if (t0 < t1) {
-            words = pages(t0);
-            next = pages(t0 + 1);
-            fetch(t0, words);
-            st.land(lds);
+    // none: 16-slot pieces of the tile on no page; all: every row of the wave sees all of it
+    auto softmax = [&](int i, uint32_t none, auto all) __attribute__((always_inline)) {
+        const int slot = decltype(all)::value ? 0 : slot_of(i) + share;
+        if (!decltype(all)::value && !all_visible(a, wpos0, wpos1, slot, slot + 32 * kU - 1)) {
+            const int off = pos - slot - 4 * static_cast<int>(half);   // less the register's place: how far back
+            if (static_cast<uint32_t>(slot) >= a.sinks) {
+                for (int p = 0; p < kU; ++p)
+                    for (int x = 0; x < 16; ++x)
+                        if (!in_reach(a, off, 32 * p + row32(x, 0))) sc[p][x] = -kInf;
+            } else {
+                for (int p = 0; p < kU; ++p)
+                    for (int x = 0; x < 16; ++x)
+                        if (!visible(a, pos, slot + 32 * p + row32(x, half))) sc[p][x] = -kInf;
+            }
         }
-        __syncthreads();
-        for (int t = t0; t < t1; ++t) {
-            uint8_t* buf = lds + ((t - t0) & 1) * St::kBytes;
-            const uint32_t none = missing(words) >> share / 16;
-            if (t + 1 < t1) {
-                words = next;
-                next = pages(t + 2);      // ahead of its tile's copies, which wait for it
-                fetch(t + 1, words);
+        if (PAGED && none)
+            for (int p = 0; p < kU; ++p)
+                for (int x = 0; x < 16; ++x)
+                    if (none >> (share / 16 + 2 * p + x / 8) & 1) sc[p][x] = -kInf;
+        float top = sc[0][0];
+        for (int p = 0; p < kU; ++p)
+            for (int x = 0; x < 16; ++x) top = fmaxf(top, sc[p][x]);
+        top = across32(top, larger);
+        if (__any(__builtin_fmaf(top, a.scale2, base) > lift + kLag<MT>)) {
+            const float low = lower_base(a, lift, base, top), f = joined(low, base);
+            if (low < base) {
+                l *= f;
+                for (int e = 0; e < kO; ++e) o[e] *= f;
+                base = low;
             }
-            const int slot = tl.slot(t, St::kSlots);
-            if (__builtin_expect(pass, 0)) {
-                St::clean(buf);
-                __syncthreads();
-            }
-            if (!skip(slot)) {
-                f32x16 sc[kU];
-                const int mine = slot + share;
-                for (int p = 0; p < kU; ++p) sc[p] = logits32<CT, QT, D>(buf + share * St::kRow, p, q, lane);
-                if (!all_visible(a, wpos0, wpos1, mine, mine + 32 * kU - 1)) {
-                    const int off = pos - mine - 4 * static_cast<int>(half);   // less the register's place: how far back
-                    if (static_cast<uint32_t>(mine) >= a.sinks) {
-                        for (int p = 0; p < kU; ++p)
-                            for (int x = 0; x < 16; ++x)
-                                if (!in_reach(a, off, 32 * p + row32(x, 0))) sc[p][x] = -kInf;
-                    } else {
-                        for (int p = 0; p < kU; ++p)
-                            for (int x = 0; x < 16; ++x)
-                                if (!visible(a, pos, mine + 32 * p + row32(x, half))) sc[p][x] = -kInf;
-                    }
+        }
+        const float from = base == kInf ? 0.0f : base;
+        for (int p = 0; p < kU; ++p)
+            for (int y = 0; y < 2; ++y) {
+                float w[8];
+                for (int x = 0; x < 8; ++x) {
+                    w[x] = __builtin_amdgcn_exp2f(__builtin_fmaf(sc[p][8 * y + x], a.scale2, from));
+                    l += w[x];
                 }
-                if (PAGED && none)
-                    for (int p = 0; p < kU; ++p)
-                        for (int x = 0; x < 16; ++x)
-                            if (none >> (2 * p + x / 8) & 1) sc[p][x] = -kInf;
-                float top = sc[0][0];
-                for (int p = 0; p < kU; ++p)
-                    for (int x = 0; x < 16; ++x) top = fmaxf(top, sc[p][x]);
-                top = across32(top, larger);
-                if (__any(__builtin_fmaf(top, a.scale2, base) > lift + kLag<MT>)) {
-                    const float low = lower_base(a, lift, base, top), f = joined(low, base);
-                    if (low < base) {
-                        l *= f;
-                        for (int e = 0; e < kO; ++e) o[e] *= f;
-                        base = low;
-                    }
-                }
-                const float from = base == kInf ? 0.0f : base;
-                for (int p = 0; p < kU; ++p)
-                    for (int x = 0; x < 16; ++x) {
-                        sc[p][x] = __builtin_amdgcn_exp2f(__builtin_fmaf(sc[p][x], a.scale2, from));
-                        l += sc[p][x];
-                    }
-                // ahead of the other workgroup's softmax while the matrix cores have work
-                __builtin_amdgcn_s_setprio(1);
-                for (int p = 0; p < kU; ++p)
-                    for (int y = 0; y < 2; ++y) {
-                        float w[8];
-                        for (int x = 0; x < 8; ++x) w[x] = sc[p][8 * y + x];
-                        u32x4 pt[NP];
-                        for (int k = 0; k < NP; ++k)
-                            pt[k] = u32x4{pack_term<MT>(w[0], w[1]), pack_term<MT>(w[2], w[3]),
-                                          pack_term<MT>(w[4], w[5]), pack_term<MT>(w[6], w[7])};
-                        for (int e = 0; e < kO; ++e) {
-                            const u32x4 v = St::values16(buf + share * St::kRow, 32 * p + 16 * y, e, lane);
-                            for (int k = NP - 1; k >= 0; --k) o[e] = mma32<MT>(v, pt[k], o[e]);
-                        }
-                    }
+                for (int k = 0; k < NP; ++k)
+                    pt[k][2 * p + y] = u32x4{pack_term<MT>(w[0], w[1]), pack_term<MT>(w[2], w[3]),
+                                             pack_term<MT>(w[4], w[5]), pack_term<MT>(w[6], w[7])};
             }
-            __builtin_amdgcn_s_setprio(0);
-            if (t + 1 < t1) st.land(lds + ((t + 1 - t0) & 1) * St::kBytes);
+    };
+    // O += the values of the tile at `values` weighed, S = the logits of the one at `keys`; among the products copy(0),
+    // copy(1), .. start what is copied meanwhile.
+    auto products = [&](auto weighs, auto scores, uint32_t values, uint32_t keys, auto copy) __attribute__((always_inline)) {
+        constexpr bool W = decltype(weighs)::value, S = decltype(scores)::value;
+        typedef short s16x4 __attribute__((ext_vector_type(4)));
+        typedef __attribute__((address_space(3))) s16x4* Values;
+        typedef const __attribute__((address_space(3))) u32x4* Keys;
+        int next = 0;
+        if constexpr (W) {
+            for (int y = 0; y < 2 * kU; ++y) {
+                for (int e = 0; e < kO; ++e) {
+                    const s16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((Values)(value_read[e][0] + (values + 16 * y * St::kRow)));
+                    const s16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((Values)(value_read[e][1] + (values + 16 * y * St::kRow)));
+                    const u32x2 v0 = __builtin_bit_cast(u32x2, lo), v1 = __builtin_bit_cast(u32x2, hi);
+                    for (int k = NP - 1; k >= 0; --k) o[e] = mma32<MT>(u32x4{v0[0], v0[1], v1[0], v1[1]}, pt[k][y], o[e]);
+                }
+                copy(next++);
+            }
+        }
+        if constexpr (S) {
+            for (int p = 0; p < kU; ++p) sc[p] = f32x16{};
+            for (int x = 0; x < kX; ++x) {
+                for (int p = 0; p < kU; ++p) {
+                    const u32x4 k = *(Keys)(key_read[x] + (keys + 32 * p * St::kRow));
+                    for (int y = NP - 1; y >= 0; --y) sc[p] = mma32<MT>(k, q.q[y][x], sc[p]);
+                }
+                if (kU == 1 || x % 2) copy(next++);
+            }
+        }
+        reads_ahead<W ? 2 * kU * kO : 0, S ? kU * kX : 0, NP>();
+    };
+    using Yes = std::true_type;
+    using No = std::false_type;
+    auto no_copy = [](int) {};
+    static_assert(2 * kU + kX / (kU == 1 ? 1 : 2) >= 2 * St::kCopies, "every copy has its place");
+
+    // Step i of a group: values of i - 1 and logits of i, meanwhile keys of i + 1 and values of i are on their way; meet;
+    // softmax of i, what is on its way waited for; meet.  The second group is a meeting behind; of shared tiles the first
+    // brings them.  What a copy overwrites was last read in front of the last meeting: keys of i - 1, values of i - 2.
+    int words = 0, next = 0;
+    bool have = false;           // weights of the step before
+    auto step = [&](int i) __attribute__((always_inline)) {
+        const uint32_t none = PAGED ? no_page<4>(a.seq, words) : 0;
+        const bool now = sees(i);
+        fetch_keys(i + 1, next);
+        fetch_values(i, words);
+        __builtin_amdgcn_s_setprio(1);
+        if (have) products(Yes(), No(), buffer(i + 1), 0, no_copy);
+        if (now) products(No(), Yes(), 0, buffer(i), no_copy);
+        have = now;
+        __builtin_amdgcn_s_setprio(0);
+        meet();
+        const int ahead = pages(i + 2);
+        if (have) softmax(i, none, No());
+        land_keys(i + 1);
+        land_values(i);
+        words = next;
+        next = ahead;
+        meet();
+    };
+    // The same for a step in the middle: its tile and the next are whole, every row of the wave sees all of it and of the
+    // one before, and its place in LDS is known (ODD: i is odd).
+    auto middle = [&](int i, auto odd) __attribute__((always_inline)) {
+        constexpr uint32_t kHere = decltype(odd)::value ? St::kBytes : 0, kOther = St::kBytes - kHere;
+        const uint32_t none = PAGED ? no_page<4>(a.seq, words) : 0;
+        const int slot = slot_of(i);
+        if constexpr (CT == PKV_FP8) {
+            fetch_keys(i + 1, next);
+            fetch_values(i, words);
+        }
+        __builtin_amdgcn_s_setprio(1);
+        products(Yes(), Yes(), kOther, kHere, [&](int x) {
+            if constexpr (CT != PKV_FP8) {
+                const int y = x % St::kCopies;
+                if (x < St::kCopies)
+                    start_copy<!kTurns>(at + kOther + kc.to + y * St::kCopyStep * St::kRow,
+                               St::template copy_from<false>(a, kp, head, next, slot + kEvery * St::kSlots, tl.high - 1,
+                                                             kc.stride, y, w4), kc.off, brings);
+                else if (x < 2 * St::kCopies)
+                    start_copy<!kTurns>(at + kHere + vc.to + y * St::kCopyStep * St::kRow,
+                               St::template copy_from<true>(a, vp, head, words, slot, tl.high - 1, vc.stride, y, w4),
+                               vc.off, brings);
+            }
+        });
+        __builtin_amdgcn_s_setprio(0);
+        meet();
+        const int ahead = pages(i + 2);
+        softmax(i, none, Yes());
+        land_keys(i + 1);
+        land_values(i);
+        words = next;
+        next = ahead;
+        meet();
+    };
+    for (int e = 0; e < kO; ++e) o[e] = f32x16{};
+    if (steps > 0) {
+        words = pages(0);
+        next = pages(1);
+        fetch_keys(0, words);
+        land_keys(0);
+        // the query is there: else the compiler waits for it at its every use, and for the copies under way with it
+        __builtin_amdgcn_s_waitcnt(0x0f70);   // vmcnt(0)
+        meet();
+        if (group) meet();
+        // middle steps: from an even one on, pairs of them.  Tiles of the list whose slots all rows of the wave see, the one
+        // before too, and whose next one is whole and there
+        const int list = tl.second - tl.first;     // tile t of the list, behind the first ones, starts at slot 64 (t + list)
+        int lo = tl.first, hi = min((wpos0 + 1) / St::kSlots, tl.high / St::kSlots - kEvery) - list;
+        if (a.window)
+            lo = max(lo, static_cast<int>(max(static_cast<int64_t>(wpos1) - a.reach + St::kSlots, static_cast<int64_t>(0)) /
+                                          St::kSlots) - list);
+        hi = min(hi, t1 - kEvery);
+        const int from = w0 <= last && wpos0 >= 0 ? (max(lo - first + kEvery - 1, 0) / kEvery + 2) & ~1 : steps;
+        const int pairs = max(hi - first + kEvery - 1, 0) / kEvery - from;       // may be negative
+        int i = 0;
+        for (; i < min(from, steps); ++i) step(i);
+        if (pairs > 1)
+            for (const int to = from + (pairs & ~1); i < to; i += 2) {
+                middle(i, No());
+                middle(i + 1, Yes());
+            }
+        for (; i < steps; ++i) step(i);
+        if (have) products(Yes(), No(), buffer(steps - 1), 0, no_copy);
+        if (!group) meet();
+    }
+    bool odd = false;
+    for (int e = 0; e < kO; ++e)
+        for (int x = 0; x < 16; ++x) odd |= (__float_as_uint(o[e][x]) & 0x7f800000u) == 0x7f800000u;
+    if (__builtin_expect(__syncthreads_or(odd && real), 0)) {
+        // both sides of step i's tile staged, by all
+        auto stage = [&](int i, int words) {
             __syncthreads();
-        }
-        if (pass < 2) {
-            bool odd = false;
+            fetch_keys(i, words);
+            fetch_values(i, words);
+            land_keys(i);
+            land_values(i);
+            __syncthreads();
+        };
+        auto cleaned = [&](int i) { return brings && there(i) && St::clean(mine + buffer(i), gt); };
+        for (int pass = 1; pass < 3; ++pass) {
+            base = kInf;
+            l = 0.0f;
+            for (int e = 0; e < kO; ++e) o[e] = f32x16{};
+#pragma unroll 1
+            for (int i = 0; i < steps; ++i) {
+                const int words = pages(i);
+                stage(i, words);
+                cleaned(i);
+                __syncthreads();
+                if (sees(i)) {
+                    products(No(), Yes(), 0, buffer(i), no_copy);
+                    softmax(i, PAGED ? no_page<4>(a.seq, words) : 0, No());
+                    products(Yes(), No(), buffer(i), 0, no_copy);
+                }
+            }
+            odd = false;
             for (int e = 0; e < kO; ++e)
                 for (int x = 0; x < 16; ++x) odd |= (__float_as_uint(o[e][x]) & 0x7f800000u) == 0x7f800000u;
             // with the values finite, from a NaN among the logits, as the weights' sum, or past the type's end
-            if (pass) odd &= !__builtin_isnan(across32(l, [](float x, float y) { return x + y; }));
-            const bool again = __syncthreads_or(odd && real);
-            if (!pass && !again) break;
-            if (!pass) continue;
-            if (again && kDown<MT>) {
-                lift -= kDown<MT>;
-                continue;
-            }
+            odd &= !__builtin_isnan(across32(l, [](float x, float y) { return x + y; }));
+            if (!kDown<MT> || pass == 2 || !__syncthreads_or(odd && real)) break;
+            lift -= kDown<MT>;
         }
         // not scaled down: that could make a weight 0
         const float from = base == kInf ? 0.0f : base + (kLift<MT> - lift);
 #pragma unroll 1
-        for (int t = t0; t < t1; ++t) {
-            const int slot = tl.slot(t, St::kSlots), here = pages(t);
-            const uint32_t none = missing(here);
-            uint8_t* buf = lds + ((t - t0) & 1) * St::kBytes;
-            fetch(t, here);
-            st.land(buf);
-            __syncthreads();
-            if (!__syncthreads_or(St::clean(buf))) continue;
-            fetch(t, here);
-            st.land(buf);
-            __syncthreads();
+        for (int i = 0; i < steps; ++i) {
+            const int words = pages(i);
+            const uint32_t none = PAGED ? no_page<4>(a.seq, words) : 0;
+            stage(i, words);
+            if (!__syncthreads_or(cleaned(i))) continue;
+            stage(i, words);
+            if (!there(i)) continue;
+            const uint8_t* buf = mine + buffer(i);
 #pragma unroll 1
             for (int j = share; j < share + 32 * kU; ++j) {
-                const bool sees = visible(a, pos, slot + j) && !(none >> j / 16 & 1);
-                if (!__any(sees)) continue;
+                const bool see = visible(a, pos, slot_of(i) + j) && !(none >> j / 16 & 1);
+                if (!__any(see)) continue;
                 uint32_t hf = half;
                 asm volatile("" : "+v"(hf));   // this rare loop's addresses are not kept over the main one
                 float dot = 0.0f;
                 for (int x = 0; x < Query<CT, QT, D>::kRegs; ++x) {
                     const u32x4 k = *reinterpret_cast<const u32x4*>(buf + St::key_at(j, 2 * x + hf));
                     for (int w = 0; w < 4; ++w)
-                        for (int y = 0; y < Query<CT, QT, D>::kTerms; ++y) dot += dot_word<MT>(k[w], q.q[y][x][w]);
+                        for (int y = 0; y < Query<CT, QT, D>::kTerms; ++y) {
+                            const uint32_t kw = k[w], qw = q.q[y][x][w];
+                            dot += dot_word<MT>(kw, qw);
+                        }
                 }
                 dot += __shfl_xor(dot, 32);
                 const float p = __builtin_amdgcn_exp2f(__builtin_fmaf(dot, a.scale2, from));
                 for (int e = 0; e < kO; ++e)
                     for (int x = 0; x < 16; ++x) {
                         const float v = St::value(buf, j, 32 * e + row32(x, hf));
-                        if (sees && (__float_as_uint(v) & 0x7f800000u) == 0x7f800000u) o[e][x] += p * v;
+                        if (see && (__float_as_uint(v) & 0x7f800000u) == 0x7f800000u) o[e][x] += p * v;
                     }
             }
-            __syncthreads();
         }
-        break;
     }
     l += __shfl_xor(l, 32);
-    constexpr int kShared = KS > 1 ? 1 : 0;   // outputs are 2^-kShared as large from here on
+    constexpr int kShared = KS == 1 ? 0 : KS == 2 ? 1 : 2;   // outputs are 2^-kShared as large from here on
     if constexpr (KS > 1) {
-        // the other share of the slots joins the first: [row block][o, base, l][lane]
-        float* to = reinterpret_cast<float*>(lds) + wave * (16 * kO + 2) * 64 + lane;
-        if (share) {
-            for (int x = 0; x < 16 * kO; ++x) to[x * 64] = o[x / 16][x % 16];
-            to[16 * kO * 64] = base;
-            to[(16 * kO + 1) * 64] = l;
+        // the other shares of the slots join the first: [share][row block][o, base, l][lane]
+        constexpr int kBlocks = 8 / KS, kBlock = (16 * kO + 2) * 64;
+        float* to = reinterpret_cast<float*>(lds) + wave * kBlock + lane;
+        const uint32_t part_of = wave_id / kBlocks;
+        __syncthreads();
+        if (part_of) {
+            float* x = to + (part_of - 1) * kBlocks * kBlock;
+            for (int e = 0; e < 16 * kO; ++e) x[e * 64] = o[e / 16][e % 16];
+            x[16 * kO * 64] = base;
+            x[(16 * kO + 1) * 64] = l;
         }
         __syncthreads();
-        if (share) return;
-        const float base2 = to[16 * kO * 64], low = fminf(base, base2);
-        const float f = joined(low, base), f2 = joined(low, base2);
-        const float of = f * kPower<-kShared>, of2 = f2 * kPower<-kShared>;
+        if (part_of) return;
+        float low = base;
+        for (int s = 0; s < KS - 1; ++s) low = fminf(low, to[s * kBlocks * kBlock + 16 * kO * 64]);
+        const float f = joined(low, base);
+        l *= f;
+        for (int e = 0; e < kO; ++e) o[e] *= f * kPower<-kShared>;
+        for (int s = 0; s < KS - 1; ++s) {
+            const float* x = to + s * kBlocks * kBlock;
+            const float f2 = joined(low, x[16 * kO * 64]);
+            l += x[(16 * kO + 1) * 64] * f2;
+            for (int e = 0; e < 16 * kO; ++e) o[e / 16][e % 16] += x[e * 64] * (f2 * kPower<-kShared>);
+        }
         base = low;
-        l = l * f + to[(16 * kO + 1) * 64] * f2;
-        for (int x = 0; x < 16 * kO; ++x) o[x / 16][x % 16] = o[x / 16][x % 16] * of + to[x * 64] * of2;
     }
     if (!real) return;
     if (part.splits > 1) {
@@ -1042,7 +1271,6 @@ struct Plan {
     uint32_t tiles, splits;        // row tiles a head at most, shares of the slots
     uint64_t rows_ml, bytes;       // the two kernels follow each other in the same workspace; all of it
 };
-constexpr uint64_t kHalf = 6;
 constexpr uint32_t kMaxShares = 64;     // of many rows
 Plan plan_of(const PagedDev& a, uint32_t dim, int cache_dtype) {
     Plan p{};
@@ -1069,19 +1297,18 @@ Plan plan_of(const PagedDev& a, uint32_t dim, int cache_dtype) {
         p.bytes = p.plan + round256(8ull * a.seq.seqs);
     }
     if (p.many) {
-        // The least time, in tenths of the 2 us that a tile takes a workgroup of 128 rows (64 rows: kHalf): as many
-        // workgroups as fit run at the speed of one, and a share costs four tiles' time for its start and end, and the
-        // passage of its outputs through memory.
-        const uint64_t fit = 256 * (dim == 64 && cache_dtype != PKV_FP8 ? 3 : 2);
+        // The least time, in tenths of a step of shared tiles (KS 1; 2 and 4 take two tiles a step): as many workgroups as
+        // there are CUs run at the speed of one, a share costs four steps' time for its start and end, and the passage of
+        // its outputs through memory.
         uint64_t least = ~0ull;
-        for (int ks = 1; ks <= 2; ++ks) {
-            const uint64_t rt = row_tile(ks);
+        for (int ks = 1; ks <= 4; ks *= 2) {
+            const uint64_t rt = rows_of_tile(ks);
             const uint64_t row_tiles = std::min((static_cast<uint64_t>(a.seq.rows) * a.group + rt - 1) / rt + a.seq.seqs,
                                                 a.seq.seqs * ((most + rt - 1) / rt));
             const uint64_t groups = a.heads * row_tiles, tiles = tiles_for(rt, 64);
             for (uint32_t n = 1; n <= kMaxShares && (n == 1 || n * 4 <= tiles); ++n) {
-                const uint64_t rounds = (groups * n + fit - 1) / fit;
-                const uint64_t cost = rounds * ((tiles + n - 1) / n + (n == 1 ? 2 : 4)) * (ks == 1 ? 10 : kHalf) +
+                const uint64_t rounds = (groups * n + 255) / 256, each = (tiles + n - 1) / n;
+                const uint64_t cost = rounds * ((ks == 1 ? each : (each + 1) / 2) + (n == 1 ? 2 : 4)) * (ks == 4 ? 8 : ks == 2 ? 12 : 10) +
                                       (n == 1 ? 0 : groups * rt * dim * 8 * n / 800000);
                 if (cost < least) {
                     least = cost;
@@ -1092,7 +1319,7 @@ Plan plan_of(const PagedDev& a, uint32_t dim, int cache_dtype) {
             }
         }
         if (p.splits > 1) {
-            const uint64_t rows = static_cast<uint64_t>(a.heads) * p.tiles * p.splits * row_tile(p.ks);
+            const uint64_t rows = static_cast<uint64_t>(a.heads) * p.tiles * p.splits * rows_of_tile(p.ks);
             p.rows_ml = round256(rows * dim * 4);
             p.bytes = std::max(p.bytes, p.rows_ml + round256(rows * 8));
         }
@@ -1112,11 +1339,12 @@ int attend_typed(const PagedDev& a, uint8_t* ws, hipStream_t st) {
         }
     if (p.many) {
         const PagedPart part{reinterpret_cast<float*>(ws), reinterpret_cast<float*>(ws + p.rows_ml), nullptr, p.tiles, 0,
-                             row_tile(p.ks), p.splits};
+                             static_cast<uint32_t>(rows_of_tile(p.ks)), p.splits};
         const int few = PAGED && p.few ? kFew : 0;
         const uint32_t grid = a.heads * p.tiles * p.splits + (p.few ? 0 : clears(a));
-        if (p.ks == 2) rows_kernel<CT, QT, D, PAGED, 2><<<grid, 256, 0, st>>>(a, part, few);
-        else rows_kernel<CT, QT, D, PAGED, 1><<<grid, 256, 0, st>>>(a, part, few);
+        if (p.ks == 4) rows_kernel<CT, QT, D, PAGED, 4><<<grid, 512, 0, st>>>(a, part, few);
+        else if (p.ks == 2) rows_kernel<CT, QT, D, PAGED, 2><<<grid, 512, 0, st>>>(a, part, few);
+        else rows_kernel<CT, QT, D, PAGED, 1><<<grid, 512, 0, st>>>(a, part, few);
         if (p.splits > 1)
             join_rows_kernel<QT, D><<<a.heads * p.tiles * (part.rows / join_rows(D)), 256, 0, st>>>(a, part, few);
     }
@@ -1160,9 +1388,9 @@ bool paged_fits(const PagedDev& a, uint32_t dim, int cache_dtype) {
     if (p.many) {
         const uint64_t tiles = static_cast<uint64_t>(a.heads) * p.tiles;
         blocks = std::max(blocks, tiles * p.splits);
-        if (p.splits > 1) blocks = std::max<uint64_t>(blocks, tiles * (row_tile(p.ks) / join_rows(dim)));
+        if (p.splits > 1) blocks = std::max<uint64_t>(blocks, tiles * (rows_of_tile(p.ks) / join_rows(dim)));
     }
-    return blocks < (1u << 24) - kClear;
+    return blocks < (1u << 23) - kClear;     // workgroups of up to 512 threads
 }
 
 uint64_t paged_workspace(const PagedDev& a, uint32_t dim, int cache_dtype) { return plan_of(a, dim, cache_dtype).bytes; }
