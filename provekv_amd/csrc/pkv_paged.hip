@@ -710,13 +710,12 @@ struct PageStage : Staged<CT, D> {
         return c;
     }
     // Where the rows that copy x takes of the tile at `slot` start: of the head's pages (rows: the head's packed row 0).
-    template <bool VALUES>
-    __device__ static const uint8_t* copy_from(const PagedDev& a, const uint8_t* rows, uint64_t head, int words, int slot,
-                                               int last, uint32_t stride, int x, uint32_t wave) {
+    __device__ static const uint8_t* copy_from(const PagedDev& a, const uint8_t* side, const uint8_t* rows, uint64_t head,
+                                               int words, int slot, int last, uint32_t stride, int x, uint32_t wave) {
         const int r = kCopyStep * x + kCopyRows * static_cast<int>(wave);
         if constexpr (PAGED) {
             const int start = piece_start(slot, r / 16, last);
-            return (VALUES ? a.v : a.k) + 2 * piece_at(a, words, r / 16, start, head) + r % 16 * stride;
+            return side + 2 * piece_at(a, words, r / 16, start, head) + r % 16 * stride;
         } else {
             return rows + static_cast<uint64_t>(slot + r) * stride;
         }
@@ -738,7 +737,7 @@ struct PageStage : Staged<CT, D> {
         } else {
             const int row = kCopyRows * static_cast<int>(wave) + static_cast<int>(lane / kPieces);
             for (int x = 0; x < kCopies; ++x) {
-                const uint8_t* at = copy_from<VALUES>(a, rows, head, words, slot, last, c.stride, x, wave);
+                const uint8_t* at = copy_from(a, from, rows, head, words, slot, last, c.stride, x, wave);
                 // the piece may start in front of the tile's part, and the row lie in front of copy_from's
                 const int r = kCopyStep * x + row, first = PAGED ? piece_start(slot, r / 16, last) + r % 16 : slot + r;
                 const int32_t back = (min(slot + r, last) - first) * static_cast<int32_t>(c.stride);
@@ -781,21 +780,12 @@ struct PageStage : Staged<CT, D> {
 };
 
 // copy_to_lds among products, free to pass LDS reads: between two meetings
-// nothing reads what a copy overwrites.  MAYBE: only if `brings`, the same in all
-// lanes, of which all are at work (a branch would part the products).
-template <bool MAYBE>
-__device__ inline void start_copy(uint32_t to, const uint8_t* from, uint32_t offset, int brings) {
+// nothing reads what a copy overwrites.
+__device__ inline void start_copy(uint32_t to, const uint8_t* from, uint32_t offset) {
     uint32_t m0;
-    if constexpr (MAYBE)
-        asm volatile("s_mov_b32 %0, m0\n\ts_mov_b32 m0, %1\n\ts_cmp_lg_u32 %4, 0\n\ts_cselect_b64 exec, -1, 0\n\t"
-                     "global_load_lds_dwordx4 %2, %3\n\ts_mov_b64 exec, -1\n\ts_mov_b32 m0, %0"
-                     : "=&s"(m0)
-                     : "s"(to), "v"(offset), "s"(from), "s"(__builtin_amdgcn_readfirstlane(brings))
-                     : "scc");
-    else
-        asm volatile("s_mov_b32 %0, m0\n\ts_mov_b32 m0, %1\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %2, %3\n\ts_mov_b32 m0, %0"
-                     : "=&s"(m0)
-                     : "s"(to), "v"(offset), "s"(from));
+    asm volatile("s_mov_b32 %0, m0\n\ts_mov_b32 m0, %1\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %2, %3\n\ts_mov_b32 m0, %0"
+                 : "=&s"(m0)
+                 : "s"(to), "v"(offset), "s"(from));
 }
 
 // The waves of a workgroup meet; nothing moves across, no copy is waited for.
@@ -831,20 +821,22 @@ __device__ inline void meet() {
 constexpr int rows_of_tile(int ks) { return 256 / ks; }
 
 // The order of V operands of two reads and K operands of one, PRODUCTS products
-// each: the reads run kAhead operands ahead of the products (left to itself the
-// compiler reads an operand, waits for it and multiplies).
+// each, in pairs: the reads run kAhead operands ahead of the products (left to
+// itself the compiler reads an operand, waits for it and multiplies).
 constexpr int kAhead = 4;
-template <int V, int K, int PRODUCTS>
+constexpr int reads_of(int v, int k, int from, int to) {
+    int n = 0;
+    for (int i = from; i < (to < v + k ? to : v + k); ++i) n += i < v ? 2 : 1;
+    return n;
+}
+template <int V, int K, int PRODUCTS, int AT = -kAhead>
 __device__ inline void reads_ahead() {
-    auto reads = [](int n) { return n < V ? 2 : n < V + K ? 1 : 0; };
-    static_assert(V + K >= kAhead && (V == 0 || V >= kAhead) && (K == 0 || K >= kAhead), "operands ahead are of one kind");
-    __builtin_amdgcn_sched_group_barrier(0x100, kAhead * (V ? 2 : 1), 0);
-#pragma unroll
-    for (int i = 0; i < V + K; ++i) {
-        __builtin_amdgcn_sched_group_barrier(0x008, PRODUCTS, 0);
-        if (reads(i + kAhead) == 2) __builtin_amdgcn_sched_group_barrier(0x100, 2, 0);
-        if (reads(i + kAhead) == 1) __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);
-    }
+    static_assert((V + K) % 2 == 0 && kAhead % 2 == 0, "pairs of operands");
+    constexpr int reads = reads_of(V, K, AT < 0 ? 0 : AT + kAhead, AT < 0 ? kAhead : AT + kAhead + 2);
+    if constexpr (AT >= 0) __builtin_amdgcn_sched_group_barrier(0x008, 2 * PRODUCTS, 0);
+    if constexpr (reads > 0) __builtin_amdgcn_sched_group_barrier(0x100, reads, 0);
+    constexpr int next = AT < 0 ? 0 : AT + 2;
+    if constexpr (next < V + K) reads_ahead<V, K, PRODUCTS, next>();
 }
 template <int CT, int QT, int D, bool PAGED, int KS>
 __global__ __launch_bounds__(512, 2) void rows_kernel(PagedDev a, PagedPart part, int few) {
@@ -853,7 +845,8 @@ __global__ __launch_bounds__(512, 2) void rows_kernel(PagedDev a, PagedPart part
     constexpr int MT = mat_type(CT), kU = KS == 4 ? 1 : 2, kO = D / 32;   // kU: 32-slot pieces a wave takes of a tile
     constexpr int NP = query_terms(CT, QT), kRowTile = rows_of_tile(KS);
     constexpr bool kTurns = KS > 1;                               // a group has tiles of its own
-    __shared__ __align__(16) uint8_t lds[(kTurns ? 4 : 2) * St::kBytes];   // two tiles a group, or of both
+    constexpr int kRing = kTurns ? 2 : 3;                         // tiles in LDS, of a group or of both: keys, then values
+    __shared__ __align__(16) uint8_t lds[(kTurns ? 2 : 1) * kRing * St::kBytes];
     const uint32_t work_blocks = a.heads * part.units * part.splits;
     if (blockIdx.x >= work_blocks) return clear_rows<QT, D, 512>(a, blockIdx.x - work_blocks);
     const uint32_t lane = threadIdx.x % 64, wave_id = __builtin_amdgcn_readfirstlane(threadIdx.x / 64);
@@ -892,22 +885,29 @@ __global__ __launch_bounds__(512, 2) void rows_kernel(PagedDev a, PagedPart part
     const uint8_t* kp = PAGED ? nullptr : a.k + 2 * (static_cast<uint64_t>(sq.row0) * a.k_slot + head);
     const uint8_t* vp = PAGED ? nullptr : a.v + 2 * (static_cast<uint64_t>(sq.row0) * a.v_slot + h * a.v_head);
 
-    uint8_t* const mine = lds + (kTurns ? group * 2 * St::kBytes : 0);
-    const bool brings = kTurns || group == 0;      // the group that copies the tiles that this one reads
+    uint8_t* const mine = lds + (kTurns ? group * kRing * St::kBytes : 0);
+    // the keys and values that a group brings: of tiles of its own both
+    const bool keys_mine = kTurns || group == 0, values_mine = kTurns || group == 1;
     const uint32_t at = static_cast<uint32_t>(reinterpret_cast<uintptr_t>((LdsByte*)mine)), w4 = wave_id % 4;
+    // places of the ring (the values' count from kKeyBytes before them)
+    auto key_place = [](int ring) { return static_cast<uint32_t>(ring) * St::kKeyBytes; };
+    auto value_place = [](int ring) { return static_cast<uint32_t>(kRing - 1 + ring) * St::kKeyBytes; };
+    auto behind = [](int ring) { return ring + 1 == kRing ? 0 : ring + 1; };
+    auto before = [](int ring) { return ring ? ring - 1 : kRing - 1; };
     float base = kInf, l = 0.0f;
     f32x16 o[kO], sc[kU];
     u32x4 pt[NP][2 * kU];
     typename St::Side ks, vs;
     const typename St::Copies kc = St::template copies<false>(a, gt), vc = St::template copies<true>(a, gt);
-    // LDS addresses of the lane's operands in the first tile: keys of slot n, values as Staged::values16 reads them
+    // LDS addresses of the lane's operands in the first place: keys of slot n, values as Staged::values16 reads them
     constexpr int kX = D / 16;
     uint32_t key_read[kX], value_read[kO][2];
     for (int x = 0; x < kX; ++x) key_read[x] = at + share * St::kRow + St::key_at(n, 2 * x + half);
     for (int e = 0; e < kO; ++e)
         for (int y = 0; y < 2; ++y) {
             const uint32_t s = lane % 16, row = lane / 32 * 4 + s / 4 + 8 * y;
-            value_read[e][y] = at + share * St::kRow + St::value_at(row, 4 * e + lane / 16 % 2 * 2 + s % 4 / 2) + s % 2 * 8;
+            value_read[e][y] = at + share * St::kRow + value_place(0) +
+                               St::value_at(row, 4 * e + lane / 16 % 2 * 2 + s % 4 / 2) + s % 2 * 8;
         }
     // the words of step i's pages (past the last tile: the last's again, unused)
     auto pages = [&](int i) {
@@ -915,17 +915,20 @@ __global__ __launch_bounds__(512, 2) void rows_kernel(PagedDev a, PagedPart part
         else return read_pages<4>(a.seq, table, tl.slot(min(tile(i), t1 - 1), St::kSlots), tl.high - 1, lane);
     };
     auto there = [&](int i) { return tile(i) < t1; };
-    auto buffer = [&](int i) { return static_cast<uint32_t>(i & 1) * St::kBytes; };
-    auto fetch_keys = [&](int i, int words) {
-        if (brings && there(i))
-            St::template fetch<false>(ks, kc, a, at + buffer(i), kp, head, words, slot_of(i), tl.high - 1, gt);
+    auto fetch_keys = [&](int i, int ring, int words) {
+        if (keys_mine && there(i))
+            St::template fetch<false>(ks, kc, a, at + key_place(ring), kp, head, words, slot_of(i), tl.high - 1, gt);
     };
-    auto fetch_values = [&](int i, int words) {
-        if (brings && there(i))
-            St::template fetch<true>(vs, vc, a, at + buffer(i), vp, head, words, slot_of(i), tl.high - 1, gt);
+    auto fetch_values = [&](int i, int ring, int words) {
+        if (values_mine && there(i))
+            St::template fetch<true>(vs, vc, a, at + value_place(ring), vp, head, words, slot_of(i), tl.high - 1, gt);
     };
-    auto land_keys = [&](int i) { if (brings && there(i)) St::template land<false>(ks, mine + buffer(i), gt); };
-    auto land_values = [&](int i) { if (brings && there(i)) St::template land<true>(vs, mine + buffer(i), gt); };
+    auto land_keys = [&](int i, int ring) {
+        if (keys_mine && there(i)) St::template land<false>(ks, mine + key_place(ring), gt);
+    };
+    auto land_values = [&](int i, int ring) {
+        if (values_mine && there(i)) St::template land<true>(vs, mine + value_place(ring), gt);
+    };
     // some row of the wave sees some of step i's tile
     auto sees = [&](int i) {
         if (!there(i)) return false;
@@ -933,25 +936,29 @@ __global__ __launch_bounds__(512, 2) void rows_kernel(PagedDev a, PagedPart part
         return slot < wt.high && (slot + 32 * kU > wt.low || static_cast<uint32_t>(slot) < a.sinks);
     };
     float lift = kLift<MT>;
-    // none: 16-slot pieces of the tile on no page; all: every row of the wave sees all of it
-    auto softmax = [&](int i, uint32_t none, auto all) __attribute__((always_inline)) {
-        const int slot = decltype(all)::value ? 0 : slot_of(i) + share;
-        if (!decltype(all)::value && !all_visible(a, wpos0, wpos1, slot, slot + 32 * kU - 1)) {
-            const int off = pos - slot - 4 * static_cast<int>(half);   // less the register's place: how far back
-            if (static_cast<uint32_t>(slot) >= a.sinks) {
-                for (int p = 0; p < kU; ++p)
-                    for (int x = 0; x < 16; ++x)
-                        if (!in_reach(a, off, 32 * p + row32(x, 0))) sc[p][x] = -kInf;
-            } else {
-                for (int p = 0; p < kU; ++p)
-                    for (int x = 0; x < 16; ++x)
-                        if (!visible(a, pos, slot + 32 * p + row32(x, half))) sc[p][x] = -kInf;
-            }
+    // logits that the rows do not see to -inf; none: 16-slot pieces of the tile on no page
+    auto hide = [&](int i) __attribute__((always_inline)) {
+        const int slot = slot_of(i) + share;
+        if (all_visible(a, wpos0, wpos1, slot, slot + 32 * kU - 1)) return;
+        const int off = pos - slot - 4 * static_cast<int>(half);   // less the register's place: how far back
+        if (static_cast<uint32_t>(slot) >= a.sinks) {
+            for (int p = 0; p < kU; ++p)
+                for (int x = 0; x < 16; ++x)
+                    if (!in_reach(a, off, 32 * p + row32(x, 0))) sc[p][x] = -kInf;
+        } else {
+            for (int p = 0; p < kU; ++p)
+                for (int x = 0; x < 16; ++x)
+                    if (!visible(a, pos, slot + 32 * p + row32(x, half))) sc[p][x] = -kInf;
         }
+    };
+    auto hide_missing = [&](uint32_t none) __attribute__((always_inline)) {
         if (PAGED && none)
             for (int p = 0; p < kU; ++p)
                 for (int x = 0; x < 16; ++x)
                     if (none >> (share / 16 + 2 * p + x / 8) & 1) sc[p][x] = -kInf;
+    };
+    // the base lowered by the largest of the logits
+    auto lower = [&]() __attribute__((always_inline)) {
         float top = sc[0][0];
         for (int p = 0; p < kU; ++p)
             for (int x = 0; x < 16; ++x) top = fmaxf(top, sc[p][x]);
@@ -964,18 +971,37 @@ __global__ __launch_bounds__(512, 2) void rows_kernel(PagedDev a, PagedPart part
                 base = low;
             }
         }
+    };
+    // weights in the logits' place, and their sums: no weight is above its piece's
+    auto weights = [&](float (&sum)[kU]) __attribute__((always_inline)) {
         const float from = base == kInf ? 0.0f : base;
-        for (int p = 0; p < kU; ++p)
+        for (int p = 0; p < kU; ++p) {
+            sum[p] = 0.0f;
+            for (int x = 0; x < 16; ++x) {
+                sc[p][x] = __builtin_amdgcn_exp2f(__builtin_fmaf(sc[p][x], a.scale2, from));
+                sum[p] += sc[p][x];
+            }
+        }
+    };
+    auto pack = [&](const float (&sum)[kU]) __attribute__((always_inline)) {
+        for (int p = 0; p < kU; ++p) {
+            l += sum[p];
             for (int y = 0; y < 2; ++y) {
                 float w[8];
-                for (int x = 0; x < 8; ++x) {
-                    w[x] = __builtin_amdgcn_exp2f(__builtin_fmaf(sc[p][8 * y + x], a.scale2, from));
-                    l += w[x];
-                }
+                for (int x = 0; x < 8; ++x) w[x] = sc[p][8 * y + x];
                 for (int k = 0; k < NP; ++k)
                     pt[k][2 * p + y] = u32x4{pack_term<MT>(w[0], w[1]), pack_term<MT>(w[2], w[3]),
                                              pack_term<MT>(w[4], w[5]), pack_term<MT>(w[6], w[7])};
             }
+        }
+    };
+    auto softmax = [&](int i, uint32_t none) __attribute__((always_inline)) {
+        float sum[kU];
+        hide(i);
+        hide_missing(none);
+        lower();
+        weights(sum);
+        pack(sum);
     };
     // O += the values of the tile at `values` weighed, S = the logits of the one at `keys`; among the products copy(0),
     // copy(1), .. start what is copied meanwhile.
@@ -1011,62 +1037,80 @@ __global__ __launch_bounds__(512, 2) void rows_kernel(PagedDev a, PagedPart part
     using Yes = std::true_type;
     using No = std::false_type;
     auto no_copy = [](int) {};
-    static_assert(2 * kU + kX / (kU == 1 ? 1 : 2) >= 2 * St::kCopies, "every copy has its place");
+    static_assert(2 * kU + kX / (kU == 1 ? 1 : 2) >= (kTurns ? 2 : 1) * St::kCopies, "every copy has its place");
 
-    // Step i of a group: values of i - 1 and logits of i, meanwhile keys of i + 1 and values of i are on their way; meet;
-    // softmax of i, what is on its way waited for; meet.  The second group is a meeting behind; of shared tiles the first
-    // brings them.  What a copy overwrites was last read in front of the last meeting: keys of i - 1, values of i - 2.
+    // Step i of a group, its tile at place `ring`: values of i - 1 and logits of i; meet; softmax of i; meet.  The second
+    // group is a meeting behind.  From the products to the end of the softmax keys of i + 1 are on their way, and values of
+    // i; of shared tiles the first group brings the keys, the second values of i + 1.  What a copy overwrites was last
+    // read in front of the last meeting: keys of i - 1 (shared: i - 2), values of i - 2.
     int words = 0, next = 0;
     bool have = false;           // weights of the step before
-    auto step = [&](int i) __attribute__((always_inline)) {
+    auto step = [&](int i, int ring) __attribute__((always_inline)) {
         const uint32_t none = PAGED ? no_page<4>(a.seq, words) : 0;
         const bool now = sees(i);
-        fetch_keys(i + 1, next);
-        fetch_values(i, words);
+        fetch_keys(i + 1, behind(ring), next);
+        if (kTurns) fetch_values(i, ring, words);
+        else fetch_values(i + 1, behind(ring), next);
         __builtin_amdgcn_s_setprio(1);
-        if (have) products(Yes(), No(), buffer(i + 1), 0, no_copy);
-        if (now) products(No(), Yes(), 0, buffer(i), no_copy);
+        if (have) products(Yes(), No(), before(ring) * St::kKeyBytes, 0, no_copy);
+        if (now) products(No(), Yes(), 0, key_place(ring), no_copy);
         have = now;
         __builtin_amdgcn_s_setprio(0);
         meet();
         const int ahead = pages(i + 2);
-        if (have) softmax(i, none, No());
-        land_keys(i + 1);
-        land_values(i);
+        if (have) softmax(i, none);
+        land_keys(i + 1, behind(ring));
+        if (kTurns) land_values(i, ring);
+        else land_values(i + 1, behind(ring));
         words = next;
         next = ahead;
         meet();
     };
     // The same for a step in the middle: its tile and the next are whole, every row of the wave sees all of it and of the
-    // one before, and its place in LDS is known (ODD: i is odd).
-    auto middle = [&](int i, auto odd) __attribute__((always_inline)) {
-        constexpr uint32_t kHere = decltype(odd)::value ? St::kBytes : 0, kOther = St::kBytes - kHere;
+    // one before, and its place is known.
+    auto middle = [&](int i, auto place) __attribute__((always_inline)) {
+        constexpr int kHere = decltype(place)::value, kNext = (kHere + 1) % kRing, kBefore = (kHere + kRing - 1) % kRing;
         const uint32_t none = PAGED ? no_page<4>(a.seq, words) : 0;
         const int slot = slot_of(i);
         if constexpr (CT == PKV_FP8) {
-            fetch_keys(i + 1, next);
-            fetch_values(i, words);
+            fetch_keys(i + 1, kNext, next);
+            if (kTurns) fetch_values(i, kHere, words);
+            else fetch_values(i + 1, kNext, next);
         }
+        // of shared tiles a group's side of the next one
+        const typename St::Copies& c = !kTurns && group ? vc : kc;
+        const uint32_t to = at + c.to + (!kTurns && group ? (kRing - 1 + kNext) * St::kKeyBytes : kNext * St::kKeyBytes);
         __builtin_amdgcn_s_setprio(1);
-        products(Yes(), Yes(), kOther, kHere, [&](int x) {
+        products(Yes(), Yes(), kBefore * St::kKeyBytes, kHere * St::kKeyBytes, [&](int x) __attribute__((always_inline)) {
             if constexpr (CT != PKV_FP8) {
                 const int y = x % St::kCopies;
                 if (x < St::kCopies)
-                    start_copy<!kTurns>(at + kOther + kc.to + y * St::kCopyStep * St::kRow,
-                               St::template copy_from<false>(a, kp, head, next, slot + kEvery * St::kSlots, tl.high - 1,
-                                                             kc.stride, y, w4), kc.off, brings);
-                else if (x < 2 * St::kCopies)
-                    start_copy<!kTurns>(at + kHere + vc.to + y * St::kCopyStep * St::kRow,
-                               St::template copy_from<true>(a, vp, head, words, slot, tl.high - 1, vc.stride, y, w4),
-                               vc.off, brings);
+                    start_copy(to + y * St::kCopyStep * St::kRow,
+                               St::copy_from(a, !kTurns && group ? a.v : a.k, !kTurns && group ? vp : kp, head, next,
+                                             slot + kEvery * St::kSlots, tl.high - 1, c.stride, y, w4), c.off);
+                else if (kTurns && x < 2 * St::kCopies)
+                    start_copy(at + vc.to + (kRing - 1 + kHere) * St::kKeyBytes + y * St::kCopyStep * St::kRow,
+                               St::copy_from(a, a.v, vp, head, words, slot, tl.high - 1, vc.stride, y, w4), vc.off);
             }
         });
         __builtin_amdgcn_s_setprio(0);
         meet();
         const int ahead = pages(i + 2);
-        softmax(i, none, Yes());
-        land_keys(i + 1);
-        land_values(i);
+        // weights by the base as it is; where their sums pass what one weight may be, from the logits again
+        float sum[kU];
+        hide_missing(none);
+        weights(sum);
+        constexpr float kMost = kPower<static_cast<int>(kLift<MT> + kLag<MT>)>;
+        if (__builtin_expect(__any(!(sum[0] <= kMost && sum[kU - 1] <= kMost) || base == kInf), 0)) {
+            products(No(), Yes(), 0, kHere * St::kKeyBytes, no_copy);
+            hide_missing(none);
+            lower();
+            weights(sum);
+        }
+        pack(sum);
+        land_keys(i + 1, kNext);
+        if (kTurns) land_values(i, kHere);
+        else land_values(i + 1, kNext);
         words = next;
         next = ahead;
         meet();
@@ -1075,47 +1119,59 @@ __global__ __launch_bounds__(512, 2) void rows_kernel(PagedDev a, PagedPart part
     if (steps > 0) {
         words = pages(0);
         next = pages(1);
-        fetch_keys(0, words);
-        land_keys(0);
+        fetch_keys(0, 0, words);
+        land_keys(0, 0);
+        if (!kTurns) {
+            fetch_values(0, 0, words);
+            land_values(0, 0);
+        }
         // the query is there: else the compiler waits for it at its every use, and for the copies under way with it
         __builtin_amdgcn_s_waitcnt(0x0f70);   // vmcnt(0)
         meet();
         if (group) meet();
-        // middle steps: from an even one on, pairs of them.  Tiles of the list whose slots all rows of the wave see, the one
-        // before too, and whose next one is whole and there
+        // middle steps, as many at a time as there are places.  Tiles of the list whose slots all rows of the wave see, the
+        // one before too, and whose next one is whole and there
         const int list = tl.second - tl.first;     // tile t of the list, behind the first ones, starts at slot 64 (t + list)
         int lo = tl.first, hi = min((wpos0 + 1) / St::kSlots, tl.high / St::kSlots - kEvery) - list;
         if (a.window)
             lo = max(lo, static_cast<int>(max(static_cast<int64_t>(wpos1) - a.reach + St::kSlots, static_cast<int64_t>(0)) /
                                           St::kSlots) - list);
         hi = min(hi, t1 - kEvery);
-        const int from = w0 <= last && wpos0 >= 0 ? (max(lo - first + kEvery - 1, 0) / kEvery + 2) & ~1 : steps;
-        const int pairs = max(hi - first + kEvery - 1, 0) / kEvery - from;       // may be negative
-        int i = 0;
-        for (; i < min(from, steps); ++i) step(i);
-        if (pairs > 1)
-            for (const int to = from + (pairs & ~1); i < to; i += 2) {
-                middle(i, No());
-                middle(i + 1, Yes());
+        const int i0 = max(lo - first + kEvery - 1, 0) / kEvery;
+        const int from = w0 <= last && wpos0 >= 0 ? (i0 + kRing) / kRing * kRing : steps;
+        const int middles = max(hi - first + kEvery - 1, 0) / kEvery - from;       // may be negative
+        int i = 0, ring = 0;
+        auto steps_to = [&](int end) {
+            for (; i < end; ++i) {
+                step(i, ring);
+                ring = behind(ring);
             }
-        for (; i < steps; ++i) step(i);
-        if (have) products(Yes(), No(), buffer(steps - 1), 0, no_copy);
+        };
+        steps_to(min(from, steps));
+        if (middles >= kRing)
+            for (const int to = from + middles / kRing * kRing; i < to; i += kRing) {
+                middle(i, std::integral_constant<int, 0>());
+                middle(i + 1, std::integral_constant<int, 1>());
+                if constexpr (kRing == 3) middle(i + 2, std::integral_constant<int, 2>());
+            }
+        steps_to(steps);
+        if (have) products(Yes(), No(), before(ring) * St::kKeyBytes, 0, no_copy);
         if (!group) meet();
     }
     bool odd = false;
     for (int e = 0; e < kO; ++e)
         for (int x = 0; x < 16; ++x) odd |= (__float_as_uint(o[e][x]) & 0x7f800000u) == 0x7f800000u;
     if (__builtin_expect(__syncthreads_or(odd && real), 0)) {
-        // both sides of step i's tile staged, by all
+        // both sides of step i's tile in the first place, by all
         auto stage = [&](int i, int words) {
             __syncthreads();
-            fetch_keys(i, words);
-            fetch_values(i, words);
-            land_keys(i);
-            land_values(i);
+            fetch_keys(i, 0, words);
+            fetch_values(i, 0, words);
+            land_keys(i, 0);
+            land_values(i, 0);
             __syncthreads();
         };
-        auto cleaned = [&](int i) { return brings && there(i) && St::clean(mine + buffer(i), gt); };
+        auto cleaned = [&](int i) { return keys_mine && there(i) && St::clean(mine + value_place(0), gt); };
         for (int pass = 1; pass < 3; ++pass) {
             base = kInf;
             l = 0.0f;
@@ -1127,9 +1183,9 @@ __global__ __launch_bounds__(512, 2) void rows_kernel(PagedDev a, PagedPart part
                 cleaned(i);
                 __syncthreads();
                 if (sees(i)) {
-                    products(No(), Yes(), 0, buffer(i), no_copy);
-                    softmax(i, PAGED ? no_page<4>(a.seq, words) : 0, No());
-                    products(Yes(), No(), buffer(i), 0, no_copy);
+                    products(No(), Yes(), 0, 0, no_copy);
+                    softmax(i, PAGED ? no_page<4>(a.seq, words) : 0);
+                    products(Yes(), No(), 0, 0, no_copy);
                 }
             }
             odd = false;
@@ -1150,7 +1206,6 @@ __global__ __launch_bounds__(512, 2) void rows_kernel(PagedDev a, PagedPart part
             if (!__syncthreads_or(cleaned(i))) continue;
             stage(i, words);
             if (!there(i)) continue;
-            const uint8_t* buf = mine + buffer(i);
 #pragma unroll 1
             for (int j = share; j < share + 32 * kU; ++j) {
                 const bool see = visible(a, pos, slot_of(i) + j) && !(none >> j / 16 & 1);
@@ -1159,7 +1214,7 @@ __global__ __launch_bounds__(512, 2) void rows_kernel(PagedDev a, PagedPart part
                 asm volatile("" : "+v"(hf));   // this rare loop's addresses are not kept over the main one
                 float dot = 0.0f;
                 for (int x = 0; x < Query<CT, QT, D>::kRegs; ++x) {
-                    const u32x4 k = *reinterpret_cast<const u32x4*>(buf + St::key_at(j, 2 * x + hf));
+                    const u32x4 k = *reinterpret_cast<const u32x4*>(mine + St::key_at(j, 2 * x + hf));
                     for (int w = 0; w < 4; ++w)
                         for (int y = 0; y < Query<CT, QT, D>::kTerms; ++y) {
                             const uint32_t kw = k[w], qw = q.q[y][x][w];
@@ -1170,7 +1225,7 @@ __global__ __launch_bounds__(512, 2) void rows_kernel(PagedDev a, PagedPart part
                 const float p = __builtin_amdgcn_exp2f(__builtin_fmaf(dot, a.scale2, from));
                 for (int e = 0; e < kO; ++e)
                     for (int x = 0; x < 16; ++x) {
-                        const float v = St::value(buf, j, 32 * e + row32(x, hf));
+                        const float v = St::value(mine + value_place(0), j, 32 * e + row32(x, hf));
                         if (see && (__float_as_uint(v) & 0x7f800000u) == 0x7f800000u) o[e][x] += p * v;
                     }
             }
