@@ -32,6 +32,12 @@ __device__ inline Seq seq_of(const SeqsDev& q, uint32_t s, uint32_t max_rows) {
     o.first = o.len - o.rows;
     return o;
 }
+// The same of a sequence that all lanes have, in scalar registers.
+__device__ inline Seq seq_of_all(const SeqsDev& q, uint32_t s, uint32_t max_rows) {
+    const Seq o = seq_of(q, s, max_rows);
+    return {__builtin_amdgcn_readfirstlane(o.row0), __builtin_amdgcn_readfirstlane(o.rows),
+            __builtin_amdgcn_readfirstlane(o.len), __builtin_amdgcn_readfirstlane(o.first)};
+}
 // The sequence of packed row r (the same in all lanes): the first that ends behind it; -1: nobody's.
 __device__ inline int seq_of_row(const SeqsDev& q, int r, uint32_t lane) {
     if (!q.starts) return r / static_cast<int>(q.each);
@@ -224,12 +230,20 @@ constexpr int kFew = 16;            // rows x group of a KV head that decode_ker
 constexpr int kStep = 32;           // slots of its tiles
 constexpr uint32_t kUnits = 1024;   // units of all heads that it aims at
 constexpr int kLeast = 4;           // tiles of a unit, one a wave
+constexpr int kLeastSteps = 8;      // rows_kernel: tiles of 64 slots of a share
 
 // The tiles that a sequence of few rows has; -1: it has no rows, or more.
 __device__ inline int few_tiles(const PagedDev& a, uint32_t s) {
     const Seq q = seq_of(a.seq, s, a.max_rows);
     if (!q.rows || static_cast<int64_t>(q.rows) * a.group > kFew) return -1;
     return tiles_of(a, q.first, q.first + q.rows - 1, kStep).count;
+}
+
+// The least whole number above all / target of the lanes' counts, and at least `least`.
+__device__ inline int share_of(int64_t all, uint32_t target, int least) {
+    for (int o = 32; o; o >>= 1) all += __shfl_xor(static_cast<long long>(all), o);
+    const double share = static_cast<double>(all) / target;   // counts stay below 2^53
+    return max(least, static_cast<int>(fmin(share, 1e9)) + 1);
 }
 
 // A share of a sequence's tiles, as units of about as many tiles for all
@@ -242,14 +256,12 @@ struct Unit {
 __device__ inline bool find_unit(const PagedDev& a, uint32_t u, uint32_t target, uint32_t lane, Unit* o) {
     const uint32_t per = (a.seq.seqs + 63) / 64, s0 = min(lane * per, a.seq.seqs), s1 = min(s0 + per, a.seq.seqs);
     int mine = -1;                      // of the run's only sequence
-    float all = 0.0f;
+    int64_t all = 0;
     for (uint32_t s = s0; s < s1; ++s) {
         mine = few_tiles(a, s);
-        all += static_cast<float>(max(mine, 0));
+        all += max(mine, 0);
     }
-    all = wave_sum(all);
-    // above the quotient, so that there are no more than target + sequences units whatever the rounding
-    const int size = max(kLeast, static_cast<int>(all * 1.000001f / static_cast<float>(target)) + 1);
+    const int size = share_of(all, target, kLeast);   // no more than target + sequences units
     auto units = [&](int tiles) { return tiles < 0 ? 0 : max(1, (tiles + size - 1) / size); };
     int n = 0;
     if (per == 1) n = units(mine);
@@ -270,11 +282,21 @@ __device__ inline bool find_unit(const PagedDev& a, uint32_t u, uint32_t target,
         if (want < first + n) break;
         first += n;
     }
-    o->seq = __builtin_amdgcn_readfirstlane(s);
-    o->first = __builtin_amdgcn_readfirstlane(first);
-    o->shares = __builtin_amdgcn_readfirstlane(n);
-    o->share = want - o->first;
+    *o = {static_cast<int>(s), want - first, n, first};
     return true;
+}
+
+// What is the same in all lanes, for the compiler to see.
+__device__ inline const uint8_t* uniform(const uint8_t* p) {
+    const uint64_t x = reinterpret_cast<uint64_t>(p);
+    const uint32_t lo = __builtin_amdgcn_readfirstlane(static_cast<uint32_t>(x)),
+                   hi = __builtin_amdgcn_readfirstlane(static_cast<uint32_t>(x >> 32));
+    return reinterpret_cast<const uint8_t*>(static_cast<uint64_t>(hi) << 32 | lo);
+}
+__device__ inline Tiles uniform(const Tiles& t) {
+    return {__builtin_amdgcn_readfirstlane(t.first), __builtin_amdgcn_readfirstlane(t.second),
+            __builtin_amdgcn_readfirstlane(t.count), __builtin_amdgcn_readfirstlane(t.low),
+            __builtin_amdgcn_readfirstlane(t.high)};
 }
 
 // Pages of a tile's 16-slot pieces: a lane reads one piece's word.  `last` is the
@@ -391,10 +413,10 @@ struct PageTile {
 
 // Shares of a unit's or a tile's rows on their way to a join.
 struct PagedPart {
-    float* o;          // [head][unit or tile][..][rows][D]
-    float* ml;         // [..][rows][2]: base, sum of the weights
-    int32_t* plan;     // [sequence][2]: first unit, units (few rows)
-    uint32_t units, target, rows, splits;
+    float* o;          // [head][unit][rows][D]
+    float* ml;         // [head][unit][rows][2]: base, sum of the weights
+    int32_t* plan;     // [sequence][2]: first unit, units; of many rows the first that is a share, shares of a tile
+    uint32_t units, target, rows, parts;
 };
 
 // The rows of a sequence of few (rows x group up to 16) against a share of its
@@ -422,17 +444,19 @@ __global__ __launch_bounds__(256, 2) void decode_kernel(PagedDev a, PagedPart pa
     const uint32_t h = blockIdx.x % a.heads, u = blockIdx.x / a.heads;
     Unit unit;
     if (!find_unit(a, u, part.target, lane, &unit)) return;
+    unit = {__builtin_amdgcn_readfirstlane(unit.seq), __builtin_amdgcn_readfirstlane(unit.share),
+            __builtin_amdgcn_readfirstlane(unit.shares), __builtin_amdgcn_readfirstlane(unit.first)};
     if (h == 0 && unit.share == 0 && threadIdx.x == 0) {
         part.plan[2 * unit.seq] = unit.first;
         part.plan[2 * unit.seq + 1] = unit.shares;
     }
-    const Seq sq = seq_of(a.seq, unit.seq, a.max_rows);
+    const Seq sq = seq_of_all(a.seq, unit.seq, a.max_rows);
     const uint32_t row = lane % 16, g = lane / 16;
     const int R = sq.rows * static_cast<int>(a.group), pos1 = sq.first + sq.rows - 1;
     const bool real = static_cast<int>(row) < R;
     const int qi = row / a.group, pos = real ? sq.first + qi : -1;
-    const Tiles tl = tiles_of(a, sq.first, pos1, kStep);
-    const int per = (tl.count + unit.shares - 1) / unit.shares;
+    const Tiles tl = uniform(tiles_of(a, sq.first, pos1, kStep));
+    const int per = __builtin_amdgcn_readfirstlane((tl.count + unit.shares - 1) / unit.shares);
     const int t0 = unit.share * per, t1 = min(t0 + per, tl.count);
     const int32_t* table = a.seq.tables + unit.seq * a.seq.table;
 
@@ -649,37 +673,75 @@ __global__ __launch_bounds__(256) void join_kernel(PagedDev a, PagedPart part) {
 }
 
 // ------------------------------------------------------------ many rows: tiles of rows through LDS
-// Row tile u of a head: sequences in order, of each its tiles from the last, whose
-// rows see most.
-struct RowTile {
-    int seq, tile;
+// A workgroup's part of a head's work: a tile of a sequence's rows against a share
+// of the slots' tiles.  Shares are as many for all tiles of a sequence, so that
+// one has at least 1 / target of all tiles there are (the last rows' counted for
+// all rows) and less than twice that: no more than `target` units are shares.
+// Units go from the longest on, of a sequence from the last rows, which see most.
+// A lane takes a run of sequences, as in find_unit.
+struct RowUnit {
+    int seq, tile, share, shares;
+    int part;                    // of the units that are shares, the tile's first
 };
-__device__ inline int row_tiles(const PagedDev& a, uint32_t s, int64_t few, int rows) {
-    const int64_t all = static_cast<int64_t>(seq_of(a.seq, s, a.max_rows).rows) * a.group;
-    return all > few ? static_cast<int>((all + rows - 1) / rows) : 0;
+struct RowWork {
+    int tiles, steps;            // row tiles, and the slots' tiles that the last of them sees
+};
+__device__ inline RowWork row_work(const PagedDev& a, uint32_t s, int64_t few, int rows) {
+    const Seq q = seq_of(a.seq, s, a.max_rows);
+    const int64_t all = static_cast<int64_t>(q.rows) * a.group;
+    RowWork w{};
+    if (all <= few) return w;
+    w.tiles = static_cast<int>((all + rows - 1) / rows);
+    const int first = (w.tiles - 1) * rows / static_cast<int>(a.group);
+    w.steps = tiles_of(a, q.first + first, q.first + q.rows - 1, 64).count;
+    return w;
 }
-__device__ inline bool find_tile(const PagedDev& a, uint32_t u, int64_t few, int rows, uint32_t lane, RowTile* o) {
+__device__ inline bool find_rows(const PagedDev& a, uint32_t u, int64_t few, int rows, uint32_t target, uint32_t lane,
+                                 RowUnit* o) {
     const uint32_t per = (a.seq.seqs + 63) / 64, s0 = min(lane * per, a.seq.seqs), s1 = min(s0 + per, a.seq.seqs);
-    int n = 0;
-    for (uint32_t s = s0; s < s1; ++s) n += row_tiles(a, s, few, rows);
-    int end = n;
-    for (int x = 1; x < 64; x <<= 1) {
-        const int y = __shfl_up(end, x);
-        if (static_cast<int>(lane) >= x) end += y;
+    RowWork mine{};
+    int64_t all = 0;
+    for (uint32_t s = s0; s < s1; ++s) {
+        mine = row_work(a, s, few, rows);
+        all += static_cast<int64_t>(mine.tiles) * mine.steps;
+    }
+    const int size = target ? share_of(all, target, kLeastSteps) : 0x7fffffff;
+    auto shares = [&](const RowWork& w) { return max(1, w.steps / size); };
+    int units = 0, parts = 0, longest = 0;
+    for (uint32_t s = s0; s < s1; ++s) {
+        const RowWork w = per == 1 ? mine : row_work(a, s, few, rows);
+        const int n = shares(w);
+        units += w.tiles * n;
+        parts += n > 1 ? w.tiles * n : 0;
+        longest = max(longest, w.steps / n);
+    }
+    // of the lanes with longer units, or as long ones and before this one
+    int first = 0, part = 0;
+    const uint32_t lanes = (a.seq.seqs + per - 1) / per;
+    for (uint32_t x = 0; x < lanes; ++x) {
+        const int len = __builtin_amdgcn_readlane(longest, x), n = __builtin_amdgcn_readlane(units, x),
+                  m = __builtin_amdgcn_readlane(parts, x);
+        const bool ahead = len > longest || (len == longest && x < lane);
+        first += ahead ? n : 0;
+        part += ahead ? m : 0;
     }
     const int want = static_cast<int>(u);
-    const uint32_t at = __popcll(__ballot(end <= want));
-    if (at == 64) return false;
-    int first = __shfl(end - n, static_cast<int>(at));
-    uint32_t s = at * per;
-    for (;; ++s) {
-        n = row_tiles(a, s, few, rows);
-        if (want < first + n) break;
-        first += n;
+    const uint64_t found = __ballot(want >= first && want < first + units);
+    if (!found) return false;
+    const int at = __ffsll(static_cast<unsigned long long>(found)) - 1;
+    first = __builtin_amdgcn_readlane(first, at);
+    part = __builtin_amdgcn_readlane(part, at);
+    for (uint32_t s = at * per;; ++s) {
+        const RowWork w = row_work(a, s, few, rows);
+        const int n = shares(w);
+        if (want < first + w.tiles * n) {
+            const int x = (want - first) / n, tile = w.tiles - 1 - x;
+            *o = {static_cast<int>(s), tile, want - first - x * n, n, part + tile * n};
+            return true;
+        }
+        first += w.tiles * n;
+        part += n > 1 ? w.tiles * n : 0;
     }
-    o->seq = __builtin_amdgcn_readfirstlane(s);
-    o->tile = __builtin_amdgcn_readfirstlane(n - 1 - (want - first));
-    return true;
 }
 
 // Staged's tiles from pages, or (PAGED false) from packed rows, a side at a time
@@ -741,7 +803,7 @@ struct PageStage : Staged<CT, D> {
                 // the piece may start in front of the tile's part, and the row lie in front of copy_from's
                 const int r = kCopyStep * x + row, first = PAGED ? piece_start(slot, r / 16, last) + r % 16 : slot + r;
                 const int32_t back = (min(slot + r, last) - first) * static_cast<int32_t>(c.stride);
-                copy_row_to_lds(lds + c.to + kCopyStep * kRow * x, at + c.off + static_cast<int64_t>(back));
+                copy_row_to_lds(__builtin_amdgcn_readfirstlane(lds + c.to + kCopyStep * kRow * x), at + c.off + static_cast<int64_t>(back));
             }
         }
     }
@@ -783,6 +845,8 @@ struct PageStage : Staged<CT, D> {
 // nothing reads what a copy overwrites.
 __device__ inline void start_copy(uint32_t to, const uint8_t* from, uint32_t offset) {
     uint32_t m0;
+    to = __builtin_amdgcn_readfirstlane(to);
+    from = uniform(from);
     asm volatile("s_mov_b32 %0, m0\n\ts_mov_b32 m0, %1\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %2, %3\n\ts_mov_b32 m0, %0"
                  : "=&s"(m0)
                  : "s"(to), "v"(offset), "s"(from));
@@ -847,23 +911,30 @@ __global__ __launch_bounds__(512, 2) void rows_kernel(PagedDev a, PagedPart part
     constexpr bool kTurns = KS > 1;                               // a group has tiles of its own
     constexpr int kRing = kTurns ? 2 : 3;                         // tiles in LDS, of a group or of both: keys, then values
     __shared__ __align__(16) uint8_t lds[(kTurns ? 2 : 1) * kRing * St::kBytes];
-    const uint32_t work_blocks = a.heads * part.units * part.splits;
+    const uint32_t work_blocks = a.heads * part.units;
     if (blockIdx.x >= work_blocks) return clear_rows<QT, D, 512>(a, blockIdx.x - work_blocks);
     const uint32_t lane = threadIdx.x % 64, wave_id = __builtin_amdgcn_readfirstlane(threadIdx.x / 64);
     const uint32_t n = lane % 32, half = lane / 32, group = wave_id / 4, gt = threadIdx.x % 256;
     const uint32_t wave = KS == 1 ? wave_id : wave_id % (8 / KS);         // its 32 rows
     const int share = KS == 4 ? static_cast<int>(wave_id / 2 % 2) * 32 : 0;   // its slots of a tile: share .. + 32 kU
     // heads fastest, so that a head's workgroups share an XCD's L2 where the heads are a multiple of 8
-    const uint32_t h = blockIdx.x % a.heads, split = blockIdx.x / a.heads % part.splits, u = blockIdx.x / a.heads / part.splits;
-    RowTile rt;
-    if (!find_tile(a, u, few, kRowTile, lane, &rt)) return;
-    const Seq sq = seq_of(a.seq, rt.seq, a.max_rows);
+    const uint32_t h = blockIdx.x % a.heads;
+    RowUnit rt;
+    if (!find_rows(a, blockIdx.x / a.heads, few, kRowTile, part.target, lane, &rt)) return;
+    rt = {__builtin_amdgcn_readfirstlane(rt.seq), __builtin_amdgcn_readfirstlane(rt.tile),
+          __builtin_amdgcn_readfirstlane(rt.share), __builtin_amdgcn_readfirstlane(rt.shares),
+          __builtin_amdgcn_readfirstlane(rt.part)};
+    if (part.target && h == 0 && rt.tile == 0 && rt.share == 0 && threadIdx.x == 0) {
+        part.plan[2 * rt.seq] = rt.part;
+        part.plan[2 * rt.seq + 1] = rt.shares;
+    }
+    const Seq sq = seq_of_all(a.seq, rt.seq, a.max_rows);
     const int R = sq.rows * static_cast<int>(a.group), r0 = rt.tile * kRowTile, G = static_cast<int>(a.group);
     const int last = min(r0 + kRowTile, R) - 1;
-    const int pos0 = sq.first + r0 / G, pos1 = sq.first + last / G;
-    const Tiles tl = tiles_of(a, pos0, pos1, St::kSlots);
-    const int per = (tl.count + static_cast<int>(part.splits) - 1) / static_cast<int>(part.splits);
-    const int t0 = static_cast<int>(split) * per, t1 = min(t0 + per, tl.count);
+    const int pos0 = sq.first + __builtin_amdgcn_readfirstlane(r0 / G), pos1 = sq.first + __builtin_amdgcn_readfirstlane(last / G);
+    const Tiles tl = uniform(tiles_of(a, pos0, pos1, St::kSlots));
+    const int per = __builtin_amdgcn_readfirstlane((tl.count + rt.shares - 1) / rt.shares);
+    const int t0 = rt.share * per, t1 = min(t0 + per, tl.count);
     // the group's tiles: t0 + first, + step, ..; as many steps for both
     constexpr int kEvery = kTurns ? 2 : 1;
     const int first = t0 + (kTurns ? static_cast<int>(group) : 0), steps = max(t1 - t0 + kEvery - 1, 0) / kEvery;
@@ -873,8 +944,9 @@ __global__ __launch_bounds__(512, 2) void rows_kernel(PagedDev a, PagedPart part
     const int w0 = r0 + 32 * static_cast<int>(wave), w1 = min(w0 + 31, last), r = w0 + static_cast<int>(n);
     const bool real = r <= last;
     const int qi = (real ? r : last) / G, pos = real ? sq.first + qi : -1;
-    const int wpos0 = sq.first + w0 / G, wpos1 = sq.first + w1 / G;   // of the wave's rows (w0 > last: none)
-    const Tiles wt = tiles_of(a, wpos0, w0 <= last ? wpos1 : -1, 1);
+    // of the wave's rows (w0 > last: none)
+    const int wpos0 = sq.first + __builtin_amdgcn_readfirstlane(w0 / G), wpos1 = sq.first + __builtin_amdgcn_readfirstlane(w1 / G);
+    const Tiles wt = uniform(tiles_of(a, wpos0, w0 <= last ? wpos1 : -1, 1));
     Query<CT, QT, D> q;
     q.load(reinterpret_cast<const T*>(a.q) + static_cast<uint64_t>(sq.row0 + qi) * a.q_row +
                (h * a.group + (real ? r : last) % G) * a.q_head,
@@ -1117,30 +1189,30 @@ __global__ __launch_bounds__(512, 2) void rows_kernel(PagedDev a, PagedPart part
     };
     for (int e = 0; e < kO; ++e) o[e] = f32x16{};
     if (steps > 0) {
+        // middle steps, as many at a time as there are places: tiles of the list whose slots all rows see, the one before
+        // too, and whose next one is whole and there
+        const int list = tl.second - tl.first;     // tile t of the list, behind the first ones, starts at slot 64 (t + list)
+        int lo = tl.first, hi = min((wpos0 + 1) / St::kSlots, tl.high / St::kSlots - kEvery) - list;
+        if (a.window)
+            lo = max(lo, static_cast<int>(max(static_cast<int64_t>(pos1) - a.reach + St::kSlots, static_cast<int64_t>(0)) /
+                                          St::kSlots) - list);
+        hi = min(hi, t1 - kEvery);
+        const int from = __builtin_amdgcn_readfirstlane(max(lo - first + kEvery - 1, 0) / kEvery + 1);
+        const int middles = __builtin_amdgcn_readfirstlane(
+            w0 <= last && wpos0 >= 0 ? max(hi - first + kEvery - 1, 0) / kEvery - from : 0);   // may be negative
+        int i = 0, ring = (kRing - from % kRing) % kRing;      // the first of the middle in the first place
         words = pages(0);
         next = pages(1);
-        fetch_keys(0, 0, words);
-        land_keys(0, 0);
+        fetch_keys(0, ring, words);
+        land_keys(0, ring);
         if (!kTurns) {
-            fetch_values(0, 0, words);
-            land_values(0, 0);
+            fetch_values(0, ring, words);
+            land_values(0, ring);
         }
         // the query is there: else the compiler waits for it at its every use, and for the copies under way with it
         __builtin_amdgcn_s_waitcnt(0x0f70);   // vmcnt(0)
         meet();
         if (group) meet();
-        // middle steps, as many at a time as there are places.  Tiles of the list whose slots all rows of the wave see, the
-        // one before too, and whose next one is whole and there
-        const int list = tl.second - tl.first;     // tile t of the list, behind the first ones, starts at slot 64 (t + list)
-        int lo = tl.first, hi = min((wpos0 + 1) / St::kSlots, tl.high / St::kSlots - kEvery) - list;
-        if (a.window)
-            lo = max(lo, static_cast<int>(max(static_cast<int64_t>(wpos1) - a.reach + St::kSlots, static_cast<int64_t>(0)) /
-                                          St::kSlots) - list);
-        hi = min(hi, t1 - kEvery);
-        const int i0 = max(lo - first + kEvery - 1, 0) / kEvery;
-        const int from = w0 <= last && wpos0 >= 0 ? (i0 + kRing) / kRing * kRing : steps;
-        const int middles = max(hi - first + kEvery - 1, 0) / kEvery - from;       // may be negative
-        int i = 0, ring = 0;
         auto steps_to = [&](int end) {
             for (; i < end; ++i) {
                 step(i, ring);
@@ -1230,6 +1302,7 @@ __global__ __launch_bounds__(512, 2) void rows_kernel(PagedDev a, PagedPart part
                     }
             }
         }
+        __syncthreads();
     }
     l += __shfl_xor(l, 32);
     constexpr int kShared = KS == 1 ? 0 : KS == 2 ? 1 : 2;   // outputs are 2^-kShared as large from here on
@@ -1260,9 +1333,9 @@ __global__ __launch_bounds__(512, 2) void rows_kernel(PagedDev a, PagedPart part
         }
         base = low;
     }
-    if (!real) return;
-    if (part.splits > 1) {
-        const uint64_t to = ((static_cast<uint64_t>(h) * part.units + u) * part.splits + split) * kRowTile + (r - r0);
+    if (rt.shares > 1) {
+        if (!real) return;
+        const uint64_t to = (static_cast<uint64_t>(h) * part.parts + rt.part + rt.share) * kRowTile + (r - r0);
         for (int e = 0; e < kO; ++e)
             for (int x = 0; x < 4; ++x)
                 *reinterpret_cast<f32x4*>(part.o + to * D + 32 * e + 8 * x + 4 * half) =
@@ -1273,44 +1346,72 @@ __global__ __launch_bounds__(512, 2) void rows_kernel(PagedDev a, PagedPart part
         }
         return;
     }
+    // through LDS, so that rows are written whole: the wave's 32 rows in 16-byte pieces at piece ^ row
+    constexpr int kPieces = D / 8;
+    uint8_t* mine_out = lds + (KS == 1 ? 32 * 2 * D : (16 * kO + 2) * 256) * wave;
     const float inv = l == 0.0f ? 0.0f : 1.0f / l * kPower<kShared>;
-    const uint32_t qh = h * a.group + static_cast<uint32_t>(r % G);
-    T* out = reinterpret_cast<T*>(a.out) + static_cast<uint64_t>(sq.row0 + qi) * a.o_row + qh * a.o_head;
+    const uint32_t qh = h * a.group + static_cast<uint32_t>((real ? r : last) % G);
     for (int e = 0; e < kO; ++e)
         for (int x = 0; x < 4; ++x) {
             typedef T T4 __attribute__((ext_vector_type(4)));
             T4 y;
             for (int k = 0; k < 4; ++k) y[k] = static_cast<T>(l == 0.0f ? 0.0f : o[e][4 * x + k] * inv);
-            *reinterpret_cast<T4*>(out + 32 * e + 8 * x + 4 * half) = y;
+            *reinterpret_cast<T4*>(mine_out + n * 2 * D + ((4 * e + x) ^ n % kPieces) * 16 + half * 8) = y;
         }
-    if (half == 0 && a.lse) a.lse[static_cast<uint64_t>(qh) * a.seq.rows + sq.row0 + qi] = lse_of(base, l);
+    const uint64_t to = static_cast<uint64_t>(sq.row0 + qi) * a.o_row + qh * a.o_head;
+    for (int x = 0; x < kPieces / 2; ++x) {
+        const uint32_t row = x * (64 / kPieces) + lane / kPieces, piece = lane % kPieces;
+        const u32x4 y = *reinterpret_cast<const u32x4*>(mine_out + row * 2 * D + (piece ^ row % kPieces) * 16);
+        const uint64_t where = __shfl(static_cast<unsigned long long>(to), static_cast<int>(row));
+        if (w0 + static_cast<int>(row) <= last)
+            *reinterpret_cast<u32x4*>(reinterpret_cast<T*>(a.out) + where + 8 * piece) = y;
+    }
+    if (real && half == 0 && a.lse) a.lse[static_cast<uint64_t>(qh) * a.seq.rows + sq.row0 + qi] = lse_of(base, l);
 }
 
-// rows_kernel's shares joined: D / 4 lanes a row, this many rows a workgroup.
-constexpr uint32_t join_rows(uint32_t dim) { return 1024 / dim; }
+// rows_kernel's shares joined, a wave a row, D / 64 channels a lane, this many rows
+// a workgroup.
+constexpr uint32_t kJoinRows = 16;
 template <int QT, int D>
 __global__ __launch_bounds__(256) void join_rows_kernel(PagedDev a, PagedPart part, int few) {
-    constexpr uint32_t kLanes = D / 4, kRows = join_rows(D);
-    const uint32_t blocks = part.rows / kRows, h = blockIdx.x % a.heads, b = blockIdx.x / a.heads % blocks;
-    const uint32_t u = blockIdx.x / a.heads / blocks;
-    RowTile rt;
-    if (!find_tile(a, u, few, static_cast<int>(part.rows), threadIdx.x % 64, &rt)) return;
-    const Seq sq = seq_of(a.seq, rt.seq, a.max_rows);
-    const uint32_t mine = b * kRows + threadIdx.x / kLanes, d = threadIdx.x % kLanes * 4;
-    const uint32_t r = static_cast<uint32_t>(rt.tile) * part.rows + mine;
-    if (r >= static_cast<uint32_t>(sq.rows) * a.group) return;
-    const uint64_t at = (static_cast<uint64_t>(h) * part.units + u) * part.splits * part.rows + mine;
-    float base = kInf, sum = 0.0f;
-    for (uint32_t s = 0; s < part.splits; ++s)
-        base = fminf(base, part.ml[2 * (at + static_cast<uint64_t>(part.rows) * s)]);
-    f32x4 o = {};
-    for (uint32_t s = 0; s < part.splits; ++s) {
-        const uint64_t x = at + static_cast<uint64_t>(part.rows) * s;
-        const float f = joined(base, part.ml[2 * x]);
-        sum += part.ml[2 * x + 1] * f;
-        o += *reinterpret_cast<const f32x4*>(part.o + x * D + d) * (f * kPower<-kJoinDown>);
+    using T = typename Elem<QT>::T;
+    constexpr int V = D / 64;
+    typedef float Vec __attribute__((ext_vector_type(V)));
+    typedef T Out __attribute__((ext_vector_type(V)));
+    const uint32_t lane = threadIdx.x % 64, wave = __builtin_amdgcn_readfirstlane(threadIdx.x / 64), all = a.seq.rows * a.group;
+    const uint32_t h = blockIdx.x % a.heads, b = blockIdx.x / a.heads * kJoinRows;
+    int s = -1;
+    Seq q{};
+    for (uint32_t x = b + wave; x < min(b + kJoinRows, all); x += 4) {
+        const int row = static_cast<int>(x / a.group);
+        if (s < 0 || row >= q.row0 + q.rows) {
+            s = seq_of_row(a.seq, row, lane);
+            if (s < 0) continue;
+            q = seq_of(a.seq, s, a.max_rows);
+        }
+        const int r = (row - q.row0) * static_cast<int>(a.group) + static_cast<int>(x % a.group);
+        if (row >= q.row0 + q.rows || static_cast<int64_t>(q.rows) * a.group <= few) continue;
+        const int first = part.plan[2 * s], shares = part.plan[2 * s + 1];
+        if (shares == 1) continue;
+        const int tile = r / static_cast<int>(part.rows);
+        const uint64_t at = (static_cast<uint64_t>(h) * part.parts + first + tile * shares) * part.rows +
+                            static_cast<uint64_t>(r - tile * static_cast<int>(part.rows));
+        float base = kInf, sum = 0.0f;
+        for (int y = 0; y < shares; ++y) base = fminf(base, part.ml[2 * (at + static_cast<uint64_t>(part.rows) * y)]);
+        Vec o = {};
+        for (int y = 0; y < shares; ++y) {
+            const uint64_t from = at + static_cast<uint64_t>(part.rows) * y;
+            const float f = joined(base, part.ml[2 * from]);
+            sum += part.ml[2 * from + 1] * f;
+            o += *reinterpret_cast<const Vec*>(part.o + from * D + V * lane) * (f * kPower<-kJoinDown>);
+        }
+        const uint32_t qh = h * a.group + x % a.group;
+        const float div = sum * kPower<-kPartDown - kJoinDown>;
+        Out y;
+        for (int e = 0; e < V; ++e) y[e] = static_cast<T>(sum == 0.0f ? 0.0f : o[e] / div);
+        *reinterpret_cast<Out*>(reinterpret_cast<T*>(a.out) + static_cast<uint64_t>(row) * a.o_row + qh * a.o_head + V * lane) = y;
+        if (lane == 0 && a.lse) a.lse[static_cast<uint64_t>(qh) * a.seq.rows + row] = lse_of(base, sum);
     }
-    write_row<QT>(a, sq.row0 + r / a.group, h * a.group + r % a.group, d, o, base, sum, kPower<-kPartDown - kJoinDown>);
 }
 
 uint32_t clears(const PagedDev& a) { return a.clear && a.seq.starts ? kClear : 0; }
@@ -1322,11 +1423,10 @@ struct Plan {
     bool few, many;                // sequences of few rows are looked for; of more
     uint32_t units, target, rows;  // decode_kernel: units a head at most, aimed at, rows of one
     uint64_t ml, plan;             // offsets in the workspace (partial outputs first)
-    int ks;                        // rows_kernel: shares of a tile's slots among a workgroup's waves
-    uint32_t tiles, splits;        // row tiles a head at most, shares of the slots
-    uint64_t rows_ml, bytes;       // the two kernels follow each other in the same workspace; all of it
+    int ks;                        // rows_kernel: 256 / ks rows a tile
+    uint32_t row_units, row_target, parts;   // units a head at most, shares aimed at (0: none), room for
+    uint64_t rows_ml, rows_plan, bytes;      // the two kernels follow each other in the same workspace; all of it
 };
-constexpr uint32_t kMaxShares = 64;     // of many rows
 Plan plan_of(const PagedDev& a, uint32_t dim, int cache_dtype) {
     Plan p{};
     const uint64_t most = static_cast<uint64_t>(a.max_rows) * a.group;
@@ -1352,35 +1452,40 @@ Plan plan_of(const PagedDev& a, uint32_t dim, int cache_dtype) {
         p.bytes = p.plan + round256(8ull * a.seq.seqs);
     }
     if (p.many) {
-        // The least time, in tenths of a step of shared tiles (KS 1; 2 and 4 take two tiles a step): as many workgroups as
-        // there are CUs run at the speed of one, a share costs four steps' time for its start and end, and the passage of
-        // its outputs through memory.
-        uint64_t least = ~0ull;
+        // The least time, in tenths of a step of shared tiles (KS 1; 2 and 4 take two tiles a step): the steps of a CU's
+        // workgroups, one after the other, and about six steps' time for the start and end of each.
+        uint64_t least = ~0ull, tiles = 0;
         for (int ks = 1; ks <= 4; ks *= 2) {
             const uint64_t rt = rows_of_tile(ks);
-            const uint64_t row_tiles = std::min((static_cast<uint64_t>(a.seq.rows) * a.group + rt - 1) / rt + a.seq.seqs,
-                                                a.seq.seqs * ((most + rt - 1) / rt));
-            const uint64_t groups = a.heads * row_tiles, tiles = tiles_for(rt, 64);
-            for (uint32_t n = 1; n <= kMaxShares && (n == 1 || n * 4 <= tiles); ++n) {
-                const uint64_t rounds = (groups * n + 255) / 256, each = (tiles + n - 1) / n;
-                const uint64_t cost = rounds * ((ks == 1 ? each : (each + 1) / 2) + (n == 1 ? 2 : 4)) * (ks == 4 ? 8 : ks == 2 ? 12 : 10) +
-                                      (n == 1 ? 0 : groups * rt * dim * 8 * n / 800000);
-                if (cost < least) {
-                    least = cost;
-                    p.splits = n;
-                    p.ks = ks;
-                    p.tiles = static_cast<uint32_t>(row_tiles);
-                }
+            const uint64_t n = std::min((static_cast<uint64_t>(a.seq.rows) * a.group + rt - 1) / rt + a.seq.seqs,
+                                        a.seq.seqs * ((most + rt - 1) / rt));
+            const uint64_t steps = (tiles_for(rt, 64) + (ks > 1 ? 1 : 0)) / (ks > 1 ? 2 : 1);
+            const uint64_t rounds = (a.heads * n + 255) / 256;
+            const uint64_t cost = rounds * (steps + 6) * (ks == 4 ? 8 : ks == 2 ? 12 : 10);
+            if (cost < least) {
+                least = cost;
+                p.ks = ks;
+                tiles = n;
             }
         }
-        if (p.splits > 1) {
-            const uint64_t rows = static_cast<uint64_t>(a.heads) * p.tiles * p.splits * rows_of_tile(p.ks);
+        // Shares, where a call has less than three row tiles a CU: of a CU's work and more, of half of that where there
+        // are more tiles than CUs (20 sequences of 600 to 6,000 slots with chunks of up to 512 rows: 267 us without).
+        const uint64_t groups = a.heads * tiles;
+        p.row_target = groups < 768 && tiles_for(rows_of_tile(p.ks), 64) >= 2 * kLeastSteps
+                           ? static_cast<uint32_t>(((groups > 256 ? 512 : 256) + a.heads - 1) / a.heads) : 0;
+        p.parts = p.row_target;
+        p.row_units = static_cast<uint32_t>(tiles) + p.row_target;
+        if (p.row_target) {
+            const uint64_t rows = static_cast<uint64_t>(a.heads) * p.parts * rows_of_tile(p.ks);
             p.rows_ml = round256(rows * dim * 4);
-            p.bytes = std::max(p.bytes, p.rows_ml + round256(rows * 8));
+            p.rows_plan = p.rows_ml + round256(rows * 8);
+            p.bytes = std::max(p.bytes, p.rows_plan + round256(8ull * a.seq.seqs));
         }
     }
     return p;
 }
+
+uint32_t join_blocks(const PagedDev& a) { return (a.seq.rows * a.group + kJoinRows - 1) / kJoinRows; }
 
 template <int CT, int QT, int D, bool PAGED>
 int attend_typed(const PagedDev& a, uint8_t* ws, hipStream_t st) {
@@ -1388,20 +1493,20 @@ int attend_typed(const PagedDev& a, uint8_t* ws, hipStream_t st) {
     if constexpr (PAGED)
         if (p.few) {
             const PagedPart part{reinterpret_cast<float*>(ws), reinterpret_cast<float*>(ws + p.ml),
-                                 reinterpret_cast<int32_t*>(ws + p.plan), p.units, p.target, p.rows, 1};
+                                 reinterpret_cast<int32_t*>(ws + p.plan), p.units, p.target, p.rows, p.units};
             decode_kernel<CT, QT, D><<<a.heads * p.units + clears(a), 256, 0, st>>>(a, part);
             if (p.units > a.seq.seqs) join_kernel<QT, D><<<a.seq.seqs * a.heads * p.rows, 256, 0, st>>>(a, part);
         }
     if (p.many) {
-        const PagedPart part{reinterpret_cast<float*>(ws), reinterpret_cast<float*>(ws + p.rows_ml), nullptr, p.tiles, 0,
-                             static_cast<uint32_t>(rows_of_tile(p.ks)), p.splits};
+        const PagedPart part{reinterpret_cast<float*>(ws), reinterpret_cast<float*>(ws + p.rows_ml),
+                             reinterpret_cast<int32_t*>(ws + p.rows_plan), p.row_units, p.row_target,
+                             static_cast<uint32_t>(rows_of_tile(p.ks)), p.parts};
         const int few = PAGED && p.few ? kFew : 0;
-        const uint32_t grid = a.heads * p.tiles * p.splits + (p.few ? 0 : clears(a));
+        const uint32_t grid = a.heads * p.row_units + (p.few ? 0 : clears(a));
         if (p.ks == 4) rows_kernel<CT, QT, D, PAGED, 4><<<grid, 512, 0, st>>>(a, part, few);
         else if (p.ks == 2) rows_kernel<CT, QT, D, PAGED, 2><<<grid, 512, 0, st>>>(a, part, few);
         else rows_kernel<CT, QT, D, PAGED, 1><<<grid, 512, 0, st>>>(a, part, few);
-        if (p.splits > 1)
-            join_rows_kernel<QT, D><<<a.heads * p.tiles * (part.rows / join_rows(D)), 256, 0, st>>>(a, part, few);
+        if (p.row_target) join_rows_kernel<QT, D><<<a.heads * join_blocks(a), 256, 0, st>>>(a, part, few);
     }
     return hipGetLastError();
 }
@@ -1441,9 +1546,8 @@ bool paged_fits(const PagedDev& a, uint32_t dim, int cache_dtype) {
     if (p.few)
         blocks = std::max(static_cast<uint64_t>(a.heads) * p.units, static_cast<uint64_t>(a.seq.seqs) * a.heads * p.rows);
     if (p.many) {
-        const uint64_t tiles = static_cast<uint64_t>(a.heads) * p.tiles;
-        blocks = std::max(blocks, tiles * p.splits);
-        if (p.splits > 1) blocks = std::max<uint64_t>(blocks, tiles * (rows_of_tile(p.ks) / join_rows(dim)));
+        blocks = std::max(blocks, static_cast<uint64_t>(a.heads) * p.row_units);
+        if (p.row_target) blocks = std::max(blocks, static_cast<uint64_t>(a.heads) * join_blocks(a));
     }
     return blocks < (1u << 23) - kClear;     // workgroups of up to 512 threads
 }
