@@ -13,10 +13,12 @@ using namespace pkv;
 
 namespace {
 
+constexpr uint32_t kMaxHeads = 1u << 16;
+
 int check_pages(const pkv_page_view& v, bool written) {
     if (v.dim != 64 && v.dim != 128) return PKV_ERR_UNSUPPORTED;
     if (v.dtype != PKV_BF16 && v.dtype != PKV_F16 && v.dtype != PKV_FP8) return PKV_ERR_INVALID_ARG;
-    if (!v.layers || !v.pages || !v.heads || v.pages > kMaxCount || v.layers > kMaxCount || v.heads > kMaxCount)
+    if (!v.layers || !v.pages || !v.heads || v.pages > kMaxCount || v.layers > kMaxCount || v.heads > kMaxHeads)
         return PKV_ERR_INVALID_ARG;
     if (v.page_slots < 16 || v.page_slots > 65536 || (v.page_slots & (v.page_slots - 1))) return PKV_ERR_INVALID_ARG;
     if (!v.d_keys || !v.d_values || !aligned(v.d_keys, 16) || !aligned(v.d_values, 16)) return PKV_ERR_INVALID_ARG;
@@ -111,7 +113,7 @@ int check_paged_shape(const pkv_paged_attend_op& op) {
     if (v.dim != 64 && v.dim != 128) return PKV_ERR_UNSUPPORTED;
     if (op.dtype != PKV_BF16 && op.dtype != PKV_F16) return PKV_ERR_INVALID_ARG;
     if (v.dtype != PKV_FP8 && op.dtype != v.dtype) return PKV_ERR_INVALID_ARG;
-    if (v.layers != 1 || !v.heads || v.page_slots < 16 || v.page_slots > 65536 || (v.page_slots & (v.page_slots - 1)))
+    if (v.layers != 1 || !v.heads || v.heads > kMaxHeads || v.page_slots < 16 || v.page_slots > 65536 || (v.page_slots & (v.page_slots - 1)))
         return PKV_ERR_INVALID_ARG;
     if (!op.q_heads || op.q_heads % v.heads || op.clear > 1) return PKV_ERR_INVALID_ARG;
     const int rc = check_counts(op.seqs, v.page_slots);
@@ -148,7 +150,7 @@ PagedDev prompts_dev(const pkv_prompts_op& op) {
 int check_prompts_shape(const pkv_prompts_op& op) {
     if (op.dim != 64 && op.dim != 128) return PKV_ERR_UNSUPPORTED;
     if (op.dtype != PKV_BF16 && op.dtype != PKV_F16) return PKV_ERR_INVALID_ARG;
-    if (!op.heads || !op.q_heads || op.q_heads % op.heads || op.clear > 1) return PKV_ERR_INVALID_ARG;
+    if (!op.heads || op.heads > kMaxHeads || !op.q_heads || op.q_heads % op.heads || op.clear > 1) return PKV_ERR_INVALID_ARG;
     if (!op.seqs || op.seqs > 1u << 24 || op.rows > kMaxRows) return PKV_ERR_INVALID_ARG;
     if (static_cast<U128>(op.rows) * op.q_heads > kMaxRows) return PKV_ERR_INVALID_ARG;
     if (op.rows && !paged_fits(prompts_dev(op), op.dim, op.dtype)) return PKV_ERR_INVALID_ARG;

@@ -87,7 +87,7 @@ __device__ inline void chunk_places(const PagedRowsDev& a, uint32_t first, int64
 // step, channels fastest, then rows, then heads: rows of a sequence that follow
 // each other are neighbours in a page, so that a step writes whole lines.
 template <int CT, int QT, int D>
-__global__ __launch_bounds__(256) void paged_store_kernel(PagedRowsDev a) {
+__global__ __launch_bounds__(256) void paged_store_kernel(PagedRowsDev a, uint32_t heads) {
     using T = typename Elem<QT>::T;
     constexpr uint32_t V = 8, kRow = D / V;
     typedef T Vec __attribute__((ext_vector_type(V)));
@@ -98,8 +98,9 @@ __global__ __launch_bounds__(256) void paged_store_kernel(PagedRowsDev a) {
     uint8_t* dst = blockIdx.y ? a.v : a.k;
     uint8_t* dsc = blockIdx.y ? a.vs : a.ks;
     chunk_places(a, chunk * kChunk, places);
-    for (uint32_t x = threadIdx.x; x < a.heads * kChunk * kRow; x += 256) {
-        const uint32_t d = x % kRow * V, i = x / kRow % kChunk, h = x / kRow / kChunk;
+    const uint32_t h0 = blockIdx.z * heads, pieces = min(heads, a.heads - h0) * kChunk * kRow;
+    for (uint32_t x = threadIdx.x; x < pieces; x += 256) {
+        const uint32_t d = x % kRow * V, i = x / kRow % kChunk, h = h0 + x / kRow / kChunk;
         const bool there = places[i] >= 0;
         // rows without a place read the chunk's first
         const uint64_t from = layer * a.layer + static_cast<uint64_t>(chunk * kChunk + (there ? i : 0)) * a.row + h * a.head;
@@ -142,7 +143,7 @@ __global__ __launch_bounds__(256) void paged_store_kernel(PagedRowsDev a) {
 
 // The same the other way, 16 bytes of the written tensor a thread and step.
 template <int CT, int QT, int D>
-__global__ __launch_bounds__(256) void paged_load_kernel(PagedRowsDev a) {
+__global__ __launch_bounds__(256) void paged_load_kernel(PagedRowsDev a, uint32_t heads) {
     using T = typename Elem<QT>::T;
     constexpr uint32_t V = QT == PKV_F32 ? 4 : 8, kRow = D / V;
     typedef T Vec __attribute__((ext_vector_type(V)));
@@ -153,8 +154,9 @@ __global__ __launch_bounds__(256) void paged_load_kernel(PagedRowsDev a) {
     const uint8_t* src = blockIdx.y ? a.v : a.k;
     const uint8_t* ssc = blockIdx.y ? a.vs : a.ks;
     chunk_places(a, chunk * kChunk, places);
-    for (uint32_t x = threadIdx.x; x < a.heads * kChunk * kRow; x += 256) {
-        const uint32_t d = x % kRow * V, i = x / kRow % kChunk, h = x / kRow / kChunk;
+    const uint32_t h0 = blockIdx.z * heads, pieces = min(heads, a.heads - h0) * kChunk * kRow;
+    for (uint32_t x = threadIdx.x; x < pieces; x += 256) {
+        const uint32_t d = x % kRow * V, i = x / kRow % kChunk, h = h0 + x / kRow / kChunk;
         if (chunk * kChunk + i >= a.seq.rows) continue;
         const bool there = places[i] >= 0;
         const uint64_t from = layer * a.p_layer + h * a.p_head + (there ? places[i] : 0) + d;   // a place that is read, not used
@@ -228,7 +230,9 @@ __device__ inline void write_row(const PagedDev& a, uint32_t r, uint32_t qh, uin
 // ------------------------------------------------------------ few rows: split over the slots
 constexpr int kFew = 16;            // rows x group of a KV head that decode_kernel takes
 constexpr int kStep = 32;           // slots of its tiles
-constexpr uint32_t kUnits = 1024;   // units of all heads that it aims at
+constexpr int wide_waves(uint32_t dim, int cache_dtype) { return dim == 64 && cache_dtype != PKV_FP8 ? 16 : 8; }
+// Units of all heads that fit the chip at once: two workgroups a CU, by their registers four of the small tiles.
+constexpr uint32_t fitting_units(uint32_t dim, int cache_dtype) { return dim == 64 ? cache_dtype == PKV_FP8 ? 768 : 1024 : 512; }
 constexpr int kLeast = 4;           // tiles of a unit, one a wave
 constexpr int kLeastSteps = 8;      // rows_kernel: tiles of 64 slots of a share
 
@@ -429,15 +433,17 @@ struct PagedPart {
 //                 in S^T: the softmax's registers are B as they are, v_perm
 //                 gathers each channel across the lane's four (x 2) slots.
 // Weights meet the values as two terms of a 16-bit type, which the bytes hide.
-// The next tile is on its way while one is worked on, and the words of the pages
+// WAVES 4, or 8 or 16 (as registers allow) where a sequence's slots are one
+// unit's, so that the call is one launch.  The next tile is on its way while one is worked on, and the words of the pages
 // of the one after it, so that no read waits for a page's number.
-template <int CT, int QT, int D>
-__global__ __launch_bounds__(256, 2) void decode_kernel(PagedDev a, PagedPart part) {
+template <int CT, int QT, int D, int WAVES>
+__global__ __launch_bounds__(64 * WAVES, WAVES > 8 ? 4 : 2) void decode_kernel(PagedDev a, PagedPart part) {
     using T = typename Elem<QT>::T;
     using Tile = PageTile<CT, D>;
     constexpr int MT = mat_type(CT), NQ = query_terms(CT, QT), NP = 2, kQ = D / 32, kO = D / 16;
+    constexpr int kDownOf = WAVES > 4 ? kPartDown + 2 : kPartDown;   // the waves' outputs together
     const uint32_t work_blocks = a.heads * part.units;
-    if (blockIdx.x >= work_blocks) return clear_rows<QT, D>(a, blockIdx.x - work_blocks);
+    if (blockIdx.x >= work_blocks) return clear_rows<QT, D, 64 * WAVES>(a, blockIdx.x - work_blocks);
     const uint32_t lane = threadIdx.x % 64, wave = __builtin_amdgcn_readfirstlane(threadIdx.x / 64);
     // heads fastest, so that a head's workgroups share an XCD's L2 (and the pages of a common prefix) where the heads
     // are a multiple of 8
@@ -567,16 +573,16 @@ __global__ __launch_bounds__(256, 2) void decode_kernel(PagedDev a, PagedPart pa
     const int first = t0 + static_cast<int>(wave);
     if (first < t1) {
         Tile even, odd;
-        int words = pages(first), next = pages(first + 4);
+        int words = pages(first), next = pages(first + WAVES);
         fetch(even, first, words);
-        for (int t = first; t < t1; t += 8) {
-            words = pages(t + 8);
-            fetch(odd, t + 4, next);
+        for (int t = first; t < t1; t += 2 * WAVES) {
+            words = pages(t + 2 * WAVES);
+            fetch(odd, t + WAVES, next);
             work(even, t, std::false_type());
-            if (t + 4 >= t1) break;
-            next = pages(t + 12);
-            fetch(even, t + 8, words);
-            work(odd, t + 4, std::false_type());
+            if (t + WAVES >= t1) break;
+            next = pages(t + 3 * WAVES);
+            fetch(even, t + 2 * WAVES, words);
+            work(odd, t + WAVES, std::false_type());
         }
         // An infinity or NaN among the values: a row that does not see it has met it with the weight 0, and the terms
         // of a weight that does see it may be 0 or negative.  Again, with those values taken out of the products and
@@ -589,7 +595,7 @@ __global__ __launch_bounds__(256, 2) void decode_kernel(PagedDev a, PagedPart pa
             l = 0.0f;
             for (int e = 0; e < kO; ++e) o[e] = f32x4{};
 #pragma unroll 1
-            for (int t = first; t < t1; t += 4) {
+            for (int t = first; t < t1; t += WAVES) {
                 fetch(even, t, pages(t));
                 work(even, t, std::true_type());
             }
@@ -608,24 +614,25 @@ __global__ __launch_bounds__(256, 2) void decode_kernel(PagedDev a, PagedPart pa
     l += __shfl_xor(l, 16);
     l += __shfl_xor(l, 32);
 
-    // the four waves' shares joined; a sequence of one unit is done
-    __shared__ float so[4][16][D + 4], sb[4][16], sl[4][16];
+    // the waves' shares joined; a sequence of one unit is done
+    __shared__ float so[WAVES][16][D + 4], sb[WAVES][16], sl[WAVES][16];
     for (int r = 0; r < 4; ++r)
         for (int e = 0; e < kO; ++e) so[wave][row][Tile::out_channel(e, r, g)] = o[e][r];
     if (g == 0) { sb[wave][row] = base; sl[wave][row] = l; }
     __syncthreads();
-    for (uint32_t x = threadIdx.x; x < static_cast<uint32_t>(R) * (D / 4); x += 256) {
+    for (uint32_t x = threadIdx.x; x < static_cast<uint32_t>(R) * (D / 4); x += 64 * WAVES) {
         const uint32_t r = x / (D / 4), d = x % (D / 4) * 4;
-        const float low = fminf(fminf(sb[0][r], sb[1][r]), fminf(sb[2][r], sb[3][r]));
+        float low = sb[0][r];
+        for (int w = 1; w < WAVES; ++w) low = fminf(low, sb[w][r]);
         float sum = 0.0f;
         f32x4 acc = {};
-        for (int w = 0; w < 4; ++w) {
+        for (int w = 0; w < WAVES; ++w) {
             const float f = joined(low, sb[w][r]);
             sum += sl[w][r] * f;
-            acc += *reinterpret_cast<const f32x4*>(&so[w][r][d]) * (f * kPower<-kPartDown>);
+            acc += *reinterpret_cast<const f32x4*>(&so[w][r][d]) * (f * kPower<-kDownOf>);
         }
         if (unit.shares == 1) {
-            write_row<QT>(a, sq.row0 + r / a.group, h * a.group + r % a.group, d, acc, low, sum, kPower<-kPartDown>);
+            write_row<QT>(a, sq.row0 + r / a.group, h * a.group + r % a.group, d, acc, low, sum, kPower<-kDownOf>);
         } else {
             const uint64_t at = (static_cast<uint64_t>(h) * part.units + u) * part.rows + r;
             *reinterpret_cast<f32x4*>(part.o + at * D + d) = acc;
@@ -1421,7 +1428,8 @@ uint64_t round256(uint64_t x) { return (x + 255) & ~255ull; }
 // The launches of a call and its workspace.
 struct Plan {
     bool few, many;                // sequences of few rows are looked for; of more
-    uint32_t units, target, rows;  // decode_kernel: units a head at most, aimed at, rows of one
+    bool wide;                     // decode_kernel: whole sequences, more waves each
+    uint32_t units, target, rows;  // units a head at most, aimed at, rows of one
     uint64_t ml, plan;             // offsets in the workspace (partial outputs first)
     int ks;                        // rows_kernel: 256 / ks rows a tile
     uint32_t row_units, row_target, parts;   // units a head at most, shares aimed at (0: none), room for
@@ -1443,8 +1451,13 @@ Plan plan_of(const PagedDev& a, uint32_t dim, int cache_dtype) {
     };
     if (p.few) {
         p.rows = static_cast<uint32_t>(std::min<uint64_t>(kFew, most));
-        p.target = (kUnits + a.heads - 1) / a.heads;
-        const uint64_t each = std::max<uint64_t>(1, (tiles_for(kFew, kStep) + kLeast - 1) / kLeast);
+        // what fits at once, less half a unit a sequence for those that are not whole
+        const uint32_t fit = fitting_units(dim, cache_dtype) / a.heads;
+        p.target = std::max(fit > a.seq.seqs / 2 ? fit - a.seq.seqs / 2 : 1, std::max(fit / 4, 1u));
+        const uint64_t tiles = tiles_for(kFew, kStep);
+        p.wide = static_cast<uint64_t>(a.seq.seqs) * a.heads <= 256 && tiles <= 4ull * wide_waves(dim, cache_dtype);
+        if (p.wide) p.target = 1;
+        const uint64_t each = p.wide ? 1 : std::max<uint64_t>(1, (tiles + kLeast - 1) / kLeast);
         p.units = static_cast<uint32_t>(std::min<uint64_t>(static_cast<uint64_t>(a.seq.seqs) + p.target, a.seq.seqs * each));
         const uint64_t rows = static_cast<uint64_t>(a.heads) * p.units * p.rows;
         p.ml = round256(rows * dim * 4);
@@ -1494,7 +1507,10 @@ int attend_typed(const PagedDev& a, uint8_t* ws, hipStream_t st) {
         if (p.few) {
             const PagedPart part{reinterpret_cast<float*>(ws), reinterpret_cast<float*>(ws + p.ml),
                                  reinterpret_cast<int32_t*>(ws + p.plan), p.units, p.target, p.rows, p.units};
-            decode_kernel<CT, QT, D><<<a.heads * p.units + clears(a), 256, 0, st>>>(a, part);
+            const uint32_t grid = a.heads * p.units + clears(a);
+            constexpr int kWide = wide_waves(D, CT);
+            if (p.wide) decode_kernel<CT, QT, D, kWide><<<grid, 64 * kWide, 0, st>>>(a, part);
+            else decode_kernel<CT, QT, D, 4><<<grid, 256, 0, st>>>(a, part);
             if (p.units > a.seq.seqs) join_kernel<QT, D><<<a.seq.seqs * a.heads * p.rows, 256, 0, st>>>(a, part);
         }
     if (p.many) {
@@ -1517,9 +1533,13 @@ int attend_dim(const PagedDev& a, uint32_t dim, uint8_t* ws, hipStream_t st) {
 
 template <int CT, int QT, int D>
 int rows_typed(const PagedRowsDev& r, bool store, hipStream_t st) {
-    const dim3 grid((r.seq.rows + kChunk - 1) / kChunk * r.layers, 2);
-    if (store) paged_store_kernel<CT, QT, D><<<grid, 256, 0, st>>>(r);
-    else paged_load_kernel<CT, QT, D><<<grid, 256, 0, st>>>(r);
+    // four workgroups a CU where there are heads enough (64 single rows of 8 heads of 128: 7.8 us with all heads in one)
+    const uint32_t chunks = (r.seq.rows + kChunk - 1) / kChunk * r.layers;
+    uint32_t heads = r.heads;
+    while (heads > 1 && 2ull * chunks * ((r.heads + heads - 1) / heads) < 1024) heads = (heads + 1) / 2;
+    const dim3 grid(chunks, 2, (r.heads + heads - 1) / heads);
+    if (store) paged_store_kernel<CT, QT, D><<<grid, 256, 0, st>>>(r, heads);
+    else paged_load_kernel<CT, QT, D><<<grid, 256, 0, st>>>(r, heads);
     return hipGetLastError();
 }
 template <int CT>
