@@ -41,6 +41,15 @@ int check_pages(const pkv_page_view& v, bool written) {
     return PKV_OK;
 }
 
+// Whether rows of a call lie on the pages that it reads or writes.
+bool over_pages(const pkv_page_view& v, const void* p, uint64_t bytes) {
+    const Axis a[4] = {{v.layer_stride, v.layers}, {v.page_stride, v.pages}, {v.head_stride, v.heads},
+                       {v.slot_stride, v.page_slots}};
+    const uint64_t e = extent(a, 4, v.dim), size = v.dtype == PKV_FP8 ? e : 2 * e;
+    if (overlap(v.d_keys, size, p, bytes) || overlap(v.d_values, size, p, bytes)) return true;
+    return v.dtype == PKV_FP8 && (overlap(v.d_key_scales, e / 32, p, bytes) || overlap(v.d_value_scales, e / 32, p, bytes));
+}
+
 // Counts only: what a workspace's size goes by.
 int check_counts(const pkv_sequences& s, uint32_t page_slots) {
     if (!s.seqs || !s.table_pages || s.reserved || s.seqs > 1u << 24 || s.rows > kMaxRows) return PKV_ERR_INVALID_ARG;
@@ -113,7 +122,8 @@ int check_paged_shape(const pkv_paged_attend_op& op) {
     if (v.dim != 64 && v.dim != 128) return PKV_ERR_UNSUPPORTED;
     if (op.dtype != PKV_BF16 && op.dtype != PKV_F16) return PKV_ERR_INVALID_ARG;
     if (v.dtype != PKV_FP8 && op.dtype != v.dtype) return PKV_ERR_INVALID_ARG;
-    if (v.layers != 1 || !v.heads || v.heads > kMaxHeads || v.page_slots < 16 || v.page_slots > 65536 || (v.page_slots & (v.page_slots - 1)))
+    if (v.layers != 1 || !v.heads || v.heads > kMaxHeads || v.page_slots < 16 || v.page_slots > 65536 ||
+        (v.page_slots & (v.page_slots - 1)))
         return PKV_ERR_INVALID_ARG;
     if (!op.q_heads || op.q_heads % v.heads || op.clear > 1) return PKV_ERR_INVALID_ARG;
     const int rc = check_counts(op.seqs, v.page_slots);
@@ -175,12 +185,15 @@ int run_rows(pkv_ctx* ctx, const pkv_paged_rows_op* op, void* stream, bool store
     if (!aligned(op->d_keys, 16) || !aligned(op->d_values, 16)) return PKV_ERR_INVALID_ARG;
     const uint64_t unit = 16 / elem_bytes(op->dtype);
     if (op->layer_stride % unit || op->row_stride % unit || op->head_stride % unit) return PKV_ERR_INVALID_ARG;
-    const Axis a[3] = {{op->layer_stride, v.layers}, {op->row_stride, std::max(op->seqs.rows, 1u)},
-                       {op->head_stride, v.heads}};
-    if (!extent(a, 3, v.dim) || (!store && !distinct(a, 3, v.dim))) return PKV_ERR_INVALID_ARG;
+    if (!op->seqs.rows || (!op->d_keys && !op->d_values)) return PKV_OK;
+    const Axis a[3] = {{op->layer_stride, v.layers}, {op->row_stride, op->seqs.rows}, {op->head_stride, v.heads}};
+    const uint64_t bytes = extent(a, 3, v.dim) * elem_bytes(op->dtype);
+    if (!bytes || (!store && !distinct(a, 3, v.dim))) return PKV_ERR_INVALID_ARG;
+    for (const void* rows : {op->d_keys, op->d_values})
+        if (rows && over_pages(v, rows, bytes)) return PKV_ERR_INVALID_ARG;
+    if (!store && op->d_keys && op->d_values && overlap(op->d_keys, bytes, op->d_values, bytes)) return PKV_ERR_INVALID_ARG;
     // the launch: a workgroup of each layer and side for every 16 rows
     if (static_cast<U128>((op->seqs.rows + 15ull) / 16) * v.layers >= 1u << 24) return PKV_ERR_INVALID_ARG;
-    if (!op->seqs.rows || (!op->d_keys && !op->d_values)) return PKV_OK;
     PagedRowsDev r{};
     r.seq = seqs_dev(op->seqs, v);
     r.k = static_cast<uint8_t*>(v.d_keys);
@@ -234,6 +247,11 @@ int pkv_paged_attend(pkv_ctx* ctx, const pkv_paged_attend_op* op, void* stream) 
     if (!rc) rc = check_pages(op->pages, false);
     if (!rc) rc = check_sequences(op->seqs, op->pages.page_slots);
     if (rc) return rc;
+    if (op->seqs.rows) {
+        const uint64_t on = row_bytes(op->d_out, op->out_row_stride, op->out_head_stride, op->seqs.rows, op->q_heads,
+                                      op->pages.dim, true);
+        if (!on || over_pages(op->pages, op->d_out, on)) return PKV_ERR_INVALID_ARG;
+    }
     return run_attend(ctx, paged_dev(*op), op->pages.dim, op->pages.dtype, op->dtype, op->scale, op->d_workspace,
                       op->workspace_bytes, stream);
 }
