@@ -74,7 +74,7 @@ __device__ inline void chunk_places(const PagedRowsDev& a, uint32_t first, int64
         if (s >= 0) {
             const Seq q = seq_of(a.seq, s, a.seq.rows);
             const int j = q.first + r - q.row0;
-            const int page = j >= 0 ? page_of(a.seq, s, j) : -1;
+            const int page = j >= 0 && j < q.len ? page_of(a.seq, s, j) : -1;   // behind it: starts that do not ascend
             if (page >= 0)
                 at = static_cast<int64_t>(page * a.page + (static_cast<uint32_t>(j) & ((1u << a.seq.shift) - 1)) * a.slot);
         }
@@ -718,7 +718,7 @@ __device__ inline bool find_rows(const PagedDev& a, uint32_t u, int64_t few, int
     for (uint32_t s = s0; s < s1; ++s) {
         const RowWork w = per == 1 ? mine : row_work(a, s, few, rows);
         const int n = shares(w);
-        units += w.tiles * n;
+        units = min(units + w.tiles * n, 1 << 24);   // no launch has as many; more where starts do not ascend
         parts += n > 1 ? w.tiles * n : 0;
         longest = max(longest, w.steps / n);
     }
@@ -1401,6 +1401,8 @@ __global__ __launch_bounds__(256) void join_rows_kernel(PagedDev a, PagedPart pa
         const int first = part.plan[2 * s], shares = part.plan[2 * s + 1];
         if (shares == 1) continue;
         const int tile = r / static_cast<int>(part.rows);
+        // starts that do not ascend may have more units than the launch, and no plan for the last
+        if (first < 0 || shares < 1 || first + (tile + 1ll) * shares > static_cast<int64_t>(part.parts)) continue;
         const uint64_t at = (static_cast<uint64_t>(h) * part.parts + first + tile * shares) * part.rows +
                             static_cast<uint64_t>(r - tile * static_cast<int>(part.rows));
         float base = kInf, sum = 0.0f;

@@ -449,3 +449,29 @@ def test_no_rows(ctx):
     assert attend_prompts(q, q[:, :2], q[:, 2:], words([0, 0])).shape == q.shape
     keys, values = cache.load(0, words(tables), words([20]))
     cache.store(keys, values, words(tables), words([20]))
+
+
+@pytest.mark.parametrize("starts", [[0, 20, 5, 6], [0, 300, 0, 300], [300, 200, 100, 0], [-5, 7, 10 ** 9, 3]])
+def test_starts_that_do_not_ascend(ctx, starts):
+    """Whose a row is, is not said, but nothing out of a sequence's own slots is
+    touched: what follows its table names a page that no call may write or read."""
+    from provekv_amd.paged import PagedKVCache, attend_prompts
+    lens, page = [320, 320, 320], 16
+    cache = PagedKVCache(1, 2, 61 + 1, page, 64, dtype=BF16)
+    cache.buf.fill_(1.0)
+    cache.buf[:, 61] = math.nan
+    wide = torch.full((3, 60), 61, dtype=torch.int32, device="cuda")
+    wide[:, :20] = torch.arange(60, dtype=torch.int32, device="cuda").view(3, 20)
+    tables, n, st = wide[:, :20], words(lens), words(starts)
+    rows = torch.full((1, 300, 2, 64), 2.0, dtype=BF16, device="cuda")
+    cache.store(rows, rows, tables, n, starts=st)
+    torch.cuda.synchronize()
+    assert torch.isnan(cache.buf[:, 61]).all() and not torch.isnan(cache.buf[:, :61]).any()
+    for back in cache.load(300, tables, n, starts=st):
+        assert not torch.isnan(back).any()
+    for G in (1, 4):
+        q = torch.ones(300, 2 * G, 64, dtype=BF16, device="cuda")
+        out = torch.zeros_like(q)
+        cache.attend(0, q, tables, n, starts=st, out=out)
+        attend_prompts(q, q[:, :2], q[:, :2], st, out=out)
+        torch.cuda.synchronize()
