@@ -676,7 +676,7 @@ int pkv_evict(pkv_ctx* ctx, const pkv_evict_op* op, void* stream);
  * power of two, 16 .. 65,536) of dim (64 or 128) elements.  Row j of (layer l,
  * page p, head h) starts at element l * layer_stride + p * page_stride + h *
  * head_stride + j * slot_stride of d_keys and of d_values; elems bounds every
- * such row's end (checked).  slot_stride is at most 2^22.
+ * such row's end (checked).  heads is at most 65,536, slot_stride at most 2^22.
  *   PKV_BF16, PKV_F16: pointers 16-byte aligned, strides a multiple of 16 bytes;
  *     scale pointers NULL.
  *   PKV_FP8: OCP MX FP8, a byte a value: e4m3 codes (no infinity; 0x7f and 0xff
@@ -732,8 +732,9 @@ typedef struct pkv_sequences {
  *     is not stored.  Two rows must not name the same place of the same page.
  *   load: the values the pages hold, rounded to dtype (exact in f32, and in bf16
  *     from PKV_FP8).  A row without a slot or a page, or nobody's, is 0.
- * layers * ceil(rows / 16) is below 2^24.  Asynchronous on `stream`; the
- * calls can be captured. */
+ * The rows lie neither on the pages nor, of a load, keys on values.  layers *
+ * ceil(rows / 16) is below 2^24.  Asynchronous on `stream`; the calls can be
+ * captured. */
 typedef struct pkv_paged_rows_op {
     pkv_page_view pages;
     pkv_sequences seqs;
@@ -767,9 +768,11 @@ int pkv_paged_load(pkv_ctx* ctx, const pkv_paged_rows_op* op, void* stream);
  * Logits, the softmax's sums and outputs' sums are held in 32 bits.  Weights meet
  * the values as two terms of a 16-bit type for sequences with up to 16 rows (rows
  * x query heads of a KV head), and of f16 queries over PKV_FP8; else as one, as
- * pkv_attend's of many rows.  rows * q_heads is at most 2^30, and every launch
- * stays below 2^24 workgroups (else PKV_ERR_INVALID_ARG).  Asynchronous on
- * `stream`; the call can be captured. */
+ * pkv_attend's of many rows.  out lies neither on q nor on the pages.  seqs is at
+ * most 2^24, rows * q_heads at most 2^30, table_pages * page_slots below it, and
+ * every launch stays below 2^23 - 64 workgroups, whose number goes by rows,
+ * max_rows, seqs and heads (else PKV_ERR_INVALID_ARG).  Asynchronous on `stream`; the call
+ * can be captured. */
 typedef struct pkv_paged_attend_op {
     pkv_page_view pages;
     pkv_sequences seqs;
@@ -792,7 +795,9 @@ int pkv_paged_attend(pkv_ctx* ctx, const pkv_paged_attend_op* op, void* stream);
 /* Attention of whole prompts on their own packed rows: row i of a sequence sees
  * that sequence's rows j <= i (and window, sinks as above).  q and out as above,
  * k and v (r, h, 0) at r * row_stride + h * head_stride; all of one dtype,
- * PKV_BF16 or PKV_F16.  d_starts as pkv_sequences', not NULL. */
+ * PKV_BF16 or PKV_F16; k_row_stride and v_row_stride are at most 2^22, and out
+ * lies on none of them.  d_starts as pkv_sequences', not NULL; max_rows, lse,
+ * workspace, clear and the limits as pkv_paged_attend's. */
 typedef struct pkv_prompts_op {
     const void* d_q;
     const void* d_k;
