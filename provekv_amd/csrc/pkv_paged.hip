@@ -1376,51 +1376,69 @@ __global__ __launch_bounds__(512, 2) void rows_kernel(PagedDev a, PagedPart part
     if (real && half == 0 && a.lse) a.lse[static_cast<uint64_t>(qh) * a.seq.rows + sq.row0 + qi] = lse_of(base, l);
 }
 
-// rows_kernel's shares joined, a wave a row, D / 64 channels a lane, this many rows
-// a workgroup.
+// rows_kernel's shares joined: 16 rows a workgroup, 16 lanes a row, which read its
+// shares' bases and sums at once and D / 16 channels each.  A row's chain of reads
+// (its sequence, the plan, the bases, the outputs) is what bounds this, so that
+// four rows a wave side by side are what counts (11,200 rows of 8 heads of 128:
+// 23.7 us with a wave a row, one row after the other).
 constexpr uint32_t kJoinRows = 16;
 template <int QT, int D>
 __global__ __launch_bounds__(256) void join_rows_kernel(PagedDev a, PagedPart part, int few) {
     using T = typename Elem<QT>::T;
-    constexpr int V = D / 64;
-    typedef float Vec __attribute__((ext_vector_type(V)));
+    constexpr int V = D / 16;
     typedef T Out __attribute__((ext_vector_type(V)));
-    const uint32_t lane = threadIdx.x % 64, wave = __builtin_amdgcn_readfirstlane(threadIdx.x / 64), all = a.seq.rows * a.group;
-    const uint32_t h = blockIdx.x % a.heads, b = blockIdx.x / a.heads * kJoinRows;
-    int s = -1;
-    Seq q{};
-    for (uint32_t x = b + wave; x < min(b + kJoinRows, all); x += 4) {
-        const int row = static_cast<int>(x / a.group);
+    const uint32_t lane = threadIdx.x % 64, wave = __builtin_amdgcn_readfirstlane(threadIdx.x / 64), i = lane % 16;
+    const uint32_t all = a.seq.rows * a.group, h = blockIdx.x % a.heads, b = blockIdx.x / a.heads * kJoinRows + 4 * wave;
+    int s = -1, mine = -1;
+    Seq q{}, sq{};
+    for (uint32_t y = 0; y < 4 && b + y < all; ++y) {   // rows of one sequence but where it ends
+        const int row = static_cast<int>((b + y) / a.group);
         if (s < 0 || row >= q.row0 + q.rows) {
-            s = seq_of_row(a.seq, row, lane);
-            if (s < 0) continue;
-            q = seq_of(a.seq, s, a.max_rows);
+            s = __builtin_amdgcn_readfirstlane(seq_of_row(a.seq, row, lane));
+            if (s >= 0) q = seq_of_all(a.seq, s, a.max_rows);
         }
-        const int r = (row - q.row0) * static_cast<int>(a.group) + static_cast<int>(x % a.group);
-        if (row >= q.row0 + q.rows || static_cast<int64_t>(q.rows) * a.group <= few) continue;
-        const int first = part.plan[2 * s], shares = part.plan[2 * s + 1];
-        if (shares == 1) continue;
-        const int tile = r / static_cast<int>(part.rows);
-        // starts that do not ascend may have more units than the launch, and no plan for the last
-        if (first < 0 || shares < 1 || first + (tile + 1ll) * shares > static_cast<int64_t>(part.parts)) continue;
-        const uint64_t at = (static_cast<uint64_t>(h) * part.parts + first + tile * shares) * part.rows +
-                            static_cast<uint64_t>(r - tile * static_cast<int>(part.rows));
-        float base = kInf, sum = 0.0f;
-        for (int y = 0; y < shares; ++y) base = fminf(base, part.ml[2 * (at + static_cast<uint64_t>(part.rows) * y)]);
-        Vec o = {};
-        for (int y = 0; y < shares; ++y) {
-            const uint64_t from = at + static_cast<uint64_t>(part.rows) * y;
-            const float f = joined(base, part.ml[2 * from]);
-            sum += part.ml[2 * from + 1] * f;
-            o += *reinterpret_cast<const Vec*>(part.o + from * D + V * lane) * (f * kPower<-kJoinDown>);
-        }
-        const uint32_t qh = h * a.group + x % a.group;
-        const float div = sum * kPower<-kPartDown - kJoinDown>;
-        Out y;
-        for (int e = 0; e < V; ++e) y[e] = static_cast<T>(sum == 0.0f ? 0.0f : o[e] / div);
-        *reinterpret_cast<Out*>(reinterpret_cast<T*>(a.out) + static_cast<uint64_t>(row) * a.o_row + qh * a.o_head + V * lane) = y;
-        if (lane == 0 && a.lse) a.lse[static_cast<uint64_t>(qh) * a.seq.rows + row] = lse_of(base, sum);
+        if (lane / 16 == y) { mine = s; sq = q; }
     }
+    const uint32_t x = b + lane / 16;
+    const int row = static_cast<int>(x / a.group);
+    int shares = 0;
+    uint64_t at = 0;
+    if (mine >= 0 && row < sq.row0 + sq.rows && static_cast<int64_t>(sq.rows) * a.group > few) {
+        const int r = (row - sq.row0) * static_cast<int>(a.group) + static_cast<int>(x % a.group);
+        const int first = part.plan[2 * mine], n = part.plan[2 * mine + 1], tile = r / static_cast<int>(part.rows);
+        // starts that do not ascend may have more units than the launch, and no plan for the last
+        if (n > 1 && first >= 0 && first + (tile + 1ll) * n <= static_cast<int64_t>(part.parts)) {
+            shares = n;
+            at = (static_cast<uint64_t>(h) * part.parts + first + static_cast<uint64_t>(tile) * n) * part.rows +
+                 static_cast<uint64_t>(r - tile * static_cast<int>(part.rows));
+        }
+    }
+    if (!__any(shares)) return;
+    const float* ml = part.ml + 2 * at;
+    const uint64_t step = 2ull * part.rows;
+    float low = kInf;
+    for (int y = static_cast<int>(i); y < shares; y += 16) low = fminf(low, ml[step * y]);
+    for (int o = 8; o; o >>= 1) low = fminf(low, __shfl_xor(low, o));
+    float sum = 0.0f;
+    f32x4 acc[V / 4] = {};
+    for (int c = 0; c < shares; c += 16) {
+        const int y = c + static_cast<int>(i), n = min(16, shares - c);
+        const float f = y < shares ? joined(low, ml[step * y]) : 0.0f;
+        if (y < shares) sum += ml[step * y + 1] * f;
+        for (int k = 0; k < n; ++k) {
+            const float w = __shfl(f, static_cast<int>(lane / 16 * 16) + k) * kPower<-kJoinDown>;
+            const float* from = part.o + (at + static_cast<uint64_t>(part.rows) * (c + k)) * D + V * i;
+            for (int e = 0; e < V / 4; ++e) acc[e] += reinterpret_cast<const f32x4*>(from)[e] * w;
+        }
+    }
+    for (int o = 8; o; o >>= 1) sum += __shfl_xor(sum, o);
+    if (!shares) return;
+    const uint32_t qh = h * a.group + x % a.group;
+    const float div = sum * kPower<-kPartDown - kJoinDown>;
+    Out y;
+    for (int e = 0; e < V; ++e) y[e] = static_cast<T>(sum == 0.0f ? 0.0f : acc[e / 4][e % 4] / div);
+    *reinterpret_cast<Out*>(reinterpret_cast<T*>(a.out) + static_cast<uint64_t>(row) * a.o_row + qh * a.o_head + V * i) = y;
+    if (i == 0 && a.lse) a.lse[static_cast<uint64_t>(qh) * a.seq.rows + row] = lse_of(low, sum);
 }
 
 uint32_t clears(const PagedDev& a) { return a.clear && a.seq.starts ? kClear : 0; }
