@@ -85,7 +85,9 @@ __device__ inline void chunk_places(const PagedRowsDev& a, uint32_t first, int64
 
 // A workgroup takes 16 packed rows of a layer and side, 8 values a thread and
 // step, channels fastest, then rows, then heads: rows of a sequence that follow
-// each other are neighbours in a page, so that a step writes whole lines.
+// each other are neighbours in a page, so that a step writes whole lines.  Bound
+// by the bytes: 24 x 32 heads x 1,391 rows of 64, keys and values, from f32 in 171 to 183 us and back
+// in 141 to 151 (4.1 TB/s; a copy reaches 4.8); 64 single rows take 5 us each way.
 template <int CT, int QT, int D>
 __global__ __launch_bounds__(256) void paged_store_kernel(PagedRowsDev a, uint32_t heads) {
     using T = typename Elem<QT>::T;
@@ -231,8 +233,14 @@ __device__ inline void write_row(const PagedDev& a, uint32_t r, uint32_t qh, uin
 constexpr int kFew = 16;            // rows x group of a KV head that decode_kernel takes
 constexpr int kStep = 32;           // slots of its tiles
 constexpr int wide_waves(uint32_t dim, int cache_dtype) { return dim == 64 && cache_dtype != PKV_FP8 ? 16 : 8; }
-// Units of all heads that fit the chip at once: two workgroups a CU, by their registers four of the small tiles.
-constexpr uint32_t fitting_units(uint32_t dim, int cache_dtype) { return dim == 64 ? cache_dtype == PKV_FP8 ? 768 : 1024 : 512; }
+// Units of all heads aimed at.  head_dim 128: two workgroups a CU (a sequence of 32,768 slots of 8 heads: 31 us; 35 with
+// fewer, 37 with twice as many, whose start costs more than it hides), and as many as fit where each still has kMany
+// tiles (24 such sequences: 541 us, 291 in 8 bits, against 596 and 333; 24 of 700 to 32,768: 168 either way).
+constexpr uint32_t fitting_units(uint32_t dim, int cache_dtype) {
+    return dim == 64 ? cache_dtype == PKV_FP8 ? 768 : 1024 : 512;
+}
+constexpr uint32_t kMostUnits = 1024;
+constexpr int kMany = 96;
 constexpr int kLeast = 4;           // tiles of a unit, one a wave
 constexpr int kLeastSteps = 8;      // rows_kernel: tiles of 64 slots of a share
 
@@ -243,9 +251,8 @@ __device__ inline int few_tiles(const PagedDev& a, uint32_t s) {
     return tiles_of(a, q.first, q.first + q.rows - 1, kStep).count;
 }
 
-// The least whole number above all / target of the lanes' counts, and at least `least`.
+// The least whole number above all / target, and at least `least`.
 __device__ inline int share_of(int64_t all, uint32_t target, int least) {
-    for (int o = 32; o; o >>= 1) all += __shfl_xor(static_cast<long long>(all), o);
     const double share = static_cast<double>(all) / target;   // counts stay below 2^53
     return max(least, static_cast<int>(fmin(share, 1e9)) + 1);
 }
@@ -257,7 +264,7 @@ __device__ inline int share_of(int64_t all, uint32_t target, int least) {
 struct Unit {
     int seq, share, shares, first;   // first: the sequence's first unit
 };
-__device__ inline bool find_unit(const PagedDev& a, uint32_t u, uint32_t target, uint32_t lane, Unit* o) {
+__device__ inline bool find_unit(const PagedDev& a, uint32_t u, uint32_t target, uint32_t most, uint32_t lane, Unit* o) {
     const uint32_t per = (a.seq.seqs + 63) / 64, s0 = min(lane * per, a.seq.seqs), s1 = min(s0 + per, a.seq.seqs);
     int mine = -1;                      // of the run's only sequence
     int64_t all = 0;
@@ -265,7 +272,9 @@ __device__ inline bool find_unit(const PagedDev& a, uint32_t u, uint32_t target,
         mine = few_tiles(a, s);
         all += max(mine, 0);
     }
-    const int size = share_of(all, target, kLeast);   // no more than target + sequences units
+    for (int x = 32; x; x >>= 1) all += __shfl_xor(static_cast<long long>(all), x);
+    // no more than target (or most) + sequences units
+    const int size = share_of(all, all >= static_cast<int64_t>(kMany) * most ? most : target, kLeast);
     auto units = [&](int tiles) { return tiles < 0 ? 0 : max(1, (tiles + size - 1) / size); };
     int n = 0;
     if (per == 1) n = units(mine);
@@ -421,6 +430,7 @@ struct PagedPart {
     float* ml;         // [head][unit][rows][2]: base, sum of the weights
     int32_t* plan;     // [sequence][2]: first unit, units; of many rows the first that is a share, shares of a tile
     uint32_t units, target, rows, parts;
+    uint32_t most;     // decode_kernel: aimed at where they are long
 };
 
 // The rows of a sequence of few (rows x group up to 16) against a share of its
@@ -434,8 +444,16 @@ struct PagedPart {
 //                 gathers each channel across the lane's four (x 2) slots.
 // Weights meet the values as two terms of a 16-bit type, which the bytes hide.
 // WAVES 4, or 8 or 16 (as registers allow) where a sequence's slots are one
-// unit's, so that the call is one launch.  The next tile is on its way while one is worked on, and the words of the pages
-// of the one after it, so that no read waits for a page's number.
+// unit's, so that the call is one launch (a row of 32 heads of 64 on 700 slots:
+// 13 us with the host's call, 23 in units of four waves and a join).  The next
+// tile is on its way while one is worked on, and the words of the pages of the
+// one after it, so that no read waits for a page's number.
+// Bound by the bytes: 5.9 TB/s of 24 x 32,768 slots of 8 heads of 128, 5.7 in 8
+// bits, 5.5 and 5.0 where the 24 sequences have 700 to 32,768; a large copy
+// reaches 4.8 on this card, a large sum 4.0.  Of short sequences by the chain
+// kernel's start, the lengths, a page's number, a tile, the joins (97 sequences
+// of 33 to 3,000 slots of 4 heads in 8 bits: 31 us and 5 of join_kernel for what
+// the bytes make 14.5).
 template <int CT, int QT, int D, int WAVES>
 __global__ __launch_bounds__(64 * WAVES, WAVES > 8 ? 4 : 2) void decode_kernel(PagedDev a, PagedPart part) {
     using T = typename Elem<QT>::T;
@@ -449,7 +467,7 @@ __global__ __launch_bounds__(64 * WAVES, WAVES > 8 ? 4 : 2) void decode_kernel(P
     // are a multiple of 8
     const uint32_t h = blockIdx.x % a.heads, u = blockIdx.x / a.heads;
     Unit unit;
-    if (!find_unit(a, u, part.target, lane, &unit)) return;
+    if (!find_unit(a, u, part.target, part.most, lane, &unit)) return;
     unit = {__builtin_amdgcn_readfirstlane(unit.seq), __builtin_amdgcn_readfirstlane(unit.share),
             __builtin_amdgcn_readfirstlane(unit.shares), __builtin_amdgcn_readfirstlane(unit.first)};
     if (h == 0 && unit.share == 0 && threadIdx.x == 0) {
@@ -712,6 +730,8 @@ __device__ inline bool find_rows(const PagedDev& a, uint32_t u, int64_t few, int
         mine = row_work(a, s, few, rows);
         all += static_cast<int64_t>(mine.tiles) * mine.steps;
     }
+    if (target)
+        for (int x = 32; x; x >>= 1) all += __shfl_xor(static_cast<long long>(all), x);
     const int size = target ? share_of(all, target, kLeastSteps) : 0x7fffffff;
     auto shares = [&](const RowWork& w) { return max(1, w.steps / size); };
     int units = 0, parts = 0, longest = 0;
@@ -873,10 +893,16 @@ __device__ inline void meet() {
 //   weights straight from those registers.
 // The workgroup's waves are two groups of four, one of each on a SIMD, that take
 // turns: while one has the matrix cores, O of the tile before and S of the next,
-// the other has the vector units for its softmax, and they meet between.  Two
-// workgroups of four waves each, which meet nobody, did one after the other (964
-// TFLOP/s for prompts of 8,192, 6,298 and 3,900 rows of 32 heads of 128, with
-// the matrix cores busy 44 % of the cycles and the vector units 47 %).
+// the other has the vector units for its softmax, and they meet between.  For
+// prompts of 8,192, 6,298 and 3,900 rows of 32 query heads of 128 that takes 850
+// us (1,160 TFLOP/s; 1,250 for one of 16,384 rows; a library's square product
+// reaches 1,330): the matrix cores are busy 62 % of the cycles, the tiles' LDS
+// reads conflict in 0.1 %, and a workgroup's start and end, 9 us that nothing
+// hides since one fills a CU's registers, take most of the rest.  Two workgroups
+// of four waves each, which meet nobody, took 1,023 (matrix cores 44 %, vector
+// units 47 %, one after the other); the turns alone made it 910, and copies by
+// both groups among the products, with the largest logit looked for only where
+// the weights' sums pass what one may be, the rest.
 // Weights are rounded once to the type of the products (f16 queries over 8-bit
 // codes: two bf16 terms), while their sum is that of the unrounded ones.
 // KS 2, 4: 128, 64 rows; the groups take the slots' tiles in turn, at 4 also two
@@ -1449,7 +1475,7 @@ uint64_t round256(uint64_t x) { return (x + 255) & ~255ull; }
 struct Plan {
     bool few, many;                // sequences of few rows are looked for; of more
     bool wide;                     // decode_kernel: whole sequences, more waves each
-    uint32_t units, target, rows;  // units a head at most, aimed at, rows of one
+    uint32_t units, target, most, rows;   // units a head at most, aimed at (most: if long), rows of one
     uint64_t ml, plan;             // offsets in the workspace (partial outputs first)
     int ks;                        // rows_kernel: 256 / ks rows a tile
     uint32_t row_units, row_target, parts;   // units a head at most, shares aimed at (0: none), room for
@@ -1472,13 +1498,18 @@ Plan plan_of(const PagedDev& a, uint32_t dim, int cache_dtype) {
     if (p.few) {
         p.rows = static_cast<uint32_t>(std::min<uint64_t>(kFew, most));
         // what fits at once, less half a unit a sequence for those that are not whole
-        const uint32_t fit = fitting_units(dim, cache_dtype) / a.heads;
-        p.target = std::max(fit > a.seq.seqs / 2 ? fit - a.seq.seqs / 2 : 1, std::max(fit / 4, 1u));
+        auto aim = [&](uint32_t all) {
+            const uint32_t fit = all / a.heads;
+            return std::max(fit > a.seq.seqs / 2 ? fit - a.seq.seqs / 2 : 1, std::max(fit / 4, 1u));
+        };
+        p.target = aim(fitting_units(dim, cache_dtype));
         const uint64_t tiles = tiles_for(kFew, kStep);
         p.wide = static_cast<uint64_t>(a.seq.seqs) * a.heads <= 256 && tiles <= 4ull * wide_waves(dim, cache_dtype);
         if (p.wide) p.target = 1;
+        p.most = p.wide ? 1 : std::max(p.target, aim(kMostUnits));
+        if (tiles * a.seq.seqs < static_cast<uint64_t>(kMany) * p.most) p.most = p.target;   // never as long
         const uint64_t each = p.wide ? 1 : std::max<uint64_t>(1, (tiles + kLeast - 1) / kLeast);
-        p.units = static_cast<uint32_t>(std::min<uint64_t>(static_cast<uint64_t>(a.seq.seqs) + p.target, a.seq.seqs * each));
+        p.units = static_cast<uint32_t>(std::min<uint64_t>(static_cast<uint64_t>(a.seq.seqs) + p.most, a.seq.seqs * each));
         const uint64_t rows = static_cast<uint64_t>(a.heads) * p.units * p.rows;
         p.ml = round256(rows * dim * 4);
         p.plan = p.ml + round256(rows * 8);
@@ -1526,7 +1557,7 @@ int attend_typed(const PagedDev& a, uint8_t* ws, hipStream_t st) {
     if constexpr (PAGED)
         if (p.few) {
             const PagedPart part{reinterpret_cast<float*>(ws), reinterpret_cast<float*>(ws + p.ml),
-                                 reinterpret_cast<int32_t*>(ws + p.plan), p.units, p.target, p.rows, p.units};
+                                 reinterpret_cast<int32_t*>(ws + p.plan), p.units, p.target, p.rows, p.units, p.most};
             const uint32_t grid = a.heads * p.units + clears(a);
             constexpr int kWide = wide_waves(D, CT);
             if (p.wide) decode_kernel<CT, QT, D, kWide><<<grid, 64 * kWide, 0, st>>>(a, part);
@@ -1536,7 +1567,7 @@ int attend_typed(const PagedDev& a, uint8_t* ws, hipStream_t st) {
     if (p.many) {
         const PagedPart part{reinterpret_cast<float*>(ws), reinterpret_cast<float*>(ws + p.rows_ml),
                              reinterpret_cast<int32_t*>(ws + p.rows_plan), p.row_units, p.row_target,
-                             static_cast<uint32_t>(rows_of_tile(p.ks)), p.parts};
+                             static_cast<uint32_t>(rows_of_tile(p.ks)), p.parts, 0};
         const int few = PAGED && p.few ? kFew : 0;
         const uint32_t grid = a.heads * p.row_units + (p.few ? 0 : clears(a));
         if (p.ks == 4) rows_kernel<CT, QT, D, PAGED, 4><<<grid, 512, 0, st>>>(a, part, few);

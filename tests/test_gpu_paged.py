@@ -475,3 +475,32 @@ def test_starts_that_do_not_ascend(ctx, starts):
         cache.attend(0, q, tables, n, starts=st, out=out)
         attend_prompts(q, q[:, :2], q[:, :2], st, out=out)
         torch.cuda.synchronize()
+
+
+@pytest.mark.parametrize("D", [64, 128])
+@pytest.mark.parametrize("cache_type", [BF16, F8], ids=["bf16", "8-bit"])
+def test_many_long_sequences(ctx, cache_type, D):
+    """Slots enough for the larger number of units; two of the heads against the plain form."""
+    from provekv_amd.paged import PagedKVCache
+    H, page, G = 16, 128, 2
+    lens = [17000, 20000, 16500, 18001, 17777, 19000, 16900, 20000, 18500, 17400, 16800, 19990]     # 217,868
+    need = [(n + page - 1) // page for n in lens]
+    g = torch.Generator().manual_seed(20)
+    order = torch.randperm(sum(need), generator=g).tolist()
+    tables = [[order.pop() for _ in range(n)] + [-1] * (max(need) - n) for n in need]
+    cache = PagedKVCache(1, H, sum(need), page, D, dtype=cache_type)
+    dg = torch.Generator(device="cuda").manual_seed(21)
+    if cache_type == F8:
+        cache.buf.random_(0, 256, generator=dg)
+        cache.buf[(cache.buf & 127) == 127] = 0
+        cache.scales.random_(118, 121, generator=dg)
+    else:
+        cache.buf.normal_(generator=dg)
+    q = torch.randn(len(lens), H * G, D, generator=g).to(BF16)
+    out = cache.attend(0, q.cuda(), words(tables), words(lens))
+    some = [0, 15]
+    pages = P.values(cache.buf[:, :, :, some], None if cache_type == BF16 else cache.scales[:, :, :, some])[0]
+    kv = [P.gathered(pages, t, n) for t, n in zip(tables, lens)]
+    spans = [(i, 1) for i in range(len(lens))]
+    rows = [h * G + y for h in some for y in range(G)]
+    P.check(out[:, rows], None, P.attend(q[:, rows].double(), kv, lens, spans, 0, 0, 1 / math.sqrt(D)), spans, BF16)
