@@ -177,8 +177,9 @@ class PagedKVCache(DeviceCalls):
         steps, each value its nearest code; a block with an infinity or NaN
         becomes NaN.  A row whose slot is negative or has no page is not stored.
         Two rows must not have the same place of the same page: sequences that
-        share pages store into pages of their own.  Rows that carry a gradient or
-        a tangent are refused."""
+        share pages store into pages of their own.  Rows that lie among the
+        pages themselves are refused (load them first), as are rows that carry a
+        gradient or a tangent."""
         some = keys if keys is not None else values
         if some is None:
             return
