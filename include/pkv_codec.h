@@ -758,7 +758,9 @@ int pkv_paged_load(pkv_ctx* ctx, const pkv_paged_rows_op* op, void* stream);
  *            were in out, or with clear = 1 become 0
  *   d_lse    NULL, or f32 [q_heads][rows]: natural log of the sum of exp(s_j)
  *            (nobody's rows left as they were)
- *   max_rows no sequence has more rows (0: rows); rows past it are not computed
+ *   max_rows no sequence has more rows (0: rows).  Of one that has, the first
+ *            max_rows are computed, each at its own slot, and the others are left
+ *            as they were in out and lse
  *   max_len  no len(s) is above it (0: table_pages * page_slots).  Both size the
  *            launch, so tight ones are faster, and a captured graph wants the
  *            largest its replays use

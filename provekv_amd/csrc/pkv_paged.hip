@@ -27,9 +27,10 @@ __device__ inline Seq seq_of(const SeqsDev& q, uint32_t s, uint32_t max_rows) {
         o.row0 = static_cast<int>(s * q.each);
         end = o.row0 + static_cast<int>(q.each);
     }
-    o.rows = min(end - o.row0, static_cast<int>(max_rows));
+    const int all = end - o.row0;
+    o.rows = min(all, static_cast<int>(max_rows));
     o.len = q.lens ? min(max(q.lens[s], 0), static_cast<int>(q.max_len)) : o.rows;
-    o.first = o.len - o.rows;
+    o.first = q.lens ? o.len - all : 0;     // of all its rows: those past max_rows have their slots too
     return o;
 }
 // The same of a sequence that all lanes have, in scalar registers.

@@ -1,0 +1,56 @@
+"""Calls whose sequences have more rows than max_rows says (a captured step that
+is replayed with longer chunks): the rows up to it are computed at their own
+slots, those past it are nobody's."""
+import math
+
+import pytest
+import torch
+
+import paged_ref as P
+from test_gpu_paged import BF16, F16, KIND_IDS, KINDS, make, prompts, running, sequences, words
+
+pytestmark = pytest.mark.gpu
+
+CUT = [  # rows of each sequence, lengths, group, max_rows
+    ([5, 1, 3], [70, 40, 33], 1, 2), ([9, 0, 2], [200, 5, 90], 4, 4), ([40, 1, 70], [130, 20, 75], 2, 33),
+    ([30, 2, 1], [25, 90, 1], 1, 20), ([300, 1, 150], [700, 300, 200], 2, 130), ([3, 4], [1, 4], 1, 2),
+]
+
+
+def cut(spans, most):
+    return [(a, min(m, most)) for a, m in spans]
+
+
+@pytest.mark.parametrize("window,sinks", [(0, 0), (9, 3)])
+@pytest.mark.parametrize("cache_type,dtype", KINDS, ids=KIND_IDS)
+@pytest.mark.parametrize("counts,lens,G,most", CUT)
+def test_rows_past_the_limit(ctx, counts, lens, G, most, cache_type, dtype, window, sinks):
+    """Row i of n stands at slot len - n + i whether or not all n are computed."""
+    cache, tables = make(cache_type, 2, 64, 16, lens, seed=30)
+    g = torch.Generator().manual_seed(31)
+    rows = 2 + sum(counts) + 3
+    st = [2 + x for x in running(counts)]
+    q = torch.randn(rows, 2 * G, 64, generator=g).to(dtype)
+    lse = torch.full((2 * G, rows), 77.0, device="cuda")
+    out = torch.full((rows, 2 * G, 64), 55.0, dtype=dtype, device="cuda")
+    cache.attend(0, q.cuda(), words(tables), words(lens), starts=words(st), window=window, sinks=sinks, lse=lse, out=out,
+                 max_rows=most)
+    spans = P.rows_of(st, len(lens), rows)
+    ref = P.attend(q.double(), sequences(cache, tables, lens), lens, spans, window, sinks, 0.125)
+    P.check(out, lse, ref, cut(spans, most), dtype, 55.0, 77.0)
+
+
+@pytest.mark.parametrize("dtype", [BF16, F16], ids=["bf16", "f16"])
+@pytest.mark.parametrize("window,sinks", [(0, 0), (50, 3)])
+def test_prompt_rows_past_the_limit(ctx, window, sinks, dtype):
+    from provekv_amd.paged import attend_prompts
+    counts, most = [100, 3, 150], 70
+    (q, k, v), (dq, dk, dv), st = prompts(dtype, counts, 2, 2, 64, before=1, behind=2, seed=32)
+    lse = torch.full((4, q.shape[0]), 77.0, device="cuda")
+    out = torch.full_like(dq, 55.0, memory_format=torch.contiguous_format)
+    attend_prompts(dq, dk, dv, words(st), window=window, sinks=sinks, lse=lse, out=out, max_rows=most)
+    spans = P.rows_of(st, 3, q.shape[0])
+    kv = [(k[a:a + m].double().transpose(0, 1), v[a:a + m].double().transpose(0, 1), torch.ones(m, dtype=torch.bool))
+          for a, m in spans]
+    ref = P.attend(q.double(), kv, counts, spans, window, sinks, 1 / math.sqrt(64))
+    P.check(out, lse, ref, cut(spans, most), dtype, 55.0, 77.0)
