@@ -754,13 +754,14 @@ int pkv_paged_load(pkv_ctx* ctx, const pkv_paged_rows_op* op, void* stream);
  * as there.
  *   q, out   element (r, g, 0) at r * row_stride + g * head_stride, of dtype: the
  *            pages', or for PKV_FP8 PKV_BF16 or PKV_F16; 16-byte aligned, strides
- *            a multiple of 16 bytes.  Rows that are nobody's are left as they
- *            were in out, or with clear = 1 become 0
+ *            a multiple of 16 bytes.  Rows that are nobody's, or past a
+ *            sequence's max_rows, are left as they were in out, or with clear = 1
+ *            become 0
  *   d_lse    NULL, or f32 [q_heads][rows]: natural log of the sum of exp(s_j)
  *            (nobody's rows left as they were)
  *   max_rows no sequence has more rows (0: rows).  Of one that has, the first
- *            max_rows are computed, each at its own slot, and the others are left
- *            as they were in out and lse
+ *            max_rows are computed, each at its own slot, and the others are
+ *            nobody's
  *   max_len  no len(s) is above it (0: table_pages * page_slots).  Both size the
  *            launch, so tight ones are faster, and a captured graph wants the
  *            largest its replays use

@@ -197,23 +197,37 @@ __device__ inline float element(const uint8_t* p, const uint8_t* scales, uint64_
     }
 }
 
-// Nobody's rows, before the first sequence's and behind the last's, to 0: the
-// workgroups behind `work`, kClear of them.
+// Nobody's rows, before the first sequence's, behind the last's and past a
+// sequence's max_rows, to 0: the workgroups behind `work`, kClear of them.
 constexpr uint32_t kClear = 64;
 template <int QT, int D, int THREADS = 256>
 __device__ void clear_rows(const PagedDev& a, uint32_t block) {
     using T = typename Elem<QT>::T;
-    const int rows = static_cast<int>(a.seq.rows), heads = static_cast<int>(a.heads * a.group);
-    const int first = min(max(a.seq.starts[0], 0), rows);
-    int last = first;                                  // the largest end, should starts not ascend
-    for (uint32_t s = threadIdx.x % 64; s < a.seq.seqs; s += 64) last = max(last, min(a.seq.starts[s + 1], rows));
-    for (int o = 32; o; o >>= 1) last = max(last, __shfl_xor(last, o));
-    const int rest = first + rows - last;
-    for (int x = static_cast<int>(block); x < rest; x += kClear) {
-        T* out = reinterpret_cast<T*>(a.out) + static_cast<uint64_t>(x < first ? x : last + x - first) * a.o_row;
+    const int rows = static_cast<int>(a.seq.rows), most = static_cast<int>(a.max_rows);
+    const int heads = static_cast<int>(a.heads * a.group);
+    auto clear = [&](int r) {
+        T* out = reinterpret_cast<T*>(a.out) + static_cast<uint64_t>(r) * a.o_row;
         for (int y = static_cast<int>(threadIdx.x); y < heads * (D / 8); y += THREADS)
             *reinterpret_cast<u32x4*>(out + static_cast<uint64_t>(y / (D / 8)) * a.o_head + y % (D / 8) * 8) = u32x4{};
+    };
+    const int first = min(max(a.seq.starts[0], 0), rows);
+    int last = first;                                  // the largest end, should starts not ascend
+    for (uint32_t s0 = 0; s0 < a.seq.seqs; s0 += 64) {
+        const uint32_t s = s0 + threadIdx.x % 64;
+        Seq q{};
+        if (s < a.seq.seqs) {
+            q = seq_of(a.seq, s, a.seq.rows);
+            last = max(last, min(a.seq.starts[s + 1], rows));
+        }
+        for (uint64_t over = __ballot(q.rows > most); over; over &= over - 1) {
+            const int i = __ffsll(static_cast<unsigned long long>(over)) - 1;
+            const int from = __builtin_amdgcn_readlane(q.row0, i) + most, n = __builtin_amdgcn_readlane(q.rows, i) - most;
+            for (int x = static_cast<int>(block); x < n; x += kClear) clear(from + x);
+        }
     }
+    for (int o = 32; o; o >>= 1) last = max(last, __shfl_xor(last, o));
+    const int rest = first + rows - last;
+    for (int x = static_cast<int>(block); x < rest; x += kClear) clear(x < first ? x : last + x - first);
 }
 
 // Four channels of an output row from their weighted sum (`down` times as large

@@ -242,7 +242,8 @@ class PagedKVCache(DeviceCalls):
         `out` that is given, and 0 in a new one.  lse: float32 [query heads,
         rows], the rows' log of the sum of exponentials.  max_rows, max_len: no
         sequence has more rows or slots (an int `lens` says so itself); they size
-        the launch.
+        the launch.  Of a sequence that has more rows, those past max_rows are no
+        sequence's; a length past max_len is taken as max_len.
 
         A q that carries a gradient or a tangent is refused: there is no
         derivative."""

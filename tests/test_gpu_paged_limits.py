@@ -54,3 +54,38 @@ def test_prompt_rows_past_the_limit(ctx, window, sinks, dtype):
           for a, m in spans]
     ref = P.attend(q.double(), kv, counts, spans, window, sinks, 1 / math.sqrt(64))
     P.check(out, lse, ref, cut(spans, most), dtype, 55.0, 77.0)
+
+
+@pytest.mark.parametrize("cache_type,dtype", KINDS, ids=KIND_IDS)
+@pytest.mark.parametrize("counts,lens,G,most", CUT)
+def test_new_outputs_are_0_past_the_limit(ctx, counts, lens, G, most, cache_type, dtype):
+    """In a new out, whatever its memory held: as the rows of nobody."""
+    from provekv_amd.paged import attend_prompts
+    cache, tables = make(cache_type, 2, 64, 16, lens, seed=33)
+    rows = 2 + sum(counts) + 3
+    st = [2 + x for x in running(counts)]
+    q = torch.randn(rows, 2 * G, 64, device="cuda").to(dtype)
+    past = torch.ones(rows, dtype=torch.bool)
+    for a, m in cut(P.rows_of(st, len(lens), rows), most):
+        past[a:a + m] = False
+
+    def new(call):
+        torch.full_like(q, 9.0)             # what the next allocation may find
+        return call()
+
+    for out in (new(lambda: cache.attend(0, q, words(tables), words(lens), starts=words(st), max_rows=most)),
+                new(lambda: attend_prompts(q, q[:, :2], q[:, :2], words(st), max_rows=most))):
+        assert not out[past].any() and out[~past].any()
+
+
+@pytest.mark.parametrize("dtype", [BF16, F16], ids=["bf16", "f16"])
+def test_many_sequences_past_the_limit(ctx, dtype):
+    """More sequences than a wave has lanes, every third of them too long."""
+    from provekv_amd.paged import attend_prompts
+    counts = [7 if i % 3 else 40 for i in range(200)]
+    (q, k, v), (dq, dk, dv), st = prompts(dtype, counts, 1, 2, 64, before=3, behind=5, seed=34)
+    torch.full((q.shape[0], 2, 64), 9.0, dtype=dtype, device="cuda")
+    out = attend_prompts(dq, dk, dv, words(st), max_rows=11)
+    want = torch.zeros_like(out)
+    attend_prompts(dq, dk, dv, words(st), max_rows=11, out=want)
+    assert torch.equal(out, want) and not out[3 + 11:3 + 40].any() and out[3 + 40].any()
