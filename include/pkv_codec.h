@@ -576,8 +576,10 @@ typedef struct pkv_kv_view {
  * the values as two or more terms of a 16-bit type (f32 caches: as they are);
  * with more than 16 rows of a KV head over a 16-bit cache, or of bf16 queries
  * over 4 bits, as one: rounded to the type, which adds to the output's own
- * rounding at most half a step of the type times sum w_j |v_j|.  Asynchronous on
- * `stream`; the call can be captured. */
+ * rounding at most half a step of the type times sum w_j |v_j|.  A w_j below
+ * 2^-126 of its row's largest may count as 0, below 2^-86 where sums of weighted
+ * values pass the end of f32 or values are not finite (f16: 2^-36).  Asynchronous
+ * on `stream`; the call can be captured. */
 typedef struct pkv_attend_op {
     pkv_kv_view cache;
     const void* d_q;
