@@ -7,7 +7,7 @@ import torch
 
 import live_ref as R
 import paged_ref as P
-from test_gpu_paged import BF16, F8, words
+from test_gpu_paged import BF16, F8, KIND_IDS, KINDS, make, running, sequences, words
 
 pytestmark = pytest.mark.gpu
 
@@ -46,3 +46,33 @@ def test_starts_that_do_not_ascend(ctx, starts, cache_type, heads):
             out = attend_prompts(q, q[:, :heads], q[:, :heads], st, out=torch.full_like(q, 55.0), max_rows=most)
             assert ((out == 1) | (out == 55)).all()
     assert R.same(P.values(cache.buf, cache.scales), now)
+
+
+@pytest.mark.parametrize("cache_type,dtype", KINDS, ids=KIND_IDS)
+@pytest.mark.parametrize("counts,G", [([1, 1, 1], 2), ([1, 1, 1], 20), ([30, 1, 65], 2)])
+@pytest.mark.parametrize("gone", [-1, 10 ** 6, -2 ** 31, 2 ** 31 - 1])
+def test_missing_pages_whatever_page_0_holds(ctx, counts, G, gone, cache_type, dtype):
+    """What stands in for a missing page is not a number."""
+    lens = [100, 200, 90]
+    cache, tables = make(cache_type, 2, 64, 16, lens, seed=60, spare=3)
+    free = [i for i in range(cache.pages) if not any(i in t for t in tables)]
+    if 0 not in free:                                     # page 0 moves
+        for x in (cache.buf, cache.scales):
+            if x is not None:
+                x[:, free[0]] = x[:, 0]
+        tables = [[free[0] if i == 0 else i for i in t] for t in tables]
+    (cache.buf if cache_type != F8 else cache.scales)[:, 0] = math.nan if cache_type != F8 else 255
+    tables[0][2], tables[1][0], tables[1][12] = gone, gone, gone
+    tables[2] = [gone] * len(tables[2])
+    g = torch.Generator().manual_seed(61)
+    rows, st = sum(counts), running(counts)
+    q = torch.randn(rows, 2 * G, 64, generator=g).to(dtype)
+    lse = torch.full((2 * G, rows), 77.0, device="cuda")
+    out = cache.attend(0, q.cuda(), words(tables), words(lens), starts=words(st), lse=lse)
+    spans = P.rows_of(st, 3, rows)
+    ref = P.attend(q.double(), sequences(cache, tables, lens), lens, spans, 0, 0, 0.125)
+    P.check(out, lse, ref, spans, dtype)
+    assert not out[-counts[2]:].any()
+    keys, values = cache.load(lens[0], words(tables[:1]), words(lens[:1]), layer=0)
+    for x in (keys, values):
+        assert torch.isfinite(x).all() and not x[32:48].any() and x[48:].any()
