@@ -149,7 +149,7 @@ template <int MT> constexpr float kLift = MT == PKV_F16 ? 11.0f : 0.0f;
 // 2^-kPartDown as large and joined 2^-kJoinDown, by as many shares as there can be.
 template <int MT> constexpr int kDown = MT == PKV_F16 ? 0 : 40;
 constexpr int kPartDown = 2;            // decode_kernel's four waves
-constexpr int kJoinDown = 10;           // shares of a row: up to 768
+constexpr int kJoinDown = 10;           // shares of a row: up to 2^10 (768 of contiguous caches, 1,024 of pages)
 constexpr float power(int x) { return x < 0 ? 0.5f * power(x + 1) : x ? 2.0f * power(x - 1) : 1.0f; }
 template <int X> constexpr float kPower = power(X);   // 2^X
 // The base with a row's logits up to `top` seen as well.

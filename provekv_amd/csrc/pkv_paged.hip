@@ -255,6 +255,8 @@ constexpr uint32_t fitting_units(uint32_t dim, int cache_dtype) {
     return dim == 64 ? cache_dtype == PKV_FP8 ? 768 : 1024 : 512;
 }
 constexpr uint32_t kMostUnits = 1024;
+static_assert(kMostUnits <= 1u << kJoinDown && fitting_units(64, PKV_BF16) <= kMostUnits && fitting_units(128, PKV_BF16) <= kMostUnits,
+              "shares of a row as they are joined");
 constexpr int kMany = 96;
 constexpr int kLeast = 4;           // tiles of a unit, one a wave
 constexpr int kLeastSteps = 8;      // rows_kernel: tiles of 64 slots of a share

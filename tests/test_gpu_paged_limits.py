@@ -7,7 +7,7 @@ import pytest
 import torch
 
 import paged_ref as P
-from test_gpu_paged import BF16, F16, KIND_IDS, KINDS, make, prompts, running, sequences, words
+from test_gpu_paged import BF16, F16, F8, KIND_IDS, KINDS, make, prompts, running, sequences, words
 
 pytestmark = pytest.mark.gpu
 
@@ -89,3 +89,23 @@ def test_many_sequences_past_the_limit(ctx, dtype):
     want = torch.zeros_like(out)
     attend_prompts(dq, dk, dv, words(st), max_rows=11, out=want)
     assert torch.equal(out, want) and not out[3 + 11:3 + 40].any() and out[3 + 40].any()
+
+
+@pytest.mark.parametrize("cache_type", [BF16, F8], ids=["bf16", "8-bit"])
+def test_as_many_shares_as_there_can_be(ctx, cache_type):
+    """One sequence and head cut into 1,024 shares, every value the largest of its
+    type and every weight the same: no sum on the way passes the end of f32."""
+    from provekv_amd.paged import PagedKVCache
+    page, slots = 65536, 97 * 1024 * 32
+    cache = PagedKVCache(1, 1, slots // page + 1, page, 64, dtype=cache_type)
+    if cache_type == F8:
+        cache.buf[:, :, 1] = 0x7e
+        cache.scales[:, :, 1] = 246
+        most = 448.0 * 2.0 ** 119
+    else:
+        most = torch.finfo(BF16).max
+        cache.buf[:, :, 1] = most
+    q = torch.ones(1, 2, 64, dtype=BF16, device="cuda")
+    out = cache.attend(0, q, words([list(range(cache.pages))]), slots)
+    # sums of f32 are off by less than half a step of bf16 here
+    assert (out.double() == most).all()
