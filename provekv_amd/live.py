@@ -91,16 +91,18 @@ class DeviceCalls:
         return type(op).from_buffer_copy(op), extra
 
     @staticmethod
-    def _served(t, call: str):
-        """No gradient or tangent of t is lost without a word."""
+    def _served(t, call: str, *more):
+        """No gradient or tangent of a call's tensors is lost without a word."""
         import torch
-        if t is None:
-            return
-        if t.requires_grad and torch.is_grad_enabled():
-            raise ValueError(f"{call} has no backward pass: detach its tensors or call it under torch.no_grad()")
         fwd = torch.autograd.forward_ad     # outside of any level nothing has a tangent
-        if getattr(fwd, "_current_level", 0) >= 0 and fwd.unpack_dual(t).tangent is not None:
-            raise ValueError(f"{call} has no forward-mode derivative: give it the primal of a dual tensor")
+        level = getattr(fwd, "_current_level", 0) >= 0
+        for x in (t, *more):
+            if x is None:
+                continue
+            if x.requires_grad and torch.is_grad_enabled():
+                raise ValueError(f"{call} has no backward pass: detach its tensors or call it under torch.no_grad()")
+            if level and fwd.unpack_dual(x).tangent is not None:
+                raise ValueError(f"{call} has no forward-mode derivative: give it the primal of a dual tensor")
 
     def _on_device(self, dev, *tensors):
         for t in tensors:

@@ -178,8 +178,8 @@ class PagedKVCache(DeviceCalls):
         becomes NaN.  A row whose slot is negative or has no page is not stored.
         Two rows must not have the same place of the same page: sequences that
         share pages store into pages of their own.  Rows that lie among the
-        pages themselves are refused (load them first), as are rows that carry a
-        gradient or a tangent."""
+        pages themselves are refused (load them first), as are rows or pages that
+        carry a gradient or a tangent."""
         some = keys if keys is not None else values
         if some is None:
             return
@@ -192,7 +192,7 @@ class PagedKVCache(DeviceCalls):
             if t.dim() != 3 + lead or t.shape != some.shape or t.shape[lead + 1:] != (self.heads, self.dim) or \
                     (lead and t.shape[0] != self.layers):
                 raise ValueError(f"keys and values must be [{'layers, ' if lead else ''}rows, {self.heads}, {self.dim}]")
-            self._served(t, "store")
+            self._served(t, "store", self.buf)
         dev = self.device
         self._tables(tables)
         self._on_device(dev, keys, values, tables)
@@ -209,13 +209,15 @@ class PagedKVCache(DeviceCalls):
         values), packed [layers, rows, heads, dim] (no layers axis for one layer)
         of dtype (bfloat16 unless given; exact in float32, and in bfloat16 from 8
         bits).  Whole sequences: starts the running sum of lens.  Rows whose slot
-        is negative or has no page, or that are no sequence's, are 0."""
+        is negative or has no page, or that are no sequence's, are 0.  Pages that
+        carry a gradient or a tangent are refused."""
         import torch
         dtype = dtype or torch.bfloat16
         if _rows_dtype(dtype) is None:
             raise TypeError("load gives float32, bfloat16 or float16")
         if rows < 0:
             raise ValueError("rows is not negative")
+        self._served(self.buf, "load")
         dev = self.device
         self._tables(tables)
         self._on_device(dev, tables)
@@ -245,13 +247,13 @@ class PagedKVCache(DeviceCalls):
         the launch.  Of a sequence that has more rows, those past max_rows are no
         sequence's; a length past max_len is taken as max_len.
 
-        A q that carries a gradient or a tangent is refused: there is no
-        derivative."""
+        Tensors that carry a gradient or a tangent, the pages among them, are
+        refused: there is no derivative."""
         import torch
         dev = self.device
         self._tables(tables)
         self._on_device(dev, q, tables, lse, out)
-        self._served(q, "attend")
+        self._served(q, "attend", self.buf, lse, out)
         sized = None      # by an int length: the call's own, so that a loop over lengths keeps one struct
         if max_len is None and not isinstance(lens, torch.Tensor):
             sized = min(max(int(lens), 1), tables.shape[1] * self.page_size)
@@ -340,8 +342,7 @@ class _Prompts(DeviceCalls):
         import torch
         dev = q.device
         self._on_device(dev, k, v, starts, lse, out)
-        for t in (q, k, v):
-            self._served(t, "attend_prompts")
+        self._served(q, "attend_prompts", k, v, lse, out)
 
         def plan(q, k, v):
             return self._plan((_like(q), _like(k), _like(v), starts.shape, window, sinks, scale, _like(lse), _like(out),
