@@ -39,12 +39,23 @@ __device__ inline Seq seq_of_all(const SeqsDev& q, uint32_t s, uint32_t max_rows
     return {__builtin_amdgcn_readfirstlane(o.row0), __builtin_amdgcn_readfirstlane(o.rows),
             __builtin_amdgcn_readfirstlane(o.len), __builtin_amdgcn_readfirstlane(o.first)};
 }
+// How many of the ascending ends of n things are at most x (both the same in all
+// lanes), 64 of them a read: whose x is, or n.
+template <class End>
+__device__ inline uint32_t ends_up_to(uint32_t n, int x, uint32_t lane, End end) {
+    uint32_t lo = 0, left = n;
+    while (left) {
+        const uint32_t step = (left + 63) / 64, last = (lane + 1) * step - 1;
+        lo += __popcll(__ballot(last < left && end(lo + last) <= x)) * step;
+        if (step == 1) break;
+        left = min(step, n - lo);
+    }
+    return lo;
+}
 // The sequence of packed row r (the same in all lanes): the first that ends behind it; -1: nobody's.
 __device__ inline int seq_of_row(const SeqsDev& q, int r, uint32_t lane) {
     if (!q.starts) return r / static_cast<int>(q.each);
-    uint32_t s = 0;
-    for (uint32_t j = 0; j < q.seqs; j += 64)
-        s += __popcll(__ballot(j + lane < q.seqs && q.starts[j + lane + 1] <= r));
+    const uint32_t s = ends_up_to(q.seqs, r, lane, [&](uint32_t x) { return q.starts[x + 1]; });
     return s < q.seqs && q.starts[s] <= r ? static_cast<int>(s) : -1;
 }
 // The page of sequence s that holds slot j (0 <= j < its length); -1: none.
@@ -278,9 +289,16 @@ __device__ inline int share_of(int64_t all, uint32_t target, int least) {
 // sequences: all their tiles by the units wanted a head, at least kLeast.  Every
 // workgroup works this out from the lengths, which only the device knows: a lane
 // takes a run of sequences, so up to 64 of them cost one read of their words.
+// That work grows with the square of the sequences: more than kCounted are
+// counted once, by a kernel ahead, and looked up.
 struct Unit {
     int seq, share, shares, first;   // first: the sequence's first unit
 };
+// Tiles of a unit: no more than target (or most) + sequences units.
+__device__ inline int unit_size(int64_t all, uint32_t target, uint32_t most) {
+    return share_of(all, all >= static_cast<int64_t>(kMany) * most ? most : target, kLeast);
+}
+__device__ inline int units_of(int tiles, int size) { return tiles < 0 ? 0 : max(1, (tiles + size - 1) / size); }
 __device__ inline bool find_unit(const PagedDev& a, uint32_t u, uint32_t target, uint32_t most, uint32_t lane, Unit* o) {
     const uint32_t per = (a.seq.seqs + 63) / 64, s0 = min(lane * per, a.seq.seqs), s1 = min(s0 + per, a.seq.seqs);
     int mine = -1;                      // of the run's only sequence
@@ -290,13 +308,11 @@ __device__ inline bool find_unit(const PagedDev& a, uint32_t u, uint32_t target,
         all += max(mine, 0);
     }
     for (int x = 32; x; x >>= 1) all += __shfl_xor(static_cast<long long>(all), x);
-    // no more than target (or most) + sequences units
-    const int size = share_of(all, all >= static_cast<int64_t>(kMany) * most ? most : target, kLeast);
-    auto units = [&](int tiles) { return tiles < 0 ? 0 : max(1, (tiles + size - 1) / size); };
+    const int size = unit_size(all, target, most);
     int n = 0;
-    if (per == 1) n = units(mine);
+    if (per == 1) n = units_of(mine, size);
     else
-        for (uint32_t s = s0; s < s1; ++s) n += units(few_tiles(a, s));
+        for (uint32_t s = s0; s < s1; ++s) n += units_of(few_tiles(a, s), size);
     int end = n;
     for (int x = 1; x < 64; x <<= 1) {
         const int y = __shfl_up(end, x);
@@ -308,11 +324,19 @@ __device__ inline bool find_unit(const PagedDev& a, uint32_t u, uint32_t target,
     int first = __shfl(end - n, static_cast<int>(at));
     uint32_t s = at * per;
     for (;; ++s) {
-        n = per == 1 ? __shfl(n, static_cast<int>(at)) : units(few_tiles(a, s));
+        n = per == 1 ? __shfl(n, static_cast<int>(at)) : units_of(few_tiles(a, s), size);
         if (want < first + n) break;
         first += n;
     }
     *o = {static_cast<int>(s), want - first, n, first};
+    return true;
+}
+// The same by the plan of few_plan_kernel.
+__device__ inline bool look_up_unit(const PagedDev& a, const int32_t* plan, uint32_t u, uint32_t lane, Unit* o) {
+    const int want = static_cast<int>(u);
+    const uint32_t s = ends_up_to(a.seq.seqs, want, lane, [&](uint32_t x) { return plan[2 * x] + plan[2 * x + 1]; });
+    if (s >= a.seq.seqs) return false;
+    *o = {static_cast<int>(s), want - plan[2 * s], plan[2 * s + 1], plan[2 * s]};
     return true;
 }
 
@@ -448,6 +472,8 @@ struct PagedPart {
     int32_t* plan;     // [sequence][2]: first unit, units; of many rows the first that is a share, shares of a tile
     uint32_t units, target, rows, parts;
     uint32_t most;     // decode_kernel: aimed at where they are long
+    int32_t* ends;     // [sequence] of many rows, counted ahead: units up to its last
+    bool counted;      // plan (and ends) are there before the kernel
 };
 
 // The rows of a sequence of few (rows x group up to 16) against a share of its
@@ -484,10 +510,11 @@ __global__ __launch_bounds__(64 * WAVES, WAVES > 8 ? 4 : 2) void decode_kernel(P
     // are a multiple of 8
     const uint32_t h = blockIdx.x % a.heads, u = blockIdx.x / a.heads;
     Unit unit;
-    if (!find_unit(a, u, part.target, part.most, lane, &unit)) return;
+    if (!(part.counted ? look_up_unit(a, part.plan, u, lane, &unit) : find_unit(a, u, part.target, part.most, lane, &unit)))
+        return;
     unit = {__builtin_amdgcn_readfirstlane(unit.seq), __builtin_amdgcn_readfirstlane(unit.share),
             __builtin_amdgcn_readfirstlane(unit.shares), __builtin_amdgcn_readfirstlane(unit.first)};
-    if (h == 0 && unit.share == 0 && threadIdx.x == 0) {
+    if (h == 0 && unit.share == 0 && threadIdx.x == 0 && !part.counted) {
         part.plan[2 * unit.seq] = unit.first;
         part.plan[2 * unit.seq + 1] = unit.shares;
     }
@@ -738,6 +765,10 @@ __device__ inline RowWork row_work(const PagedDev& a, uint32_t s, int64_t few, i
     w.steps = tiles_of(a, q.first + first, q.first + q.rows - 1, 64).count;
     return w;
 }
+__device__ inline int rows_size(int64_t all, uint32_t target) {
+    return target ? share_of(all, target, kLeastSteps) : 0x7fffffff;
+}
+__device__ inline int shares_of(const RowWork& w, int size) { return max(1, w.steps / size); }
 __device__ inline bool find_rows(const PagedDev& a, uint32_t u, int64_t few, int rows, uint32_t target, uint32_t lane,
                                  RowUnit* o) {
     const uint32_t per = (a.seq.seqs + 63) / 64, s0 = min(lane * per, a.seq.seqs), s1 = min(s0 + per, a.seq.seqs);
@@ -749,8 +780,8 @@ __device__ inline bool find_rows(const PagedDev& a, uint32_t u, int64_t few, int
     }
     if (target)
         for (int x = 32; x; x >>= 1) all += __shfl_xor(static_cast<long long>(all), x);
-    const int size = target ? share_of(all, target, kLeastSteps) : 0x7fffffff;
-    auto shares = [&](const RowWork& w) { return max(1, w.steps / size); };
+    const int size = rows_size(all, target);
+    auto shares = [&](const RowWork& w) { return shares_of(w, size); };
     int units = 0, parts = 0, longest = 0;
     for (uint32_t s = s0; s < s1; ++s) {
         const RowWork w = per == 1 ? mine : row_work(a, s, few, rows);
@@ -785,6 +816,93 @@ __device__ inline bool find_rows(const PagedDev& a, uint32_t u, int64_t few, int
         }
         first += w.tiles * n;
         part += n > 1 ? w.tiles * n : 0;
+    }
+}
+// The same by the plan of rows_plan_kernel, in the sequences' order.
+__device__ inline bool look_up_rows(const PagedDev& a, const int32_t* plan, const int32_t* ends, uint32_t u, int64_t few,
+                                    int rows, uint32_t lane, RowUnit* o) {
+    const int want = static_cast<int>(u);
+    const uint32_t s = ends_up_to(a.seq.seqs, want, lane, [&](uint32_t x) { return ends[x]; });
+    if (s >= a.seq.seqs) return false;
+    const int n = plan[2 * s + 1], at = want - (s ? ends[s - 1] : 0), x = at / n;
+    const int tile = row_work(a, s, few, rows).tiles - 1 - x;
+    *o = {static_cast<int>(s), tile, at - x * n, n, plan[2 * s] + tile * n};
+    return true;
+}
+
+// ------------------------------------------------------------ many sequences: counted once
+// More sequences than this are counted by one workgroup ahead of the kernel, whose
+// launch costs about what the counting by every workgroup does here: 256 single
+// tokens on 20 slots of 8 heads of 64 take 27 us, 23 counted ahead, of 4 heads 17
+// and 21; 1,024 of 8 heads 182 and 48, 4,096 prompts of 4 rows 9,900 and 690.
+constexpr uint32_t kCounted = 256;
+constexpr uint32_t kCounters = 1024;   // its threads
+
+// The sum of x over the workgroup's threads before this one; *all: over all of them.
+__device__ inline int64_t sum_before(int64_t x, int64_t* all, int64_t (&waves)[kCounters / 64]) {
+    const uint32_t lane = threadIdx.x % 64, wave = threadIdx.x / 64;
+    int64_t end = x;
+    for (uint32_t o = 1; o < 64; o <<= 1) {
+        const int64_t y = __shfl_up(static_cast<long long>(end), o);
+        if (lane >= o) end += y;
+    }
+    __syncthreads();                   // the last call's sums have been read
+    if (lane == 63) waves[wave] = end;
+    __syncthreads();
+    int64_t before = 0;
+    *all = 0;
+    for (uint32_t w = 0; w < kCounters / 64; ++w) {
+        before += w < wave ? waves[w] : 0;
+        *all += waves[w];
+    }
+    return before + end - x;
+}
+
+// decode_kernel's units: plan[2 s] the first of sequence s, plan[2 s + 1] how many.
+__global__ __launch_bounds__(kCounters) void few_plan_kernel(PagedDev a, PagedPart part) {
+    __shared__ int64_t waves[kCounters / 64];
+    int64_t mine = 0, all, first = 0;
+    for (uint32_t s = threadIdx.x; s < a.seq.seqs; s += kCounters) mine += max(few_tiles(a, s), 0);
+    sum_before(mine, &all, waves);
+    const int size = unit_size(all, part.target, part.most);
+    for (uint32_t s0 = 0; s0 < a.seq.seqs; s0 += kCounters) {
+        const uint32_t s = s0 + threadIdx.x;
+        const int n = s < a.seq.seqs ? units_of(few_tiles(a, s), size) : 0;
+        const int64_t before = sum_before(n, &all, waves);
+        if (s < a.seq.seqs) {
+            part.plan[2 * s] = static_cast<int32_t>(first + before);
+            part.plan[2 * s + 1] = n;
+        }
+        first += all;
+    }
+}
+
+// rows_kernel's: ends[s] the units up to sequence s's last, plan[2 s] the first of
+// its units that are shares, plan[2 s + 1] the shares of a tile.
+__global__ __launch_bounds__(kCounters) void rows_plan_kernel(PagedDev a, PagedPart part, int few) {
+    __shared__ int64_t waves[kCounters / 64];
+    int64_t mine = 0, all, units = 0, parts = 0;
+    for (uint32_t s = threadIdx.x; s < a.seq.seqs; s += kCounters) {
+        const RowWork w = row_work(a, s, few, static_cast<int>(part.rows));
+        mine += static_cast<int64_t>(w.tiles) * w.steps;
+    }
+    sum_before(mine, &all, waves);
+    const int size = rows_size(all, part.target);
+    for (uint32_t s0 = 0; s0 < a.seq.seqs; s0 += kCounters) {
+        const uint32_t s = s0 + threadIdx.x;
+        RowWork w{};
+        if (s < a.seq.seqs) w = row_work(a, s, few, static_cast<int>(part.rows));
+        const int n = shares_of(w, size);
+        const int64_t own = static_cast<int64_t>(w.tiles) * n, shares = n > 1 ? own : 0;
+        const int64_t end = units + own + sum_before(own, &all, waves);
+        units += all;
+        const int64_t at = parts + sum_before(shares, &all, waves);
+        parts += all;
+        if (s < a.seq.seqs) {
+            part.ends[s] = static_cast<int32_t>(min(end, static_cast<int64_t>(0x7fffffff)));   // more where starts do not ascend
+            part.plan[2 * s] = static_cast<int32_t>(at);
+            part.plan[2 * s + 1] = n;
+        }
     }
 }
 
@@ -970,11 +1088,14 @@ __global__ __launch_bounds__(512, 2) void rows_kernel(PagedDev a, PagedPart part
     // heads fastest, so that a head's workgroups share an XCD's L2 where the heads are a multiple of 8
     const uint32_t h = blockIdx.x % a.heads;
     RowUnit rt;
-    if (!find_rows(a, blockIdx.x / a.heads, few, kRowTile, part.target, lane, &rt)) return;
+    const uint32_t u = blockIdx.x / a.heads;
+    if (!(part.counted ? look_up_rows(a, part.plan, part.ends, u, few, kRowTile, lane, &rt)
+                       : find_rows(a, u, few, kRowTile, part.target, lane, &rt)))
+        return;
     rt = {__builtin_amdgcn_readfirstlane(rt.seq), __builtin_amdgcn_readfirstlane(rt.tile),
           __builtin_amdgcn_readfirstlane(rt.share), __builtin_amdgcn_readfirstlane(rt.shares),
           __builtin_amdgcn_readfirstlane(rt.part)};
-    if (part.target && h == 0 && rt.tile == 0 && rt.share == 0 && threadIdx.x == 0) {
+    if (part.target && h == 0 && rt.tile == 0 && rt.share == 0 && threadIdx.x == 0 && !part.counted) {
         part.plan[2 * rt.seq] = rt.part;
         part.plan[2 * rt.seq + 1] = rt.shares;
     }
@@ -1497,12 +1618,14 @@ struct Plan {
     int ks;                        // rows_kernel: 256 / ks rows a tile
     uint32_t row_units, row_target, parts;   // units a head at most, shares aimed at (0: none), room for
     uint64_t rows_ml, rows_plan, bytes;      // the two kernels follow each other in the same workspace; all of it
+    bool counted;                  // by the plan kernels
 };
 Plan plan_of(const PagedDev& a, uint32_t dim, int cache_dtype) {
     Plan p{};
     const uint64_t most = static_cast<uint64_t>(a.max_rows) * a.group;
     p.few = a.seq.paged && (!a.seq.each || most <= kFew);
     p.many = !a.seq.paged || most > kFew;
+    p.counted = a.seq.seqs > kCounted;
     // tiles of `step` slots that `rows` rows can see: all, or the window, the rows before the last and the sinks, rounded
     // to tiles apart
     auto tiles_for = [&](uint64_t rows, uint64_t step) {
@@ -1556,11 +1679,11 @@ Plan plan_of(const PagedDev& a, uint32_t dim, int cache_dtype) {
                            ? static_cast<uint32_t>(((groups > 256 ? 512 : 256) + a.heads - 1) / a.heads) : 0;
         p.parts = p.row_target;
         p.row_units = static_cast<uint32_t>(tiles) + p.row_target;
-        if (p.row_target) {
+        if (p.row_target || p.counted) {
             const uint64_t rows = static_cast<uint64_t>(a.heads) * p.parts * rows_of_tile(p.ks);
             p.rows_ml = round256(rows * dim * 4);
             p.rows_plan = p.rows_ml + round256(rows * 8);
-            p.bytes = std::max(p.bytes, p.rows_plan + round256(8ull * a.seq.seqs));
+            p.bytes = std::max(p.bytes, p.rows_plan + round256((p.counted ? 12ull : 8ull) * a.seq.seqs));
         }
     }
     return p;
@@ -1574,7 +1697,9 @@ int attend_typed(const PagedDev& a, uint8_t* ws, hipStream_t st) {
     if constexpr (PAGED)
         if (p.few) {
             const PagedPart part{reinterpret_cast<float*>(ws), reinterpret_cast<float*>(ws + p.ml),
-                                 reinterpret_cast<int32_t*>(ws + p.plan), p.units, p.target, p.rows, p.units, p.most};
+                                 reinterpret_cast<int32_t*>(ws + p.plan), p.units, p.target, p.rows, p.units, p.most, nullptr,
+                                 p.counted};
+            if (p.counted) few_plan_kernel<<<1, kCounters, 0, st>>>(a, part);
             const uint32_t grid = a.heads * p.units + clears(a);
             constexpr int kWide = wide_waves(D, CT);
             if (p.wide) decode_kernel<CT, QT, D, kWide><<<grid, 64 * kWide, 0, st>>>(a, part);
@@ -1584,8 +1709,10 @@ int attend_typed(const PagedDev& a, uint8_t* ws, hipStream_t st) {
     if (p.many) {
         const PagedPart part{reinterpret_cast<float*>(ws), reinterpret_cast<float*>(ws + p.rows_ml),
                              reinterpret_cast<int32_t*>(ws + p.rows_plan), p.row_units, p.row_target,
-                             static_cast<uint32_t>(rows_of_tile(p.ks)), p.parts, 0};
+                             static_cast<uint32_t>(rows_of_tile(p.ks)), p.parts, 0,
+                             reinterpret_cast<int32_t*>(ws + p.rows_plan) + 2ull * a.seq.seqs, p.counted};
         const int few = PAGED && p.few ? kFew : 0;
+        if (p.counted) rows_plan_kernel<<<1, kCounters, 0, st>>>(a, part, few);
         const uint32_t grid = a.heads * p.row_units + (p.few ? 0 : clears(a));
         if (p.ks == 4) rows_kernel<CT, QT, D, PAGED, 4><<<grid, 512, 0, st>>>(a, part, few);
         else if (p.ks == 2) rows_kernel<CT, QT, D, PAGED, 2><<<grid, 512, 0, st>>>(a, part, few);
