@@ -192,7 +192,7 @@ class PagedKVCache(DeviceCalls):
             if t.dim() != 3 + lead or t.shape != some.shape or t.shape[lead + 1:] != (self.heads, self.dim) or \
                     (lead and t.shape[0] != self.layers):
                 raise ValueError(f"keys and values must be [{'layers, ' if lead else ''}rows, {self.heads}, {self.dim}]")
-            self._served(t, "store", self.buf)
+        self._served(keys, "store", values, self.buf)
         dev = self.device
         self._tables(tables)
         self._on_device(dev, keys, values, tables)
