@@ -488,9 +488,10 @@ struct PagedPart {
 // Weights meet the values as two terms of a 16-bit type, which the bytes hide.
 // WAVES 4, or 8 or 16 (as registers allow) where a sequence's slots are one
 // unit's, so that the call is one launch (a row of 32 heads of 64 on 700 slots:
-// 13 us with the host's call, 23 in units of four waves and a join).  The next
-// tile is on its way while one is worked on, and the words of the pages of the
-// one after it, so that no read waits for a page's number.
+// 14 us with the host's call, 16 in units of four waves and a join; in a graph 12
+// and 9.6, and eight such rows on about 900 slots 16.5 and 19.4).  The next tile
+// is on its way while one is worked on, and the words of the pages of the one
+// after it, so that no read waits for a page's number.
 // Bound by the bytes: 5.9 TB/s of 24 x 32,768 slots of 8 heads of 128, 5.7 in 8
 // bits, 5.5 and 5.0 where the 24 sequences have 700 to 32,768; a large copy
 // reaches 4.8 on this card, a large sum 4.0.  Of short sequences by the chain
@@ -1029,9 +1030,9 @@ __device__ inline void meet() {
 // The workgroup's waves are two groups of four, one of each on a SIMD, that take
 // turns: while one has the matrix cores, O of the tile before and S of the next,
 // the other has the vector units for its softmax, and they meet between.  For
-// prompts of 8,192, 6,298 and 3,900 rows of 32 query heads of 128 that takes 850
-// us (1,160 TFLOP/s; 1,250 for one of 16,384 rows; a library's square product
-// reaches 1,330): the matrix cores are busy 62 % of the cycles, the tiles' LDS
+// prompts of 8,192, 5,920 and 4,278 rows of 32 query heads of 128 that takes 841
+// to 905 us, card by card (1,170 to 1,090 TFLOP/s; 1,250 for one of 16,384 rows; a
+// library's square product reaches 1,330): the matrix cores are busy 62 % of the cycles, the tiles' LDS
 // reads conflict in 0.1 %, and a workgroup's start and end, 9 us that nothing
 // hides since one fills a CU's registers, take most of the rest.  Two workgroups
 // of four waves each, which meet nobody, took 1,023 (matrix cores 44 %, vector
