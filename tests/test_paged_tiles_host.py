@@ -56,6 +56,11 @@ def expect(names, pages, queries, D, paged, rows, joined, what):
     assert any("16join_rows_kernelI" in x for x in names) == joined, (what, names)
 
 
+def counted(names):
+    """Plan kernels ahead of the others."""
+    return sum("plan_kernel" in x for x in names)
+
+
 if __name__ == "__main__":
     hip = C.CDLL(sys.argv[1], mode=C.RTLD_GLOBAL)   # found ahead of the runtime's own
     hip.host_hip_launched.restype = C.c_char_p
@@ -82,3 +87,15 @@ if __name__ == "__main__":
                                  5 + sum(counts), H, hq, D, max(counts), window, sinks, 0)
                 got = kernels(hip, lambda: lib.pkv_prompts(ctx, C.byref(op), None))
                 expect(got, dtype, dtype, D, False, tile, joined, name)
+    # up to 256 sequences are counted by every workgroup, more by a kernel ahead of each that cuts them
+    for seqs, ahead in ((1, 0), (64, 0), (256, 0), (257, 1), (5000, 1)):
+        side = 2 * 16 * 64
+        for starts, rows, most, kinds in ((None, seqs, 0, 1), (STARTS, seqs, 1, 1), (STARTS, seqs + 40, 0, 2)):
+            v = L.PageView(K, V, None, None, 200 * 2 * side, 2 * side, 16 * 64, 64, 200 * 2 * side - side, 1, 200, 2, 16, 64, 1)
+            s = L.Sequences(TABLES, 9, LENS, starts, seqs, 9, rows, 0)
+            op = L.PagedAttendOp(v, s, Q, OUT, 128, 64, 128, 64, None, WORK, 1 << 40, 0.125, 1, 2, most, 0, 0, 0, 0)
+            got = counted(kernels(hip, lambda: lib.pkv_paged_attend(ctx, C.byref(op), None)))
+            assert got == kinds * ahead, (seqs, kinds, got)
+        op = L.PromptsOp(Q, K, V, OUT, 384, 64, 384, 64, 384, 64, 128, 64, STARTS, None, WORK, 1 << 40, 0.125, 1, seqs, seqs + 40, 2,
+                         2, 64, 0, 0, 0, 0)
+        assert counted(kernels(hip, lambda: lib.pkv_prompts(ctx, C.byref(op), None))) == ahead
